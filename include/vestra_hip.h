@@ -487,6 +487,127 @@ int vk_attention_into_f32(vk_runtime* rt, const vk_tensor* q,
                           size_t heads, size_t rows, size_t head_dim,
                           vk_tensor* out);
 
+/* ------------------------------------------------------------------ */
+/* views that come one after another: rotary axes, a cache, attention   */
+/* over it                                                              */
+/* ------------------------------------------------------------------ */
+
+/* Rotary positions with several axes (time, height, width): the 32 pairs of
+ * a row of head_dim 64 are shared out over `count` axes, pairs[a] of them to
+ * axis a (their sum is 32; an axis may have none).
+ *   blocks (default): axis a owns 2*pairs[a] consecutive elements, the axes
+ *     one after another; pair i of an axis is its elements (i, i + pairs[a])
+ *     (VK_ROPE_ROTATE_HALF) or (2i, 2i + 1) (VK_ROPE_INTERLEAVED) and turns by
+ *     p * freq^(-2i/(2*pairs[a])) (VK_ROPE_EXP_HALF: over the axis's own
+ *     elements) or p * freq^(-2i/64) (VK_ROPE_EXP_HEAD).  Two axes of 16 pairs
+ *     are the 2D RoPE above.
+ *   VK_ROPE_SECTIONS: pair j is the row's elements (j, j + 32) or (2j, 2j + 1)
+ *     and turns by p * freq^(-2j/64); pairs 0..pairs[0]-1 take axis 0's
+ *     coordinate, the next pairs[1] axis 1's, and so on. */
+#define VK_ROPE_SECTIONS 4u
+#define VK_ROPE_MAX_AXES 4
+typedef struct vk_rope_axes {
+  size_t count;                     /* 1 .. VK_ROPE_MAX_AXES */
+  unsigned pairs[VK_ROPE_MAX_AXES]; /* 32 in all */
+  float freq;                       /* > 0 */
+  unsigned mode;                    /* VK_ROPE_* flags */
+} vk_rope_axes;
+
+/* Q/K LayerNorm (as vk_qk_norm_rope_f32, in the runtime's LayerNorm order;
+ * q_gamma .. k_beta all NULL: none) and the rotation above.  q holds
+ * sequences*n tokens of `heads` heads, k of `kv_heads` (which may differ;
+ * k and k_out NULL: q alone), each [heads, sequences, n, 64]
+ * (VK_QK_HEADS_OUTER) or [sequences, heads, n, 64] (VK_QK_VIEWS_OUTER).
+ * positions [sequences*n, count]: f32 (taken as they are, fractions
+ * included), i32 or i64.  The angle is held in 64 bits, so far positions turn
+ * exactly (to 1e-7 of a turn up to |p| = 2^31).  No table: nothing is
+ * allocated.  q_out may be q (in place) or a tensor that overlaps no other;
+ * k_out likewise.  head_dim 64.  No counterpart in the reference. */
+int vk_qk_norm_rope_axes_f32(vk_runtime* rt, const vk_tensor* q,
+                             const vk_tensor* k, const vk_tensor* q_gamma,
+                             const vk_tensor* q_beta, const vk_tensor* k_gamma,
+                             const vk_tensor* k_beta,
+                             const vk_tensor* positions, size_t sequences,
+                             size_t heads, size_t kv_heads, size_t n,
+                             size_t head_dim, const vk_rope_axes* axes,
+                             vk_qk_layout layout, float eps, vk_tensor* q_out,
+                             vk_tensor* k_out);
+
+/* A cache of K and V rows in 8 bits a value: codes u8 [sequences, heads,
+ * capacity, 64] and one f32 scale a row [sequences, heads, capacity]; a value
+ * is code * scale.  The four tensors are the caller's (zeroed or not: only
+ * written slots are read). */
+typedef enum vk_cache_format {
+  VK_CACHE_Q8 = 0, /* int8, scale = largest |x| of the row / 127             */
+  VK_CACHE_F8 = 1  /* 4 exponent and 3 mantissa bits (e4m3, no infinities),
+                      scale = largest |x| / 448                              */
+} vk_cache_format;
+typedef struct vk_kv_cache {
+  vk_tensor* k;       /* u8 codes */
+  vk_tensor* v;
+  vk_tensor* k_scale; /* f32 */
+  vk_tensor* v_scale;
+  size_t sequences, heads, capacity, head_dim; /* head_dim 64 */
+  int format;
+} vk_kv_cache;
+
+/* Which rows a call is about: row i < counts[s] of sequence s (i < n) is slot
+ * starts[s] + i.  starts and counts are i32 [sequences] on the device, read
+ * when the work runs (a captured graph follows them); NULL: 0 and n.  A row
+ * whose slot lies outside 0 .. capacity-1 is left out, as is a row past
+ * counts[s]: nothing of it is written.
+ *
+ * Quantises k and v (f32, [heads, sequences, n, 64] or [sequences, heads, n,
+ * 64] by `layout`) into the cache: scale = largest |x| / 127 (448) rounded to
+ * f32, code = x / scale rounded to f32 and then to the nearest code (ties to
+ * even).  A row whose scale would be below 2^-100 is held as zeros, scale 0; a
+ * row with an infinity or a NaN gets the scale NaN and codes 0, and reads back
+ * as NaN. */
+int vk_kv_cache_write_f32(vk_runtime* rt, const vk_kv_cache* cache,
+                          const vk_tensor* k, const vk_tensor* v, size_t n,
+                          const vk_tensor* starts, const vk_tensor* counts,
+                          vk_qk_layout layout);
+/* The rows back as f32, code * scale (k or v may be NULL: not read). */
+int vk_kv_cache_read_f32(vk_runtime* rt, const vk_kv_cache* cache, size_t n,
+                         const vk_tensor* starts, const vk_tensor* counts,
+                         vk_tensor* k, vk_tensor* v, vk_qk_layout layout);
+
+/* What a query may see and how it is scored.  All zeros: every held key, by
+ * q.k / 8.  The order is scale, cap, bias, masks, softmax. */
+typedef struct vk_attention_rules {
+  float scale;             /* of q.k; 0: 1/sqrt(64) */
+  float cap;               /* > 0: score = cap * tanh(score / cap) */
+  const vk_tensor* slopes; /* f32 [heads]: score -= slopes[h] * |p - j| for a
+                              query at position p and the key of slot j */
+  int causal;              /* key j only where j <= p */
+  const vk_tensor* prefix; /* i32 [sequences], with causal: keys j < prefix[s]
+                              are seen by every query */
+  const vk_tensor* q_docs; /* i32 [sequences, n] and */
+  const vk_tensor* k_docs; /* i32 [sequences, capacity]: key only where its
+                              document is the query's; */
+  int docs_ordered;        /* or, when set, where it is not a later one */
+} vk_attention_rules;
+
+/* Attention of `n` queries a sequence over the cache: query i < counts[s] is
+ * at position p = starts[s] + i and sees the keys of slots 0 .. starts[s] +
+ * counts[s] - 1 (inside the capacity, and below max_length where that is not
+ * 0) that `rules` (NULL: none) leave it; the call after
+ * vk_kv_cache_write_f32 of the same starts and counts.  max_length is what
+ * the host knows of the longest sequence's rows after the write: the work is
+ * shared out by it.  `heads` queries share the cache's heads (heads a multiple
+ * of them; head h reads head h / (heads / cache heads)).  q and out f32,
+ * [heads, sequences, n, 64] or [sequences, heads, n, 64] by `layout`; out
+ * overlaps no other tensor.  A query that sees nothing gets zeros; rows past
+ * counts[s] are left as they were.  A query that sees a key that reads back
+ * as NaN gets NaN; keys that it does not see have no effect whatever they
+ * hold.  Scores, weights and sums are held as in f32: the values of the cache
+ * are exact in f16, queries and weights are taken as two f16 parts. */
+int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache,
+                            const vk_tensor* q, size_t heads, size_t n,
+                            const vk_tensor* starts, const vk_tensor* counts,
+                            size_t max_length, const vk_attention_rules* rules,
+                            vk_qk_layout layout, vk_tensor* out);
+
 /* CudaRuntime::prepend_cls_add_pos_f32(patches, cls, pos, n_patches, embed)
  * (patch_embed.rs:234-240): row 0 = cls + pos[0]; row 1+p = patch_p + pos[1+p]. */
 int vk_prepend_cls_add_pos_f32(vk_runtime* rt, const vk_tensor* patches,

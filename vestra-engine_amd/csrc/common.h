@@ -186,6 +186,13 @@ int split_weights(vk_linear* lin, bool f16_values);
 // run the sequence once eagerly first.  The buffer it replaces is retired,
 // not freed.
 int ensure_work(vk_runtime* rt, size_t floats, const char* who);
+// VK_ERR_INVALID unless `t` lies on the runtime's device.
+int check_device(const vk_runtime* rt, const vk_tensor* t, const char* what);
+// VK_ERR_INVALID unless `t` is f32 [len], 16-byte aligned and on the runtime's
+// device.
+int check_f32(const vk_runtime* rt, const vk_tensor* t, size_t len, const char* what);
+// Whether two tensors (either may be null or empty) share memory.
+bool overlap(const vk_tensor* a, const vk_tensor* b);
 // Stream-ordered device-to-device copy of `bytes` bytes as a kernel (a
 // captured sequence then holds kernel nodes only).
 int device_copy(vk_runtime* rt, void* dst, const void* src, size_t bytes);

@@ -172,6 +172,24 @@ int ensure_work(vk_runtime* rt, size_t floats, const char* who) {
   return VK_OK;
 }
 
+int check_device(const vk_runtime* rt, const vk_tensor* t, const char* what) {
+  VK_REQUIRE(t && t->rt && t->rt->device == rt->device, "%s: a tensor of another device", what);
+  return VK_OK;
+}
+
+int check_f32(const vk_runtime* rt, const vk_tensor* t, size_t len, const char* what) {
+  VK_REQUIRE(t && t->dtype == VK_F32 && t->len == len, "%s must be f32 [%zu] (holds %zu)", what, len,
+             t ? t->len : 0);
+  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0, "%s must be 16-byte aligned", what);
+  return check_device(rt, t, what);
+}
+
+bool overlap(const vk_tensor* a, const vk_tensor* b) {
+  if (!a || !b || a->len == 0 || b->len == 0) return false;
+  const uintptr_t x = reinterpret_cast<uintptr_t>(a->ptr), y = reinterpret_cast<uintptr_t>(b->ptr);
+  return x < y + b->len * dtype_size(b->dtype) && y < x + a->len * dtype_size(a->dtype);
+}
+
 // Device-to-device copies as kernels.  16-byte aligned copies: persistent
 // single-wave workgroups over 3 KiB chunks (three float4 per lane), wave w
 // taking chunks w, w + W, ... (W = vk::stream_waves), the next chunk loaded

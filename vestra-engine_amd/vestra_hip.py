@@ -34,6 +34,8 @@ VK_F32, VK_F16, VK_U8, VK_I32, VK_I64 = 0, 1, 2, 3, 4
 VK_ROPE_ROTATE_HALF, VK_ROPE_INTERLEAVED = 0, 1
 VK_ROPE_EXP_HALF, VK_ROPE_EXP_HEAD = 0, 2
 VK_ROPE_DEFAULT = 0
+VK_ROPE_SECTIONS, VK_ROPE_MAX_AXES = 4, 4
+VK_CACHE_Q8, VK_CACHE_F8 = 0, 1
 VK_QK_HEADS_OUTER, VK_QK_VIEWS_OUTER = 0, 1
 # LayerNorm summation order of a runtime (vk_runtime_set_layernorm_order)
 VK_LN_ORDER_TREE, VK_LN_ORDER_SEQUENTIAL = 0, 1
@@ -101,6 +103,21 @@ class VitBlockWeights(C.Structure):
 
 class VitBlockWorkspace(C.Structure):
     _fields_ = [(n, _vp) for n in ("ln", "q", "k", "v", "attn", "hidden")]
+
+
+class _RopeAxes(C.Structure):
+    _fields_ = [("count", _sz), ("pairs", C.c_uint * VK_ROPE_MAX_AXES), ("freq", _f),
+                ("mode", C.c_uint)]
+
+
+class _KvCache(C.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("sequences", _sz),
+                ("heads", _sz), ("capacity", _sz), ("head_dim", _sz), ("format", _i)]
+
+
+class _AttentionRules(C.Structure):
+    _fields_ = [("scale", _f), ("cap", _f), ("slopes", _vp), ("causal", _i), ("prefix", _vp),
+                ("q_docs", _vp), ("k_docs", _vp), ("docs_ordered", _i)]
 
 
 _SIGS = {
@@ -190,6 +207,16 @@ _SIGS = {
     "vk_normalize_u8_hwc_nchw_f32": ([_vp, _vp, _sz, _sz, _vp, _vp, _vp], _i),
     "vk_attention_online_f32": ([_vp, _vp, _vp, _vp, _sz, _sz, _sz, _pp], _i),
     "vk_attention_into_f32": ([_vp, _vp, _vp, _vp, _sz, _sz, _sz, _vp], _i),
+    "vk_qk_norm_rope_axes_f32": (
+        [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _sz, _sz, C.POINTER(_RopeAxes), _i,
+         _f, _vp, _vp], _i),
+    "vk_kv_cache_write_f32": (
+        [_vp, C.POINTER(_KvCache), _vp, _vp, _sz, _vp, _vp, _i], _i),
+    "vk_kv_cache_read_f32": (
+        [_vp, C.POINTER(_KvCache), _sz, _vp, _vp, _vp, _vp, _i], _i),
+    "vk_attention_cached_f32": (
+        [_vp, C.POINTER(_KvCache), _vp, _sz, _sz, _vp, _vp, _sz, C.POINTER(_AttentionRules), _i,
+         _vp], _i),
     "vk_prepend_cls_add_pos_f32": ([_vp, _vp, _vp, _vp, _sz, _sz, _pp], _i),
     "vk_pos_embed_bicubic_f32": ([_vp, _vp, _sz, _sz, _sz, _sz, _f, _pp], _i),
     "vk_patch_embed_u8": ([_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp], _i),
@@ -408,6 +435,47 @@ class Graph:
             pass
 
 
+class RopeAxes:
+    """Rotary axes: pairs per axis (32 in all), frequency base, convention
+    (``vk_rope_axes``)."""
+
+    def __init__(self, pairs: Sequence[int], freq: float = 100.0, sections: bool = False,
+                 interleaved: bool = False, exp_head: bool = False):
+        if not 1 <= len(pairs) <= VK_ROPE_MAX_AXES or min(pairs) < 0:
+            raise VestraError(VK_ERR_INVALID, f"1 to {VK_ROPE_MAX_AXES} axes with pairs >= 0")
+        self.struct = _RopeAxes(
+            len(pairs), (C.c_uint * VK_ROPE_MAX_AXES)(*pairs), freq,
+            (VK_ROPE_SECTIONS if sections else 0) | (VK_ROPE_INTERLEAVED if interleaved else 0)
+            | (VK_ROPE_EXP_HEAD if exp_head else 0))
+
+
+class KvCache:
+    """K and V rows of `sequences` sequences in 8 bits a value (``vk_kv_cache``):
+    codes u8 [sequences, heads, capacity, 64] and scales f32 [sequences, heads,
+    capacity], tensors that it keeps alive.  ``Runtime.kv_cache`` makes one with
+    tensors of its own."""
+
+    def __init__(self, fmt: int, sequences: int, heads: int, capacity: int, k: Tensor, v: Tensor,
+                 k_scale: Tensor, v_scale: Tensor):
+        self.format, self.sequences, self.heads, self.capacity = fmt, sequences, heads, capacity
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.struct = _KvCache(k.handle, v.handle, k_scale.handle, v_scale.handle, sequences,
+                               heads, capacity, 64, fmt)
+
+
+class AttentionRules:
+    """What a query of ``Runtime.attention_cached_f32`` may see and how it is
+    scored (``vk_attention_rules``); keeps its tensors alive."""
+
+    def __init__(self, scale: float = 0.0, cap: float = 0.0, slopes: Optional[Tensor] = None,
+                 causal: bool = False, prefix: Optional[Tensor] = None,
+                 q_docs: Optional[Tensor] = None, k_docs: Optional[Tensor] = None,
+                 docs_ordered: bool = False):
+        self.tensors = (slopes, prefix, q_docs, k_docs)
+        self.struct = _AttentionRules(scale, cap, _h(slopes), 1 if causal else 0, _h(prefix),
+                                      _h(q_docs), _h(k_docs), 1 if docs_ordered else 0)
+
+
 class Runtime:
     """``vestra_kernels::cuda::CudaRuntime`` on one MI355X (one HIP stream)."""
 
@@ -610,6 +678,48 @@ class Runtime:
                            head_dim: int, out: Tensor) -> None:
         _check(lib.vk_attention_into_f32(self.handle, q.handle, k.handle, v.handle, heads,
                                          rows, head_dim, out.handle))
+
+    def kv_cache(self, fmt: int, sequences: int, heads: int, capacity: int) -> KvCache:
+        """A cache with tensors of its own (their contents undefined)."""
+        rows = sequences * heads * capacity
+        return KvCache(fmt, sequences, heads, capacity, self.alloc_u8(rows * 64),
+                       self.alloc_u8(rows * 64), self.alloc_f32(rows), self.alloc_f32(rows))
+
+    def kv_cache_write_f32(self, cache: KvCache, k: Tensor, v: Tensor, n: int,
+                           starts: Optional[Tensor] = None, counts: Optional[Tensor] = None,
+                           layout: int = VK_QK_HEADS_OUTER) -> None:
+        """Quantise row i < counts[s] of sequence s of k and v into slot starts[s] + i."""
+        _check(lib.vk_kv_cache_write_f32(self.handle, cache.struct, k.handle, v.handle, n,
+                                         _h(starts), _h(counts), layout))
+
+    def kv_cache_read_f32(self, cache: KvCache, n: int, starts: Optional[Tensor],
+                          counts: Optional[Tensor], k: Optional[Tensor], v: Optional[Tensor],
+                          layout: int = VK_QK_HEADS_OUTER) -> None:
+        """The cache's rows back as f32."""
+        _check(lib.vk_kv_cache_read_f32(self.handle, cache.struct, n, _h(starts), _h(counts),
+                                        _h(k), _h(v), layout))
+
+    def attention_cached_f32(self, cache: KvCache, q: Tensor, heads: int, n: int,
+                             starts: Optional[Tensor], counts: Optional[Tensor],
+                             max_length: int, rules: Optional[AttentionRules], out: Tensor,
+                             layout: int = VK_QK_HEADS_OUTER) -> None:
+        """Attention of n queries a sequence over the cache, by `rules`."""
+        _check(lib.vk_attention_cached_f32(self.handle, cache.struct, q.handle, heads, n,
+                                           _h(starts), _h(counts), max_length,
+                                           None if rules is None else rules.struct, layout,
+                                           out.handle))
+
+    def qk_norm_rope_axes_f32(self, q: Tensor, k: Optional[Tensor], q_gamma: Optional[Tensor],
+                              q_beta: Optional[Tensor], k_gamma: Optional[Tensor],
+                              k_beta: Optional[Tensor], positions: Tensor, heads: int,
+                              kv_heads: int, n: int, axes: RopeAxes, eps: float, q_out: Tensor,
+                              k_out: Optional[Tensor], sequences: int = 1,
+                              layout: int = VK_QK_HEADS_OUTER) -> None:
+        """Q/K LayerNorm and rotary positions of several axes."""
+        _check(lib.vk_qk_norm_rope_axes_f32(
+            self.handle, q.handle, _h(k), _h(q_gamma), _h(q_beta), _h(k_gamma), _h(k_beta),
+            positions.handle, sequences, heads, kv_heads, n, 64, axes.struct, layout, eps,
+            q_out.handle, _h(k_out)))
 
     def gelu_f32_in_place(self, x: Tensor) -> None:
         _check(lib.vk_gelu_f32_inplace(self.handle, x.handle))

@@ -80,7 +80,14 @@ def attention(q, kv, vv, v_scale, n, starts, counts, rules, limit=0, pick=None):
     roundings of a 64-term sum with room), the scale, the cap (tanh to 8 u of the cap), the
     bias and the running reference (a rounding each, at their size), 2^x and the
     weight's own two parts (64 u with the constant terms).  The output then moves by sum_j
-    p_j e_j |v_j - o|, and the value sum rounds (2 sqrt(n) + blocks + 8) u of sum p |v|."""
+    p_j e_j |v_j - o|, and the value sum rounds (2 sqrt(n) + blocks + 8) u of sum p |v|.
+
+    Two floors beside these.  A query's values are scaled so that its largest is at least 1,
+    and their second part is a multiple of 2^-24: off by 2^-25 = u / 2 of the row's largest
+    |q| at most, whatever the value's own size, which moves a score by that times sum
+    |k_d|.  A weight (2^x times V's scale) is at least 2^11 for the largest and its second part
+    a multiple of 2^-24: off by 2^-36 of the largest at most, whatever its own size (and
+    left out below), which moves the output by that times sum_j |code_j|."""
     S, H, _, _ = q.shape
     KV, cap = kv.shape[1], kv.shape[2]
     out = np.full(q.shape, np.nan)
@@ -104,6 +111,7 @@ def attention(q, kv, vv, v_scale, n, starts, counts, rules, limit=0, pick=None):
                 u = ks @ x * scale
                 terms = np.abs(ks) @ np.abs(x) * abs(scale)
                 e = 16 * terms + 8 * np.abs(u) + 64 + 2 * lsv[seen]
+                e = e + 0.5 * np.abs(x).max() * np.abs(ks).sum(1) * abs(scale)
                 if c:
                     u = c * np.tanh(u / c)
                     e = e + 8 * c
@@ -120,6 +128,8 @@ def attention(q, kv, vv, v_scale, n, starts, counts, rules, limit=0, pick=None):
                 size = p @ np.abs(vs)
                 tol[s, h, i] = (p * e) @ np.abs(vs - o) + 2 * U * np.abs(o) + (
                     2 * np.sqrt(len(p)) + len(p) / 64 + 8) * U * size + 1e-38
+                sv = np.maximum(v_scale[s, h * KV // H, :end][seen].astype(np.float64), LEAST)
+                tol[s, h, i] += 2.0 ** -36 * (p * sv).max() * (np.abs(vs) / sv[:, None]).sum(0)
     return out, tol
 
 
@@ -134,10 +144,20 @@ def set_i32(rt, t, a):
 
 
 def captured(rt, run):
-    """The graph of what `run` enqueues."""
-    rt.begin_capture()
-    run()
-    return rt.end_capture()
+    """The graph of what `run` enqueues.  Tensors of earlier tests that the collector
+    frees meanwhile would end the capture."""
+    import gc
+    gc.collect()
+    gc.disable()
+    try:
+        rt.begin_capture()
+        try:
+            run()
+        finally:
+            graph = rt.end_capture()
+    finally:
+        gc.enable()
+    return graph
 
 
 def heads_outer(x):

@@ -318,7 +318,7 @@ def test_a_video_step_by_step(rt, rng):
 def test_refusals(rt):
     S, H, cap, n = 2, 4, 8, 3
     c = rt.kv_cache(0, S, 2, cap)
-    q, o = rt.alloc_f32(S * H * n * 64), rt.alloc_f32(S * H * n * 64)
+    q, o = rt.upload_f32(np.ones(S * H * n * 64)), rt.alloc_f32(S * H * n * 64)
     z = rt.upload_i32(np.zeros(S, np.int32))
     slopes, docs = rt.upload_f32(np.ones(H)), rt.upload_i32(np.zeros(S * cap, np.int32))
     R = vh.AttentionRules
@@ -356,12 +356,12 @@ def test_capture_refuses_to_grow_the_work_buffer(rng):
     q, out = own.upload_f32(c.q), own.alloc_f32(c.q.size)
     st = own.upload_i32(c.starts)
     args = (c.cache, q, c.H, c.n, st, None, 0, None, out)
-    own.begin_capture()
-    try:
+
+    def refused():
         with pytest.raises(vh.VestraError):
             own.attention_cached_f32(*args)
-    finally:
-        own.end_capture()
+
+    cached.captured(own, refused)
     own.attention_cached_f32(*args)
     want = out.numpy()
     graph = cached.captured(own, lambda: own.attention_cached_f32(*args))

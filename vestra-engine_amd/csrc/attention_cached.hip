@@ -6,8 +6,11 @@
 // sums of values) over the keys that it meets; the lanes are joined once, at the
 // end.
 #include <cmath>
+#include <type_traits>
+#include <utility>
 
 #include "kv_cache.h"
+#include "split_f16.h"
 
 namespace {
 
@@ -29,7 +32,7 @@ struct Shape {
   Rules rules;
   uint32_t heads, group;  // query heads, and how many of them share a cache head
   uint32_t limit;         // keys at or past it are not seen (capacity, max_length)
-  uint32_t splits;
+  uint32_t splits, tiles;
 };
 
 // Keys of sequence s: those of slots 0 .. keys_of - 1.
@@ -181,6 +184,575 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   }
 }
 
+// ---------------------------------------------------------------------------
+// 32 queries a wave on the f16 matrix cores
+// ---------------------------------------------------------------------------
+using vks::f32x16;
+using vks::f32x4;
+using vks::u32x4;
+
+constexpr int KB = 64;          // keys of a block
+constexpr int kKPitch = 144;    // bytes of a K row in LDS: 64 f16 + 16
+constexpr int kVPitch = 192;    // of a V row: 64 f16 + 64
+constexpr float kPBits = 11.0f, kSlack = 2.0f;
+constexpr float kLowest = -3e38f;       // the running reference before any key
+constexpr float kSumDown = 0x1p-5f;     // of the denominators
+constexpr float kFarBits = 64.0f;
+constexpr int kQUp = 10;                // binary digits that Q is scaled up by
+constexpr int kFlush = 8;
+
+// Lane R of each 16-lane row, to all of the row.
+template <int R>
+__device__ __forceinline__ float bcast(float v) {
+  return __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(
+      static_cast<int>(__float_as_uint(v)), 0x150 | R, 0xf, 0xf, true)));
+}
+
+template <int I>
+using Int = std::integral_constant<int, I>;
+
+template <typename F, int... I>
+__device__ __forceinline__ void each(F f, std::integer_sequence<int, I...>) {
+  (f(Int<I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void each(F f) {
+  each(f, std::make_integer_sequence<int, N>{});
+}
+
+__device__ __forceinline__ float other_half(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                  false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// Eight codes as f16 (exact).
+template <int FORMAT>
+__device__ __forceinline__ u32x4 decode8(uint2 w) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  u32x4 r;
+  if constexpr (FORMAT == VK_CACHE_Q8) {
+    // code + 128 in the low byte of 1024 + .., and 1152 taken off
+    const uint32_t a = w.x ^ 0x80808080u, b = w.y ^ 0x80808080u;
+    const f16x2 off = {static_cast<_Float16>(1152.0f), static_cast<_Float16>(1152.0f)};
+    const uint32_t p[4] = {__builtin_amdgcn_perm(a, 0x64646464u, 0x00050004u),
+                           __builtin_amdgcn_perm(a, 0x64646464u, 0x00070006u),
+                           __builtin_amdgcn_perm(b, 0x64646464u, 0x00050004u),
+                           __builtin_amdgcn_perm(b, 0x64646464u, 0x00070006u)};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const f16x2 x = __builtin_bit_cast(f16x2, p[i]) - off;
+      r[i] = __builtin_bit_cast(uint32_t, x);
+    }
+  } else {
+    const auto a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w.x), 1.0f, false);
+    const auto b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w.x), 1.0f, true);
+    const auto c = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w.y), 1.0f, false);
+    const auto d = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(static_cast<int>(w.y), 1.0f, true);
+    r = u32x4{__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b),
+              __builtin_bit_cast(uint32_t, c), __builtin_bit_cast(uint32_t, d)};
+  }
+  return r;
+}
+
+// Four keys' values of one d a lane, out of LDS rows [key][d] of f16: in each 16
+// lanes, lane 4 r + c gives the address of key r's values d = 4 c .. 4 c + 3, and lane d
+// receives its d of keys 0 .. 3.
+__device__ __forceinline__ uint2 read_tr(const char* p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4 lds_t;
+  const s16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (lds_t*)(const_cast<char*>(p)));
+  return __builtin_bit_cast(uint2, v);
+}
+
+// What a block's keys bring beside their codes, in LDS: 64 of each, key 32 t + 8
+// (r / 4) + 4 half + r % 4 at 32 t + 16 half + r.
+struct KeyData {
+  float ks[KB];   // K's scale / 2^kQUp; 0 past the end
+  float lsv[KB];  // log2 of V's scale; -inf past the end
+  float rs[KB];   // kSumDown / V's scale; 0 past the end and where the scale is not a number
+  int doc[KB];
+  float low, high;  // least and largest lsv (keys past the end left out)
+};
+
+__device__ __forceinline__ int key_slot(int key) {
+  return (key & 32) | (key & 4) << 2 | (key & 24) >> 1 | (key & 3);
+}
+
+// tanh to a few units of the last place: the odd series to x^11 below 0.35, (e - 1) / (e + 1)
+// as 1 - 2 / (e + 1) from there.
+__device__ __forceinline__ float tanh1(float x) {
+  const float y = x * x;
+  float p = __builtin_fmaf(y, -0.008863236f, 0.021869488f);
+  p = __builtin_fmaf(y, p, -0.053968254f);
+  p = __builtin_fmaf(y, p, 0.13333334f);
+  p = __builtin_fmaf(y, p, -0.33333334f);
+  p = __builtin_fmaf(x * y, p, x);
+  const float e = __builtin_amdgcn_exp2f(x * 2.8853900817779268f);
+  const float b = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
+  return fabsf(x) < 0.35f ? p : b;
+}
+
+// A wave's 32 queries: lane l and lane l ^ 32 hold query l % 32.
+struct Queries {
+  u32x4 q[4][2];         // two f16 parts, d = 16 ks + 8 half + j
+  float back;            // 1, or what the row's own scale has to be undone by
+  bool own_scale;        // uniform: some row has one
+  float slope, cap_up;   // per unit of distance and cap, in base 2
+  int pre, doc;
+  long long pos;
+  f32x16 o[2], total[2];
+  float m, l;            // running reference, this lane's denominators
+};
+
+__device__ __forceinline__ void load_queries(Queries& w, const float* row, float c, int half) {
+  f32x4 x[4][2];
+  float m = 0.0f;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      x[ks][i] = *reinterpret_cast<const f32x4*>(row + 16 * ks + 8 * half + 4 * i) * c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[ks][i][e]));
+    }
+  m = fmaxf(m, other_half(m));
+  const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+  const bool usual = m == 0.0f || (e >= -10 && e < 5);
+  int up = usual ? kQUp : 14 - e;
+  up = up > 120 ? 120 : up;
+  const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
+  w.back = __uint_as_float(static_cast<uint32_t>(127 + kQUp - up) << 23);
+  w.own_scale = __builtin_amdgcn_ballot_w64(up != kQUp) != 0;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) {
+    uint32_t h[4], l[4];
+    const f32x4 a = x[ks][0] * f, b = x[ks][1] * f;
+    vks::split2_plain(a[0], a[1], &h[0], &l[0]);
+    vks::split2_plain(a[2], a[3], &h[1], &l[1]);
+    vks::split2_plain(b[0], b[1], &h[2], &l[2]);
+    vks::split2_plain(b[2], b[3], &h[3], &l[3]);
+    w.q[ks][0] = u32x4{h[0], h[1], h[2], h[3]};
+    w.q[ks][1] = u32x4{l[0], l[1], l[2], l[3]};
+  }
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w.o[dt][r] = w.total[dt][r] = 0.0f;
+  w.m = kLowest;
+  w.l = 0.0f;
+}
+
+__device__ __forceinline__ void flush(Queries& w) {
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      w.total[dt][r] += w.o[dt][r];
+      w.o[dt][r] = 0.0f;
+    }
+}
+
+// One block of keys: K rows and V rows as f16 in LDS.  `k0` is its first key,
+// `masked` (uniform) says whether some query of the wave may not see some key
+// of it, `far` whether V's scales differ enough for the denominators to need
+// a second look.
+template <bool SCORE, bool MASK>
+__device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const char* k,
+                                           const char* v, const KeyData& kd, int k0, bool masked,
+                                           bool far) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int at = 16 * half + (lane & 15);
+  f32x16 s[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
+  const char* kf = k + (lane & 31) * kKPitch + 16 * half;
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const u32x4 f = *reinterpret_cast<const u32x4*>(kf + 32 * t * kKPitch + 32 * ks);
+      s[t] = vks::mfma32(f, w.q[ks][1], s[t]);
+      s[t] = vks::mfma32(f, w.q[ks][0], s[t]);
+    }
+  float lsv[2], rs[2];
+  float mb = kLowest;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const float ksv = kd.ks[32 * t + at];
+    lsv[t] = kd.lsv[32 * t + at];
+    rs[t] = kd.rs[32 * t + at];
+    each<16>([&](auto r) { s[t][r()] *= bcast<r>(ksv); });
+    if (w.own_scale) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] *= w.back;
+    }
+    if constexpr (SCORE) {
+      if (ru.cap > 0.0f) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[t][r] = tanh1(s[t][r]) * w.cap_up;
+      }
+      if (ru.slopes) {
+        const float base = static_cast<float>(w.pos - (k0 + 32 * t + 4 * half));
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (8 * (r / 4) + r % 4)), s[t][r]);
+      }
+    }
+    each<16>([&](auto r) { s[t][r()] += bcast<r>(lsv[t]); });
+    if constexpr (MASK) {
+      if (masked) {
+        if (ru.causal) {
+          // keys j <= pos or j < pre, that is j < most
+          const long long most = w.pos + 1 > w.pre ? w.pos + 1 : w.pre;
+          const long long left = most - (k0 + 32 * t + 4 * half);
+          const int lim = left > 64 ? 64 : (left < 0 ? 0 : static_cast<int>(left));
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
+        }
+        if (ru.q_docs) {
+          const float doc = __int_as_float(kd.doc[32 * t + at]);
+          if (ru.docs_ordered) {
+            each<16>([&](auto r) {
+              s[t][r()] = __float_as_int(bcast<r>(doc)) <= w.doc ? s[t][r()] : -INFINITY;
+            });
+          } else {
+            each<16>([&](auto r) {
+              s[t][r()] = __float_as_int(bcast<r>(doc)) == w.doc ? s[t][r()] : -INFINITY;
+            });
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) mb = fmaxf(mb, s[t][r]);
+  }
+  if (__builtin_amdgcn_ballot_w64(mb > w.m + kSlack) != 0) {
+    mb = fmaxf(mb, other_half(mb));
+    const bool moves = mb > w.m + kSlack;
+    // in two steps: V's scales may be far apart
+    const float f = moves ? __builtin_amdgcn_exp2f(0.5f * (w.m - mb)) : 1.0f;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        w.o[dt][r] = w.o[dt][r] * f * f;
+        w.total[dt][r] = w.total[dt][r] * f * f;
+      }
+    w.l = w.l * f * f;
+    w.m = moves ? mb : w.m;
+  }
+  const float ref = w.m - kPBits;
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[t][r] -= ref;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  if (__builtin_expect(far, 0)) {
+    // a key whose V is small beside those met: its weight, which carries V's scale, may have
+    // left f32's range where its share of the denominator has not
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      each<16>([&](auto r) {
+        const float x = __builtin_amdgcn_exp2f(s[t][r()] - bcast<r>(lsv[t])) * kSumDown;
+        const bool lost = s[t][r()] < -100.0f && s[t][r()] > -INFINITY;
+        sum[r() & 3] += lost ? x : 0.0f;
+        if (lost) s[t][r()] = -INFINITY;
+      });
+  }
+  // the transposed reads: key 16 ch + 4 half + (l % 16) / 4 (+ 8), d 32 dt + 16 (l / 16 % 2) + 4 (l % 4)
+  const char* vf = v + (4 * half + ((lane & 15) >> 2)) * kVPitch + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+#pragma unroll
+  for (int ch = 0; ch < 4; ++ch) {
+    constexpr int kStep = 8 * kVPitch;
+    u32x4 vv[2];
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) {
+      const uint2 a = read_tr(vf + 2 * ch * kStep + 64 * dt);
+      const uint2 b = read_tr(vf + (2 * ch + 1) * kStep + 64 * dt);
+      vv[dt] = u32x4{a.x, a.y, b.x, b.y};
+    }
+    u32x4 p0, p1;
+    each<4>([&](auto j) {
+      constexpr int r0 = 2 * j;
+      const int t = ch >> 1;
+      float a, b;
+      if (ch & 1) {
+        a = __builtin_amdgcn_exp2f(s[t][8 + r0]);
+        b = __builtin_amdgcn_exp2f(s[t][8 + r0 + 1]);
+        sum[0] = __builtin_fmaf(bcast<8 + r0>(rs[t]), a, sum[0]);
+        sum[1] = __builtin_fmaf(bcast<8 + r0 + 1>(rs[t]), b, sum[1]);
+      } else {
+        a = __builtin_amdgcn_exp2f(s[t][r0]);
+        b = __builtin_amdgcn_exp2f(s[t][r0 + 1]);
+        sum[2] = __builtin_fmaf(bcast<r0>(rs[t]), a, sum[2]);
+        sum[3] = __builtin_fmaf(bcast<r0 + 1>(rs[t]), b, sum[3]);
+      }
+      uint32_t x, y;
+      vks::split2_plain(a, b, &x, &y);
+      p0[j()] = x;
+      p1[j()] = y;
+    });
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) w.o[dt] = vks::mfma32(vv[dt], p1, w.o[dt]);
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt) w.o[dt] = vks::mfma32(vv[dt], p0, w.o[dt]);
+  }
+  w.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+}
+
+// Staging of a block by all threads: eight codes of K and of V a thread and
+// row, and wave 0's keys' scales and documents.
+template <int FORMAT, int THREADS>
+struct Stage {
+  static constexpr int kPer = KB * 8 / THREADS;
+  uint2 k[kPer], v[kPer];
+  float ks, vs;
+  int doc;
+
+  __device__ __forceinline__ void load(const Shape& a, size_t first, size_t doc_first, int k0,
+                                       int keys) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int key = k0 + (tid >> 3) + i * (THREADS / 8);
+      const size_t at = (first + (key < keys ? key : keys - 1)) * HD + 8 * (tid & 7);
+      k[i] = *reinterpret_cast<const uint2*>(a.cache.k + at);
+      v[i] = *reinterpret_cast<const uint2*>(a.cache.v + at);
+    }
+    if (tid < KB) {
+      const int key = k0 + tid;
+      const int c = key < keys ? key : keys - 1;
+      ks = a.cache.ks[first + c];
+      vs = a.cache.vs[first + c];
+      if (a.rules.k_docs) doc = a.rules.k_docs[doc_first + c];
+    }
+  }
+
+  __device__ __forceinline__ void store(const Shape& a, char* kl, char* vl, KeyData& kd, int k0,
+                                        int keys) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int key = (tid >> 3) + i * (THREADS / 8);
+      *reinterpret_cast<u32x4*>(kl + key * kKPitch + 16 * (tid & 7)) = decode8<FORMAT>(k[i]);
+      *reinterpret_cast<u32x4*>(vl + key * kVPitch + 16 * (tid & 7)) = decode8<FORMAT>(v[i]);
+    }
+    if (tid < KB) {
+      const bool in = k0 + tid < keys;
+      const int at = key_slot(tid);
+      const float c = fmaxf(vs, vkc::kLeastScale);  // a NaN: the least
+      const bool nan = vs != vs;
+      const float l = nan ? vs : log2f(c);
+      kd.ks[at] = in ? ks * (1.0f / (1 << kQUp)) : 0.0f;
+      kd.lsv[at] = in ? l : -INFINITY;
+      kd.rs[at] = in && !nan ? kSumDown / c : 0.0f;
+      if (a.rules.k_docs) kd.doc[at] = doc;
+      const bool number = in && !nan;
+      const float low = -wave_max(number ? -l : -INFINITY);
+      const float high = wave_max(number ? l : -INFINITY);
+      if (tid == 0) {
+        kd.low = low;
+        kd.high = high;
+      }
+    }
+  }
+};
+
+constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
+
+template <int FORMAT, bool SCORE, bool MASK, int QW>
+__global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float* __restrict__ q,
+                                                                    float* __restrict__ out,
+                                                                    float* __restrict__ part,
+                                                                    Shape a) {
+  constexpr int kThreads = 64 * QW, kRows = 32 * QW;
+  __shared__ __align__(16) char kl[2][KB * kKPitch];
+  __shared__ __align__(16) char vl[2][KB * kVPitch];
+  __shared__ KeyData kd[2];
+  __shared__ uint16_t list[MASK ? kList : 1];
+  __shared__ int wave_count[QW], doc_low[QW], doc_high[QW];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  __builtin_assume(tid < kThreads);
+  const Rules& ru = a.rules;
+
+  // XCD-major numbering: the tiles of one cache head share an XCD's L2.  A
+  // sequence's later tiles come first: with a causal mask they take longest.
+  const uint32_t all = vkd::xcd_tile(blockIdx.x, gridDim.x);
+  const uint32_t split = all % a.splits, u = all / a.splits;
+  const uint32_t tile = a.tiles - 1 - u % a.tiles, sh = u / a.tiles;
+  const uint32_t kh = sh % a.cache.heads, s = sh / a.cache.heads;
+  const int count = vkc::count_of(a.rows, s);
+  const int rows = count > 0 ? count * static_cast<int>(a.group) : 0;  // query i's heads side by side
+  const int row0 = static_cast<int>(tile) * kRows;
+  if (row0 >= rows) return;
+  const int keys = keys_of(a, s);
+  const long long start = vkc::start_of(a.rows, s);
+  const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
+  const size_t doc_first = static_cast<size_t>(s) * a.cache.capacity;
+  const bool live = row0 + 32 * wave < rows;  // uniform over the wave
+  const int row = row0 + 32 * wave + (lane & 31);
+  const int my = row < rows ? row : rows - 1;
+  const uint32_t i = my / a.group, h = kh * a.group + my % a.group;
+
+  Queries w;
+  load_queries(w, q + vkc::row_at(a.rows, a.heads, s, h, i),
+               ru.cap > 0.0f ? ru.scale / ru.cap : ru.scale * kLog2e, half);
+  w.cap_up = ru.cap * kLog2e;
+  w.slope = SCORE && ru.slopes ? ru.slopes[h] * kLog2e : 0.0f;
+  w.pos = start + i;
+  w.pre = MASK && ru.prefix ? ru.prefix[s] : 0;
+  w.doc = MASK && ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + i] : 0;
+
+  const int blocks = (keys + KB - 1) / KB;
+  // the tile's positions and documents
+  const long long p_low = start + row0 / static_cast<int>(a.group);
+  const int row_last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
+  const long long p_high = start + row_last / static_cast<int>(a.group);
+  int q_low = 0, q_high = 0;
+  if (MASK && ru.q_docs) {
+    int lo = w.doc, hi = w.doc;
+    if (live) {
+#pragma unroll
+      for (int m = 16; m; m >>= 1) {
+        lo = min(lo, __shfl_xor(lo, m, 64));
+        hi = max(hi, __shfl_xor(hi, m, 64));
+      }
+    } else {
+      lo = 0x7fffffff;
+      hi = -0x7fffffff - 1;
+    }
+    if (lane == 0) {
+      doc_low[wave] = lo;
+      doc_high[wave] = hi;
+    }
+    __syncthreads();
+    q_low = doc_low[0];
+    q_high = doc_high[0];
+#pragma unroll
+    for (int x = 1; x < QW; ++x) {
+      q_low = min(q_low, doc_low[x]);
+      q_high = max(q_high, doc_high[x]);
+    }
+  }
+
+  float high = -INFINITY;  // largest lsv met
+  int taken = 0;
+  Stage<FORMAT, kThreads> st;
+  // blocks listed (MASK) or all of them, a run of kList at a time
+  for (int seg = 0; seg < blocks; seg += kList) {
+    int listed = blocks - seg < kList ? blocks - seg : kList;
+    if constexpr (MASK) {
+      int filled = 0;
+      const int seg_end = seg + listed;
+      for (int b0 = seg; b0 < seg_end; b0 += kThreads) {
+        const int b = b0 + tid;
+        bool any = b < seg_end, full = true;
+        if (any) {
+          const long long k0 = static_cast<long long>(b) * KB;
+          const long long k1 = k0 + KB < keys ? k0 + KB - 1 : keys - 1;  // last key
+          if (ru.causal) {
+            any = k0 <= p_high || k0 < w.pre;
+            full = k1 <= p_low || k1 < w.pre;
+          }
+          if (any && ru.q_docs) {
+            int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+            for (long long j = k0; j <= k1; ++j) {
+              const int d = ru.k_docs[doc_first + j];
+              lo = min(lo, d);
+              hi = max(hi, d);
+            }
+            if (ru.docs_ordered) {
+              any = lo <= q_high;
+              full = full && hi <= q_low;
+            } else {
+              any = lo <= q_high && hi >= q_low;
+              full = full && lo == hi && q_low == q_high && lo == q_low;
+            }
+          }
+        }
+        const uint64_t m = __builtin_amdgcn_ballot_w64(any);
+        __syncthreads();  // the counts of the run before are read
+        if (lane == 0) wave_count[wave] = __popcll(m);
+        __syncthreads();
+        int at = filled;
+#pragma unroll
+        for (int x = 0; x < QW; ++x) {
+          if (x < wave) at += wave_count[x];
+          filled += wave_count[x];
+        }
+        if (any)
+          list[at + __popcll(m & ((1ull << lane) - 1))] =
+              static_cast<uint16_t>((b - seg) << 1 | (full ? 0 : 1));
+      }
+      listed = filled;
+      __syncthreads();
+    }
+    const int b_begin = static_cast<int>(static_cast<long long>(split) * listed / a.splits);
+    const int b_end = static_cast<int>(static_cast<long long>(split + 1) * listed / a.splits);
+    if (b_begin == b_end) continue;  // uniform over the workgroup
+    auto entry = [&](int x) { return MASK ? static_cast<int>(list[x]) : x << 1; };
+    int e = entry(b_begin);
+    int k0 = (seg + (e >> 1)) * KB;
+    st.load(a, first, doc_first, k0, keys);
+    st.store(a, kl[0], vl[0], kd[0], k0, keys);
+    __syncthreads();
+    for (int x = b_begin; x < b_end; ++x) {
+      const int buf = (x - b_begin) & 1;
+      const bool more = x + 1 < b_end;
+      const int e_next = more ? entry(x + 1) : 0;
+      const int k0_next = (seg + (e_next >> 1)) * KB;
+      if (more) st.load(a, first, doc_first, k0_next, keys);
+      __builtin_amdgcn_sched_barrier(0);
+      high = fmaxf(high, kd[buf].high);
+      if (live) {
+        if (taken % kFlush == kFlush - 1) flush(w);
+        take_block<SCORE, MASK>(w, ru, kl[buf], vl[buf], kd[buf], k0, (e & 1) != 0,
+                                kd[buf].low < high - kFarBits);
+      }
+      ++taken;
+      if (more) st.store(a, kl[buf ^ 1], vl[buf ^ 1], kd[buf ^ 1], k0_next, keys);
+      e = e_next;
+      k0 = k0_next;
+      __syncthreads();
+    }
+  }
+  flush(w);
+  const float l = w.l + other_half(w.l);
+  if (!live || row >= rows) return;
+  if (part) {
+    const size_t all_rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
+    const size_t at = static_cast<size_t>(split) * all_rows +
+                      (static_cast<size_t>(s) * a.heads + h) * a.rows.n + i;
+    float* po = part + at * HD + 4 * half;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) =
+            f32x4{w.total[dt][4 * r], w.total[dt][4 * r + 1], w.total[dt][4 * r + 2],
+                  w.total[dt][4 * r + 3]};
+    if (half == 0)
+      *reinterpret_cast<float2*>(part + a.splits * all_rows * HD + 2 * at) = make_float2(w.m, l);
+  } else {
+    float* po = out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * half;
+    const bool none = l == 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        f32x4 t;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.total[dt][4 * r + c] / l * kSumDown;
+        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) = t;
+      }
+  }
+}
+
 // Joins the key splits of a row, in split order: 16 threads a row.
 __global__ __launch_bounds__(256) void attention_join_kernel(const float* __restrict__ part,
                                                              float* __restrict__ out, float up,
@@ -201,13 +773,14 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
   float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
   for (uint32_t sp = 0; sp < a.splits; ++sp) {
     const float2 x = ml[sp * rows + row];
-    const float w = x.x == -INFINITY && x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(x.x - m);
+    // in two steps: V's scales, which the references carry, may be far apart
+    const float w = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(0.5f * (x.x - m));
     const float4 y = *reinterpret_cast<const float4*>(part + (sp * rows + row) * HD + 4 * c);
-    l += x.y * w;
-    o.x += y.x * w;
-    o.y += y.y * w;
-    o.z += y.z * w;
-    o.w += y.w * w;
+    l += x.y * w * w;
+    o.x += y.x * w * w;
+    o.y += y.y * w * w;
+    o.z += y.z * w * w;
+    o.w += y.w * w * w;
   }
   if (l == 0.0f)
     o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -290,32 +863,58 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
       max_length > 0 && max_length < cache->capacity ? max_length : cache->capacity;
   a.limit = static_cast<uint32_t>(limit);
 
-  const int cus = rt->cu_count > 0 ? rt->cu_count : 256;
-  const size_t blocks = (limit + 63) / 64;
+  const auto* Q = static_cast<const float*>(q->ptr);
+  auto* O = static_cast<float*>(out->ptr);
+  const size_t blocks = (limit + KB - 1) / KB;
+  const size_t tile_rows = 256, tiles = (a.group * n + tile_rows - 1) / tile_rows;
+  const bool few = a.group * n <= 4;
+  const size_t cus = rt->cu_count > 0 ? rt->cu_count : 256;
+  const size_t units = few ? rows : cache->sequences * cache->heads * tiles;
   size_t splits = 1;
-  while (splits < 64 && rows * splits < 4 * static_cast<size_t>(cus) &&
-         blocks / (2 * splits) >= 2 * kRowWaves)
-    splits *= 2;
-  VK_UNSUPPORTED_IF(rows * splits > 0x7fffffffULL, "attention_cached: %zu queries", rows);
+  if (few) {
+    while (splits < 64 && rows * splits < 4 * cus && blocks / (2 * splits) >= 2 * kRowWaves)
+      splits *= 2;
+  } else {
+    splits = cus / units;
+    splits = splits > 16 ? 16 : splits;
+    splits = splits > blocks / 4 ? blocks / 4 : splits;
+    splits = splits < 1 ? 1 : splits;
+  }
+  VK_UNSUPPORTED_IF(units * splits > 0x7fffffffULL, "attention_cached: %zu queries", rows);
   a.splits = static_cast<uint32_t>(splits);
+  a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
   if (splits > 1) {
     VK_TRY(vk::ensure_work(rt, splits * rows * (HD + 2), "attention_cached"));
     part = rt->work;
   }
-  const auto* Q = static_cast<const float*>(q->ptr);
-  auto* O = static_cast<float*>(out->ptr);
-  const dim3 grid(static_cast<unsigned>(rows * splits));
-  if (cache->format == VK_CACHE_Q8)
-    hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_Q8>, grid, dim3(64 * kRowWaves), 0, rt->stream,
-                       Q, O, part, a);
-  else
-    hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_F8>, grid, dim3(64 * kRowWaves), 0, rt->stream,
-                       Q, O, part, a);
-  VK_TRY(vk::check_launch("attention_row_kernel"));
+  const dim3 grid(static_cast<unsigned>(units * splits));
+  const bool q8 = cache->format == VK_CACHE_Q8;
+  if (few) {
+    if (q8)
+      hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_Q8>, grid, dim3(64 * kRowWaves), 0,
+                         rt->stream, Q, O, part, a);
+    else
+      hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_F8>, grid, dim3(64 * kRowWaves), 0,
+                         rt->stream, Q, O, part, a);
+  } else {
+    const bool score = ru.cap > 0.0f || ru.slopes, mask = ru.causal || ru.q_docs;
+#define VK_TILE(F, S, M)                                                                          \
+  hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 8>), grid, dim3(512), 0, rt->stream, Q, O, \
+                     part, a)
+#define VK_TILE_F(F)                        \
+  if (score && mask) VK_TILE(F, true, true); \
+  else if (score) VK_TILE(F, true, false);   \
+  else if (mask) VK_TILE(F, false, true);    \
+  else VK_TILE(F, false, false)
+    if (q8) { VK_TILE_F(VK_CACHE_Q8); } else { VK_TILE_F(VK_CACHE_F8); }
+#undef VK_TILE_F
+#undef VK_TILE
+  }
+  VK_TRY(vk::check_launch("attention_cached"));
   if (splits == 1) return VK_OK;
   hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
-                     dim3(256), 0, rt->stream, part, O, 0x1p24f, a);
+                     dim3(256), 0, rt->stream, part, O, few ? 0x1p24f : kSumDown, a);
   return vk::check_launch("attention_join_kernel");
 }
 

@@ -44,10 +44,22 @@ __device__ __forceinline__ int keys_of(const Shape& a, uint32_t s) {
   return end > 0 ? static_cast<int>(end) : 0;
 }
 
+// Largest over the wave, without a round trip through LDS: rotations inside rows of
+// 16 lanes, then swaps of rows and of halves.
 __device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int m = 32; m; m >>= 1) v = fmaxf(v, __shfl_xor(v, m, 64));
-  return v;
+#define VK_ROR(n)                                                                            \
+  v = fmaxf(v, __uint_as_float(static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(               \
+                   static_cast<int>(__float_as_uint(v)), 0x120 | n, 0xf, 0xf, true))));
+  VK_ROR(8) VK_ROR(4) VK_ROR(2) VK_ROR(1)
+#undef VK_ROR
+  const auto a =
+      __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const uint32_t a0 = a[0], a1 = a[1];
+  v = fmaxf(__uint_as_float(a0), __uint_as_float(a1));
+  const auto b =
+      __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  const uint32_t b0 = b[0], b1 = b[1];
+  return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
 
 constexpr int kRowWaves = 4;
@@ -196,8 +208,7 @@ constexpr int kKPitch = 144;    // bytes of a K row in LDS: 64 f16 + 16
 constexpr int kVPitch = 192;    // of a V row: 64 f16 + 64
 constexpr float kPBits = 11.0f, kSlack = 2.0f;
 constexpr float kLowest = -3e38f;       // the running reference before any key
-constexpr float kSumDown = 0x1p-5f;     // of the denominators
-constexpr float kFarBits = 64.0f;
+constexpr float kLeastLsv = -88.0f;     // of a key's V in the choice of the reference
 constexpr int kQUp = 10;                // binary digits that Q is scaled up by
 constexpr int kFlush = 8;
 
@@ -269,11 +280,10 @@ __device__ __forceinline__ uint2 read_tr(const char* p) {
 // What a block's keys bring beside their codes, in LDS: 64 of each, key 32 t + 8
 // (r / 4) + 4 half + r % 4 at 32 t + 16 half + r.
 struct KeyData {
-  float ks[KB];   // K's scale / 2^kQUp; 0 past the end
-  float lsv[KB];  // log2 of V's scale; -inf past the end
-  float rs[KB];   // kSumDown / V's scale; 0 past the end and where the scale is not a number
+  float ks[KB];   // K's scale / 2^kQUp (a NaN where V's scale is one)
+  float lsv[KB];  // log2 of V's scale, at least kLeastLsv
+  float sv[KB];   // V's scale (0 where it is a NaN)
   int doc[KB];
-  float low, high;  // least and largest lsv (keys past the end left out)
 };
 
 __device__ __forceinline__ int key_slot(int key) {
@@ -344,6 +354,18 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
   w.l = 0.0f;
 }
 
+// Two weights as f16 parts, packed: the remainder by one mixed-precision FMA each.
+// `one` is 1.0 that the compiler does not see through: it would take the FMA apart.
+__device__ __forceinline__ void split_weights2(float a, float b, float one, uint32_t* p0,
+                                               uint32_t* p1) {
+  const vks::f16x2 h = __builtin_convertvector((vks::f32x2{a, b}), vks::f16x2);
+  const vks::f16x2 l = {
+      static_cast<_Float16>(__builtin_fmaf(a, one, -static_cast<float>(h[0]))),
+      static_cast<_Float16>(__builtin_fmaf(b, one, -static_cast<float>(h[1])))};
+  *p0 = __builtin_bit_cast(uint32_t, h);
+  *p1 = __builtin_bit_cast(uint32_t, l);
+}
+
 __device__ __forceinline__ void flush(Queries& w) {
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
@@ -354,41 +376,46 @@ __device__ __forceinline__ void flush(Queries& w) {
     }
 }
 
-// One block of keys: K rows and V rows as f16 in LDS.  `k0` is its first key,
-// `masked` (uniform) says whether some query of the wave may not see some key
-// of it, `far` whether V's scales differ enough for the denominators to need
-// a second look.
-template <bool SCORE, bool MASK>
-__device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const char* k,
-                                           const char* v, const KeyData& kd, int k0, bool masked,
-                                           bool far) {
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int at = 16 * half + (lane & 15);
-  f32x16 s[2];
+// One step of 16 d of S^T = K Q^T for a block of 64 keys: the small products first.
+__device__ __forceinline__ void score_step(f32x16 (&s)[2], const Queries& w, const char* k, int ks) {
+  const int lane = threadIdx.x & 63;
+  const char* kf = k + (lane & 31) * kKPitch + 16 * (lane >> 5) + 32 * ks;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const u32x4 f = *reinterpret_cast<const u32x4*>(kf + 32 * t * kKPitch);
+    s[t] = vks::mfma32(f, w.q[ks][1], s[t]);
+    s[t] = vks::mfma32(f, w.q[ks][0], s[t]);
+  }
+}
+
+__device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
-  const char* kf = k + (lane & 31) * kKPitch + 16 * half;
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks)
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const u32x4 f = *reinterpret_cast<const u32x4*>(kf + 32 * t * kKPitch + 32 * ks);
-      s[t] = vks::mfma32(f, w.q[ks][1], s[t]);
-      s[t] = vks::mfma32(f, w.q[ks][0], s[t]);
-    }
-  float lsv[2], rs[2];
+}
+
+// The scores of a block from the products: scales, cap, bias and masks, base 2;
+// `left` keys of it are held, `masked` (uniform) says whether a query of the wave may
+// not see some of them.  Moves the reference of queries whose weights would leave
+// f16's upper end: it follows the largest of score + log2 of V's scale, the size of a key's
+// part of the value sum, once that passes it by kSlack.
+template <bool SCORE, bool MASK>
+__device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Rules& ru,
+                                            const KeyData& kd, long long k0, int left, bool masked) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int at = 16 * half + (lane & 15);
   float mb = kLowest;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const float ksv = kd.ks[32 * t + at];
-    lsv[t] = kd.lsv[32 * t + at];
-    rs[t] = kd.rs[32 * t + at];
+    float lsv = kd.lsv[32 * t + at];
     each<16>([&](auto r) { s[t][r()] *= bcast<r>(ksv); });
-    if (w.own_scale) {
+    if (__builtin_expect(w.own_scale, 0)) {
+      float back = w.back;
+      asm volatile("" : "+v"(back));  // keeps the products in this branch
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] *= w.back;
+      for (int r = 0; r < 16; ++r) s[t][r] *= back;
     }
     if constexpr (SCORE) {
       if (ru.cap > 0.0f) {
@@ -402,17 +429,20 @@ __device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const ch
           s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (8 * (r / 4) + r % 4)), s[t][r]);
       }
     }
-    each<16>([&](auto r) { s[t][r()] += bcast<r>(lsv[t]); });
+    if (__builtin_expect(left < KB, 0)) {
+      const int lim = left - 32 * t - 4 * half;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
+    }
     if constexpr (MASK) {
       if (masked) {
         if (ru.causal) {
           // keys j <= pos or j < pre, that is j < most
           const long long most = w.pos + 1 > w.pre ? w.pos + 1 : w.pre;
-          const long long left = most - (k0 + 32 * t + 4 * half);
-          const int lim = left > 64 ? 64 : (left < 0 ? 0 : static_cast<int>(left));
+          const long long far = most - (k0 + 32 * t + 4 * half);
+          const int lim = far > 64 ? 64 : (far < 0 ? 0 : static_cast<int>(far));
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
+          for (int r = 0; r < 16; ++r) s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
         }
         if (ru.q_docs) {
           const float doc = __int_as_float(kd.doc[32 * t + at]);
@@ -428,13 +458,13 @@ __device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const ch
         }
       }
     }
-#pragma unroll
-    for (int r = 0; r < 16; ++r) mb = fmaxf(mb, s[t][r]);
+    asm volatile("" : "+v"(lsv));  // the broadcasts stay here, part of the additions
+    each<16>([&](auto r) { mb = fmaxf(mb, s[t][r()] + bcast<r>(lsv)); });
   }
   if (__builtin_amdgcn_ballot_w64(mb > w.m + kSlack) != 0) {
     mb = fmaxf(mb, other_half(mb));
     const bool moves = mb > w.m + kSlack;
-    // in two steps: V's scales may be far apart
+    // in two steps: V's scales, which the references carry, may be far apart
     const float f = moves ? __builtin_amdgcn_exp2f(0.5f * (w.m - mb)) : 1.0f;
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
@@ -446,29 +476,25 @@ __device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const ch
     w.l = w.l * f * f;
     w.m = moves ? mb : w.m;
   }
+}
+
+// The weights of a block's scores, p = 2^(score - reference), their sum, and O^T += V^T
+// (p V's scale)^T; beside them the products of the next block (its K at `k_next`).
+__device__ __forceinline__ void value_block(f32x16 (&s)[2], f32x16 (&next)[2], Queries& w,
+                                            const char* v, const KeyData& kd, const char* k_next) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  const int at = 16 * half + (lane & 15);
   const float ref = w.m - kPBits;
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s[t][r] -= ref;
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-  if (__builtin_expect(far, 0)) {
-    // a key whose V is small beside those met: its weight, which carries V's scale, may have
-    // left f32's range where its share of the denominator has not
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      each<16>([&](auto r) {
-        const float x = __builtin_amdgcn_exp2f(s[t][r()] - bcast<r>(lsv[t])) * kSumDown;
-        const bool lost = s[t][r()] < -100.0f && s[t][r()] > -INFINITY;
-        sum[r() & 3] += lost ? x : 0.0f;
-        if (lost) s[t][r()] = -INFINITY;
-      });
-  }
+  const float sv[2] = {kd.sv[at], kd.sv[32 + at]};
+  float one = 1.0f;
+  asm("" : "+s"(one));
+  clear(next);
+  float sum[2] = {0.0f, 0.0f};
   // the transposed reads: key 16 ch + 4 half + (l % 16) / 4 (+ 8), d 32 dt + 16 (l / 16 % 2) + 4 (l % 4)
-  const char* vf = v + (4 * half + ((lane & 15) >> 2)) * kVPitch + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
-#pragma unroll
-  for (int ch = 0; ch < 4; ++ch) {
-    constexpr int kStep = 8 * kVPitch;
+  const char* vf =
+      v + (4 * half + ((lane & 15) >> 2)) * kVPitch + 32 * ((lane >> 4) & 1) + 8 * (lane & 3);
+  each<4>([&](auto ch) {
+    constexpr int kStep = 8 * kVPitch, t = ch >> 1, r0 = 8 * (ch & 1);
     u32x4 vv[2];
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt) {
@@ -476,24 +502,16 @@ __device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const ch
       const uint2 b = read_tr(vf + (2 * ch + 1) * kStep + 64 * dt);
       vv[dt] = u32x4{a.x, a.y, b.x, b.y};
     }
+    score_step(next, w, k_next, ch);
     u32x4 p0, p1;
     each<4>([&](auto j) {
-      constexpr int r0 = 2 * j;
-      const int t = ch >> 1;
-      float a, b;
-      if (ch & 1) {
-        a = __builtin_amdgcn_exp2f(s[t][8 + r0]);
-        b = __builtin_amdgcn_exp2f(s[t][8 + r0 + 1]);
-        sum[0] = __builtin_fmaf(bcast<8 + r0>(rs[t]), a, sum[0]);
-        sum[1] = __builtin_fmaf(bcast<8 + r0 + 1>(rs[t]), b, sum[1]);
-      } else {
-        a = __builtin_amdgcn_exp2f(s[t][r0]);
-        b = __builtin_amdgcn_exp2f(s[t][r0 + 1]);
-        sum[2] = __builtin_fmaf(bcast<r0>(rs[t]), a, sum[2]);
-        sum[3] = __builtin_fmaf(bcast<r0 + 1>(rs[t]), b, sum[3]);
-      }
+      constexpr int r = r0 + 2 * j;
+      const float a = __builtin_amdgcn_exp2f(s[t][r] - ref);
+      const float b = __builtin_amdgcn_exp2f(s[t][r + 1] - ref);
+      sum[0] += a;
+      sum[1] += b;
       uint32_t x, y;
-      vks::split2_plain(a, b, &x, &y);
+      split_weights2(a * bcast<r>(sv[t]), b * bcast<r + 1>(sv[t]), one, &x, &y);
       p0[j()] = x;
       p1[j()] = y;
     });
@@ -501,65 +519,57 @@ __device__ __forceinline__ void take_block(Queries& w, const Rules& ru, const ch
     for (int dt = 0; dt < 2; ++dt) w.o[dt] = vks::mfma32(vv[dt], p1, w.o[dt]);
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt) w.o[dt] = vks::mfma32(vv[dt], p0, w.o[dt]);
-  }
-  w.l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  });
+  w.l += sum[0] + sum[1];
 }
 
-// Staging of a block by all threads: eight codes of K and of V a thread and
-// row, and wave 0's keys' scales and documents.
+// Staging by all threads: eight codes of K (or V) a thread and row.
 template <int FORMAT, int THREADS>
-struct Stage {
+struct StageRows {
   static constexpr int kPer = KB * 8 / THREADS;
-  uint2 k[kPer], v[kPer];
+  uint2 w[kPer];
+
+  __device__ __forceinline__ void load(const uint8_t* codes, size_t first, int k0, int keys) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int key = k0 + (tid >> 3) + i * (THREADS / 8);
+      w[i] = *reinterpret_cast<const uint2*>(
+          codes + (first + (key < keys ? key : keys - 1)) * HD + 8 * (tid & 7));
+    }
+  }
+
+  template <int PITCH>
+  __device__ __forceinline__ void store(char* to) const {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      *reinterpret_cast<u32x4*>(to + ((tid >> 3) + i * (THREADS / 8)) * PITCH + 16 * (tid & 7)) =
+          decode8<FORMAT>(w[i]);
+  }
+};
+
+// A key's scales and document, one a thread of the first wave.
+struct StageKeys {
   float ks, vs;
   int doc;
 
   __device__ __forceinline__ void load(const Shape& a, size_t first, size_t doc_first, int k0,
                                        int keys) {
-    const int tid = threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int key = k0 + (tid >> 3) + i * (THREADS / 8);
-      const size_t at = (first + (key < keys ? key : keys - 1)) * HD + 8 * (tid & 7);
-      k[i] = *reinterpret_cast<const uint2*>(a.cache.k + at);
-      v[i] = *reinterpret_cast<const uint2*>(a.cache.v + at);
-    }
-    if (tid < KB) {
-      const int key = k0 + tid;
-      const int c = key < keys ? key : keys - 1;
-      ks = a.cache.ks[first + c];
-      vs = a.cache.vs[first + c];
-      if (a.rules.k_docs) doc = a.rules.k_docs[doc_first + c];
-    }
+    const int key = k0 + static_cast<int>(threadIdx.x);
+    const int c = key < keys ? key : keys - 1;
+    ks = a.cache.ks[first + c];
+    vs = a.cache.vs[first + c];
+    if (a.rules.k_docs) doc = a.rules.k_docs[doc_first + c];
   }
 
-  __device__ __forceinline__ void store(const Shape& a, char* kl, char* vl, KeyData& kd, int k0,
-                                        int keys) {
-    const int tid = threadIdx.x;
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int key = (tid >> 3) + i * (THREADS / 8);
-      *reinterpret_cast<u32x4*>(kl + key * kKPitch + 16 * (tid & 7)) = decode8<FORMAT>(k[i]);
-      *reinterpret_cast<u32x4*>(vl + key * kVPitch + 16 * (tid & 7)) = decode8<FORMAT>(v[i]);
-    }
-    if (tid < KB) {
-      const bool in = k0 + tid < keys;
-      const int at = key_slot(tid);
-      const float c = fmaxf(vs, vkc::kLeastScale);  // a NaN: the least
-      const bool nan = vs != vs;
-      const float l = nan ? vs : log2f(c);
-      kd.ks[at] = in ? ks * (1.0f / (1 << kQUp)) : 0.0f;
-      kd.lsv[at] = in ? l : -INFINITY;
-      kd.rs[at] = in && !nan ? kSumDown / c : 0.0f;
-      if (a.rules.k_docs) kd.doc[at] = doc;
-      const bool number = in && !nan;
-      const float low = -wave_max(number ? -l : -INFINITY);
-      const float high = wave_max(number ? l : -INFINITY);
-      if (tid == 0) {
-        kd.low = low;
-        kd.high = high;
-      }
-    }
+  __device__ __forceinline__ void store(const Shape& a, KeyData& kd) const {
+    const int at = key_slot(threadIdx.x);
+    const bool nan = vs != vs;
+    kd.ks[at] = nan ? vs : ks * (1.0f / (1 << kQUp));
+    kd.lsv[at] = fmaxf(__builtin_amdgcn_logf(fmaxf(vs, vkc::kLeastScale)), kLeastLsv);
+    kd.sv[at] = nan ? 0.0f : vs;
+    if (a.rules.k_docs) kd.doc[at] = doc;
   }
 };
 
@@ -640,9 +650,9 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
     }
   }
 
-  float high = -INFINITY;  // largest lsv met
   int taken = 0;
-  Stage<FORMAT, kThreads> st;
+  StageRows<FORMAT, kThreads> rows_k, rows_v;
+  StageKeys keys_d;
   // blocks listed (MASK) or all of them, a run of kList at a time
   for (int seg = 0; seg < blocks; seg += kList) {
     int listed = blocks - seg < kList ? blocks - seg : kList;
@@ -696,30 +706,54 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
     const int b_end = static_cast<int>(static_cast<long long>(split + 1) * listed / a.splits);
     if (b_begin == b_end) continue;  // uniform over the workgroup
     auto entry = [&](int x) { return MASK ? static_cast<int>(list[x]) : x << 1; };
+    auto key_of = [&](int e) { return (seg + (e >> 1)) * KB; };
+    // K runs a block ahead of V: block x + 1's products are taken beside block x's weights
     int e = entry(b_begin);
-    int k0 = (seg + (e >> 1)) * KB;
-    st.load(a, first, doc_first, k0, keys);
-    st.store(a, kl[0], vl[0], kd[0], k0, keys);
+    int e1 = entry(b_begin + 1 < b_end ? b_begin + 1 : b_begin);
+    {
+      rows_k.load(a.cache.k, first, key_of(e), keys);
+      rows_v.load(a.cache.v, first, key_of(e), keys);
+      if (wave == 0) keys_d.load(a, first, doc_first, key_of(e), keys);
+      rows_k.template store<kKPitch>(kl[0]);
+      rows_v.template store<kVPitch>(vl[0]);
+      if (wave == 0) keys_d.store(a, kd[0]);
+      rows_k.load(a.cache.k, first, key_of(e1), keys);
+      rows_k.template store<kKPitch>(kl[1]);
+    }
     __syncthreads();
-    for (int x = b_begin; x < b_end; ++x) {
-      const int buf = (x - b_begin) & 1;
-      const bool more = x + 1 < b_end;
-      const int e_next = more ? entry(x + 1) : 0;
-      const int k0_next = (seg + (e_next >> 1)) * KB;
-      if (more) st.load(a, first, doc_first, k0_next, keys);
+    f32x16 sc[2][2];
+    clear(sc[0]);
+    if (live)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) score_step(sc[0], w, kl[0], ks);
+    __syncthreads();  // kl[0] is read
+    auto step = [&](int x, auto buf_c) {
+      constexpr int buf = buf_c;
+      const int e2 = entry(x + 2 < b_end ? x + 2 : b_end - 1);
+      const int k0 = key_of(e);
+      rows_k.load(a.cache.k, first, key_of(e2), keys);
+      rows_v.load(a.cache.v, first, key_of(e1), keys);
+      if (wave == 0) keys_d.load(a, first, doc_first, key_of(e1), keys);
       __builtin_amdgcn_sched_barrier(0);
-      high = fmaxf(high, kd[buf].high);
       if (live) {
         if (taken % kFlush == kFlush - 1) flush(w);
-        take_block<SCORE, MASK>(w, ru, kl[buf], vl[buf], kd[buf], k0, (e & 1) != 0,
-                                kd[buf].low < high - kFarBits);
+        score_block<SCORE, MASK>(sc[buf], w, ru, kd[buf], k0, keys - k0, (e & 1) != 0);
+        value_block(sc[buf], sc[buf ^ 1], w, vl[buf], kd[buf], kl[buf ^ 1]);
       }
       ++taken;
-      if (more) st.store(a, kl[buf ^ 1], vl[buf ^ 1], kd[buf ^ 1], k0_next, keys);
-      e = e_next;
-      k0 = k0_next;
+      rows_k.template store<kKPitch>(kl[buf]);
+      rows_v.template store<kVPitch>(vl[buf ^ 1]);
+      if (wave == 0) keys_d.store(a, kd[buf ^ 1]);
+      e = e1;
+      e1 = e2;
       __syncthreads();
+    };
+    int x = b_begin;
+    for (; x + 1 < b_end; x += 2) {
+      step(x, Int<0>{});
+      step(x + 1, Int<1>{});
     }
+    if (x < b_end) step(x, Int<0>{});
   }
   flush(w);
   const float l = w.l + other_half(w.l);
@@ -747,7 +781,7 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
       for (int r = 0; r < 4; ++r) {
         f32x4 t;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.total[dt][4 * r + c] / l * kSumDown;
+        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.total[dt][4 * r + c] / l;
         *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) = t;
       }
   }
@@ -914,7 +948,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   VK_TRY(vk::check_launch("attention_cached"));
   if (splits == 1) return VK_OK;
   hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
-                     dim3(256), 0, rt->stream, part, O, few ? 0x1p24f : kSumDown, a);
+                     dim3(256), 0, rt->stream, part, O, few ? 0x1p24f : 1.0f, a);
   return vk::check_launch("attention_join_kernel");
 }
 

@@ -85,8 +85,8 @@ def attention(q, kv, vv, v_scale, n, starts, counts, rules, limit=0, pick=None):
     Two floors beside these.  A query's values are scaled so that its largest is at least 1,
     and their second part is a multiple of 2^-24: off by 2^-25 = u / 2 of the row's largest
     |q| at most, whatever the value's own size, which moves a score by that times sum
-    |k_d|.  A weight (2^x times V's scale) is at least 2^11 for the largest and its second part
-    a multiple of 2^-24: off by 2^-36 of the largest at most, whatever its own size (and
+    |k_d|.  A weight (2^x times V's scale) is at least 2^9 for the largest and its second part
+    a multiple of 2^-24: off by 2^-34 of the largest at most, whatever its own size (and
     left out below), which moves the output by that times sum_j |code_j|."""
     S, H, _, _ = q.shape
     KV, cap = kv.shape[1], kv.shape[2]
@@ -129,7 +129,7 @@ def attention(q, kv, vv, v_scale, n, starts, counts, rules, limit=0, pick=None):
                 tol[s, h, i] = (p * e) @ np.abs(vs - o) + 2 * U * np.abs(o) + (
                     2 * np.sqrt(len(p)) + len(p) / 64 + 8) * U * size + 1e-38
                 sv = np.maximum(v_scale[s, h * KV // H, :end][seen].astype(np.float64), LEAST)
-                tol[s, h, i] += 2.0 ** -36 * (p * sv).max() * (np.abs(vs) / sv[:, None]).sum(0)
+                tol[s, h, i] += 2.0 ** -34 * (p * sv).max() * (np.abs(vs) / sv[:, None]).sum(0)
     return out, tol
 
 

@@ -44,6 +44,12 @@ __device__ __forceinline__ int keys_of(const Shape& a, uint32_t s) {
   return end > 0 ? static_cast<int>(end) : 0;
 }
 
+// Position of row i; every key lies below the largest.
+__device__ __forceinline__ int position(int start, uint32_t i) {
+  const long long p = static_cast<long long>(start) + i;
+  return p < 0x7ffffffe ? static_cast<int>(p) : 0x7ffffffe;
+}
+
 // Largest over the wave, without a round trip through LDS: rotations inside rows of
 // 16 lanes, then swaps of rows and of halves.
 __device__ __forceinline__ float wave_max(float v) {
@@ -79,7 +85,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   if (static_cast<int>(i) >= vkc::count_of(a.rows, s)) return;
   const uint32_t kh = h / a.group;
   const int keys = keys_of(a, s);
-  const long long p = static_cast<long long>(vkc::start_of(a.rows, s)) + i;
+  const int p = position(vkc::start_of(a.rows, s), i);
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
   const float* qr = q + vkc::row_at(a.rows, a.heads, s, h, i);
   const Rules& ru = a.rules;
@@ -121,7 +127,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     float t = ((u[0] + u[1]) + (u[2] + u[3])) * a.cache.ks[slot] * ru.scale;
     if (ru.cap > 0.0f) t = ru.cap * tanhf(t / ru.cap);
     if (ru.slopes) {
-      const long long far = p > j ? p - j : j - p;
+      const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
       t -= slope * static_cast<float>(far);
     }
     t *= kLog2e;
@@ -206,11 +212,10 @@ using vks::u32x4;
 constexpr int KB = 64;          // keys of a block
 constexpr int kKPitch = 144;    // bytes of a K row in LDS: 64 f16 + 16
 constexpr int kVPitch = 192;    // of a V row: 64 f16 + 64
-constexpr float kPBits = 11.0f, kSlack = 2.0f;
+constexpr float kPBits = 9.0f, kSlack = 6.0f;
 constexpr float kLowest = -3e38f;       // the running reference before any key
 constexpr float kLeastLsv = -88.0f;     // of a key's V in the choice of the reference
 constexpr int kQUp = 10;                // binary digits that Q is scaled up by
-constexpr int kFlush = 8;
 
 // Lane R of each 16-lane row, to all of the row.
 template <int R>
@@ -310,9 +315,9 @@ struct Queries {
   float back;            // 1, or what the row's own scale has to be undone by
   bool own_scale;        // uniform: some row has one
   float slope, cap_up;   // per unit of distance and cap, in base 2
-  int pre, doc;
-  long long pos;
-  f32x16 o[2], total[2];
+  int pos, doc;
+  int seen;              // causal: keys below it are seen
+  f32x16 o[2];
   float m, l;            // running reference, this lane's denominators
 };
 
@@ -349,7 +354,7 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-    for (int r = 0; r < 16; ++r) w.o[dt][r] = w.total[dt][r] = 0.0f;
+    for (int r = 0; r < 16; ++r) w.o[dt][r] = 0.0f;
   w.m = kLowest;
   w.l = 0.0f;
 }
@@ -364,16 +369,6 @@ __device__ __forceinline__ void split_weights2(float a, float b, float one, uint
       static_cast<_Float16>(__builtin_fmaf(b, one, -static_cast<float>(h[1])))};
   *p0 = __builtin_bit_cast(uint32_t, h);
   *p1 = __builtin_bit_cast(uint32_t, l);
-}
-
-__device__ __forceinline__ void flush(Queries& w) {
-#pragma unroll
-  for (int dt = 0; dt < 2; ++dt)
-#pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      w.total[dt][r] += w.o[dt][r];
-      w.o[dt][r] = 0.0f;
-    }
 }
 
 // One step of 16 d of S^T = K Q^T for a block of 64 keys: the small products first.
@@ -402,7 +397,7 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 // part of the value sum, once that passes it by kSlack.
 template <bool SCORE, bool MASK>
 __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Rules& ru,
-                                            const KeyData& kd, long long k0, int left, bool masked) {
+                                            const KeyData& kd, int k0, int left, bool masked) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int at = 16 * half + (lane & 15);
   float mb = kLowest;
@@ -423,40 +418,29 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
         for (int r = 0; r < 16; ++r) s[t][r] = tanh1(s[t][r]) * w.cap_up;
       }
       if (ru.slopes) {
-        const float base = static_cast<float>(w.pos - (k0 + 32 * t + 4 * half));
+        const float base =
+            static_cast<float>(static_cast<long long>(w.pos) - (k0 + 32 * t + 4 * half));
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (8 * (r / 4) + r % 4)), s[t][r]);
       }
     }
-    if (__builtin_expect(left < KB, 0)) {
-      const int lim = left - 32 * t - 4 * half;
+    const bool causal = MASK && masked && ru.causal;
+    if (__builtin_expect(left < KB || causal, 0)) {
+      int lim = left;
+      if (causal) lim = min(lim, w.seen - k0);
+      lim -= 32 * t + 4 * half;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
     }
-    if constexpr (MASK) {
-      if (masked) {
-        if (ru.causal) {
-          // keys j <= pos or j < pre, that is j < most
-          const long long most = w.pos + 1 > w.pre ? w.pos + 1 : w.pre;
-          const long long far = most - (k0 + 32 * t + 4 * half);
-          const int lim = far > 64 ? 64 : (far < 0 ? 0 : static_cast<int>(far));
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
-        }
-        if (ru.q_docs) {
-          const float doc = __int_as_float(kd.doc[32 * t + at]);
-          if (ru.docs_ordered) {
-            each<16>([&](auto r) {
-              s[t][r()] = __float_as_int(bcast<r>(doc)) <= w.doc ? s[t][r()] : -INFINITY;
-            });
-          } else {
-            each<16>([&](auto r) {
-              s[t][r()] = __float_as_int(bcast<r>(doc)) == w.doc ? s[t][r()] : -INFINITY;
-            });
-          }
-        }
-      }
+    if (MASK && masked && ru.q_docs) {
+      const float doc = __int_as_float(kd.doc[32 * t + at]);
+      // a later document, or any other
+      const int least = ru.docs_ordered ? -0x7fffffff - 1 : w.doc;
+      each<16>([&](auto r) {
+        const int d = __float_as_int(bcast<r>(doc));
+        s[t][r()] = d <= w.doc && d >= least ? s[t][r()] : -INFINITY;
+      });
     }
     asm volatile("" : "+v"(lsv));  // the broadcasts stay here, part of the additions
     each<16>([&](auto r) { mb = fmaxf(mb, s[t][r()] + bcast<r>(lsv)); });
@@ -469,26 +453,22 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
 #pragma unroll
     for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        w.o[dt][r] = w.o[dt][r] * f * f;
-        w.total[dt][r] = w.total[dt][r] * f * f;
-      }
+      for (int r = 0; r < 16; ++r) w.o[dt][r] = w.o[dt][r] * f * f;
     w.l = w.l * f * f;
     w.m = moves ? mb : w.m;
   }
 }
 
 // The weights of a block's scores, p = 2^(score - reference), their sum, and O^T += V^T
-// (p V's scale)^T; beside them the products of the next block (its K at `k_next`).
-__device__ __forceinline__ void value_block(f32x16 (&s)[2], f32x16 (&next)[2], Queries& w,
-                                            const char* v, const KeyData& kd, const char* k_next) {
+// (p V's scale)^T.
+__device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, const char* v,
+                                            const KeyData& kd) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int at = 16 * half + (lane & 15);
   const float ref = w.m - kPBits;
   const float sv[2] = {kd.sv[at], kd.sv[32 + at]};
   float one = 1.0f;
   asm("" : "+s"(one));
-  clear(next);
   float sum[2] = {0.0f, 0.0f};
   // the transposed reads: key 16 ch + 4 half + (l % 16) / 4 (+ 8), d 32 dt + 16 (l / 16 % 2) + 4 (l % 4)
   const char* vf =
@@ -502,7 +482,6 @@ __device__ __forceinline__ void value_block(f32x16 (&s)[2], f32x16 (&next)[2], Q
       const uint2 b = read_tr(vf + (2 * ch + 1) * kStep + 64 * dt);
       vv[dt] = u32x4{a.x, a.y, b.x, b.y};
     }
-    score_step(next, w, k_next, ch);
     u32x4 p0, p1;
     each<4>([&](auto j) {
       constexpr int r = r0 + 2 * j;
@@ -576,7 +555,7 @@ struct StageKeys {
 constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
 
 template <int FORMAT, bool SCORE, bool MASK, int QW>
-__global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float* __restrict__ q,
+__global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float* __restrict__ q,
                                                                     float* __restrict__ out,
                                                                     float* __restrict__ part,
                                                                     Shape a) {
@@ -601,7 +580,7 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
   const int row0 = static_cast<int>(tile) * kRows;
   if (row0 >= rows) return;
   const int keys = keys_of(a, s);
-  const long long start = vkc::start_of(a.rows, s);
+  const int start = vkc::start_of(a.rows, s);
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
   const size_t doc_first = static_cast<size_t>(s) * a.cache.capacity;
   const bool live = row0 + 32 * wave < rows;  // uniform over the wave
@@ -614,15 +593,16 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
                ru.cap > 0.0f ? ru.scale / ru.cap : ru.scale * kLog2e, half);
   w.cap_up = ru.cap * kLog2e;
   w.slope = SCORE && ru.slopes ? ru.slopes[h] * kLog2e : 0.0f;
-  w.pos = start + i;
-  w.pre = MASK && ru.prefix ? ru.prefix[s] : 0;
+  w.pos = position(start, i);
+  const int pre = MASK && ru.prefix ? ru.prefix[s] : 0;
+  w.seen = max(max(w.pos + 1, pre), 0);
   w.doc = MASK && ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + i] : 0;
 
   const int blocks = (keys + KB - 1) / KB;
   // the tile's positions and documents
-  const long long p_low = start + row0 / static_cast<int>(a.group);
+  const int p_low = position(start, row0 / a.group);
   const int row_last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
-  const long long p_high = start + row_last / static_cast<int>(a.group);
+  const int p_high = position(start, row_last / a.group);
   int q_low = 0, q_high = 0;
   if (MASK && ru.q_docs) {
     int lo = w.doc, hi = w.doc;
@@ -650,7 +630,6 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
     }
   }
 
-  int taken = 0;
   StageRows<FORMAT, kThreads> rows_k, rows_v;
   StageKeys keys_d;
   // blocks listed (MASK) or all of them, a run of kList at a time
@@ -666,8 +645,8 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
           const long long k0 = static_cast<long long>(b) * KB;
           const long long k1 = k0 + KB < keys ? k0 + KB - 1 : keys - 1;  // last key
           if (ru.causal) {
-            any = k0 <= p_high || k0 < w.pre;
-            full = k1 <= p_low || k1 < w.pre;
+            any = k0 <= p_high || k0 < pre;
+            full = k1 <= p_low || k1 < pre;
           }
           if (any && ru.q_docs) {
             int lo = 0x7fffffff, hi = -0x7fffffff - 1;
@@ -702,60 +681,42 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
       listed = filled;
       __syncthreads();
     }
-    const int b_begin = static_cast<int>(static_cast<long long>(split) * listed / a.splits);
-    const int b_end = static_cast<int>(static_cast<long long>(split + 1) * listed / a.splits);
+    const int b_begin = static_cast<int>(split * static_cast<uint32_t>(listed) / a.splits);
+    const int b_end = static_cast<int>((split + 1) * static_cast<uint32_t>(listed) / a.splits);
     if (b_begin == b_end) continue;  // uniform over the workgroup
     auto entry = [&](int x) { return MASK ? static_cast<int>(list[x]) : x << 1; };
     auto key_of = [&](int e) { return (seg + (e >> 1)) * KB; };
-    // K runs a block ahead of V: block x + 1's products are taken beside block x's weights
     int e = entry(b_begin);
-    int e1 = entry(b_begin + 1 < b_end ? b_begin + 1 : b_begin);
-    {
-      rows_k.load(a.cache.k, first, key_of(e), keys);
-      rows_v.load(a.cache.v, first, key_of(e), keys);
-      if (wave == 0) keys_d.load(a, first, doc_first, key_of(e), keys);
-      rows_k.template store<kKPitch>(kl[0]);
-      rows_v.template store<kVPitch>(vl[0]);
-      if (wave == 0) keys_d.store(a, kd[0]);
-      rows_k.load(a.cache.k, first, key_of(e1), keys);
-      rows_k.template store<kKPitch>(kl[1]);
-    }
+    rows_k.load(a.cache.k, first, key_of(e), keys);
+    rows_v.load(a.cache.v, first, key_of(e), keys);
+    if (wave == 0) keys_d.load(a, first, doc_first, key_of(e), keys);
+    rows_k.template store<kKPitch>(kl[0]);
+    rows_v.template store<kVPitch>(vl[0]);
+    if (wave == 0) keys_d.store(a, kd[0]);
     __syncthreads();
-    f32x16 sc[2][2];
-    clear(sc[0]);
-    if (live)
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) score_step(sc[0], w, kl[0], ks);
-    __syncthreads();  // kl[0] is read
-    auto step = [&](int x, auto buf_c) {
-      constexpr int buf = buf_c;
-      const int e2 = entry(x + 2 < b_end ? x + 2 : b_end - 1);
+    for (int x = b_begin; x < b_end; ++x) {
+      const int buf = (x - b_begin) & 1;
+      const int e1 = entry(x + 1 < b_end ? x + 1 : x);
       const int k0 = key_of(e);
-      rows_k.load(a.cache.k, first, key_of(e2), keys);
+      rows_k.load(a.cache.k, first, key_of(e1), keys);
       rows_v.load(a.cache.v, first, key_of(e1), keys);
       if (wave == 0) keys_d.load(a, first, doc_first, key_of(e1), keys);
       __builtin_amdgcn_sched_barrier(0);
       if (live) {
-        if (taken % kFlush == kFlush - 1) flush(w);
-        score_block<SCORE, MASK>(sc[buf], w, ru, kd[buf], k0, keys - k0, (e & 1) != 0);
-        value_block(sc[buf], sc[buf ^ 1], w, vl[buf], kd[buf], kl[buf ^ 1]);
+        f32x16 sc[2];
+        clear(sc);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) score_step(sc, w, kl[buf], ks);
+        score_block<SCORE, MASK>(sc, w, ru, kd[buf], k0, keys - k0, (e & 1) != 0);
+        value_block(sc, w, vl[buf], kd[buf]);
       }
-      ++taken;
-      rows_k.template store<kKPitch>(kl[buf]);
+      rows_k.template store<kKPitch>(kl[buf ^ 1]);
       rows_v.template store<kVPitch>(vl[buf ^ 1]);
       if (wave == 0) keys_d.store(a, kd[buf ^ 1]);
       e = e1;
-      e1 = e2;
       __syncthreads();
-    };
-    int x = b_begin;
-    for (; x + 1 < b_end; x += 2) {
-      step(x, Int<0>{});
-      step(x + 1, Int<1>{});
     }
-    if (x < b_end) step(x, Int<0>{});
   }
-  flush(w);
   const float l = w.l + other_half(w.l);
   if (!live || row >= rows) return;
   if (part) {
@@ -768,8 +729,8 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
 #pragma unroll
       for (int r = 0; r < 4; ++r)
         *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) =
-            f32x4{w.total[dt][4 * r], w.total[dt][4 * r + 1], w.total[dt][4 * r + 2],
-                  w.total[dt][4 * r + 3]};
+            f32x4{w.o[dt][4 * r], w.o[dt][4 * r + 1], w.o[dt][4 * r + 2],
+                  w.o[dt][4 * r + 3]};
     if (half == 0)
       *reinterpret_cast<float2*>(part + a.splits * all_rows * HD + 2 * at) = make_float2(w.m, l);
   } else {
@@ -781,7 +742,7 @@ __global__ __launch_bounds__(64 * QW, 2) void attention_tile_kernel(const float*
       for (int r = 0; r < 4; ++r) {
         f32x4 t;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.total[dt][4 * r + c] / l;
+        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.o[dt][4 * r + c] / l;
         *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) = t;
       }
   }
@@ -900,7 +861,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const auto* Q = static_cast<const float*>(q->ptr);
   auto* O = static_cast<float*>(out->ptr);
   const size_t blocks = (limit + KB - 1) / KB;
-  const size_t tile_rows = 256, tiles = (a.group * n + tile_rows - 1) / tile_rows;
+  const size_t tile_rows = 128, tiles = (a.group * n + tile_rows - 1) / tile_rows;
   const bool few = a.group * n <= 4;
   const size_t cus = rt->cu_count > 0 ? rt->cu_count : 256;
   const size_t units = few ? rows : cache->sequences * cache->heads * tiles;
@@ -909,7 +870,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
     while (splits < 64 && rows * splits < 4 * cus && blocks / (2 * splits) >= 2 * kRowWaves)
       splits *= 2;
   } else {
-    splits = cus / units;
+    splits = 3 * cus / units;
     splits = splits > 16 ? 16 : splits;
     splits = splits > blocks / 4 ? blocks / 4 : splits;
     splits = splits < 1 ? 1 : splits;
@@ -934,7 +895,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   } else {
     const bool score = ru.cap > 0.0f || ru.slopes, mask = ru.causal || ru.q_docs;
 #define VK_TILE(F, S, M)                                                                          \
-  hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 8>), grid, dim3(512), 0, rt->stream, Q, O, \
+  hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 4>), grid, dim3(256), 0, rt->stream, Q, O, \
                      part, a)
 #define VK_TILE_F(F)                        \
   if (score && mask) VK_TILE(F, true, true); \

@@ -502,19 +502,24 @@ __device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, co
   w.l += sum[0] + sum[1];
 }
 
-// Staging by all threads: eight codes of K (or V) a thread and row.
+// Staging by all threads: eight codes of K (or V) a thread and row.  The block's
+// rows are a buffer of their own (its base and the bytes left of it in scalar registers), so
+// a load has no address arithmetic and keys past the end read zeros.
 template <int FORMAT, int THREADS>
 struct StageRows {
   static constexpr int kPer = KB * 8 / THREADS;
   uint2 w[kPer];
 
   __device__ __forceinline__ void load(const uint8_t* codes, size_t first, int k0, int keys) {
-    const int tid = threadIdx.x;
+    typedef int i32x2_t __attribute__((ext_vector_type(2)));
+    const int left = keys - k0 < KB ? keys - k0 : KB;
+    const __amdgpu_buffer_rsrc_t r =
+        vkd::buffer_rsrc(codes + (first + k0) * HD, static_cast<uint32_t>(left * HD));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const int key = k0 + (tid >> 3) + i * (THREADS / 8);
-      w[i] = *reinterpret_cast<const uint2*>(
-          codes + (first + (key < keys ? key : keys - 1)) * HD + 8 * (tid & 7));
+      const i32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(
+          r, static_cast<int>(8 * threadIdx.x), 8 * THREADS * i, 0);
+      w[i] = make_uint2(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
     }
   }
 
@@ -535,11 +540,15 @@ struct StageKeys {
 
   __device__ __forceinline__ void load(const Shape& a, size_t first, size_t doc_first, int k0,
                                        int keys) {
-    const int key = k0 + static_cast<int>(threadIdx.x);
-    const int c = key < keys ? key : keys - 1;
-    ks = a.cache.ks[first + c];
-    vs = a.cache.vs[first + c];
-    if (a.rules.k_docs) doc = a.rules.k_docs[doc_first + c];
+    const int left = keys - k0 < KB ? keys - k0 : KB;
+    const int at = 4 * static_cast<int>(threadIdx.x), bytes = 4 * left;
+    ks = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+        vkd::buffer_rsrc(a.cache.ks + first + k0, bytes), at, 0, 0));
+    vs = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+        vkd::buffer_rsrc(a.cache.vs + first + k0, bytes), at, 0, 0));
+    if (a.rules.k_docs)
+      doc = static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(
+          vkd::buffer_rsrc(a.rules.k_docs + doc_first + k0, bytes), at, 0, 0));
   }
 
   __device__ __forceinline__ void store(const Shape& a, KeyData& kd) const {
@@ -748,7 +757,9 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
   }
 }
 
-// Joins the key splits of a row, in split order: 16 threads a row.
+// Joins the key splits of a row, in split order: 16 threads a row, every load before the
+// first sum.
+template <int MOST>
 __global__ __launch_bounds__(256) void attention_join_kernel(const float* __restrict__ part,
                                                              float* __restrict__ out, float up,
                                                              Shape a) {
@@ -762,26 +773,32 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
   const uint32_t h = sh % a.heads, s = sh / a.heads;
   if (static_cast<int>(i) >= vkc::count_of(a.rows, s)) return;
   const float2* ml = reinterpret_cast<const float2*>(part + a.splits * rows * HD);
+  float2 x[MOST];
+  f32x4 y[MOST];
+#pragma unroll
+  for (int sp = 0; sp < MOST; ++sp) {
+    const size_t at = (sp < static_cast<int>(a.splits) ? sp : 0) * rows + row;
+    x[sp] = ml[at];
+    y[sp] = *reinterpret_cast<const f32x4*>(part + at * HD + 4 * c);
+  }
   float m = -INFINITY;
-  for (uint32_t sp = 0; sp < a.splits; ++sp) m = fmaxf(m, ml[sp * rows + row].x);
+#pragma unroll
+  for (int sp = 0; sp < MOST; ++sp) m = fmaxf(m, x[sp].x);  // again the first past the last
   float l = 0.0f;
-  float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  for (uint32_t sp = 0; sp < a.splits; ++sp) {
-    const float2 x = ml[sp * rows + row];
+  f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int sp = 0; sp < MOST; ++sp) {
     // in two steps: V's scales, which the references carry, may be far apart
-    const float w = x.y == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(0.5f * (x.x - m));
-    const float4 y = *reinterpret_cast<const float4*>(part + (sp * rows + row) * HD + 4 * c);
-    l += x.y * w * w;
-    o.x += y.x * w * w;
-    o.y += y.y * w * w;
-    o.z += y.z * w * w;
-    o.w += y.w * w * w;
+    const bool in = sp < static_cast<int>(a.splits) && x[sp].y != 0.0f;
+    const float w = in ? __builtin_amdgcn_exp2f(0.5f * (x[sp].x - m)) : 0.0f;
+    l += x[sp].y * w * w;
+    o += y[sp] * w * w;
   }
   if (l == 0.0f)
-    o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   else
-    o = make_float4(o.x / l * up, o.y / l * up, o.z / l * up, o.w / l * up);
-  *reinterpret_cast<float4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * c) = o;
+    o = f32x4{o[0] / l * up, o[1] / l * up, o[2] / l * up, o[3] / l * up};
+  *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * c) = o;
 }
 
 int check_i32(const vk_runtime* rt, const vk_tensor* t, size_t len, const char* what) {
@@ -908,8 +925,15 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   }
   VK_TRY(vk::check_launch("attention_cached"));
   if (splits == 1) return VK_OK;
-  hipLaunchKernelGGL(attention_join_kernel, dim3(static_cast<unsigned>((rows * 16 + 255) / 256)),
-                     dim3(256), 0, rt->stream, part, O, few ? 0x1p24f : 1.0f, a);
+  const dim3 jgrid(static_cast<unsigned>((rows * 16 + 255) / 256));
+#define VK_JOIN(N)                                                                          \
+  hipLaunchKernelGGL(attention_join_kernel<N>, jgrid, dim3(256), 0, rt->stream, part, O, up, a)
+  const float up = few ? 0x1p24f : 1.0f;
+  if (splits <= 4) VK_JOIN(4);
+  else if (splits <= 8) VK_JOIN(8);
+  else if (splits <= 16) VK_JOIN(16);
+  else VK_JOIN(64);
+#undef VK_JOIN
   return vk::check_launch("attention_join_kernel");
 }
 

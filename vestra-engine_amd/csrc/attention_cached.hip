@@ -33,6 +33,9 @@ struct Shape {
   uint32_t heads, group;  // query heads, and how many of them share a cache head
   uint32_t limit;         // keys at or past it are not seen (capacity, max_length)
   uint32_t splits, tiles;
+  struct {
+    uint32_t share, heads;
+  } order;
 };
 
 // Keys of sequence s: those of slots 0 .. keys_of - 1.
@@ -400,51 +403,58 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
                                             const KeyData& kd, int k0, int left, bool masked) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
   const int at = 16 * half + (lane & 15);
-  float mb = kLowest;
+  const float ksv[2] = {kd.ks[at], kd.ks[32 + at]};
+  each<32>([&](auto i) { s[i / 16][i % 16] *= bcast<i % 16>(ksv[i / 16]); });
+  if (__builtin_expect(w.own_scale, 0)) {
+    float back = w.back;
+    asm volatile("" : "+v"(back));  // keeps the products in this branch
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
-    const float ksv = kd.ks[32 * t + at];
-    float lsv = kd.lsv[32 * t + at];
-    each<16>([&](auto r) { s[t][r()] *= bcast<r>(ksv); });
-    if (__builtin_expect(w.own_scale, 0)) {
-      float back = w.back;
-      asm volatile("" : "+v"(back));  // keeps the products in this branch
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] *= back;
-    }
-    if constexpr (SCORE) {
-      if (ru.cap > 0.0f) {
+  }
+  if constexpr (SCORE) {
+    if (ru.cap > 0.0f) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[t][r] = tanh1(s[t][r]) * w.cap_up;
-      }
-      if (ru.slopes) {
-        const float base =
-            static_cast<float>(static_cast<long long>(w.pos) - (k0 + 32 * t + 4 * half));
+    }
+    if (ru.slopes) {
+      const float base = static_cast<float>(static_cast<long long>(w.pos) - (k0 + 4 * half));
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-          s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (8 * (r / 4) + r % 4)), s[t][r]);
-      }
+          s[t][r] =
+              __builtin_fmaf(-w.slope, fabsf(base - (32 * t + 8 * (r / 4) + r % 4)), s[t][r]);
     }
-    const bool causal = MASK && masked && ru.causal;
-    if (__builtin_expect(left < KB || causal, 0)) {
-      int lim = left;
-      if (causal) lim = min(lim, w.seen - k0);
-      lim -= 32 * t + 4 * half;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] = 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
-    }
-    if (MASK && masked && ru.q_docs) {
-      const float doc = __int_as_float(kd.doc[32 * t + at]);
-      // a later document, or any other
-      const int least = ru.docs_ordered ? -0x7fffffff - 1 : w.doc;
-      each<16>([&](auto r) {
-        const int d = __float_as_int(bcast<r>(doc));
-        s[t][r()] = d <= w.doc && d >= least ? s[t][r()] : -INFINITY;
-      });
-    }
-    asm volatile("" : "+v"(lsv));  // the broadcasts stay here, part of the additions
-    each<16>([&](auto r) { mb = fmaxf(mb, s[t][r()] + bcast<r>(lsv)); });
   }
+  const bool causal = MASK && masked && ru.causal;
+  if (__builtin_expect(left < KB || causal, 0)) {
+    int lim = left;
+    if (causal) lim = min(lim, w.seen - k0);
+    lim -= 4 * half;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[t][r] = 32 * t + 8 * (r / 4) + r % 4 < lim ? s[t][r] : -INFINITY;
+  }
+  if (MASK && masked && ru.q_docs) {
+    // a later document, or any other
+    const int least = ru.docs_ordered ? -0x7fffffff - 1 : w.doc;
+    const float doc[2] = {__int_as_float(kd.doc[at]), __int_as_float(kd.doc[32 + at])};
+    each<32>([&](auto i) {
+      const int d = __float_as_int(bcast<i % 16>(doc[i / 16]));
+      s[i / 16][i % 16] = d <= w.doc && d >= least ? s[i / 16][i % 16] : -INFINITY;
+    });
+  }
+  float lsv[2] = {kd.lsv[at], kd.lsv[32 + at]};
+  // the broadcasts stay here, part of the additions
+  asm volatile("" : "+v"(lsv[0]), "+v"(lsv[1]));
+  float mb = kLowest;
+  each<32>([&](auto i) { mb = fmaxf(mb, s[i / 16][i % 16] + bcast<i % 16>(lsv[i / 16])); });
   if (__builtin_amdgcn_ballot_w64(mb > w.m + kSlack) != 0) {
     mb = fmaxf(mb, other_half(mb));
     const bool moves = mb > w.m + kSlack;
@@ -578,11 +588,15 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
   __builtin_assume(tid < kThreads);
   const Rules& ru = a.rules;
 
-  // XCD-major numbering: the tiles of one cache head share an XCD's L2.  A
-  // sequence's later tiles come first: with a causal mask they take longest.
-  const uint32_t all = vkd::xcd_tile(blockIdx.x, gridDim.x);
-  const uint32_t split = all % a.splits, u = all / a.splits;
-  const uint32_t tile = a.tiles - 1 - u % a.tiles, sh = u / a.tiles;
+  // Workgroups go round the 8 XCDs.  `order.share` of them take a group of `order.heads`
+  // (sequence, cache head) pairs between them, so that a pair's K and V stay in few L2s;
+  // in a group the last tiles come first: with a causal mask they take longest.
+  const uint32_t xcd = blockIdx.x & 7;
+  const uint32_t in = (blockIdx.x >> 3) * a.order.share + xcd % a.order.share;
+  if (in >= a.order.heads * a.splits * a.tiles) return;
+  const uint32_t pair = in % a.order.heads, u = in / a.order.heads;
+  const uint32_t split = u % a.splits, tile = a.tiles - 1 - u / a.splits;
+  const uint32_t sh = xcd / a.order.share * a.order.heads + pair;
   const uint32_t kh = sh % a.cache.heads, s = sh / a.cache.heads;
   const int count = vkc::count_of(a.rows, s);
   const int rows = count > 0 ? count * static_cast<int>(a.group) : 0;  // query i's heads side by side
@@ -900,7 +914,13 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
     VK_TRY(vk::ensure_work(rt, splits * rows * (HD + 2), "attention_cached"));
     part = rt->work;
   }
-  const dim3 grid(static_cast<unsigned>(units * splits));
+  // 8 / share groups of `heads` pairs each
+  const size_t pairs = cache->sequences * cache->heads;
+  const uint32_t groups = pairs % 8 == 0 ? 8 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
+  a.order.share = 8 / groups;
+  a.order.heads = static_cast<uint32_t>(pairs / groups);
+  const size_t slots = (a.order.heads * tiles * splits + a.order.share - 1) / a.order.share;
+  const dim3 grid(static_cast<unsigned>(few ? units * splits : 8 * slots));
   const bool q8 = cache->format == VK_CACHE_Q8;
   if (few) {
     if (q8)

@@ -16,6 +16,9 @@ namespace {
 
 constexpr int HD = 64;
 constexpr float kLog2e = 1.44269504088896341f;
+// V's scale in the single row's sums: room for weights up to 2^4 and 2^20 keys of the largest
+// numbers.
+constexpr float kRowDown = 0x1p-24f, kRowUp = 0x1p24f;
 
 struct Rules {
   float scale, cap;
@@ -71,9 +74,13 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
 
-constexpr int kRowWaves = 4;
+constexpr int kRowWaves = 8;
 constexpr float kRoom = 4.0f;  // a lane's maximum follows scores that pass it by 2^kRoom
 
+// One query a sequence and cache head: a workgroup a query and key split, a lane a key.  The
+// lane's 64 products are F32 FMAs with the query in scalar registers (four running sums), and
+// it keeps a softmax of its own (maximum, sum and 64 sums of values) over the keys that it
+// meets; the lanes are joined once, at the end, halving: lane d is left with d.
 template <int FORMAT>
 __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const float* __restrict__ q,
                                                                        float* __restrict__ out,
@@ -83,18 +90,18 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   __shared__ float sm[kRowWaves], sl[kRowWaves];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
   const uint32_t split = blockIdx.x % a.splits, row = blockIdx.x / a.splits;
-  const uint32_t i = row % a.rows.n, sh = row / a.rows.n;
-  const uint32_t h = sh % a.heads, s = sh / a.heads;
-  if (static_cast<int>(i) >= vkc::count_of(a.rows, s)) return;
-  const uint32_t kh = h / a.group;
-  const int keys = keys_of(a, s);
-  const int p = position(vkc::start_of(a.rows, s), i);
-  const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
-  const float* qr = q + vkc::row_at(a.rows, a.heads, s, h, i);
+  const uint32_t h = row % a.heads, s = row / a.heads;
   const Rules& ru = a.rules;
+  // every scalar together: none waits for another
+  const int count = vkc::count_of(a.rows, s), start = vkc::start_of(a.rows, s);
   const float slope = ru.slopes ? ru.slopes[h] : 0.0f;
   const int pre = ru.prefix ? ru.prefix[s] : 0;
-  const int doc = ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + i] : 0;
+  const int doc = ru.q_docs ? ru.q_docs[s] : 0;
+  const float* qr = q + vkc::row_at(a.rows, a.heads, s, h, 0);
+  if (count <= 0) return;
+  const int keys = keys_of(a, s);
+  const int p = position(start, 0);
+  const size_t first = (static_cast<size_t>(s) * a.cache.heads + h) * a.cache.capacity;
 
   float m = -INFINITY, l = 0.0f, acc[HD];
 #pragma unroll
@@ -104,20 +111,26 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const int b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / a.splits);
   for (int b = b0 + wave; b < b1; b += kRowWaves) {
     const int j = b * 64 + lane;
+    // the key's codes and scales, all at once (past the end the last key's)
+    const size_t slot = first + (j < keys ? j : keys - 1);
+    const uint4* kc = reinterpret_cast<const uint4*>(a.cache.k + slot * HD);
+    const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD);
+    uint4 kw[4], vw[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) kw[c] = kc[c];
+    const float ks = a.cache.ks[slot], vs = a.cache.vs[slot];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) vw[c] = vc[c];
     bool seen = j < keys;
     if (ru.causal) seen = seen && (j <= p || j < pre);
-    if (seen && ru.q_docs) {
+    if (ru.q_docs && seen) {
       const int kd = ru.k_docs[static_cast<size_t>(s) * a.cache.capacity + j];
       seen = ru.docs_ordered ? kd <= doc : kd == doc;
     }
-    if (!seen) continue;
-    const size_t slot = first + j;
     float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const uint4* kc = reinterpret_cast<const uint4*>(a.cache.k + slot * HD);
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 w = kc[c];
-      const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+      const uint32_t ws[4] = {kw[c].x, kw[c].y, kw[c].z, kw[c].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float4 x = vkc::decode4<FORMAT>(ws[e]);
@@ -127,29 +140,27 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
         u[3] = __builtin_fmaf(qr[16 * c + 4 * e + 3], x.w, u[3]);
       }
     }
-    float t = ((u[0] + u[1]) + (u[2] + u[3])) * a.cache.ks[slot] * ru.scale;
+    float t = ((u[0] + u[1]) + (u[2] + u[3])) * ks * ru.scale;
     if (ru.cap > 0.0f) t = ru.cap * tanhf(t / ru.cap);
     if (ru.slopes) {
       const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
       t -= slope * static_cast<float>(far);
     }
     t *= kLog2e;
-    if (t == -INFINITY) continue;
-    if (t > m + kRoom) {
+    seen = seen && !(t == -INFINITY);
+    if (seen && t > m + kRoom) {
       const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - t);
       l *= f;
 #pragma unroll
       for (int d = 0; d < HD; ++d) acc[d] *= f;
       m = t;
     }
-    const float w = __builtin_amdgcn_exp2f(t - m);
+    const float w = seen ? __builtin_amdgcn_exp2f(t - m) : 0.0f;
     l += w;
-    const float wv = w * (a.cache.vs[slot] * 0x1p-24f);
-    const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD);
+    const float wv = seen ? w * (vs * kRowDown) : 0.0f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint4 x4 = vc[c];
-      const uint32_t ws[4] = {x4.x, x4.y, x4.z, x4.w};
+      const uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float4 x = vkc::decode4<FORMAT>(ws[e]);
@@ -161,22 +172,37 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
       }
     }
   }
-  // the wave: one maximum, the sums halved over the lanes, lane d left with d
   const float mw = wave_max(m);
   const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mw);
   l *= f;
 #pragma unroll
   for (int d = 0; d < HD; ++d) acc[d] *= f;
+  // halving by swaps of halves and of rows of 16, then by exchanges inside them
 #pragma unroll
-  for (int w = 32; w; w >>= 1) {
+  for (int d = 0; d < 32; ++d) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[d]),
+                                                    __float_as_uint(acc[d + 32]), false, false);
+    const uint32_t x = r[0], y = r[1];
+    acc[d] = __uint_as_float(x) + __uint_as_float(y);
+  }
+#pragma unroll
+  for (int d = 0; d < 16; ++d) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[d]),
+                                                    __float_as_uint(acc[d + 16]), false, false);
+    const uint32_t x = r[0], y = r[1];
+    acc[d] = __uint_as_float(x) + __uint_as_float(y);
+  }
+#pragma unroll
+  for (int w = 8; w; w >>= 1) {
     const bool up = (lane & w) != 0;
 #pragma unroll
     for (int d = 0; d < w; ++d) {
       const float send = up ? acc[d] : acc[d + w];
       acc[d] = (up ? acc[d + w] : acc[d]) + __shfl_xor(send, w, 64);
     }
-    l += __shfl_xor(l, w, 64);
   }
+#pragma unroll
+  for (int w = 32; w; w >>= 1) l += __shfl_xor(l, w, 64);
   so[wave][lane] = acc[0];
   if (lane == 0) {
     sm[wave] = mw;
@@ -195,13 +221,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     lg += sl[w] * g;
   }
   if (part) {
-    const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
+    const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads;
     const size_t at = static_cast<size_t>(split) * rows + row;
     part[at * HD + lane] = o;
     if (lane == 0)
       *reinterpret_cast<float2*>(part + a.splits * rows * HD + 2 * at) = make_float2(mg, lg);
   } else {
-    out[vkc::row_at(a.rows, a.heads, s, h, i) + lane] = lg == 0.0f ? 0.0f : o / lg * 0x1p24f;
+    out[vkc::row_at(a.rows, a.heads, s, h, 0) + lane] = lg == 0.0f ? 0.0f : o / lg * kRowUp;
   }
 }
 
@@ -294,6 +320,33 @@ struct KeyData {
   int doc[KB];
 };
 
+// The same as a lane of a wave takes them: of the keys of its row of 16 lanes, its own.
+struct KeyRegs {
+  float ks[2], lsv[2], sv[2];  // of the 32 keys t
+  int doc[2];
+};
+
+__device__ __forceinline__ KeyRegs key_regs(const KeyData& kd, bool docs) {
+  const int lane = threadIdx.x & 63, at = 16 * (lane >> 5) + (lane & 15);
+  KeyRegs k;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    k.ks[t] = kd.ks[32 * t + at];
+    k.lsv[t] = kd.lsv[32 * t + at];
+    k.sv[t] = kd.sv[32 * t + at];
+    k.doc[t] = docs ? kd.doc[32 * t + at] : 0;
+  }
+  return k;
+}
+
+// ks, lsv and sv from the scales of a row of K and of V.
+__device__ __forceinline__ void key_values(float k, float v, float* ks, float* lsv, float* sv) {
+  const bool nan = v != v;
+  *ks = nan ? v : k * (1.0f / (1 << kQUp));
+  *lsv = fmaxf(__builtin_amdgcn_logf(fmaxf(v, vkc::kLeastScale)), kLeastLsv);
+  *sv = nan ? 0.0f : v;
+}
+
 __device__ __forceinline__ int key_slot(int key) {
   return (key & 32) | (key & 4) << 2 | (key & 24) >> 1 | (key & 3);
 }
@@ -314,7 +367,7 @@ __device__ __forceinline__ float tanh1(float x) {
 
 // A wave's 32 queries: lane l and lane l ^ 32 hold query l % 32.
 struct Queries {
-  u32x4 q[4][2];         // two f16 parts, d = 16 ks + 8 half + j
+  u32x4 q[4][2];         // two f16 parts of eight values, four steps of 16 d
   float back;            // 1, or what the row's own scale has to be undone by
   bool own_scale;        // uniform: some row has one
   float slope, cap_up;   // per unit of distance and cap, in base 2
@@ -324,6 +377,8 @@ struct Queries {
   float m, l;            // running reference, this lane's denominators
 };
 
+// The order of d: element j of step ks is d = DK ks + DH half + j.
+template <int DK, int DH>
 __device__ __forceinline__ void load_queries(Queries& w, const float* row, float c, int half) {
   f32x4 x[4][2];
   float m = 0.0f;
@@ -331,7 +386,7 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
   for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[ks][i] = *reinterpret_cast<const f32x4*>(row + 16 * ks + 8 * half + 4 * i) * c;
+      x[ks][i] = *reinterpret_cast<const f32x4*>(row + DK * ks + DH * half + 4 * i) * c;
 #pragma unroll
       for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[ks][i][e]));
     }
@@ -400,11 +455,9 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 // part of the value sum, once that passes it by kSlack.
 template <bool SCORE, bool MASK>
 __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Rules& ru,
-                                            const KeyData& kd, int k0, int left, bool masked) {
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int at = 16 * half + (lane & 15);
-  const float ksv[2] = {kd.ks[at], kd.ks[32 + at]};
-  each<32>([&](auto i) { s[i / 16][i % 16] *= bcast<i % 16>(ksv[i / 16]); });
+                                            const KeyRegs& key, int k0, int left, bool masked) {
+  const int half = (threadIdx.x & 63) >> 5;
+  each<32>([&](auto i) { s[i / 16][i % 16] *= bcast<i % 16>(key.ks[i / 16]); });
   if (__builtin_expect(w.own_scale, 0)) {
     float back = w.back;
     asm volatile("" : "+v"(back));  // keeps the products in this branch
@@ -444,13 +497,12 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
   if (MASK && masked && ru.q_docs) {
     // a later document, or any other
     const int least = ru.docs_ordered ? -0x7fffffff - 1 : w.doc;
-    const float doc[2] = {__int_as_float(kd.doc[at]), __int_as_float(kd.doc[32 + at])};
     each<32>([&](auto i) {
-      const int d = __float_as_int(bcast<i % 16>(doc[i / 16]));
+      const int d = __float_as_int(bcast<i % 16>(__int_as_float(key.doc[i / 16])));
       s[i / 16][i % 16] = d <= w.doc && d >= least ? s[i / 16][i % 16] : -INFINITY;
     });
   }
-  float lsv[2] = {kd.lsv[at], kd.lsv[32 + at]};
+  float lsv[2] = {key.lsv[0], key.lsv[1]};
   // the broadcasts stay here, part of the additions
   asm volatile("" : "+v"(lsv[0]), "+v"(lsv[1]));
   float mb = kLowest;
@@ -472,11 +524,9 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
 // The weights of a block's scores, p = 2^(score - reference), their sum, and O^T += V^T
 // (p V's scale)^T.
 __device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, const char* v,
-                                            const KeyData& kd) {
+                                            const KeyRegs& key) {
   const int lane = threadIdx.x & 63, half = lane >> 5;
-  const int at = 16 * half + (lane & 15);
   const float ref = w.m - kPBits;
-  const float sv[2] = {kd.sv[at], kd.sv[32 + at]};
   float one = 1.0f;
   asm("" : "+s"(one));
   float sum[2] = {0.0f, 0.0f};
@@ -500,7 +550,7 @@ __device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, co
       sum[0] += a;
       sum[1] += b;
       uint32_t x, y;
-      split_weights2(a * bcast<r>(sv[t]), b * bcast<r + 1>(sv[t]), one, &x, &y);
+      split_weights2(a * bcast<r>(key.sv[t]), b * bcast<r + 1>(key.sv[t]), one, &x, &y);
       p0[j()] = x;
       p1[j()] = y;
     });
@@ -510,6 +560,141 @@ __device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, co
     for (int dt = 0; dt < 2; ++dt) w.o[dt] = vks::mfma32(vv[dt], p0, w.o[dt]);
   });
   w.l += sum[0] + sum[1];
+}
+
+// The queries of a wave: row `row` of cache head kh's, whose query heads lie side by side.
+template <bool SCORE, bool MASK, int DK, int DH>
+__device__ __forceinline__ void take_queries(Queries& w, const float* __restrict__ q, const Shape& a,
+                                             uint32_t s, uint32_t kh, uint32_t row, uint32_t* i,
+                                             uint32_t* h) {
+  const Rules& ru = a.rules;
+  *i = row / a.group;
+  *h = kh * a.group + (row - *i * a.group);
+  load_queries<DK, DH>(w, q + vkc::row_at(a.rows, a.heads, s, *h, *i),
+                       ru.cap > 0.0f ? ru.scale / ru.cap : ru.scale * kLog2e,
+                       (threadIdx.x & 63) >> 5);
+  w.cap_up = ru.cap * kLog2e;
+  w.slope = SCORE && ru.slopes ? ru.slopes[*h] * kLog2e : 0.0f;
+  w.pos = position(vkc::start_of(a.rows, s), *i);
+  const int pre = MASK && ru.prefix ? ru.prefix[s] : 0;
+  w.seen = max(max(w.pos + 1, pre), 0);
+  w.doc = MASK && ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + *i] : 0;
+}
+
+// What a tile's queries may see, as a whole.
+struct Span {
+  int p_low, p_high, pre;  // positions and prefix
+  int q_low, q_high;       // documents
+};
+
+// Of rows row_first .. row_last of a workgroup of WAVES waves; `range` is LDS.
+template <int WAVES>
+__device__ __forceinline__ Span tile_span(const Queries& w, const Shape& a, uint32_t s,
+                                          int row_first, int row_last, bool live, int* range) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int start = vkc::start_of(a.rows, s);
+  Span p{position(start, row_first / a.group), position(start, row_last / a.group),
+         a.rules.prefix ? a.rules.prefix[s] : 0, 0, 0};
+  if (a.rules.q_docs) {
+    int lo = w.doc, hi = w.doc;
+#pragma unroll
+    for (int m = 16; m; m >>= 1) {
+      lo = min(lo, __shfl_xor(lo, m, 64));
+      hi = max(hi, __shfl_xor(hi, m, 64));
+    }
+    if (lane == 0) {
+      range[wave] = live ? lo : 0x7fffffff;
+      range[WAVES + wave] = live ? hi : -0x7fffffff - 1;
+    }
+    __syncthreads();
+    p.q_low = range[0];
+    p.q_high = range[WAVES];
+#pragma unroll
+    for (int x = 1; x < WAVES; ++x) {
+      p.q_low = min(p.q_low, range[x]);
+      p.q_high = max(p.q_high, range[WAVES + x]);
+    }
+  }
+  return p;
+}
+
+constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
+
+// Lists the blocks of seg .. seg_end - 1 that some query of the tile may see, in order: the
+// block less seg, times two, plus one where not every query sees all of it.  A thread takes a
+// block; `count` is LDS.
+template <int WAVES>
+__device__ __forceinline__ int list_blocks(uint16_t* list, int* count, const Shape& a,
+                                           const Span& p, int seg, int seg_end, int keys,
+                                           size_t doc_first) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const Rules& ru = a.rules;
+  int filled = 0;
+  for (int b0 = seg; b0 < seg_end; b0 += 64 * WAVES) {
+    const int b = b0 + static_cast<int>(threadIdx.x);
+    bool any = b < seg_end, full = true;
+    if (any) {
+      const int k0 = b * KB;
+      const int k1 = keys - k0 < KB ? keys - 1 : k0 + KB - 1;  // last key
+      if (ru.causal) {
+        any = k0 <= p.p_high || k0 < p.pre;
+        full = k1 <= p.p_low || k1 < p.pre;
+      }
+      if (any && ru.q_docs) {
+        int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+        const int* d = ru.k_docs + doc_first + k0;
+        for (int j = 0; j <= k1 - k0; ++j) {
+          lo = min(lo, d[j]);
+          hi = max(hi, d[j]);
+        }
+        if (ru.docs_ordered) {
+          any = lo <= p.q_high;
+          full = full && hi <= p.q_low;
+        } else {
+          any = lo <= p.q_high && hi >= p.q_low;
+          full = full && lo == hi && p.q_low == p.q_high && lo == p.q_low;
+        }
+      }
+    }
+    const uint64_t m = __builtin_amdgcn_ballot_w64(any);
+    __syncthreads();  // the counts of the run before are read
+    if (lane == 0) count[wave] = __popcll(m);
+    __syncthreads();
+    int at = filled;
+#pragma unroll
+    for (int x = 0; x < WAVES; ++x) {
+      if (x < wave) at += count[x];
+      filled += count[x];
+    }
+    if (any)
+      list[at + __popcll(m & ((1ull << lane) - 1))] =
+          static_cast<uint16_t>((b - seg) << 1 | (full ? 0 : 1));
+  }
+  __syncthreads();
+  return filled;
+}
+
+// A query's share of the result: its sums and their denominators to `part` (and the
+// reference they stand in), or their quotient to `out`.
+__device__ __forceinline__ void store_part(float* part, const Shape& a, uint32_t split, uint32_t s,
+                                           uint32_t h, uint32_t i, int d, const f32x4& o) {
+  const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
+  const size_t at = static_cast<size_t>(split) * rows +
+                    (static_cast<size_t>(s) * a.heads + h) * a.rows.n + i;
+  *reinterpret_cast<f32x4*>(part + at * HD + d) = o;
+}
+
+__device__ __forceinline__ void store_ml(float* part, const Shape& a, uint32_t split, uint32_t s,
+                                         uint32_t h, uint32_t i, float m, float l) {
+  const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
+  const size_t at = static_cast<size_t>(split) * rows +
+                    (static_cast<size_t>(s) * a.heads + h) * a.rows.n + i;
+  *reinterpret_cast<float2*>(part + a.splits * rows * HD + 2 * at) = make_float2(m, l);
+}
+
+__device__ __forceinline__ f32x4 quotient(const f32x4& o, float l) {
+  if (l == 0.0f) return f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  return f32x4{o[0] / l, o[1] / l, o[2] / l, o[3] / l};
 }
 
 // Staging by all threads: eight codes of K (or V) a thread and row.  The block's
@@ -563,15 +748,10 @@ struct StageKeys {
 
   __device__ __forceinline__ void store(const Shape& a, KeyData& kd) const {
     const int at = key_slot(threadIdx.x);
-    const bool nan = vs != vs;
-    kd.ks[at] = nan ? vs : ks * (1.0f / (1 << kQUp));
-    kd.lsv[at] = fmaxf(__builtin_amdgcn_logf(fmaxf(vs, vkc::kLeastScale)), kLeastLsv);
-    kd.sv[at] = nan ? 0.0f : vs;
+    key_values(ks, vs, &kd.ks[at], &kd.lsv[at], &kd.sv[at]);
     if (a.rules.k_docs) kd.doc[at] = doc;
   }
 };
-
-constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
 
 template <int FORMAT, bool SCORE, bool MASK, int QW>
 __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float* __restrict__ q,
@@ -579,12 +759,13 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
                                                                     float* __restrict__ part,
                                                                     Shape a) {
   constexpr int kThreads = 64 * QW, kRows = 32 * QW;
+  static_assert(kRows == vk::kTileRows, "the plan's tiles");
   __shared__ __align__(16) char kl[2][KB * kKPitch];
   __shared__ __align__(16) char vl[2][KB * kVPitch];
   __shared__ KeyData kd[2];
   __shared__ uint16_t list[MASK ? kList : 1];
-  __shared__ int wave_count[QW], doc_low[QW], doc_high[QW];
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  __shared__ int wave_count[QW], doc_range[2 * QW];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   __builtin_assume(tid < kThreads);
   const Rules& ru = a.rules;
 
@@ -603,107 +784,25 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
   const int row0 = static_cast<int>(tile) * kRows;
   if (row0 >= rows) return;
   const int keys = keys_of(a, s);
-  const int start = vkc::start_of(a.rows, s);
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
   const size_t doc_first = static_cast<size_t>(s) * a.cache.capacity;
   const bool live = row0 + 32 * wave < rows;  // uniform over the wave
   const int row = row0 + 32 * wave + (lane & 31);
-  const int my = row < rows ? row : rows - 1;
-  const uint32_t i = my / a.group, h = kh * a.group + my % a.group;
-
+  uint32_t i, h;
   Queries w;
-  load_queries(w, q + vkc::row_at(a.rows, a.heads, s, h, i),
-               ru.cap > 0.0f ? ru.scale / ru.cap : ru.scale * kLog2e, half);
-  w.cap_up = ru.cap * kLog2e;
-  w.slope = SCORE && ru.slopes ? ru.slopes[h] * kLog2e : 0.0f;
-  w.pos = position(start, i);
-  const int pre = MASK && ru.prefix ? ru.prefix[s] : 0;
-  w.seen = max(max(w.pos + 1, pre), 0);
-  w.doc = MASK && ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + i] : 0;
+  take_queries<SCORE, MASK, 16, 8>(w, q, a, s, kh, row < rows ? row : rows - 1, &i, &h);
 
   const int blocks = (keys + KB - 1) / KB;
-  // the tile's positions and documents
-  const int p_low = position(start, row0 / a.group);
-  const int row_last = row0 + kRows < rows ? row0 + kRows - 1 : rows - 1;
-  const int p_high = position(start, row_last / a.group);
-  int q_low = 0, q_high = 0;
-  if (MASK && ru.q_docs) {
-    int lo = w.doc, hi = w.doc;
-    if (live) {
-#pragma unroll
-      for (int m = 16; m; m >>= 1) {
-        lo = min(lo, __shfl_xor(lo, m, 64));
-        hi = max(hi, __shfl_xor(hi, m, 64));
-      }
-    } else {
-      lo = 0x7fffffff;
-      hi = -0x7fffffff - 1;
-    }
-    if (lane == 0) {
-      doc_low[wave] = lo;
-      doc_high[wave] = hi;
-    }
-    __syncthreads();
-    q_low = doc_low[0];
-    q_high = doc_high[0];
-#pragma unroll
-    for (int x = 1; x < QW; ++x) {
-      q_low = min(q_low, doc_low[x]);
-      q_high = max(q_high, doc_high[x]);
-    }
-  }
-
+  Span span;
+  if constexpr (MASK)
+    span = tile_span<QW>(w, a, s, row0, row0 + kRows < rows ? row0 + kRows - 1 : rows - 1, live, doc_range);
   StageRows<FORMAT, kThreads> rows_k, rows_v;
   StageKeys keys_d;
   // blocks listed (MASK) or all of them, a run of kList at a time
   for (int seg = 0; seg < blocks; seg += kList) {
     int listed = blocks - seg < kList ? blocks - seg : kList;
-    if constexpr (MASK) {
-      int filled = 0;
-      const int seg_end = seg + listed;
-      for (int b0 = seg; b0 < seg_end; b0 += kThreads) {
-        const int b = b0 + tid;
-        bool any = b < seg_end, full = true;
-        if (any) {
-          const long long k0 = static_cast<long long>(b) * KB;
-          const long long k1 = k0 + KB < keys ? k0 + KB - 1 : keys - 1;  // last key
-          if (ru.causal) {
-            any = k0 <= p_high || k0 < pre;
-            full = k1 <= p_low || k1 < pre;
-          }
-          if (any && ru.q_docs) {
-            int lo = 0x7fffffff, hi = -0x7fffffff - 1;
-            for (long long j = k0; j <= k1; ++j) {
-              const int d = ru.k_docs[doc_first + j];
-              lo = min(lo, d);
-              hi = max(hi, d);
-            }
-            if (ru.docs_ordered) {
-              any = lo <= q_high;
-              full = full && hi <= q_low;
-            } else {
-              any = lo <= q_high && hi >= q_low;
-              full = full && lo == hi && q_low == q_high && lo == q_low;
-            }
-          }
-        }
-        const uint64_t m = __builtin_amdgcn_ballot_w64(any);
-        __syncthreads();  // the counts of the run before are read
-        if (lane == 0) wave_count[wave] = __popcll(m);
-        __syncthreads();
-        int at = filled;
-#pragma unroll
-        for (int x = 0; x < QW; ++x) {
-          if (x < wave) at += wave_count[x];
-          filled += wave_count[x];
-        }
-        if (any)
-          list[at + __popcll(m & ((1ull << lane) - 1))] =
-              static_cast<uint16_t>((b - seg) << 1 | (full ? 0 : 1));
-      }
-      listed = filled;
-      __syncthreads();
-    }
+    if constexpr (MASK)
+      listed = list_blocks<QW>(list, wave_count, a, span, seg, seg + listed, keys, doc_first);
     const int b_begin = static_cast<int>(split * static_cast<uint32_t>(listed) / a.splits);
     const int b_end = static_cast<int>((split + 1) * static_cast<uint32_t>(listed) / a.splits);
     if (b_begin == b_end) continue;  // uniform over the workgroup
@@ -730,8 +829,9 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
         clear(sc);
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) score_step(sc, w, kl[buf], ks);
-        score_block<SCORE, MASK>(sc, w, ru, kd[buf], k0, keys - k0, (e & 1) != 0);
-        value_block(sc, w, vl[buf], kd[buf]);
+        const KeyRegs key = key_regs(kd[buf], MASK && ru.q_docs);
+        score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0);
+        value_block(sc, w, vl[buf], key);
       }
       rows_k.template store<kKPitch>(kl[buf ^ 1]);
       rows_v.template store<kVPitch>(vl[buf ^ 1]);
@@ -740,46 +840,195 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
       __syncthreads();
     }
   }
+  const int half = lane >> 5;
   const float l = w.l + other_half(w.l);
   if (!live || row >= rows) return;
-  if (part) {
-    const size_t all_rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
-    const size_t at = static_cast<size_t>(split) * all_rows +
-                      (static_cast<size_t>(s) * a.heads + h) * a.rows.n + i;
-    float* po = part + at * HD + 4 * half;
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
+  for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) =
-            f32x4{w.o[dt][4 * r], w.o[dt][4 * r + 1], w.o[dt][4 * r + 2],
-                  w.o[dt][4 * r + 3]};
-    if (half == 0)
-      *reinterpret_cast<float2*>(part + a.splits * all_rows * HD + 2 * at) = make_float2(w.m, l);
-  } else {
-    float* po = out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * half;
-    const bool none = l == 0.0f;
+    for (int r = 0; r < 4; ++r) {
+      const f32x4 o = {w.o[dt][4 * r], w.o[dt][4 * r + 1], w.o[dt][4 * r + 2], w.o[dt][4 * r + 3]};
+      const int d = 32 * dt + 8 * r + 4 * half;
+      if (part)
+        store_part(part, a, split, s, h, i, d, o);
+      else
+        *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + d) = quotient(o, l);
+    }
+  if (part && half == 0) store_ml(part, a, split, s, h, i, w.m, l);
+}
+
+// 32 rows or fewer of a cache head: the waves of a workgroup hold the same queries and
+// take blocks of keys in turn, each for itself: K straight from memory as the products' operand
+// (d = 32 half + 8 ks + j: a lane's 32 codes of a key lie side by side), V through 12
+// KiB of LDS of the wave's own for the transposed reads, a block ahead in registers.  No
+// barrier until the waves are joined at the end.
+constexpr int kFewWaves = 4;
+
+template <int FORMAT, bool SCORE, bool MASK>
+__global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
+    const float* __restrict__ q, float* __restrict__ out, float* __restrict__ part, Shape a) {
+  __shared__ __align__(16) char vl[kFewWaves][KB * kVPitch];
+  __shared__ float sm[kFewWaves][32], sl[kFewWaves][32];
+  __shared__ uint16_t list[MASK ? kList : 1];
+  __shared__ int wave_count[kFewWaves], doc_range[2 * kFewWaves];
+  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
+  __builtin_assume(tid < 64 * kFewWaves);
+  const Rules& ru = a.rules;
+  const uint32_t split = blockIdx.x % a.splits, sh = blockIdx.x / a.splits;
+  const uint32_t kh = sh % a.cache.heads, s = sh / a.cache.heads;
+  const int count = vkc::count_of(a.rows, s);
+  if (count <= 0) return;
+  const int rows = count * static_cast<int>(a.group);
+  const int keys = keys_of(a, s);
+  const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
+  const size_t doc_first = static_cast<size_t>(s) * a.cache.capacity;
+  const int row = lane & 31;
+  uint32_t i, h;
+  Queries w;
+  take_queries<SCORE, MASK, 8, 32>(w, q, a, s, kh, row < rows ? row : rows - 1, &i, &h);
+  const int blocks = (keys + KB - 1) / KB;
+  Span span;
+  if constexpr (MASK) span = tile_span<kFewWaves>(w, a, s, 0, rows - 1, true, doc_range);
+
+  // a block's codes and scales in registers: K rows 32 t + l % 32, bytes 32 half ..; V rows
+  // 16 x + l / 4, 16 bytes at l % 4; scales of keys 32 t + 8 (i / 4) + 4 half + i % 4, i = l % 16
+  typedef int i32x4_t __attribute__((ext_vector_type(4)));
+  i32x4_t kr[2][2], vr[4];
+  float kss[2], vss[2];
+  int docs[2];
+  auto load = [&](int k0) {
+    const int left = keys - k0 < KB ? keys - k0 : KB;
+    const __amdgpu_buffer_rsrc_t kb =
+        vkd::buffer_rsrc(a.cache.k + (first + k0) * HD, static_cast<uint32_t>(left * HD));
+    const __amdgpu_buffer_rsrc_t vb =
+        vkd::buffer_rsrc(a.cache.v + (first + k0) * HD, static_cast<uint32_t>(left * HD));
+    const int k_off = (lane & 31) * HD + 32 * half;
 #pragma unroll
-    for (int dt = 0; dt < 2; ++dt)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        f32x4 t;
+      for (int x = 0; x < 2; ++x)
+        kr[t][x] = __builtin_amdgcn_raw_buffer_load_b128(kb, k_off, 32 * HD * t + 16 * x, 0);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) t[c] = none ? 0.0f : w.o[dt][4 * r + c] / l;
-        *reinterpret_cast<f32x4*>(po + 32 * dt + 8 * r) = t;
+    for (int x = 0; x < 4; ++x)
+      vr[x] = __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * lane, 1024 * x, 0);
+    const __amdgpu_buffer_rsrc_t ksb = vkd::buffer_rsrc(a.cache.ks + first + k0, 4 * left);
+    const __amdgpu_buffer_rsrc_t vsb = vkd::buffer_rsrc(a.cache.vs + first + k0, 4 * left);
+    const int at = 4 * (8 * ((lane & 15) >> 2) + 4 * half + (lane & 3));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      kss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksb, at, 128 * t, 0));
+      vss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsb, at, 128 * t, 0));
+    }
+    if (MASK && ru.q_docs) {
+      const __amdgpu_buffer_rsrc_t db =
+          vkd::buffer_rsrc(ru.k_docs + doc_first + k0, 4 * left);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        docs[t] = static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(db, at, 128 * t, 0));
+    }
+  };
+  char* vw = vl[wave];
+
+  for (int seg = 0; seg < blocks; seg += kList) {
+    int listed = blocks - seg < kList ? blocks - seg : kList;
+    if constexpr (MASK)
+      listed = list_blocks<kFewWaves>(list, wave_count, a, span, seg, seg + listed, keys, doc_first);
+    const int b_begin = static_cast<int>(split * static_cast<uint32_t>(listed) / a.splits) + wave;
+    const int b_end = static_cast<int>((split + 1) * static_cast<uint32_t>(listed) / a.splits);
+    auto entry = [&](int x) {
+      return MASK ? __builtin_amdgcn_readfirstlane(static_cast<int>(list[x])) : x << 1;
+    };
+    auto key_of = [&](int e) { return (seg + (e >> 1)) * KB; };
+    int e = 0;
+    if (b_begin < b_end) {
+      e = entry(b_begin);
+      load(key_of(e));
+    }
+    for (int x = b_begin; x < b_end; x += kFewWaves) {
+      // this block's operands out of the loads' registers
+      const int k0 = key_of(e);
+      KeyRegs key;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        key_values(kss[t], vss[t], &key.ks[t], &key.lsv[t], &key.sv[t]);
+        key.doc[t] = MASK && ru.q_docs ? docs[t] : 0;
       }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        char* to = vw + (16 * y + (lane >> 2)) * kVPitch + 32 * (lane & 3);
+        *reinterpret_cast<u32x4*>(to) = decode8<FORMAT>(make_uint2(vr[y][0], vr[y][1]));
+        *reinterpret_cast<u32x4*>(to + 16) = decode8<FORMAT>(make_uint2(vr[y][2], vr[y][3]));
+      }
+      f32x16 sc[2];
+      clear(sc);
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          const i32x4_t c = kr[t][ks >> 1];
+          const u32x4 f = decode8<FORMAT>(ks & 1 ? make_uint2(c[2], c[3]) : make_uint2(c[0], c[1]));
+          sc[t] = vks::mfma32(f, w.q[ks][1], sc[t]);
+          sc[t] = vks::mfma32(f, w.q[ks][0], sc[t]);
+        }
+      const int e1 = entry(x + kFewWaves < b_end ? x + kFewWaves : x);
+      load(key_of(e1));
+      vkd::wave_lds_fence();
+      score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0);
+      value_block(sc, w, vw, key);
+      vkd::wave_lds_fence();
+      e = e1;
+    }
+    if constexpr (MASK) __syncthreads();  // the list is read
+  }
+  // the waves together, in their order: o through each wave's LDS as [query][d]
+  w.l += other_half(w.l);
+  float* so = reinterpret_cast<float*>(vw);
+  constexpr int kOPitch = 68;
+  static_assert(32 * kOPitch * 4 <= KB * kVPitch, "a wave's sums fit its LDS");
+#pragma unroll
+  for (int dt = 0; dt < 2; ++dt)
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      *reinterpret_cast<f32x4*>(so + row * kOPitch + 32 * dt + 8 * r + 4 * half) =
+          f32x4{w.o[dt][4 * r], w.o[dt][4 * r + 1], w.o[dt][4 * r + 2], w.o[dt][4 * r + 3]};
+  if (half == 0) {
+    sm[wave][row] = w.m;
+    sl[wave][row] = w.l;
+  }
+  __syncthreads();
+  for (int x = tid; x < 16 * rows; x += 64 * kFewWaves) {
+    const int r = x >> 4, d = 4 * (x & 15);
+    float m = sm[0][r];
+#pragma unroll
+    for (int y = 1; y < kFewWaves; ++y) m = fmaxf(m, sm[y][r]);
+    float l = 0.0f;
+    f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int y = 0; y < kFewWaves; ++y) {
+      // in two steps: V's scales, which the references carry, may be far apart
+      const float f = sl[y][r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(0.5f * (sm[y][r] - m));
+      l += sl[y][r] * f * f;
+      o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vl[y]) + r * kOPitch + d) *
+           f * f;
+    }
+    const uint32_t ri = r / a.group, rh = kh * a.group + (r - ri * a.group);
+    if (part) {
+      store_part(part, a, split, s, rh, ri, d, o);
+      if (d == 0) store_ml(part, a, split, s, rh, ri, m, l);
+    } else {
+      *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, rh, ri) + d) = quotient(o, l);
+    }
   }
 }
 
-// Joins the key splits of a row, in split order: 16 threads a row, every load before the
-// first sum.
-template <int MOST>
+// Joins the key splits of a row: a wave a row, its 16-lane rows g taking splits g, g + 4, ..
+// in order (every load before the first sum), and then the four together.
+template <int PER>
 __global__ __launch_bounds__(256) void attention_join_kernel(const float* __restrict__ part,
                                                              float* __restrict__ out, float up,
                                                              Shape a) {
-  const size_t idx = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
-  const size_t row = idx >> 4;
-  const int c = static_cast<int>(idx & 15);
+  const size_t row = static_cast<size_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int g = (threadIdx.x & 63) >> 4, c = static_cast<int>(threadIdx.x & 15);
   const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
   if (row >= rows) return;
   const uint32_t i = static_cast<uint32_t>(row % a.rows.n);
@@ -787,32 +1036,39 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
   const uint32_t h = sh % a.heads, s = sh / a.heads;
   if (static_cast<int>(i) >= vkc::count_of(a.rows, s)) return;
   const float2* ml = reinterpret_cast<const float2*>(part + a.splits * rows * HD);
-  float2 x[MOST];
-  f32x4 y[MOST];
+  float2 x[PER];
+  f32x4 y[PER];
 #pragma unroll
-  for (int sp = 0; sp < MOST; ++sp) {
-    const size_t at = (sp < static_cast<int>(a.splits) ? sp : 0) * rows + row;
-    x[sp] = ml[at];
-    y[sp] = *reinterpret_cast<const f32x4*>(part + at * HD + 4 * c);
+  for (int j = 0; j < PER; ++j) {
+    const uint32_t sp = g + 4 * j;
+    const size_t at = (sp < a.splits ? sp : 0) * rows + row;
+    x[j] = ml[at];
+    y[j] = *reinterpret_cast<const f32x4*>(part + at * HD + 4 * c);
+    if (sp >= a.splits) x[j].y = 0.0f;
   }
   float m = -INFINITY;
 #pragma unroll
-  for (int sp = 0; sp < MOST; ++sp) m = fmaxf(m, x[sp].x);  // again the first past the last
+  for (int j = 0; j < PER; ++j) m = fmaxf(m, x[j].x);  // again the first past the last
+  m = fmaxf(m, __shfl_xor(m, 16, 64));
+  m = fmaxf(m, __shfl_xor(m, 32, 64));
   float l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int sp = 0; sp < MOST; ++sp) {
+  for (int j = 0; j < PER; ++j) {
     // in two steps: V's scales, which the references carry, may be far apart
-    const bool in = sp < static_cast<int>(a.splits) && x[sp].y != 0.0f;
-    const float w = in ? __builtin_amdgcn_exp2f(0.5f * (x[sp].x - m)) : 0.0f;
-    l += x[sp].y * w * w;
-    o += y[sp] * w * w;
+    const float w = x[j].y != 0.0f ? __builtin_amdgcn_exp2f(0.5f * (x[j].x - m)) : 0.0f;
+    l += x[j].y * w * w;
+    o += y[j] * w * w;
   }
-  if (l == 0.0f)
-    o = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-  else
-    o = f32x4{o[0] / l * up, o[1] / l * up, o[2] / l * up, o[3] / l * up};
-  *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * c) = o;
+#pragma unroll
+  for (int w = 16; w <= 32; w <<= 1) {
+    l += __shfl_xor(l, w, 64);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += __shfl_xor(o[e], w, 64);
+  }
+  if (g == 0)
+    *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + 4 * c) =
+        quotient(o, l) * up;
 }
 
 int check_i32(const vk_runtime* rt, const vk_tensor* t, size_t len, const char* what) {
@@ -892,21 +1148,13 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const auto* Q = static_cast<const float*>(q->ptr);
   auto* O = static_cast<float*>(out->ptr);
   const size_t blocks = (limit + KB - 1) / KB;
-  const size_t tile_rows = 128, tiles = (a.group * n + tile_rows - 1) / tile_rows;
-  const bool few = a.group * n <= 4;
+  const size_t pairs = cache->sequences * cache->heads;
   const size_t cus = rt->cu_count > 0 ? rt->cu_count : 256;
-  const size_t units = few ? rows : cache->sequences * cache->heads * tiles;
-  size_t splits = 1;
-  if (few) {
-    while (splits < 64 && rows * splits < 4 * cus && blocks / (2 * splits) >= 2 * kRowWaves)
-      splits *= 2;
-  } else {
-    splits = 3 * cus / units;
-    splits = splits > 16 ? 16 : splits;
-    splits = splits > blocks / 4 ? blocks / 4 : splits;
-    splits = splits < 1 ? 1 : splits;
-  }
-  VK_UNSUPPORTED_IF(units * splits > 0x7fffffffULL, "attention_cached: %zu queries", rows);
+  const vk::CachedPlan plan = vk::cached_plan(cus, pairs, a.group * n, rows, blocks);
+  const size_t tiles = (a.group * n + vk::kTileRows - 1) / vk::kTileRows;
+  const size_t units = plan.form == vk::kTile ? pairs * tiles : pairs;
+  const size_t splits = plan.splits;
+  VK_UNSUPPORTED_IF(units * splits > 0x7ffffff0ULL, "attention_cached: %zu queries", rows);
   a.splits = static_cast<uint32_t>(splits);
   a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
@@ -915,44 +1163,50 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
     part = rt->work;
   }
   // 8 / share groups of `heads` pairs each
-  const size_t pairs = cache->sequences * cache->heads;
   const uint32_t groups = pairs % 8 == 0 ? 8 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
   a.order.share = 8 / groups;
   a.order.heads = static_cast<uint32_t>(pairs / groups);
   const size_t slots = (a.order.heads * tiles * splits + a.order.share - 1) / a.order.share;
-  const dim3 grid(static_cast<unsigned>(few ? units * splits : 8 * slots));
+  const dim3 grid(static_cast<unsigned>(plan.form == vk::kTile ? 8 * slots : units * splits));
   const bool q8 = cache->format == VK_CACHE_Q8;
-  if (few) {
+  const bool score = ru.cap > 0.0f || ru.slopes, mask = ru.causal || ru.q_docs;
+#define VK_FORM(F, S, M)                                                                       \
+  if (plan.form == vk::kFew)                                                                            \
+    hipLaunchKernelGGL((attention_few_kernel<F, S, M>), grid, dim3(64 * kFewWaves), 0,         \
+                       rt->stream, Q, O, part, a);                                             \
+  else                                                                                         \
+    hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 4>), grid, dim3(256), 0, rt->stream, Q, \
+                       O, part, a)
+#define VK_RULES(F)                                             \
+  if (score && mask) { VK_FORM(F, true, true); }                \
+  else if (score) { VK_FORM(F, true, false); }                  \
+  else if (mask) { VK_FORM(F, false, true); }                   \
+  else { VK_FORM(F, false, false); }
+  if (plan.form == vk::kRow) {
     if (q8)
       hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_Q8>, grid, dim3(64 * kRowWaves), 0,
                          rt->stream, Q, O, part, a);
     else
       hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_F8>, grid, dim3(64 * kRowWaves), 0,
                          rt->stream, Q, O, part, a);
+  } else if (q8) {
+    VK_RULES(VK_CACHE_Q8)
   } else {
-    const bool score = ru.cap > 0.0f || ru.slopes, mask = ru.causal || ru.q_docs;
-#define VK_TILE(F, S, M)                                                                          \
-  hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 4>), grid, dim3(256), 0, rt->stream, Q, O, \
-                     part, a)
-#define VK_TILE_F(F)                        \
-  if (score && mask) VK_TILE(F, true, true); \
-  else if (score) VK_TILE(F, true, false);   \
-  else if (mask) VK_TILE(F, false, true);    \
-  else VK_TILE(F, false, false)
-    if (q8) { VK_TILE_F(VK_CACHE_Q8); } else { VK_TILE_F(VK_CACHE_F8); }
-#undef VK_TILE_F
-#undef VK_TILE
+    VK_RULES(VK_CACHE_F8)
   }
+#undef VK_RULES
+#undef VK_FORM
   VK_TRY(vk::check_launch("attention_cached"));
   if (splits == 1) return VK_OK;
-  const dim3 jgrid(static_cast<unsigned>((rows * 16 + 255) / 256));
+  const dim3 jgrid(static_cast<unsigned>((rows + 3) / 4));
 #define VK_JOIN(N)                                                                          \
   hipLaunchKernelGGL(attention_join_kernel<N>, jgrid, dim3(256), 0, rt->stream, part, O, up, a)
-  const float up = few ? 0x1p24f : 1.0f;
-  if (splits <= 4) VK_JOIN(4);
-  else if (splits <= 8) VK_JOIN(8);
-  else if (splits <= 16) VK_JOIN(16);
-  else VK_JOIN(64);
+  const float up = plan.form == vk::kRow ? kRowUp : 1.0f;
+  if (splits <= 4) VK_JOIN(1);
+  else if (splits <= 8) VK_JOIN(2);
+  else if (splits <= 16) VK_JOIN(4);
+  else if (splits <= 32) VK_JOIN(8);
+  else VK_JOIN(16);
 #undef VK_JOIN
   return vk::check_launch("attention_join_kernel");
 }

@@ -460,6 +460,13 @@ __device__ __forceinline__ void st_stream(float4* p, float4 v) {
 // then not held up behind a backlog of the wave's writes).
 __device__ __forceinline__ void wait_memory() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+// Orders a wave's LDS accesses before it against those after it, where a wave exchanges
+// values through LDS of its own (its lanes are in step: no barrier).
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 __device__ __forceinline__ float f16_to_f32(uint16_t h) {
   return static_cast<float>(__builtin_bit_cast(_Float16, h));
 }

@@ -209,4 +209,57 @@ inline AttentionPlan attention_plan(int cus, size_t sequences, size_t n, int pro
   return best;
 }
 
+// ---------------------------------------------------------------------------
+// Attention over the 8-bit cache (attention_cached.hip)
+// ---------------------------------------------------------------------------
+// Which kernel a call takes, and over how many workgroups the keys of a query are
+// shared out (each writes its part of 66 floats a query, and a second pass joins them).
+// `pairs`: sequences x cache heads, `queries` of each, `rows` in all, `blocks` of 64 keys.
+enum CachedForm { kRow, kFew, kTile };
+constexpr int kTileRows = 128;
+struct CachedPlan {
+  CachedForm form;
+  int splits;
+};
+
+// kRow (one query a pair, a lane a key): a workgroup a CU, four blocks of keys at
+// least; up to 24 blocks (three a wave) one workgroup and no join: 12 x 866 keys 7.6 us
+// unsplit, 8.5 in 16; 12 x 5,000 18.2 and 9.3; 16 x 124,704 348 and 46.
+// kFew (up to 32 queries a pair, a wave a block): a workgroup a CU, six blocks at least; two
+// a CU where each still has 16 blocks: 12 x 10,392 keys and 32 queries 80 us unsplit, 20 in
+// 8, 15 in 16, 20 in 64; 4 x 30,000 231, 36, 22, 13.
+// kTile (128 queries a workgroup, a block a step for all): a step takes 1.5 us with one
+// workgroup on the CU and 1.3 of the CU's time with two or three; a split adds its parts'
+// traffic and the join: 12 x 866 over 10,392 keys 236 us unsplit, 90 in 3, 79 in 6 and in 9.
+// One query: against the second kernel 16 x 124,704 46 us (64), 12 x 866 7.6 (9.2).
+inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t rows,
+                              size_t blocks) {
+  const auto between = [](size_t v, size_t most) { return v < 1 ? size_t{1} : v > most ? most : v; };
+  if (queries == 1) {
+    if (blocks <= 24) return CachedPlan{kRow, 1};
+    const size_t per = cus / pairs < blocks / 4 ? cus / pairs : blocks / 4;
+    return CachedPlan{kRow, static_cast<int>(between(per, 64))};
+  }
+  if (queries <= 32) {
+    size_t sp = cus / pairs;
+    if (2 * sp * 16 <= blocks) sp *= 2;
+    if (sp > blocks / 6) sp = blocks / 6;
+    return CachedPlan{kFew, static_cast<int>(between(sp, 64))};
+  }
+  const size_t tiles = pairs * ((queries + kTileRows - 1) / kTileRows);
+  int best = 1;
+  double best_us = 0.0;
+  for (int sp = 1; sp <= 64 && (sp == 1 || static_cast<size_t>(4 * sp) <= blocks); ++sp) {
+    const double load = static_cast<double>((tiles * sp + cus - 1) / cus);
+    const double steps = static_cast<double>((blocks + sp - 1) / sp);
+    double us = steps * (load > 1.0 ? 1.3 * load : 1.5);
+    if (sp > 1) us += 4.0 + 2.0 * 264.0 * sp * static_cast<double>(rows) / 4.5e6;
+    if (best_us == 0.0 || us < best_us) {
+      best = sp;
+      best_us = us;
+    }
+  }
+  return CachedPlan{kTile, best};
+}
+
 }  // namespace vk

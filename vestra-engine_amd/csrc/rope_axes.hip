@@ -50,11 +50,6 @@ __device__ __forceinline__ float row_inv(float q, float eps) {
   return SEQ ? 1.0f / sqrtf(var + eps) : __builtin_amdgcn_rsqf(var + eps);
 }
 
-__device__ __forceinline__ void wave_lds_fence() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
-
 // A row's 64 values left to right, from LDS.
 __device__ __forceinline__ float row_chain(const float* r) {
   float s = 0.0f;
@@ -142,9 +137,9 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
       if constexpr (SEQ) {
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
-        wave_lds_fence();
+        vkd::wave_lds_fence();
         float st = l < kHeads ? row_chain(mine + l * kPitch) / 64.0f : 0.0f;
-        wave_lds_fence();
+        vkd::wave_lds_fence();
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) {
           mean[j] = __shfl(st, j, 16);
@@ -155,9 +150,9 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
           d.w = v[j].w - mean[j]; d.w = d.w * d.w;
           *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = d;
         }
-        wave_lds_fence();
+        vkd::wave_lds_fence();
         st = l < kHeads ? row_inv<true>(row_chain(mine + l * kPitch), eps) : 0.0f;
-        wave_lds_fence();
+        vkd::wave_lds_fence();
 #pragma unroll
         for (int j = 0; j < kHeads; ++j) inv[j] = __shfl(st, j, 16);
       } else {
@@ -186,7 +181,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
     }
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
-    wave_lds_fence();
+    vkd::wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < kHeads; ++j) {
       const float* r = mine + j * kPitch;
@@ -197,7 +192,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
       o.w = v[j].w * c[3] + r[partner[3]] * sn[3];
       v[j] = o;
     }
-    wave_lds_fence();
+    vkd::wave_lds_fence();
 #pragma unroll
     for (int j = 0; j < kHeads; ++j)
       if (live && h + j < h1)

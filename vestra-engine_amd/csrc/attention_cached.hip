@@ -643,9 +643,16 @@ __device__ __forceinline__ int list_blocks(uint16_t* list, int* count, const Sha
       if (any && ru.q_docs) {
         int lo = 0x7fffffff, hi = -0x7fffffff - 1;
         const int* d = ru.k_docs + doc_first + k0;
-        for (int j = 0; j <= k1 - k0; ++j) {
-          lo = min(lo, d[j]);
-          hi = max(hi, d[j]);
+        const int last = k1 - k0;
+        for (int j = 0; j <= last; j += 16) {  // sixteen loads in flight
+          int x[16];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) x[y] = d[min(j + y, last)];
+#pragma unroll
+          for (int y = 0; y < 16; ++y) {
+            lo = min(lo, x[y]);
+            hi = max(hi, x[y]);
+          }
         }
         if (ru.docs_ordered) {
           any = lo <= p.q_high;

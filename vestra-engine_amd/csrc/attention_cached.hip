@@ -244,6 +244,7 @@ constexpr int kVPitch = 192;    // of a V row: 64 f16 + 64
 constexpr float kPBits = 9.0f, kSlack = 6.0f;
 constexpr float kLowest = -3e38f;       // the running reference before any key
 constexpr float kLeastLsv = -88.0f;     // of a key's V in the choice of the reference
+constexpr int kCap = 1, kBias = 2;      // what SCORE does to a product beside its scale
 constexpr int kQUp = 10;                // binary digits that Q is scaled up by
 
 // Lane R of each 16-lane row, to all of the row.
@@ -351,18 +352,23 @@ __device__ __forceinline__ int key_slot(int key) {
   return (key & 32) | (key & 4) << 2 | (key & 24) >> 1 | (key & 3);
 }
 
-// tanh to a few units of the last place: the odd series to x^11 below 0.35, (e - 1) / (e + 1)
-// as 1 - 2 / (e + 1) from there.
-__device__ __forceinline__ float tanh1(float x) {
+// tanh to a few units of the last place: the odd series to x^11 below kTanhSeries, (e - 1) /
+// (e + 1) as 1 - 2 / (e + 1) from there.
+constexpr float kTanhSeries = 0.35f;
+
+__device__ __forceinline__ float tanh_series(float x) {
   const float y = x * x;
   float p = __builtin_fmaf(y, -0.008863236f, 0.021869488f);
   p = __builtin_fmaf(y, p, -0.053968254f);
   p = __builtin_fmaf(y, p, 0.13333334f);
   p = __builtin_fmaf(y, p, -0.33333334f);
-  p = __builtin_fmaf(x * y, p, x);
+  return __builtin_fmaf(x * y, p, x);
+}
+
+__device__ __forceinline__ float tanh1(float x) {
   const float e = __builtin_amdgcn_exp2f(x * 2.8853900817779268f);
   const float b = __builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(e + 1.0f), 1.0f);
-  return fabsf(x) < 0.35f ? p : b;
+  return fabsf(x) < kTanhSeries ? tanh_series(x) : b;
 }
 
 // A wave's 32 queries: lane l and lane l ^ 32 hold query l % 32.
@@ -453,7 +459,7 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 // not see some of them.  Moves the reference of queries whose weights would leave
 // f16's upper end: it follows the largest of score + log2 of V's scale, the size of a key's
 // part of the value sum, once that passes it by kSlack.
-template <bool SCORE, bool MASK>
+template <int SCORE, bool MASK>
 __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Rules& ru,
                                             const KeyRegs& key, int k0, int left, bool masked) {
   const int half = (threadIdx.x & 63) >> 5;
@@ -466,23 +472,37 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[t][r] *= back;
   }
-  if constexpr (SCORE) {
-    if (ru.cap > 0.0f) {
+  if constexpr (SCORE != 0) __builtin_amdgcn_sched_barrier(0);
+  if constexpr ((SCORE & kCap) != 0) {
+    // scores far below the cap, the usual case, are the series' alone (3 x 16 x 1,301 queries
+    // over up to 2,600 keys: 110 us, 138 where they are not; both for every score 131)
+    float top = 0.0f;
 #pragma unroll
-      for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < 2; ++t)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[t][r] = tanh1(s[t][r]) * w.cap_up;
-    }
-    if (ru.slopes) {
-      const float base = static_cast<float>(static_cast<long long>(w.pos) - (k0 + 4 * half));
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[t][r] =
-              __builtin_fmaf(-w.slope, fabsf(base - (32 * t + 8 * (r / 4) + r % 4)), s[t][r]);
+      for (int r = 0; r < 16; ++r) top = fmaxf(top, fabsf(s[t][r]));
+    if (__builtin_amdgcn_ballot_w64(top >= kTanhSeries) == 0) {
+      each<32>([&](auto i) {
+        s[i / 16][i % 16] = tanh_series(s[i / 16][i % 16]) * w.cap_up;
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four at a time: registers
+      });
+    } else {
+      each<32>([&](auto i) {
+        s[i / 16][i % 16] = tanh1(s[i / 16][i % 16]) * w.cap_up;
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      });
     }
   }
+  if constexpr ((SCORE & kBias) != 0) {
+    const float base = static_cast<float>(static_cast<long long>(w.pos) - (k0 + 4 * half));
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (32 * t + 8 * (r / 4) + r % 4)), s[t][r]);
+  }
+  // nothing of the rules' work is begun ahead of it, in registers that the tile has not
+  if constexpr (SCORE != 0) __builtin_amdgcn_sched_barrier(0);
   const bool causal = MASK && masked && ru.causal;
   if (__builtin_expect(left < KB || causal, 0)) {
     int lim = left;
@@ -563,7 +583,7 @@ __device__ __forceinline__ void value_block(const f32x16 (&s)[2], Queries& w, co
 }
 
 // The queries of a wave: row `row` of cache head kh's, whose query heads lie side by side.
-template <bool SCORE, bool MASK, int DK, int DH>
+template <int SCORE, bool MASK, int DK, int DH>
 __device__ __forceinline__ void take_queries(Queries& w, const float* __restrict__ q, const Shape& a,
                                              uint32_t s, uint32_t kh, uint32_t row, uint32_t* i,
                                              uint32_t* h) {
@@ -574,18 +594,28 @@ __device__ __forceinline__ void take_queries(Queries& w, const float* __restrict
                        ru.cap > 0.0f ? ru.scale / ru.cap : ru.scale * kLog2e,
                        (threadIdx.x & 63) >> 5);
   w.cap_up = ru.cap * kLog2e;
-  w.slope = SCORE && ru.slopes ? ru.slopes[*h] * kLog2e : 0.0f;
+  w.slope = (SCORE & kBias) != 0 ? ru.slopes[*h] * kLog2e : 0.0f;
   w.pos = position(vkc::start_of(a.rows, s), *i);
   const int pre = MASK && ru.prefix ? ru.prefix[s] : 0;
   w.seen = max(max(w.pos + 1, pre), 0);
   w.doc = MASK && ru.q_docs ? ru.q_docs[static_cast<size_t>(s) * a.rows.n + *i] : 0;
 }
 
-// What a tile's queries may see, as a whole.
+// What a tile's queries may see, as a whole, and a wave's of them.
 struct Span {
   int p_low, p_high, pre;  // positions and prefix
   int q_low, q_high;       // documents
+  int w_high, w_doc_low, w_doc_high;  // the wave's last position, its documents
 };
+
+// Whether some query of the wave may see a key of the block of keys k0 ..
+__device__ __forceinline__ bool wave_sees(const Span& p, const Rules& ru, const KeyData& kd,
+                                          int k0) {
+  if (ru.causal && k0 > p.w_high && k0 >= p.pre) return false;
+  if (!ru.q_docs) return true;
+  const int d = kd.doc[threadIdx.x & 63];
+  return __builtin_amdgcn_ballot_w64(d <= p.w_doc_high && (ru.docs_ordered || d >= p.w_doc_low)) != 0;
+}
 
 // Of rows row_first .. row_last of a workgroup of WAVES waves; `range` is LDS.
 template <int WAVES>
@@ -594,7 +624,8 @@ __device__ __forceinline__ Span tile_span(const Queries& w, const Shape& a, uint
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int start = vkc::start_of(a.rows, s);
   Span p{position(start, row_first / a.group), position(start, row_last / a.group),
-         a.rules.prefix ? a.rules.prefix[s] : 0, 0, 0};
+         a.rules.prefix ? a.rules.prefix[s] : 0, 0, 0, 0, 0, 0};
+  p.w_high = position(start, min(row_first + 32 * wave + 31, row_last) / a.group);
   if (a.rules.q_docs) {
     int lo = w.doc, hi = w.doc;
 #pragma unroll
@@ -602,6 +633,8 @@ __device__ __forceinline__ Span tile_span(const Queries& w, const Shape& a, uint
       lo = min(lo, __shfl_xor(lo, m, 64));
       hi = max(hi, __shfl_xor(hi, m, 64));
     }
+    p.w_doc_low = __builtin_amdgcn_readfirstlane(lo);
+    p.w_doc_high = __builtin_amdgcn_readfirstlane(hi);
     if (lane == 0) {
       range[wave] = live ? lo : 0x7fffffff;
       range[WAVES + wave] = live ? hi : -0x7fffffff - 1;
@@ -620,51 +653,74 @@ __device__ __forceinline__ Span tile_span(const Queries& w, const Shape& a, uint
 
 constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
 
+// Smallest and largest of a 16-lane row.
+__device__ __forceinline__ void row16_range(int* lo, int* hi) {
+#define VK_ROR(n)                                                              \
+  *lo = min(*lo, __builtin_amdgcn_mov_dpp(*lo, 0x120 | n, 0xf, 0xf, true));    \
+  *hi = max(*hi, __builtin_amdgcn_mov_dpp(*hi, 0x120 | n, 0xf, 0xf, true));
+  VK_ROR(8) VK_ROR(4) VK_ROR(2) VK_ROR(1)
+#undef VK_ROR
+}
+
 // Lists the blocks of seg .. seg_end - 1 that some query of the tile may see, in order: the
-// block less seg, times two, plus one where not every query sees all of it.  A thread takes a
-// block; `count` is LDS.
+// block less seg, times two, plus one where not every query sees all of it.  First the documents'
+// part, 16 lanes a block and 16 blocks a wave in flight (1,000 workgroups over 163 blocks,
+// with the attention: a thread a block 157 us, so 131), as 2 (some) + 1 (not all) in the block's
+// place; then a thread a block takes the order in and closes the gaps.  `count` is LDS.
 template <int WAVES>
 __device__ __forceinline__ int list_blocks(uint16_t* list, int* count, const Shape& a,
                                            const Span& p, int seg, int seg_end, int keys,
                                            size_t doc_first) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Rules& ru = a.rules;
+  if (ru.causal) {  // blocks with a key that is not behind every query
+    const int top = max(max(p.p_high + 1, p.pre), 0);
+    seg_end = min(seg_end, top / KB + (top % KB != 0));
+  }
+  if (ru.q_docs) {
+    const int* d = ru.k_docs + doc_first;
+    for (int base = seg; base < seg_end; base += 16 * WAVES) {
+      int x[4][4];
+#pragma unroll
+      for (int y = 0; y < 4; ++y)
+#pragma unroll
+        for (int z = 0; z < 4; ++z) {
+          const int b = base + 4 * WAVES * y + 4 * wave + (lane >> 4);
+          x[y][z] = d[min(b * KB + 16 * z + (lane & 15), keys - 1)];
+        }
+#pragma unroll
+      for (int y = 0; y < 4; ++y) {
+        const int b = base + 4 * WAVES * y + 4 * wave + (lane >> 4);
+        int lo = min(min(x[y][0], x[y][1]), min(x[y][2], x[y][3]));
+        int hi = max(max(x[y][0], x[y][1]), max(x[y][2], x[y][3]));
+        row16_range(&lo, &hi);
+        const bool any = lo <= p.q_high && (ru.docs_ordered || hi >= p.q_low);
+        const bool full = ru.docs_ordered
+                              ? hi <= p.q_low
+                              : lo == hi && p.q_low == p.q_high && lo == p.q_low;
+        if ((lane & 15) == 0 && b < seg_end)
+          list[b - seg] = static_cast<uint16_t>((any ? 2 : 0) | (full ? 0 : 1));
+      }
+    }
+    __syncthreads();
+  }
   int filled = 0;
   for (int b0 = seg; b0 < seg_end; b0 += 64 * WAVES) {
     const int b = b0 + static_cast<int>(threadIdx.x);
     bool any = b < seg_end, full = true;
     if (any) {
-      const int k0 = b * KB;
-      const int k1 = keys - k0 < KB ? keys - 1 : k0 + KB - 1;  // last key
       if (ru.causal) {
-        any = k0 <= p.p_high || k0 < p.pre;
+        const int k1 = min(b * KB + KB, keys) - 1;  // last key
         full = k1 <= p.p_low || k1 < p.pre;
       }
-      if (any && ru.q_docs) {
-        int lo = 0x7fffffff, hi = -0x7fffffff - 1;
-        const int* d = ru.k_docs + doc_first + k0;
-        const int last = k1 - k0;
-        for (int j = 0; j <= last; j += 16) {  // sixteen loads in flight
-          int x[16];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) x[y] = d[min(j + y, last)];
-#pragma unroll
-          for (int y = 0; y < 16; ++y) {
-            lo = min(lo, x[y]);
-            hi = max(hi, x[y]);
-          }
-        }
-        if (ru.docs_ordered) {
-          any = lo <= p.q_high;
-          full = full && hi <= p.q_low;
-        } else {
-          any = lo <= p.q_high && hi >= p.q_low;
-          full = full && lo == hi && p.q_low == p.q_high && lo == p.q_low;
-        }
+      if (ru.q_docs) {
+        const int x = list[b - seg];
+        any = (x & 2) != 0;
+        full = full && (x & 1) == 0;
       }
     }
     const uint64_t m = __builtin_amdgcn_ballot_w64(any);
-    __syncthreads();  // the counts of the run before are read
+    __syncthreads();  // the counts of the run before are read, and the marks of this one
     if (lane == 0) count[wave] = __popcll(m);
     __syncthreads();
     int at = filled;
@@ -760,8 +816,10 @@ struct StageKeys {
   }
 };
 
-template <int FORMAT, bool SCORE, bool MASK, int QW>
-__global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float* __restrict__ q,
+// Three workgroups a CU; two with a cap, whose work a score wants the registers (in 168 of
+// them it spills: 122 us for 110).
+template <int FORMAT, int SCORE, bool MASK, int QW>
+__global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_kernel(const float* __restrict__ q,
                                                                     float* __restrict__ out,
                                                                     float* __restrict__ part,
                                                                     Shape a) {
@@ -831,7 +889,7 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
       rows_v.load(a.cache.v, first, key_of(e1), keys);
       if (wave == 0) keys_d.load(a, first, doc_first, key_of(e1), keys);
       __builtin_amdgcn_sched_barrier(0);
-      if (live) {
+      if (live && !(MASK && (e & 1) && !wave_sees(span, ru, kd[buf], k0))) {
         f32x16 sc[2];
         clear(sc);
 #pragma unroll
@@ -871,7 +929,7 @@ __global__ __launch_bounds__(64 * QW, 3) void attention_tile_kernel(const float*
 // barrier until the waves are joined at the end.
 constexpr int kFewWaves = 4;
 
-template <int FORMAT, bool SCORE, bool MASK>
+template <int FORMAT, int SCORE, bool MASK>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
     const float* __restrict__ q, float* __restrict__ out, float* __restrict__ part, Shape a) {
   __shared__ __align__(16) char vl[kFewWaves][KB * kVPitch];
@@ -1176,19 +1234,22 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const size_t slots = (a.order.heads * tiles * splits + a.order.share - 1) / a.order.share;
   const dim3 grid(static_cast<unsigned>(plan.form == vk::kTile ? 8 * slots : units * splits));
   const bool q8 = cache->format == VK_CACHE_Q8;
-  const bool score = ru.cap > 0.0f || ru.slopes, mask = ru.causal || ru.q_docs;
+  const int score = (ru.cap > 0.0f ? kCap : 0) | (ru.slopes ? kBias : 0);
+  const bool mask = ru.causal || ru.q_docs;
 #define VK_FORM(F, S, M)                                                                       \
-  if (plan.form == vk::kFew)                                                                            \
+  if (plan.form == vk::kFew)                                                                   \
     hipLaunchKernelGGL((attention_few_kernel<F, S, M>), grid, dim3(64 * kFewWaves), 0,         \
                        rt->stream, Q, O, part, a);                                             \
   else                                                                                         \
     hipLaunchKernelGGL((attention_tile_kernel<F, S, M, 4>), grid, dim3(256), 0, rt->stream, Q, \
                        O, part, a)
-#define VK_RULES(F)                                             \
-  if (score && mask) { VK_FORM(F, true, true); }                \
-  else if (score) { VK_FORM(F, true, false); }                  \
-  else if (mask) { VK_FORM(F, false, true); }                   \
-  else { VK_FORM(F, false, false); }
+#define VK_RULE(F, S)                      \
+  case S:                                  \
+    if (mask) { VK_FORM(F, S, true); }     \
+    else { VK_FORM(F, S, false); }         \
+    break;
+#define VK_RULES(F) \
+  switch (score) { VK_RULE(F, 0) VK_RULE(F, kCap) VK_RULE(F, kBias) VK_RULE(F, (kCap | kBias)) }
   if (plan.form == vk::kRow) {
     if (q8)
       hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_Q8>, grid, dim3(64 * kRowWaves), 0,
@@ -1202,6 +1263,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
     VK_RULES(VK_CACHE_F8)
   }
 #undef VK_RULES
+#undef VK_RULE
 #undef VK_FORM
   VK_TRY(vk::check_launch("attention_cached"));
   if (splits == 1) return VK_OK;

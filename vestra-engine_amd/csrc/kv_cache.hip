@@ -153,7 +153,7 @@ int check_cache(const vk_runtime* rt, const vk_kv_cache* c) {
   VK_REQUIRE(c->format == VK_CACHE_Q8 || c->format == VK_CACHE_F8, "kv_cache: unknown format %d",
              c->format);
   VK_REQUIRE(c->heads > 0, "kv_cache: no heads");
-  VK_UNSUPPORTED_IF(c->capacity > 0x7fffff00ULL || c->sequences > 0xffffff || c->heads > 0xffff,
+  VK_UNSUPPORTED_IF(c->capacity > 0x7fff0000ULL || c->sequences > 0xffffff || c->heads > 0xffff,
                     "kv_cache: %zu sequences of %zu heads and %zu slots", c->sequences, c->heads,
                     c->capacity);
   VK_UNSUPPORTED_IF(c->capacity > 0 && c->sequences * c->heads > (size_t{1} << 48) / c->capacity,

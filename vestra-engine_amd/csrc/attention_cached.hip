@@ -36,6 +36,7 @@ struct Shape {
   uint32_t heads, group;  // query heads, and how many of them share a cache head
   uint32_t limit;         // keys at or past it are not seen (capacity, max_length)
   uint32_t splits, tiles;
+  uint32_t parts;         // workgroups a tile and split: 2 with documents apart (document_part)
   struct {
     uint32_t share, heads;
   } order;
@@ -651,6 +652,34 @@ __device__ __forceinline__ Span tile_span(const Queries& w, const Shape& a, uint
   return p;
 }
 
+// A tile across the border of two documents would take the blocks of both, one after the
+// other, for half of its queries each (10,392 queries over documents of 866, most tiles in one
+// of them: 143 us, so 100).  It has two workgroups, and where its first rows have a document that
+// no later row has, the first takes those and the second the rest; else the second has nothing
+// (documents of 8 x 128: 89 us, so 91).  Ordered documents hold the earlier ones' keys too and
+// gain nothing (407 us, 480 so).  Row bounds in, and out; false: no row.
+__device__ __forceinline__ bool document_part(const Shape& a, uint32_t s, uint32_t part, int* row0,
+                                              int* row_end) {
+  static_assert(vk::kTileRows == 128, "two rows a lane");
+  const int lane = threadIdx.x & 63, rows = *row_end - *row0;
+  const int* docs = a.rules.q_docs + static_cast<size_t>(s) * a.rows.n;
+  const auto doc_of = [&](int i) {
+    return docs[static_cast<uint32_t>(*row0 + min(i, rows - 1)) / a.group];
+  };
+  const int d0 = doc_of(0), x = doc_of(lane), y = doc_of(64 + lane);
+  const uint64_t e0 = __builtin_amdgcn_ballot_w64(x == d0 && lane < rows);
+  const uint64_t e1 = __builtin_amdgcn_ballot_w64(y == d0 && lane + 64 < rows);
+  const int same = __popcll(e0) + __popcll(e1);
+  // the same rows are the first ones
+  const bool first = ~e0 ? __builtin_ctzll(~e0) == same : !~e1 || 64 + __builtin_ctzll(~e1) == same;
+  if (!first || same == rows) return part == 0;
+  if (part == 0)
+    *row_end = *row0 + same;
+  else
+    *row0 += same;
+  return true;
+}
+
 constexpr int kList = 2048;  // blocks whose visibility is worked out at a time
 
 // Smallest and largest of a 16-lane row.
@@ -839,28 +868,32 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
   // in a group the last tiles come first: with a causal mask they take longest.
   const uint32_t xcd = blockIdx.x & 7;
   const uint32_t in = (blockIdx.x >> 3) * a.order.share + xcd % a.order.share;
-  if (in >= a.order.heads * a.splits * a.tiles) return;
+  if (in >= a.order.heads * a.splits * a.tiles * a.parts) return;
   const uint32_t pair = in % a.order.heads, u = in / a.order.heads;
-  const uint32_t split = u % a.splits, tile = a.tiles - 1 - u / a.splits;
+  const uint32_t split = u % a.splits, v = u / a.splits;
+  // (the second parts first: most of them end at once)
+  const uint32_t tile = a.tiles - 1 - v % a.tiles, piece = a.parts - 1 - v / a.tiles;
   const uint32_t sh = xcd / a.order.share * a.order.heads + pair;
   const uint32_t kh = sh % a.cache.heads, s = sh / a.cache.heads;
   const int count = vkc::count_of(a.rows, s);
   const int rows = count > 0 ? count * static_cast<int>(a.group) : 0;  // query i's heads side by side
-  const int row0 = static_cast<int>(tile) * kRows;
+  int row0 = static_cast<int>(tile) * kRows;
   if (row0 >= rows) return;
+  int row_end = row0 + kRows < rows ? row0 + kRows : rows;
+  if (MASK && a.parts > 1 && !document_part(a, s, piece, &row0, &row_end)) return;
   const int keys = keys_of(a, s);
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + kh) * a.cache.capacity;
   const size_t doc_first = static_cast<size_t>(s) * a.cache.capacity;
-  const bool live = row0 + 32 * wave < rows;  // uniform over the wave
+  const bool live = row0 + 32 * wave < row_end;  // uniform over the wave
   const int row = row0 + 32 * wave + (lane & 31);
   uint32_t i, h;
   Queries w;
-  take_queries<SCORE, MASK, 16, 8>(w, q, a, s, kh, row < rows ? row : rows - 1, &i, &h);
+  take_queries<SCORE, MASK, 16, 8>(w, q, a, s, kh, row < row_end ? row : row_end - 1, &i, &h);
 
   const int blocks = (keys + KB - 1) / KB;
   Span span;
   if constexpr (MASK)
-    span = tile_span<QW>(w, a, s, row0, row0 + kRows < rows ? row0 + kRows - 1 : rows - 1, live, doc_range);
+    span = tile_span<QW>(w, a, s, row0, row_end - 1, live, doc_range);
   StageRows<FORMAT, kThreads> rows_k, rows_v;
   StageKeys keys_d;
   // blocks listed (MASK) or all of them, a run of kList at a time
@@ -907,7 +940,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
   }
   const int half = lane >> 5;
   const float l = w.l + other_half(w.l);
-  if (!live || row >= rows) return;
+  if (!live || row >= row_end) return;
 #pragma unroll
   for (int dt = 0; dt < 2; ++dt)
 #pragma unroll
@@ -1219,7 +1252,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const size_t tiles = (a.group * n + vk::kTileRows - 1) / vk::kTileRows;
   const size_t units = plan.form == vk::kTile ? pairs * tiles : pairs;
   const size_t splits = plan.splits;
-  VK_UNSUPPORTED_IF(units * splits > 0x7ffffff0ULL, "attention_cached: %zu queries", rows);
+  VK_UNSUPPORTED_IF(2 * units * splits > 0x7ffffff0ULL, "attention_cached: %zu queries", rows);
   a.splits = static_cast<uint32_t>(splits);
   a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
@@ -1231,7 +1264,9 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const uint32_t groups = pairs % 8 == 0 ? 8 : pairs % 4 == 0 ? 4 : pairs % 2 == 0 ? 2 : 1;
   a.order.share = 8 / groups;
   a.order.heads = static_cast<uint32_t>(pairs / groups);
-  const size_t slots = (a.order.heads * tiles * splits + a.order.share - 1) / a.order.share;
+  a.parts = a.rules.q_docs && !a.rules.docs_ordered ? 2 : 1;
+  const size_t slots =
+      (a.order.heads * tiles * splits * a.parts + a.order.share - 1) / a.order.share;
   const dim3 grid(static_cast<unsigned>(plan.form == vk::kTile ? 8 * slots : units * splits));
   const bool q8 = cache->format == VK_CACHE_Q8;
   const int score = (ru.cap > 0.0f ? kCap : 0) | (ru.slopes ? kBias : 0);

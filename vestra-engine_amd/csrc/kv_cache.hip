@@ -69,9 +69,10 @@ __device__ __forceinline__ bool place(const Split& sp, const vkc::Rows& r, const
   if (g >= sp.groups) return false;
   const uint32_t sh = vkd::fdiv(g, sp.by_n), i = g - sh * r.n;
   const uint32_t s = vkd::fdiv(sh, sp.by_heads), h = sh - s * c.heads;
-  if (static_cast<int>(i) >= vkc::count_of(r, s)) return false;
-  const long long at = static_cast<long long>(vkc::start_of(r, s)) + i;
-  if (at < 0 || at >= static_cast<long long>(c.capacity)) return false;
+  const int count = vkc::count_of(r, s), start = vkc::start_of(r, s);  // one wait for both
+  const long long at = static_cast<long long>(start) + i;
+  if (static_cast<int>(i) >= count || at < 0 || at >= static_cast<long long>(c.capacity))
+    return false;
   *f32_at = vkc::row_at(r, c.heads, s, h, i);
   *slot = (static_cast<size_t>(s) * c.heads + h) * c.capacity + static_cast<size_t>(at);
   return true;

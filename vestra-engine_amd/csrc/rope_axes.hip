@@ -23,10 +23,12 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroups = kThreads / 16;  // tokens of a workgroup
-constexpr int kHeads = 4;               // rows of a group in flight
+// Rows of a group in flight.  866 tokens of 24 heads: 4.1 us; 4.7 with four rows (half the
+// workgroups), 5.3 with one (a token's angles for one row).  10,392: 24.2, 24.7, 34.
+constexpr int kHeads = 2;
 constexpr int kPitch = 68;              // floats of a row in LDS
 
-struct AxesTable {
+struct alignas(16) AxesTable {
   double turns[64];     // f / (2 pi) of the element's pair
   uint8_t axis[64];     // its axis
   uint8_t partner[64];  // the pair's other element
@@ -64,15 +66,6 @@ __device__ __forceinline__ float row_chain(const float* r) {
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ double position(const void* p, size_t i) {
-  return static_cast<double>(static_cast<const T*>(p)[i]);
-}
-
-__device__ __forceinline__ float lane4(const float4& v, int i) {
-  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
-}
-
 template <typename PT, typename POS, bool NORM, bool SEQ>
 __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
     const float* q, const float* k, float* q_out, float* k_out, const PT* __restrict__ qg,
@@ -101,8 +94,19 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
     return h < sh.heads ? row(h, sh.heads) : row(h - sh.heads, sh.kv_heads);
   };
 
+  // the table's and the positions' loads first: the angles hang on both, one after the other
   float c[4], sn[4];
-  int partner[4];
+  const uint32_t axis4 = reinterpret_cast<const uint32_t*>(tab.axis)[l];
+  const uint32_t partner4 = reinterpret_cast<const uint32_t*>(tab.partner)[l];
+  const uint32_t second4 = reinterpret_cast<const uint32_t*>(tab.second)[l];
+  double f[4];
+  POS at_axis[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    f[e] = tab.turns[4 * l + e];
+    at_axis[e] = static_cast<const POS*>(pos)[static_cast<size_t>(t) * sh.axes +
+                                              (axis4 >> 8 * e & 0xff)];
+  }
   bool have = false;
   for (uint32_t h = h0; h < h1; h += kHeads) {
     float4 v[kHeads];
@@ -116,9 +120,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
       have = true;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int d = 4 * l + e;
-        const double turns =
-            position<POS>(pos, static_cast<size_t>(t) * sh.axes + tab.axis[d]) * tab.turns[d];
+        const double turns = static_cast<double>(at_axis[e]) * f[e];
         const double quarter = rint(4.0 * turns);
         const float r = static_cast<float>(turns - 0.25 * quarter);  // within 1/8
         float sr, cr;
@@ -128,8 +130,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
         if (quad == 1 || quad == 2) ca = -ca;
         if (quad >= 2) sa = -sa;
         c[e] = ca;
-        sn[e] = tab.second[d] ? sa : -sa;
-        partner[e] = tab.partner[d];
+        sn[e] = second4 >> 8 * e & 1 ? sa : -sa;
       }
     }
     if constexpr (NORM) {
@@ -186,10 +187,10 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
     for (int j = 0; j < kHeads; ++j) {
       const float* r = mine + j * kPitch;
       float4 o;
-      o.x = v[j].x * c[0] + r[partner[0]] * sn[0];
-      o.y = v[j].y * c[1] + r[partner[1]] * sn[1];
-      o.z = v[j].z * c[2] + r[partner[2]] * sn[2];
-      o.w = v[j].w * c[3] + r[partner[3]] * sn[3];
+      o.x = v[j].x * c[0] + r[partner4 >> 0 & 0xff] * sn[0];
+      o.y = v[j].y * c[1] + r[partner4 >> 8 & 0xff] * sn[1];
+      o.z = v[j].z * c[2] + r[partner4 >> 16 & 0xff] * sn[2];
+      o.w = v[j].w * c[3] + r[partner4 >> 24 & 0xff] * sn[3];
       v[j] = o;
     }
     vkd::wave_lds_fence();

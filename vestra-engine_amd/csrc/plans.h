@@ -231,6 +231,7 @@ struct CachedPlan {
 // kTile (128 queries a workgroup, a block a step for all): a step takes 1.5 us with one
 // workgroup on the CU and 1.3 of the CU's time with two or three; a split adds its parts'
 // traffic and the join: 12 x 866 over 10,392 keys 236 us unsplit, 90 in 3, 79 in 6 and in 9.
+// Twelve workgroups a CU are the most: past that the parts (then 104 MB) grow for little.
 // One query: against the second kernel 16 x 124,704 46 us (64), 12 x 866 7.6 (9.2).
 inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t rows,
                               size_t blocks) {
@@ -249,7 +250,8 @@ inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t r
   const size_t tiles = pairs * ((queries + kTileRows - 1) / kTileRows);
   int best = 1;
   double best_us = 0.0;
-  for (int sp = 1; sp <= 64 && (sp == 1 || static_cast<size_t>(4 * sp) <= blocks); ++sp) {
+  for (int sp = 1; sp <= 64 && (sp == 1 || (static_cast<size_t>(4 * sp) <= blocks &&
+                                            tiles * sp <= 12 * cus)); ++sp) {
     const double load = static_cast<double>((tiles * sp + cus - 1) / cus);
     const double steps = static_cast<double>((blocks + sp - 1) / sp);
     double us = steps * (load > 1.0 ? 1.3 * load : 1.5);

@@ -562,7 +562,8 @@ typedef struct vk_kv_cache {
  * f32, code = x / scale rounded to f32 and then to the nearest code (ties to
  * even).  A row whose scale would be below 2^-100 is held as zeros, scale 0; a
  * row with an infinity or a NaN gets the scale NaN and codes 0, and reads back
- * as NaN. */
+ * as NaN.  The scale is at most the one whose largest code reads back finite.
+ * No counterpart in the reference. */
 int vk_kv_cache_write_f32(vk_runtime* rt, const vk_kv_cache* cache,
                           const vk_tensor* k, const vk_tensor* v, size_t n,
                           const vk_tensor* starts, const vk_tensor* counts,
@@ -601,7 +602,12 @@ typedef struct vk_attention_rules {
  * counts[s] are left as they were.  A query that sees a key that reads back
  * as NaN gets NaN; keys that it does not see have no effect whatever they
  * hold.  Scores, weights and sums are held as in f32: the values of the cache
- * are exact in f16, queries and weights are taken as two f16 parts. */
+ * are exact in f16, queries and weights are taken as two f16 parts (a query's
+ * value to 2^-25 of its row's largest, a weight times V's scale to 2^-34 of
+ * the largest; one query: f32 throughout).  Positions past 2^31 - 2 count as
+ * 2^31 - 2.  The same call gives the same bits.  A large call splits its keys
+ * and keeps partial results in the runtime's work buffer (run it once before
+ * a capture, which cannot grow it).  No counterpart in the reference. */
 int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache,
                             const vk_tensor* q, size_t heads, size_t n,
                             const vk_tensor* starts, const vk_tensor* counts,

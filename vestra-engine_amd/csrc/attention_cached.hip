@@ -1,10 +1,29 @@
 // Attention over the 8-bit cache of K and V rows (kv_cache.h), with capped
 // scores, a bias by distance, and causal, prefix and document masks.
 //
-// attention_row_kernel: a query a workgroup.  A lane takes a key, its 64 values
-// and scores in F32, and keeps a softmax of its own (running maximum, sum and 64
-// sums of values) over the keys that it meets; the lanes are joined once, at the
-// end.
+// The mathematics.  A held value is code * scale, one scale a row, and both kinds of
+// code (int8, e4m3) are exact in f16.  So the products run over codes: score_j = K's
+// scale_j * (q . code_j), and out = sum_j (p_j * V's scale_j) code_j / sum_j p_j with
+// p_j = 2^(score_j - m) in base 2, m a reference that follows the row's largest score.  An
+// f32 factor (q; p times V's scale) is taken as two f16 parts of 11 bits each, so each of the
+// two products is two on the f16 matrix cores, summed in f32: twice the time of
+// one f16 product, where the f32 matrix cores take seven times that of one.
+//
+// Three kernels (plans.h says which, and over how many workgroups the keys are split), and one
+// that joins the splits:
+//   attention_row_kernel   one query: a lane a key, f32 on the vector units.  Bound by memory (16 x
+//                          124,704 keys: 45.9 us, 5.9 TB/s); a short cache by one CU's vector
+//                          units (12 x 866 keys: 7.1 us).
+//   attention_few_kernel   up to 32 queries of a cache head: a wave a block of 64 keys.  Bound
+//                          by the latency of a block's chain (12 x 10,392 keys, 32 queries:
+//                          13.7 us).
+//   attention_tile_kernel  128 queries a workgroup, the blocks through LDS.  Bound by the vector
+//                          units beside the matrix cores (softmax and the splitting of weights: 64% and
+//                          42% of the time; 12 x 10,392 rows over the frames before theirs: 407 us,
+//                          883 TFLOP/s of f16 products where a large library product reaches
+//                          1,080).
+// No atomics and no order that depends on timing: the same call gives the same bits, and a
+// row's do not depend on the values of other queries.
 #include <cmath>
 #include <type_traits>
 #include <utility>
@@ -235,6 +254,17 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
 // ---------------------------------------------------------------------------
 // 32 queries a wave on the f16 matrix cores
 // ---------------------------------------------------------------------------
+// S^T = K Q^T by 32x32x16 products, a block of 64 keys x 32 queries in 32 registers: a lane
+// holds one query (lane l and l ^ 32 query l % 32), so maxima, references and denominators stay
+// in the lane, S^T's registers are O^T += V^T P^T's operand as they stand, and no weight goes
+// through LDS.  What belongs to a key (scales, documents) is spread over the 16 lanes of a row and
+// broadcast by the instruction that uses it.
+//
+// The reference does not follow the maximum at every block: weights may be up to 2^(kPBits +
+// kSlack) = 2^15, f16's upper end, and it moves once a row's largest score * V's scale
+// passes it by 2^kSlack.  It holds V's scale too, so that the weights that matter have all
+// their bits in f16 however small V is: a row's largest is at least 2^kPBits, its second
+// part's last place 2^-24, which is 2^-33 of it (a rounding 2^-34).
 using vks::f32x16;
 using vks::f32x4;
 using vks::u32x4;

@@ -5,8 +5,9 @@
 // of the same token to a group.  The scale is the row's largest |x| / 127 (448),
 // a code the quotient rounded to f32 and then to the code: both divisions are
 // the correctly rounded ones, so a program that quantises on the host gets the
-// same codes.  Streams of one pass, bound by HBM from a few thousand rows on
-// and by the launch below.
+// same codes.  Streams of one pass, bound by HBM from some hundred thousand rows on
+// (12 heads of 10,392 read back: 13.5 us, 6.0 TB/s; 16 x 8 x 866 written 14.5, 5.0 TB/s) and by
+// the launch and one chain of loads below (10,392 rows: written 3.8 us, read 2.9, in a graph).
 #include "kv_cache.h"
 
 namespace {

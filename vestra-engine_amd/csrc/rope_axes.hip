@@ -11,6 +11,9 @@
 // lie wherever the convention puts them: the normalised row goes through LDS (a
 // row is its group's alone: no barrier, the lanes of a wave are in step).
 //
+// Bound by HBM for many tokens (10,392 of 24 heads: 24.2 us, 5.3 TB/s, of a copy's 5.0) and by
+// the chain of loads (table, position, angle) for few (866: 4.1 us in a graph).
+//
 // The angle: turns = position * f_j / (2 pi) in 64 bits, reduced there to an
 // eighth of a turn either side of a quarter, then single precision; a position
 // of 2^31 is held to 2^-22 of a turn.

@@ -520,7 +520,7 @@ typedef struct vk_rope_axes {
  * (VK_QK_HEADS_OUTER) or [sequences, heads, n, 64] (VK_QK_VIEWS_OUTER).
  * positions [sequences*n, count]: f32 (taken as they are, fractions
  * included), i32 or i64.  The angle is held in 64 bits, so far positions turn
- * exactly (to 1e-7 of a turn up to |p| = 2^31).  No table: nothing is
+ * exactly (to 1e-7 of a turn up to |p| = 2^31 where freq >= 1).  No table: nothing is
  * allocated.  q_out may be q (in place) or a tensor that overlaps no other;
  * k_out likewise.  head_dim 64.  No counterpart in the reference. */
 int vk_qk_norm_rope_axes_f32(vk_runtime* rt, const vk_tensor* q,
@@ -577,7 +577,8 @@ int vk_kv_cache_read_f32(vk_runtime* rt, const vk_kv_cache* cache, size_t n,
  * q.k / 8.  The order is scale, cap, bias, masks, softmax. */
 typedef struct vk_attention_rules {
   float scale;             /* of q.k; 0: 1/sqrt(64) */
-  float cap;               /* > 0: score = cap * tanh(score / cap) */
+  float cap;               /* > 0: score = cap * tanh(score / cap); |scale| and
+                              |scale| / cap lie in 2^-40 .. 2^40 */
   const vk_tensor* slopes; /* f32 [heads]: score -= slopes[h] * |p - j| for a
                               query at position p and the key of slot j */
   int causal;              /* key j only where j <= p */
@@ -601,13 +602,15 @@ typedef struct vk_attention_rules {
  * overlaps no other tensor.  A query that sees nothing gets zeros; rows past
  * counts[s] are left as they were.  A query that sees a key that reads back
  * as NaN gets NaN; keys that it does not see have no effect whatever they
- * hold.  Scores, weights and sums are held as in f32: the values of the cache
- * are exact in f16, queries and weights are taken as two f16 parts (a query's
- * value to 2^-25 of its row's largest, a weight times V's scale to 2^-34 of
- * the largest; one query: f32 throughout).  Positions past 2^31 - 2 count as
- * 2^31 - 2.  The same call gives the same bits.  A large call splits its keys
- * and keeps partial results in the runtime's work buffer (run it once before
- * a capture, which cannot grow it).  No counterpart in the reference. */
+ * hold, slots that nothing wrote too (codes 0x7f and 0xff of VK_CACHE_F8,
+ * which the write never makes, count as zeros in V).  Scores, weights and
+ * sums are held as in f32: the values of the cache are exact in f16, queries
+ * and weights are taken as two f16 parts (a query's value to 2^-25 of its
+ * row's largest, a weight times V's scale to 2^-34 of the largest; one query:
+ * f32 throughout).  Positions past 2^31 - 2 count as 2^31 - 2.  The same call
+ * gives the same bits.  A large call splits its keys and keeps partial
+ * results in the runtime's work buffer (run it once before a capture, which
+ * cannot grow it).  No counterpart in the reference. */
 int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache,
                             const vk_tensor* q, size_t heads, size_t n,
                             const vk_tensor* starts, const vk_tensor* counts,

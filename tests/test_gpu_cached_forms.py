@@ -214,3 +214,86 @@ def test_keys_and_values_of_one_tensor(rt, rng):
     held = cached.values(*cached.quantise(x, 1), 1).astype(np.float32)
     for got in (k.numpy().reshape(x.shape), v.numpy().reshape(x.shape)):
         assert np.array_equal(got[0, :, :30], held[0, :, :30]) and np.array_equal(got[1], held[1])
+
+
+def garbage(rng, c, slots):
+    """Fills `slots` of every sequence and head of a cache with bytes and scales of every kind."""
+    def put(t, width, dtype, values):
+        a = np.empty(len(t), dtype)
+        if dtype == np.uint8:
+            assert vh.lib.vk_download_u8(c.rt.handle, t.handle, a.ctypes.data, a.size) == 0
+        else:
+            a = t.numpy()
+        a = a.reshape(c.S, c.KV, c.cap, width)
+        a[:, :, slots] = rng.choice(values, a[:, :, slots].shape)
+        t.write(np.ascontiguousarray(a.reshape(-1)))
+    for t in (c.cache.k, c.cache.v):
+        put(t, 64, np.uint8, np.array([0x7f, 0xff, 0x80, 0, 0x7e, 0xfe, 1, 77], np.uint8))
+    for t in (c.cache.k_scale, c.cache.v_scale):
+        put(t, 1, np.float32, np.array([np.nan, np.inf, -np.inf, 3.4e38, -3.4e38, 1e-44, -0.0, 5.0],
+                                       np.float32))
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("n,cap", [(1, 300), (1, 3000), (11, 300), (11, 3000), (150, 500)])
+@pytest.mark.parametrize("rule", [{}, {"cap": 20.0}])
+def test_slots_that_nothing_wrote(rt, rng, fmt, n, cap, rule):
+    """Slots of another document, of later positions and past the length may hold anything:
+    the same bits."""
+    end = cap - 40
+    c = Case(rt, rng, fmt, 2, 2, 1, cap, n, [end - n] * 2).fill()
+    r = {**rule, "causal": True, "q_docs": np.zeros((2, n), np.int32),
+         "k_docs": np.zeros((2, cap), np.int32)}
+    hidden = np.concatenate([np.arange(0, 70), np.arange(100, end - n, 7)])
+    r["k_docs"][:, hidden] = 1
+    want = c.check(r, pick=[0, n // 2, n - 1])
+    later = np.arange(end - n // 2, cap)  # behind the length, and behind the first queries
+    garbage(rng, c, np.concatenate([hidden, np.arange(end, cap)]))
+    assert np.array_equal(c.run(r), want)
+    garbage(rng, c, later)
+    keep = n - n // 2
+    assert np.array_equal(c.run(r)[:, :, :keep], want[:, :, :keep])
+
+
+@pytest.mark.parametrize("n", [1, 11, 150])
+def test_codes_that_are_no_number(rt, rng, n):
+    """e4m3's codes 0x7f and 0xff, put there by hand: zeros in V, NaN to who sees them in K."""
+    c = Case(rt, rng, 1, 1, 2, 2, 300, n, [300 - n]).fill()
+    clean = c.run()
+    codes = cached.quantise(c.v, 1)[0]
+    codes[0, 0, 100, ::3], codes[0, 1, 5, 7] = 0x7f, 0xff
+    c.cache.v.write(codes.reshape(-1))
+    c.vheld = np.nan_to_num(cached.values(codes, c.v_scale, 1), nan=0.0)
+    got = c.check()
+    assert not np.array_equal(got, clean)
+    codes = cached.quantise(c.k, 1)[0]
+    codes[0, 1, 200, 9] = 0x7f
+    c.cache.k.write(codes.reshape(-1))
+    assert np.array_equal(c.run()[:, 0], got[:, 0]) and np.isnan(c.got()[:, 1]).all()
+
+
+def test_scales_out_of_range_are_refused(rt):
+    c = rt.kv_cache(0, 1, 1, 4)
+    q, o = rt.upload_f32(np.ones(64)), rt.alloc_f32(64)
+    for args in (dict(scale=1e-13), dict(scale=-1e13), dict(cap=1e-14), dict(cap=1e12),
+                 dict(scale=1e6, cap=1e-7), dict(scale=1e-44)):
+        with pytest.raises(vh.UnsupportedShape):
+            rt.attention_cached_f32(c, q, 1, 1, None, None, 0, vh.AttentionRules(**args), o)
+
+
+@pytest.mark.parametrize("n", [1, 11, 150])
+@pytest.mark.parametrize("rule", [{"scale": -0.25}, {"scale": 2.0 ** -39}, {"scale": -0.5, "cap": 3.0},
+                                  {"scale": 0.125, "cap": 1e11}, {"scale": 0.125, "cap": 2e-13}])
+def test_scales_at_the_ends_of_the_range(rt, rng, n, rule):
+    c = Case(rt, rng, n % 2, 1, 2, 1, 260, n, [260 - n]).fill()
+    c.check(rule)
+
+
+def test_more_workgroups_than_a_launch_holds_are_refused(rt):
+    """16,777,215 sequences of one query: 2^33 threads."""
+    S = 0xffffff
+    c = rt.kv_cache(0, S, 1, 1)
+    q, o = rt.alloc_f32(S * 64), rt.alloc_f32(S * 64)
+    with pytest.raises(vh.UnsupportedShape):
+        rt.attention_cached_f32(c, q, 1, 1, None, None, 0, None, o)
+    rt.synchronize()

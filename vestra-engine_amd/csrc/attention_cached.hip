@@ -94,6 +94,9 @@ __device__ __forceinline__ float wave_max(float v) {
   return fmaxf(__uint_as_float(b0), __uint_as_float(b1));
 }
 
+template <int FORMAT, int N>
+__device__ __forceinline__ void drop_nan(uint32_t (&w)[N]);
+
 constexpr int kRowWaves = 8;
 constexpr float kRoom = 4.0f;  // a lane's maximum follows scores that pass it by 2^kRoom
 
@@ -180,7 +183,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     const float wv = seen ? w * (vs * kRowDown) : 0.0f;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
-      const uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
+      uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
+      drop_nan<FORMAT>(ws);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float4 x = vkc::decode4<FORMAT>(ws[e]);
@@ -332,6 +336,24 @@ __device__ __forceinline__ u32x4 decode8(uint2 w) {
   return r;
 }
 
+// V's codes that are no number (e4m3's 0x7f and 0xff, which the cache's write never makes, but
+// a slot that nothing wrote may hold) as zeros: a weight of 0 does not take them away.
+template <int FORMAT, int N>
+__device__ __forceinline__ void drop_nan(uint32_t (&w)[N]) {
+  if constexpr (FORMAT == VK_CACHE_F8) {
+    uint32_t any = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) any |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
+    if (__builtin_expect((any & 0x80808080u) != 0, 0)) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const uint32_t bad = ((w[i] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        w[i] &= ~((bad << 1) - (bad >> 7));  // all of a byte
+      }
+    }
+  }
+}
+
 // Four keys' values of one d a lane, out of LDS rows [key][d] of f16: in each 16
 // lanes, lane 4 r + c gives the address of key r's values d = 4 c .. 4 c + 3, and lane d
 // receives its d of keys 0 .. 3.
@@ -346,9 +368,9 @@ __device__ __forceinline__ uint2 read_tr(const char* p) {
 // What a block's keys bring beside their codes, in LDS: 64 of each, key 32 t + 8
 // (r / 4) + 4 half + r % 4 at 32 t + 16 half + r.
 struct KeyData {
-  float ks[KB];   // K's scale / 2^kQUp (a NaN where V's scale is one)
+  float ks[KB];   // K's scale / 2^kQUp (a NaN where V's scale is one, or infinite)
   float lsv[KB];  // log2 of V's scale, at least kLeastLsv
-  float sv[KB];   // V's scale (0 where it is a NaN)
+  float sv[KB];   // V's scale (0 there)
   int doc[KB];
 };
 
@@ -373,10 +395,10 @@ __device__ __forceinline__ KeyRegs key_regs(const KeyData& kd, bool docs) {
 
 // ks, lsv and sv from the scales of a row of K and of V.
 __device__ __forceinline__ void key_values(float k, float v, float* ks, float* lsv, float* sv) {
-  const bool nan = v != v;
-  *ks = nan ? v : k * (1.0f / (1 << kQUp));
-  *lsv = fmaxf(__builtin_amdgcn_logf(fmaxf(v, vkc::kLeastScale)), kLeastLsv);
+  const bool nan = !(fabsf(v) <= 3.4028235e38f);
+  *ks = nan ? NAN : k * (1.0f / (1 << kQUp));
   *sv = nan ? 0.0f : v;
+  *lsv = fmaxf(__builtin_amdgcn_logf(fmaxf(*sv, vkc::kLeastScale)), kLeastLsv);
 }
 
 __device__ __forceinline__ int key_slot(int key) {
@@ -840,9 +862,17 @@ struct StageRows {
     }
   }
 
-  template <int PITCH>
-  __device__ __forceinline__ void store(char* to) const {
+  template <int PITCH, bool V = false>
+  __device__ __forceinline__ void store(char* to) {
     const int tid = threadIdx.x;
+    if constexpr (V) {
+      uint32_t x[2 * kPer];
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) x[2 * i] = w[i].x, x[2 * i + 1] = w[i].y;
+      drop_nan<FORMAT>(x);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) w[i] = make_uint2(x[2 * i], x[2 * i + 1]);
+    }
 #pragma unroll
     for (int i = 0; i < kPer; ++i)
       *reinterpret_cast<u32x4*>(to + ((tid >> 3) + i * (THREADS / 8)) * PITCH + 16 * (tid & 7)) =
@@ -943,7 +973,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
     rows_v.load(a.cache.v, first, key_of(e), keys);
     if (wave == 0) keys_d.load(a, first, doc_first, key_of(e), keys);
     rows_k.template store<kKPitch>(kl[0]);
-    rows_v.template store<kVPitch>(vl[0]);
+    rows_v.template store<kVPitch, true>(vl[0]);
     if (wave == 0) keys_d.store(a, kd[0]);
     __syncthreads();
     for (int x = b_begin; x < b_end; ++x) {
@@ -969,7 +999,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
         if constexpr (MASK) __builtin_amdgcn_s_setprio(0);
       }
       rows_k.template store<kKPitch>(kl[buf ^ 1]);
-      rows_v.template store<kVPitch>(vl[buf ^ 1]);
+      rows_v.template store<kVPitch, true>(vl[buf ^ 1]);
       if (wave == 0) keys_d.store(a, kd[buf ^ 1]);
       e = e1;
       if constexpr (!MASK) __builtin_amdgcn_s_setprio(0);
@@ -1092,8 +1122,12 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
 #pragma unroll
       for (int y = 0; y < 4; ++y) {
         char* to = vw + (16 * y + (lane >> 2)) * kVPitch + 32 * (lane & 3);
-        *reinterpret_cast<u32x4*>(to) = decode8<FORMAT>(make_uint2(vr[y][0], vr[y][1]));
-        *reinterpret_cast<u32x4*>(to + 16) = decode8<FORMAT>(make_uint2(vr[y][2], vr[y][3]));
+        const int c0 = vr[y][0], c1 = vr[y][1], c2 = vr[y][2], c3 = vr[y][3];
+        uint32_t c[4] = {static_cast<uint32_t>(c0), static_cast<uint32_t>(c1),
+                         static_cast<uint32_t>(c2), static_cast<uint32_t>(c3)};
+        drop_nan<FORMAT>(c);
+        *reinterpret_cast<u32x4*>(to) = decode8<FORMAT>(make_uint2(c[0], c[1]));
+        *reinterpret_cast<u32x4*>(to + 16) = decode8<FORMAT>(make_uint2(c[2], c[3]));
       }
       f32x16 sc[2];
       clear(sc);
@@ -1239,6 +1273,13 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   VK_REQUIRE(std::isfinite(ru.scale), "attention_cached: scale %g", static_cast<double>(ru.scale));
   VK_REQUIRE(std::isfinite(ru.cap) && ru.cap >= 0.0f, "attention_cached: cap %g",
              static_cast<double>(ru.cap));
+  // what a query is multiplied by keeps its values normal numbers
+  const float scale = ru.scale == 0.0f ? 0.125f : ru.scale;
+  const float by = std::fabs(ru.cap > 0.0f ? scale / ru.cap : scale);
+  VK_UNSUPPORTED_IF(!(by >= 0x1p-40f && by <= 0x1p40f && std::fabs(scale) >= 0x1p-40f &&
+                      std::fabs(scale) <= 0x1p40f),
+                    "attention_cached: scale %g with cap %g (scale and scale / cap: 2^-40 to 2^40)",
+                    static_cast<double>(ru.scale), static_cast<double>(ru.cap));
   if (ru.slopes) {
     VK_REQUIRE(ru.slopes->dtype == VK_F32 && ru.slopes->len == heads,
                "slopes must be f32 [%zu] (holds %zu)", heads, ru.slopes->len);
@@ -1267,7 +1308,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   Shape a;
   a.cache = vk::cache_args(cache);
   a.rows = vk::rows_args(starts, counts, cache->sequences, n, layout);
-  a.rules.scale = ru.scale == 0.0f ? 0.125f : ru.scale;
+  a.rules.scale = scale;
   a.rules.cap = ru.cap;
   a.rules.slopes = ru.slopes ? static_cast<const float*>(ru.slopes->ptr) : nullptr;
   a.rules.prefix = ints(ru.prefix);
@@ -1290,7 +1331,6 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   const size_t tiles = (a.group * n + vk::kTileRows - 1) / vk::kTileRows;
   const size_t units = plan.form == vk::kTile ? pairs * tiles : pairs;
   const size_t splits = plan.splits;
-  VK_UNSUPPORTED_IF(2 * units * splits > 0x7ffffff0ULL, "attention_cached: %zu queries", rows);
   a.splits = static_cast<uint32_t>(splits);
   a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
@@ -1305,7 +1345,10 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   a.parts = a.rules.q_docs && !a.rules.docs_ordered ? 2 : 1;
   const size_t slots =
       (a.order.heads * tiles * splits * a.parts + a.order.share - 1) / a.order.share;
-  const dim3 grid(static_cast<unsigned>(plan.form == vk::kTile ? 8 * slots : units * splits));
+  const size_t wgs = plan.form == vk::kTile ? 8 * slots : units * splits;
+  VK_UNSUPPORTED_IF(wgs * (plan.form == vk::kRow ? 64 * kRowWaves : 256) > 0xffffffffULL,
+                    "attention_cached: %zu workgroups", wgs);
+  const dim3 grid(static_cast<unsigned>(wgs));
   const bool q8 = cache->format == VK_CACHE_Q8;
   const int score = (ru.cap > 0.0f ? kCap : 0) | (ru.slopes ? kBias : 0);
   const bool mask = ru.causal || ru.q_docs;

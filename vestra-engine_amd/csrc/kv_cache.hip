@@ -65,6 +65,10 @@ struct Split {
   uint32_t groups;
 };
 
+__device__ __forceinline__ uint32_t group_id() {
+  return (blockIdx.y * gridDim.x + blockIdx.x) * kGroups + (threadIdx.x >> 4);
+}
+
 __device__ __forceinline__ bool place(const Split& sp, const vkc::Rows& r, const vkc::Cache& c,
                                       uint32_t g, size_t* f32_at, size_t* slot) {
   if (g >= sp.groups) return false;
@@ -86,7 +90,7 @@ __global__ __launch_bounds__(kThreads) void kv_cache_write_kernel(const float* _
                                                                   Split sp) {
   const int l = threadIdx.x & 15;
   size_t from, slot;
-  if (!place(sp, r, c, blockIdx.x * kGroups + (threadIdx.x >> 4), &from, &slot)) return;
+  if (!place(sp, r, c, group_id(), &from, &slot)) return;
   const float4 a = vkd::ld_stream(reinterpret_cast<const float4*>(k + from) + l);
   const float4 b = vkd::ld_stream(reinterpret_cast<const float4*>(v + from) + l);
   float da, db;
@@ -112,7 +116,7 @@ __global__ __launch_bounds__(kThreads) void kv_cache_read_kernel(float* __restri
                                                                  Split sp) {
   const int l = threadIdx.x & 15;
   size_t to, slot;
-  if (!place(sp, r, c, blockIdx.x * kGroups + (threadIdx.x >> 4), &to, &slot)) return;
+  if (!place(sp, r, c, group_id(), &to, &slot)) return;
   uint32_t wa = 0, wb = 0;
   float da = 0.0f, db = 0.0f;
   if (k) {
@@ -134,6 +138,12 @@ int make_split(const vk_kv_cache* c, size_t n, Split* sp) {
   sp->by_heads = vkd::make_fastdiv(static_cast<uint32_t>(c->heads));
   sp->groups = static_cast<uint32_t>(groups);
   return VK_OK;
+}
+
+// 2^20 workgroups a row of the grid: a launch holds at most 2^32 threads a dimension.
+dim3 make_grid(const Split& sp) {
+  const uint32_t wgs = (sp.groups + kGroups - 1) / kGroups, x = wgs < (1u << 20) ? wgs : 1u << 20;
+  return dim3(x, (wgs + x - 1) / x);
 }
 
 int check_rows(const vk_kv_cache* c, size_t n, vk_qk_layout layout) {
@@ -210,7 +220,7 @@ int vk_kv_cache_write_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_ten
   if (len == 0 || cache->capacity == 0) return VK_OK;
   Split sp;
   VK_TRY(make_split(cache, n, &sp));
-  const dim3 grid((sp.groups + kGroups - 1) / kGroups);
+  const dim3 grid = make_grid(sp);
   const auto* K = static_cast<const float*>(k->ptr);
   const auto* V = static_cast<const float*>(v->ptr);
   const vkc::Cache c = vk::cache_args(cache);
@@ -245,7 +255,7 @@ int vk_kv_cache_read_f32(vk_runtime* rt, const vk_kv_cache* cache, size_t n,
   if (len == 0 || cache->capacity == 0) return VK_OK;
   Split sp;
   VK_TRY(make_split(cache, n, &sp));
-  const dim3 grid((sp.groups + kGroups - 1) / kGroups);
+  const dim3 grid = make_grid(sp);
   float* K = k ? static_cast<float*>(k->ptr) : nullptr;
   float* V = v ? static_cast<float*>(v->ptr) : nullptr;
   const vkc::Cache c = vk::cache_args(cache);

@@ -300,8 +300,8 @@ int vk_qk_norm_rope_axes_f32(vk_runtime* rt, const vk_tensor* q, const vk_tensor
   VK_REQUIRE(pairs == 32, "qk_norm_rope_axes: the axes have %llu pairs (32)", pairs);
   VK_REQUIRE(heads > 0, "qk_norm_rope_axes: no heads");
   VK_UNSUPPORTED_IF(sequences > 0x7fffffffULL || n > 0x7fffffffULL || heads > 0xffff ||
-                        kv_heads > 0xffff || sequences * n > 0x7fffffffULL,
-                    "qk_norm_rope_axes: too large");
+                        kv_heads > 0xffff || sequences * n > 0xffffff0ULL,
+                    "qk_norm_rope_axes: too large");  // 16 threads a token, 2^32 a launch
   const size_t rows = sequences * n;
   VK_TRY(vk::check_f32(rt, q, heads * rows * 64, "q"));
   VK_TRY(vk::check_f32(rt, q_out, heads * rows * 64, "q_out"));

@@ -297,3 +297,15 @@ def test_more_workgroups_than_a_launch_holds_are_refused(rt):
     with pytest.raises(vh.UnsupportedShape):
         rt.attention_cached_f32(c, q, 1, 1, None, None, 0, None, o)
     rt.synchronize()
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("S,H,keys", [(1, 1, 1), (1, 64, 130), (1, 65, 130), (16, 4, 1536),
+                                      (13, 5, 65), (2, 3, 1537)])
+def test_single_rows_of_few_and_many_heads(rt, rng, fmt, S, H, keys):
+    """Rows whose columns are shared out over workgroups (64 at most on 256 CUs) and rows of
+    one, up to the longest unsplit cache and a key past it."""
+    starts = [max(keys - 1 - 7 * s, 0) for s in range(S)]
+    c = Case(rt, rng, fmt, S, H, H, keys, 1, starts, layout=fmt).fill()
+    c.check()
+    c.check({"causal": True, "cap": 10.0, "slopes": np.linspace(0.0, 0.2, H, dtype=np.float32)})

@@ -12,8 +12,8 @@
 // Three kernels (plans.h says which, and over how many workgroups the keys are split), and one
 // that joins the splits:
 //   attention_row_kernel   one query: a lane a key, f32 on the vector units.  Bound by memory (16 x
-//                          124,704 keys: 45.9 us, 5.9 TB/s); a short cache by one CU's vector
-//                          units (12 x 866 keys: 7.1 us).
+//                          124,704 keys: 45.9 us, 5.9 TB/s); a short cache by its CUs'
+//                          vector units (12 x 866 keys: 5.9 us).
 //   attention_few_kernel   up to 32 queries of a cache head: a wave a block of 64 keys.  Bound
 //                          by the latency of a block's chain (12 x 10,392 keys, 32 queries:
 //                          13.7 us).
@@ -103,16 +103,22 @@ constexpr float kRoom = 4.0f;  // a lane's maximum follows scores that pass it b
 // One query a sequence and cache head: a workgroup a query and key split, a lane a key.  The
 // lane's 64 products are F32 FMAs with the query in scalar registers (four running sums), and
 // it keeps a softmax of its own (maximum, sum and 64 sums of values) over the keys that it
-// meets; the lanes are joined once, at the end, halving: lane d is left with d.
-template <int FORMAT>
+// meets; the lanes are joined once, at the end, halving: lane d is left with d.  A short cache's
+// few rows have four workgroups each (PARTS), which share V's columns and all take the scores: a
+// CU has 60% of the vector work (12 x 866 keys 5.9 us, 7.1 in one).
+template <int FORMAT, int PARTS>
 __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const float* __restrict__ q,
                                                                        float* __restrict__ out,
                                                                        float* __restrict__ part,
                                                                        Shape a) {
-  __shared__ float so[kRowWaves][HD];
+  constexpr int ND = HD / PARTS;
+  __shared__ float so[kRowWaves][ND];
   __shared__ float sm[kRowWaves], sl[kRowWaves];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const uint32_t split = blockIdx.x % a.splits, row = blockIdx.x / a.splits;
+  const uint32_t all = a.rows.sequences * a.heads;
+  const uint32_t split = PARTS > 1 ? 0 : blockIdx.x % a.splits;
+  const uint32_t row = PARTS > 1 ? blockIdx.x % all : blockIdx.x / a.splits;
+  const int d0 = PARTS > 1 ? static_cast<int>(blockIdx.x / all) * ND : 0;
   const uint32_t h = row % a.heads, s = row / a.heads;
   const Rules& ru = a.rules;
   // every scalar together: none waits for another
@@ -126,9 +132,9 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const int p = position(start, 0);
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + h) * a.cache.capacity;
 
-  float m = -INFINITY, l = 0.0f, acc[HD];
+  float m = -INFINITY, l = 0.0f, acc[ND];
 #pragma unroll
-  for (int d = 0; d < HD; ++d) acc[d] = 0.0f;
+  for (int d = 0; d < ND; ++d) acc[d] = 0.0f;
   const int blocks = (keys + 63) / 64;
   const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / a.splits);
   const int b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / a.splits);
@@ -137,13 +143,13 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     // the key's codes and scales, all at once (past the end the last key's)
     const size_t slot = first + (j < keys ? j : keys - 1);
     const uint4* kc = reinterpret_cast<const uint4*>(a.cache.k + slot * HD);
-    const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD);
-    uint4 kw[4], vw[4];
+    const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD + d0);
+    uint4 kw[4], vw[ND / 16];
 #pragma unroll
     for (int c = 0; c < 4; ++c) kw[c] = kc[c];
     const float ks = a.cache.ks[slot], vs = a.cache.vs[slot];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) vw[c] = vc[c];
+    for (int c = 0; c < ND / 16; ++c) vw[c] = vc[c];
     bool seen = j < keys;
     if (ru.causal) seen = seen && (j <= p || j < pre);
     if (ru.q_docs && seen) {
@@ -175,14 +181,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
       const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - t);
       l *= f;
 #pragma unroll
-      for (int d = 0; d < HD; ++d) acc[d] *= f;
+      for (int d = 0; d < ND; ++d) acc[d] *= f;
       m = t;
     }
     const float w = seen ? __builtin_amdgcn_exp2f(t - m) : 0.0f;
     l += w;
     const float wv = seen ? w * (vs * kRowDown) : 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
+    for (int c = 0; c < ND / 16; ++c) {
       uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
       drop_nan<FORMAT>(ws);
 #pragma unroll
@@ -200,40 +206,46 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mw);
   l *= f;
 #pragma unroll
-  for (int d = 0; d < HD; ++d) acc[d] *= f;
-  // halving by swaps of halves and of rows of 16, then by exchanges inside them
+  for (int d = 0; d < ND; ++d) acc[d] *= f;
+  // halving by swaps of halves and of rows of 16, then by exchanges inside them (sums of the
+  // same element once each lane has but one): lane x is left with element x / PARTS
 #pragma unroll
-  for (int d = 0; d < 32; ++d) {
+  for (int d = 0; d < ND / 2; ++d) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(acc[d]),
-                                                    __float_as_uint(acc[d + 32]), false, false);
+                                                    __float_as_uint(acc[d + ND / 2]), false, false);
     const uint32_t x = r[0], y = r[1];
     acc[d] = __uint_as_float(x) + __uint_as_float(y);
   }
 #pragma unroll
-  for (int d = 0; d < 16; ++d) {
+  for (int d = 0; d < ND / 4; ++d) {
     const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(acc[d]),
-                                                    __float_as_uint(acc[d + 16]), false, false);
+                                                    __float_as_uint(acc[d + ND / 4]), false, false);
     const uint32_t x = r[0], y = r[1];
     acc[d] = __uint_as_float(x) + __uint_as_float(y);
   }
 #pragma unroll
   for (int w = 8; w; w >>= 1) {
+    const int half = w / PARTS;  // elements left after the step (0: one before it, too)
     const bool up = (lane & w) != 0;
+    if (half == 0) {
+      acc[0] += __shfl_xor(acc[0], w, 64);
+      continue;
+    }
 #pragma unroll
-    for (int d = 0; d < w; ++d) {
-      const float send = up ? acc[d] : acc[d + w];
-      acc[d] = (up ? acc[d + w] : acc[d]) + __shfl_xor(send, w, 64);
+    for (int d = 0; d < half; ++d) {
+      const float send = up ? acc[d] : acc[d + half];
+      acc[d] = (up ? acc[d + half] : acc[d]) + __shfl_xor(send, w, 64);
     }
   }
 #pragma unroll
   for (int w = 32; w; w >>= 1) l += __shfl_xor(l, w, 64);
-  so[wave][lane] = acc[0];
+  if (lane % PARTS == 0) so[wave][lane / PARTS] = acc[0];
   if (lane == 0) {
     sm[wave] = mw;
     sl[wave] = l;
   }
   __syncthreads();
-  if (wave != 0) return;
+  if (wave != 0 || lane >= ND) return;
   float mg = sm[0];
 #pragma unroll
   for (int w = 1; w < kRowWaves; ++w) mg = fmaxf(mg, sm[w]);
@@ -244,14 +256,14 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     o += so[w][lane] * g;
     lg += sl[w] * g;
   }
-  if (part) {
+  if (PARTS == 1 && part) {
     const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads;
     const size_t at = static_cast<size_t>(split) * rows + row;
     part[at * HD + lane] = o;
     if (lane == 0)
       *reinterpret_cast<float2*>(part + a.splits * rows * HD + 2 * at) = make_float2(mg, lg);
   } else {
-    out[vkc::row_at(a.rows, a.heads, s, h, 0) + lane] = lg == 0.0f ? 0.0f : o / lg * kRowUp;
+    out[vkc::row_at(a.rows, a.heads, s, h, 0) + d0 + lane] = lg == 0.0f ? 0.0f : o / lg * kRowUp;
   }
 }
 
@@ -1367,12 +1379,18 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
 #define VK_RULES(F) \
   switch (score) { VK_RULE(F, 0) VK_RULE(F, kCap) VK_RULE(F, kBias) VK_RULE(F, (kCap | kBias)) }
   if (plan.form == vk::kRow) {
-    if (q8)
-      hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_Q8>, grid, dim3(64 * kRowWaves), 0,
-                         rt->stream, Q, O, part, a);
-    else
-      hipLaunchKernelGGL(attention_row_kernel<VK_CACHE_F8>, grid, dim3(64 * kRowWaves), 0,
-                         rt->stream, Q, O, part, a);
+#define VK_ROW(F, P)                                                                        \
+  hipLaunchKernelGGL((attention_row_kernel<F, P>), dim3(grid.x * P), dim3(64 * kRowWaves), 0, \
+                     rt->stream, Q, O, part, a)
+    const bool parts = splits == 1 && 4 * rows <= cus;  // where the card has the CUs
+    if (q8) {
+      if (parts) VK_ROW(VK_CACHE_Q8, 4);
+      else VK_ROW(VK_CACHE_Q8, 1);
+    } else {
+      if (parts) VK_ROW(VK_CACHE_F8, 4);
+      else VK_ROW(VK_CACHE_F8, 1);
+    }
+#undef VK_ROW
   } else if (q8) {
     VK_RULES(VK_CACHE_Q8)
   } else {

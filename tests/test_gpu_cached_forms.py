@@ -309,3 +309,55 @@ def test_single_rows_of_few_and_many_heads(rt, rng, fmt, S, H, keys):
     c = Case(rt, rng, fmt, S, H, H, keys, 1, starts, layout=fmt).fill()
     c.check()
     c.check({"causal": True, "cap": 10.0, "slopes": np.linspace(0.0, 0.2, H, dtype=np.float32)})
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("qs,ks", [(1e-36, 1e36), (1e-34, 1e37), (1e36, 1e-26), (1e30, 1e-28),
+                                   (1e-36, 1.0)])
+@pytest.mark.parametrize("n", [1, 9, 70])
+def test_queries_at_the_ends_of_f32(rt, rng, fmt, qs, ks, n):
+    """Products that stay in range, of factors that do not: the largest and the smallest
+    queries with keys the other way round."""
+    c = Case(rt, rng, fmt, 1, 2, 1, 330, n, [330 - n], qs=qs, ks=ks).fill()
+    c.check(label=f"{qs} {ks}")
+
+
+def test_misaligned_tensors_are_refused(rt):
+    import ctypes
+    c = rt.kv_cache(0, 2, 1, 4)
+    q, o = rt.upload_f32(np.ones(128)), rt.alloc_f32(128)
+    raw = rt.upload_i32(np.zeros(8, np.int32))
+    h = ctypes.c_void_p()
+    if vh.lib.vk_tensor_wrap(rt.handle, vh.VK_I32, raw.device_ptr + 2, 2, ctypes.byref(h)) != 0:
+        return
+    odd = vh.Tensor(rt, h)
+    for call in (lambda: rt.kv_cache_write_f32(c, q, q, 1, odd),
+                 lambda: rt.kv_cache_read_f32(c, 1, None, odd, o, None),
+                 lambda: rt.attention_cached_f32(c, q, 1, 1, odd, None, 0, None, o),
+                 lambda: rt.attention_cached_f32(c, q, 1, 1, None, None, 0,
+                                                 vh.AttentionRules(causal=True, prefix=odd), o)):
+        with pytest.raises(vh.VestraError) as e:
+            call()
+        assert e.value.code == vh.VK_ERR_INVALID
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("n,cap,seen", [(1, 300, 100), (1, 4000, 2500), (9, 300, 100), (9, 4000, 2500),
+                                        (150, 500, 100), (150, 4000, 2500)])
+@pytest.mark.parametrize("slope", [2.0 ** 7, 2.0 ** 14, 2.0 ** 20])
+@pytest.mark.parametrize("vs", [1e-5, 1.0, 1e8])
+def test_scores_far_from_zero(rt, rng, fmt, n, cap, seen, slope, vs):
+    """Keys all far from the queries under a steep bias: scores of -2^17 to -2^32, where f32's
+    step is up to 512; the nearest key outweighs the next by 2^100 at least."""
+    c = Case(rt, rng, fmt, 1, 3, 3, cap, n, [cap - n], vs=vs).fill()
+    c.check({"slopes": np.array([slope, slope, 0.0], np.float32)}, max_length=seen,
+            pick=[0, n // 2, n - 1])
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("n", [1, 20, 70])
+def test_single_heads_at_the_ends_of_f32(rt, rng, fmt, n):
+    """As the test of both ends above, a head to a cache head."""
+    for qs, ks in ((1e36, 1e-26), (1e-36, 1e36), (3e37, 1e-28)):
+        c = Case(rt, rng, fmt, 1, 2, 2, 200, n, [200 - n], qs=qs, ks=ks).fill()
+        c.check(label=f"{qs} {ks}")

@@ -133,75 +133,91 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const size_t first = (static_cast<size_t>(s) * a.cache.heads + h) * a.cache.capacity;
 
   float m = -INFINITY, l = 0.0f, acc[ND];
-#pragma unroll
-  for (int d = 0; d < ND; ++d) acc[d] = 0.0f;
   const int blocks = (keys + 63) / 64;
   const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / a.splits);
   const int b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / a.splits);
-  for (int b = b0 + wave; b < b1; b += kRowWaves) {
-    const int j = b * 64 + lane;
-    // the key's codes and scales, all at once (past the end the last key's)
-    const size_t slot = first + (j < keys ? j : keys - 1);
-    const uint4* kc = reinterpret_cast<const uint4*>(a.cache.k + slot * HD);
-    const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD + d0);
-    uint4 kw[4], vw[ND / 16];
+  // The wave's blocks; whether q . code went past f32's range somewhere, which K's scale may
+  // bring it back into: `small` takes the codes times kDown.
+  const auto run = [&](auto small) {
+    constexpr bool kSmall = decltype(small)::value;
+    constexpr float kDown = 0x1p-24f;
+    bool past = false;
+    m = -INFINITY;
+    l = 0.0f;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) kw[c] = kc[c];
-    const float ks = a.cache.ks[slot], vs = a.cache.vs[slot];
+    for (int d = 0; d < ND; ++d) acc[d] = 0.0f;
+    for (int b = b0 + wave; b < b1; b += kRowWaves) {
+      const int j = b * 64 + lane;
+      // the key's codes and scales, all at once (past the end the last key's)
+      const size_t slot = first + (j < keys ? j : keys - 1);
+      const uint4* kc = reinterpret_cast<const uint4*>(a.cache.k + slot * HD);
+      const uint4* vc = reinterpret_cast<const uint4*>(a.cache.v + slot * HD + d0);
+      uint4 kw[4], vw[ND / 16];
 #pragma unroll
-    for (int c = 0; c < ND / 16; ++c) vw[c] = vc[c];
-    bool seen = j < keys;
-    if (ru.causal) seen = seen && (j <= p || j < pre);
-    if (ru.q_docs && seen) {
-      const int kd = ru.k_docs[static_cast<size_t>(s) * a.cache.capacity + j];
-      seen = ru.docs_ordered ? kd <= doc : kd == doc;
-    }
-    float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int c = 0; c < 4; ++c) kw[c] = kc[c];
+      const float ks = a.cache.ks[slot], vs = a.cache.vs[slot];
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t ws[4] = {kw[c].x, kw[c].y, kw[c].z, kw[c].w};
+      for (int c = 0; c < ND / 16; ++c) vw[c] = vc[c];
+      bool seen = j < keys;
+      if (ru.causal) seen = seen && (j <= p || j < pre);
+      if (ru.q_docs && seen) {
+        const int kd = ru.k_docs[static_cast<size_t>(s) * a.cache.capacity + j];
+        seen = ru.docs_ordered ? kd <= doc : kd == doc;
+      }
+      float u[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 x = vkc::decode4<FORMAT>(ws[e]);
-        u[0] = __builtin_fmaf(qr[16 * c + 4 * e], x.x, u[0]);
-        u[1] = __builtin_fmaf(qr[16 * c + 4 * e + 1], x.y, u[1]);
-        u[2] = __builtin_fmaf(qr[16 * c + 4 * e + 2], x.z, u[2]);
-        u[3] = __builtin_fmaf(qr[16 * c + 4 * e + 3], x.w, u[3]);
+      for (int c = 0; c < 4; ++c) {
+        const uint32_t ws[4] = {kw[c].x, kw[c].y, kw[c].z, kw[c].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float4 x = vkc::decode4<FORMAT>(ws[e]);
+          if constexpr (kSmall) x = make_float4(x.x * kDown, x.y * kDown, x.z * kDown, x.w * kDown);
+          u[0] = __builtin_fmaf(qr[16 * c + 4 * e], x.x, u[0]);
+          u[1] = __builtin_fmaf(qr[16 * c + 4 * e + 1], x.y, u[1]);
+          u[2] = __builtin_fmaf(qr[16 * c + 4 * e + 2], x.z, u[2]);
+          u[3] = __builtin_fmaf(qr[16 * c + 4 * e + 3], x.w, u[3]);
+        }
+      }
+      const float dot = (u[0] + u[1]) + (u[2] + u[3]);
+      float t = dot * ks * ru.scale;
+      if constexpr (kSmall) t *= 1.0f / kDown;
+      past = past || !(fabsf(dot) <= 3.4028235e38f);
+      if (ru.cap > 0.0f) t = ru.cap * tanhf(t / ru.cap);
+      if (ru.slopes) {
+        const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
+        t -= slope * static_cast<float>(far);
+      }
+      t *= kLog2e;
+      seen = seen && !(t == -INFINITY);
+      if (seen && t > m + kRoom) {
+        const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - t);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < ND; ++d) acc[d] *= f;
+        m = t;
+      }
+      const float w = seen ? __builtin_amdgcn_exp2f(t - m) : 0.0f;
+      l += w;
+      const float wv = seen ? w * (vs * kRowDown) : 0.0f;
+#pragma unroll
+      for (int c = 0; c < ND / 16; ++c) {
+        uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
+        drop_nan<FORMAT>(ws);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4 x = vkc::decode4<FORMAT>(ws[e]);
+          const int d = 16 * c + 4 * e;
+          acc[d] = __builtin_fmaf(wv, x.x, acc[d]);
+          acc[d + 1] = __builtin_fmaf(wv, x.y, acc[d + 1]);
+          acc[d + 2] = __builtin_fmaf(wv, x.z, acc[d + 2]);
+          acc[d + 3] = __builtin_fmaf(wv, x.w, acc[d + 3]);
+        }
       }
     }
-    float t = ((u[0] + u[1]) + (u[2] + u[3])) * ks * ru.scale;
-    if (ru.cap > 0.0f) t = ru.cap * tanhf(t / ru.cap);
-    if (ru.slopes) {
-      const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
-      t -= slope * static_cast<float>(far);
-    }
-    t *= kLog2e;
-    seen = seen && !(t == -INFINITY);
-    if (seen && t > m + kRoom) {
-      const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - t);
-      l *= f;
-#pragma unroll
-      for (int d = 0; d < ND; ++d) acc[d] *= f;
-      m = t;
-    }
-    const float w = seen ? __builtin_amdgcn_exp2f(t - m) : 0.0f;
-    l += w;
-    const float wv = seen ? w * (vs * kRowDown) : 0.0f;
-#pragma unroll
-    for (int c = 0; c < ND / 16; ++c) {
-      uint32_t ws[4] = {vw[c].x, vw[c].y, vw[c].z, vw[c].w};
-      drop_nan<FORMAT>(ws);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float4 x = vkc::decode4<FORMAT>(ws[e]);
-        const int d = 16 * c + 4 * e;
-        acc[d] = __builtin_fmaf(wv, x.x, acc[d]);
-        acc[d + 1] = __builtin_fmaf(wv, x.y, acc[d + 1]);
-        acc[d + 2] = __builtin_fmaf(wv, x.z, acc[d + 2]);
-        acc[d + 3] = __builtin_fmaf(wv, x.w, acc[d + 3]);
-      }
-    }
-  }
+    return past;
+  };
+  if (__builtin_expect(__builtin_amdgcn_ballot_w64(run(std::false_type{})) != 0, 0))
+    run(std::true_type{});
   const float mw = wave_max(m);
   const float f = m == -INFINITY && l == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m - mw);
   l *= f;
@@ -261,7 +277,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
     const size_t at = static_cast<size_t>(split) * rows + row;
     part[at * HD + lane] = o;
     if (lane == 0)
-      *reinterpret_cast<float2*>(part + a.splits * rows * HD + 2 * at) = make_float2(mg, lg);
+      *reinterpret_cast<float4*>(part + a.splits * rows * HD + 4 * at) =
+          make_float4(mg, 0.0f, lg, 0.0f);
   } else {
     out[vkc::row_at(a.rows, a.heads, s, h, 0) + d0 + lane] = lg == 0.0f ? 0.0f : o / lg * kRowUp;
   }
@@ -290,6 +307,7 @@ constexpr int kKPitch = 144;    // bytes of a K row in LDS: 64 f16 + 16
 constexpr int kVPitch = 192;    // of a V row: 64 f16 + 64
 constexpr float kPBits = 9.0f, kSlack = 6.0f;
 constexpr float kLowest = -3e38f;       // the running reference before any key
+constexpr float kFar = 65536.0f;        // scores of this size are taken from the row's own base
 constexpr float kLeastLsv = -88.0f;     // of a key's V in the choice of the reference
 constexpr int kCap = 1, kBias = 2;      // what SCORE does to a product beside its scale
 constexpr int kQUp = 10;                // binary digits that Q is scaled up by
@@ -441,6 +459,7 @@ struct Queries {
   u32x4 q[4][2];         // two f16 parts of eight values, four steps of 16 d
   float back;            // 1, or what the row's own scale has to be undone by
   bool own_scale;        // uniform: some row has one
+  bool far;              // uniform: some row has a base
   float slope, cap_up;   // per unit of distance and cap, in base 2
   int pos, doc;
   int seen;              // causal: keys below it are seen
@@ -465,7 +484,7 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
   const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
   const bool usual = m == 0.0f || (e >= -10 && e < 5);
   int up = usual ? kQUp : 14 - e;
-  up = up > 120 ? 120 : up;
+  up = up > 127 ? 127 : up;
   const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
   w.back = __uint_as_float(static_cast<uint32_t>(127 + kQUp - up) << 23);
   w.own_scale = __builtin_amdgcn_ballot_w64(up != kQUp) != 0;
@@ -486,6 +505,17 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
     for (int r = 0; r < 16; ++r) w.o[dt][r] = 0.0f;
   w.m = kLowest;
   w.l = 0.0f;
+  w.far = false;
+}
+
+// A row's base in LDS, 0 at first: once a row's reference passes +-kFar its scores are taken as
+// differences from the base (exact near it), and so are the references, which hold V's scales
+// and kPBits: beside a score of 2^26 f32 has no bits for those.
+__device__ __forceinline__ float& base_of(float* bases) { return bases[threadIdx.x & 31]; }
+
+// The reference of a join: (reference, base) pairs by their exact difference.
+__device__ __forceinline__ float apart(const float2& a, const float2& b) {
+  return (a.y - b.y) + (a.x - b.x);
 }
 
 // Two weights as f16 parts, packed: the remainder by one mixed-precision FMA each.
@@ -519,6 +549,17 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
     for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
 }
 
+// Half (the second half: `rest` 1) of the undoing of a row's own scale, a power of two.
+__device__ __forceinline__ void unscale(f32x16 (&s)[2], float back, int rest) {
+  asm volatile("" : "+v"(back));  // keeps the work in the branch around it
+  const int x = static_cast<int>(__float_as_uint(back) >> 23) - 127;
+  const float f = __uint_as_float(static_cast<uint32_t>(127 + ((x + rest) >> 1)) << 23);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[t][r] *= f;
+}
+
 // The scores of a block from the products: scales, cap, bias and masks, base 2;
 // `left` keys of it are held, `masked` (uniform) says whether a query of the wave may
 // not see some of them.  Moves the reference of queries whose weights would leave
@@ -526,17 +567,13 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
 // part of the value sum, once that passes it by kSlack.
 template <int SCORE, bool MASK>
 __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Rules& ru,
-                                            const KeyRegs& key, int k0, int left, bool masked) {
+                                            const KeyRegs& key, int k0, int left, bool masked,
+                                            float* bases) {
   const int half = (threadIdx.x & 63) >> 5;
+  // a row's own scale is undone in two steps about K's: either alone may leave f32's range
+  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.back, 0);
   each<32>([&](auto i) { s[i / 16][i % 16] *= bcast<i % 16>(key.ks[i / 16]); });
-  if (__builtin_expect(w.own_scale, 0)) {
-    float back = w.back;
-    asm volatile("" : "+v"(back));  // keeps the products in this branch
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s[t][r] *= back;
-  }
+  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.back, 1);
   if constexpr (SCORE != 0) __builtin_amdgcn_sched_barrier(0);
   if constexpr ((SCORE & kCap) != 0) {
     // scores far below the cap, the usual case, are the series' alone (3 x 16 x 1,301 queries
@@ -566,6 +603,13 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
       for (int r = 0; r < 16; ++r)
         s[t][r] = __builtin_fmaf(-w.slope, fabsf(base - (32 * t + 8 * (r / 4) + r % 4)), s[t][r]);
   }
+  if (__builtin_expect(w.far, 0)) {
+    const float base = base_of(bases);
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[t][r] -= base;
+  }
   // nothing of the rules' work is begun ahead of it, in registers that the tile has not
   if constexpr (SCORE != 0) __builtin_amdgcn_sched_barrier(0);
   const bool causal = MASK && masked && ru.causal;
@@ -594,7 +638,22 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
   each<32>([&](auto i) { mb = fmaxf(mb, s[i / 16][i % 16] + bcast<i % 16>(lsv[i / 16])); });
   if (__builtin_amdgcn_ballot_w64(mb > w.m + kSlack) != 0) {
     mb = fmaxf(mb, other_half(mb));
-    const bool moves = mb > w.m + kSlack;
+    bool moves = mb > w.m + kSlack;
+    if (__builtin_expect(__builtin_amdgcn_ballot_w64(moves && fabsf(mb) >= kFar) != 0, 0)) {
+      // the base moves there, and what V's scales add is seen again without the score's rounding
+      const float by = moves && fabsf(mb) >= kFar ? mb : 0.0f, base = base_of(bases);
+      const float to = base + by, shift = to - base;
+      base_of(bases) = to;
+      vkd::wave_lds_fence();
+      w.far = true;
+      w.m = fmaxf(w.m - shift, kLowest);
+      float again = kLowest;
+      each<32>([&](auto i) {
+        s[i / 16][i % 16] -= shift;
+        again = fmaxf(again, s[i / 16][i % 16] + bcast<i % 16>(lsv[i / 16]));
+      });
+      mb = fmaxf(again, other_half(again));
+    }
     // in two steps: V's scales, which the references carry, may be far apart
     const float f = moves ? __builtin_amdgcn_exp2f(0.5f * (w.m - mb)) : 1.0f;
 #pragma unroll
@@ -841,11 +900,11 @@ __device__ __forceinline__ void store_part(float* part, const Shape& a, uint32_t
 }
 
 __device__ __forceinline__ void store_ml(float* part, const Shape& a, uint32_t split, uint32_t s,
-                                         uint32_t h, uint32_t i, float m, float l) {
+                                         uint32_t h, uint32_t i, float m, float l, float base) {
   const size_t rows = static_cast<size_t>(a.rows.sequences) * a.heads * a.rows.n;
   const size_t at = static_cast<size_t>(split) * rows +
                     (static_cast<size_t>(s) * a.heads + h) * a.rows.n + i;
-  *reinterpret_cast<float2*>(part + a.splits * rows * HD + 2 * at) = make_float2(m, l);
+  *reinterpret_cast<float4*>(part + a.splits * rows * HD + 4 * at) = make_float4(m, base, l, 0.0f);
 }
 
 __device__ __forceinline__ f32x4 quotient(const f32x4& o, float l) {
@@ -931,6 +990,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
   __shared__ KeyData kd[2];
   __shared__ uint16_t list[MASK ? kList : 1];
   __shared__ int wave_count[QW], doc_range[2 * QW];
+  __shared__ float base[QW][32];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
   __builtin_assume(tid < kThreads);
   const Rules& ru = a.rules;
@@ -964,6 +1024,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
   Queries w;
   take_queries<SCORE, MASK, 16, 8>(w, q, a, s, kh, row < row_end ? row : row_end - 1, &i, &h);
 
+  base_of(base[wave]) = 0.0f;  // (both lanes of a query, the same)
   const int blocks = (keys + KB - 1) / KB;
   Span span;
   if constexpr (MASK)
@@ -1002,7 +1063,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) score_step(sc, w, kl[buf], ks);
         const KeyRegs key = key_regs(kd[buf], MASK && ru.q_docs);
-        score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0);
+        score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0, base[wave]);
         // ahead of the CU's other waves while it feeds the matrix cores (12 x 866 queries over
         // 10,392 keys 79.7 us without, 76.3 so; masked 413 and 408), and up to the barrier where
         // its blocks go by in step with theirs (73.4; masked 413)
@@ -1032,7 +1093,7 @@ __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_
       else
         *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, h, i) + d) = quotient(o, l);
     }
-  if (part && half == 0) store_ml(part, a, split, s, h, i, w.m, l);
+  if (part && half == 0) store_ml(part, a, split, s, h, i, w.m, l, base_of(base[wave]));
 }
 
 // 32 rows or fewer of a cache head: the waves of a workgroup hold the same queries and
@@ -1046,7 +1107,8 @@ template <int FORMAT, int SCORE, bool MASK>
 __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
     const float* __restrict__ q, float* __restrict__ out, float* __restrict__ part, Shape a) {
   __shared__ __align__(16) char vl[kFewWaves][KB * kVPitch];
-  __shared__ float sm[kFewWaves][32], sl[kFewWaves][32];
+  __shared__ float2 sm[kFewWaves][32];  // reference, base
+  __shared__ float sl[kFewWaves][32], base[kFewWaves][32];
   __shared__ uint16_t list[MASK ? kList : 1];
   __shared__ int wave_count[kFewWaves], doc_range[2 * kFewWaves];
   const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, half = lane >> 5;
@@ -1064,6 +1126,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
   uint32_t i, h;
   Queries w;
   take_queries<SCORE, MASK, 8, 32>(w, q, a, s, kh, row < rows ? row : rows - 1, &i, &h);
+  base_of(base[wave]) = 0.0f;
   const int blocks = (keys + KB - 1) / KB;
   Span span;
   if constexpr (MASK) span = tile_span<kFewWaves>(w, a, s, 0, rows - 1, true, doc_range);
@@ -1155,7 +1218,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
       const int e1 = entry(x + kFewWaves < b_end ? x + kFewWaves : x);
       load(key_of(e1));
       vkd::wave_lds_fence();
-      score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0);
+      score_block<SCORE, MASK>(sc, w, ru, key, k0, keys - k0, (e & 1) != 0, base[wave]);
       value_block(sc, w, vw, key);
       vkd::wave_lds_fence();
       e = e1;
@@ -1174,21 +1237,21 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
       *reinterpret_cast<f32x4*>(so + row * kOPitch + 32 * dt + 8 * r + 4 * half) =
           f32x4{w.o[dt][4 * r], w.o[dt][4 * r + 1], w.o[dt][4 * r + 2], w.o[dt][4 * r + 3]};
   if (half == 0) {
-    sm[wave][row] = w.m;
+    sm[wave][row] = make_float2(w.m, base_of(base[wave]));
     sl[wave][row] = w.l;
   }
   __syncthreads();
   for (int x = tid; x < 16 * rows; x += 64 * kFewWaves) {
     const int r = x >> 4, d = 4 * (x & 15);
-    float m = sm[0][r];
+    float2 m = sm[0][r];
 #pragma unroll
-    for (int y = 1; y < kFewWaves; ++y) m = fmaxf(m, sm[y][r]);
+    for (int y = 1; y < kFewWaves; ++y) m = apart(sm[y][r], m) > 0.0f ? sm[y][r] : m;
     float l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int y = 0; y < kFewWaves; ++y) {
       // in two steps: V's scales, which the references carry, may be far apart
-      const float f = sl[y][r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(0.5f * (sm[y][r] - m));
+      const float f = sl[y][r] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(0.5f * apart(sm[y][r], m));
       l += sl[y][r] * f * f;
       o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(vl[y]) + r * kOPitch + d) *
            f * f;
@@ -1196,7 +1259,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
     const uint32_t ri = r / a.group, rh = kh * a.group + (r - ri * a.group);
     if (part) {
       store_part(part, a, split, s, rh, ri, d, o);
-      if (d == 0) store_ml(part, a, split, s, rh, ri, m, l);
+      if (d == 0) store_ml(part, a, split, s, rh, ri, m.x, l, m.y);
     } else {
       *reinterpret_cast<f32x4*>(out + vkc::row_at(a.rows, a.heads, s, rh, ri) + d) = quotient(o, l);
     }
@@ -1217,8 +1280,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
   const uint32_t sh = static_cast<uint32_t>(row / a.rows.n);
   const uint32_t h = sh % a.heads, s = sh / a.heads;
   if (static_cast<int>(i) >= vkc::count_of(a.rows, s)) return;
-  const float2* ml = reinterpret_cast<const float2*>(part + a.splits * rows * HD);
-  float2 x[PER];
+  const float4* ml = reinterpret_cast<const float4*>(part + a.splits * rows * HD);
+  float4 x[PER];  // reference, base, denominator
   f32x4 y[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -1226,20 +1289,24 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
     const size_t at = (sp < a.splits ? sp : 0) * rows + row;
     x[j] = ml[at];
     y[j] = *reinterpret_cast<const f32x4*>(part + at * HD + 4 * c);
-    if (sp >= a.splits) x[j].y = 0.0f;
+    if (sp >= a.splits) x[j].z = 0.0f;
   }
-  float m = -INFINITY;
+  float2 m = make_float2(x[0].x, x[0].y);  // again the first past the last
+  const auto larger = [&](const float2& o) { m = apart(o, m) > 0.0f ? o : m; };
 #pragma unroll
-  for (int j = 0; j < PER; ++j) m = fmaxf(m, x[j].x);  // again the first past the last
-  m = fmaxf(m, __shfl_xor(m, 16, 64));
-  m = fmaxf(m, __shfl_xor(m, 32, 64));
+  for (int j = 1; j < PER; ++j) larger(make_float2(x[j].x, x[j].y));
+#pragma unroll
+  for (int w = 16; w <= 32; w <<= 1)
+    larger(make_float2(__shfl_xor(m.x, w, 64), __shfl_xor(m.y, w, 64)));
   float l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
     // in two steps: V's scales, which the references carry, may be far apart
-    const float w = x[j].y != 0.0f ? __builtin_amdgcn_exp2f(0.5f * (x[j].x - m)) : 0.0f;
-    l += x[j].y * w * w;
+    const float w = x[j].z != 0.0f
+                        ? __builtin_amdgcn_exp2f(0.5f * apart(make_float2(x[j].x, x[j].y), m))
+                        : 0.0f;
+    l += x[j].z * w * w;
     o += y[j] * w * w;
   }
 #pragma unroll
@@ -1347,7 +1414,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
   if (splits > 1) {
-    VK_TRY(vk::ensure_work(rt, splits * rows * (HD + 2), "attention_cached"));
+    VK_TRY(vk::ensure_work(rt, splits * rows * (HD + 4), "attention_cached"));
     part = rt->work;
   }
   // 8 / share groups of `heads` pairs each

@@ -186,7 +186,8 @@ int split_weights(vk_linear* lin, bool f16_values);
 // run the sequence once eagerly first.  The buffer it replaces is retired,
 // not freed.
 int ensure_work(vk_runtime* rt, size_t floats, const char* who);
-// VK_ERR_INVALID unless `t` lies on the runtime's device.
+// VK_ERR_INVALID unless `t` lies on the runtime's device, at a multiple of its
+// values' size.
 int check_device(const vk_runtime* rt, const vk_tensor* t, const char* what);
 // VK_ERR_INVALID unless `t` is f32 [len], 16-byte aligned and on the runtime's
 // device.

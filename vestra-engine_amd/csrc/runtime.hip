@@ -174,6 +174,8 @@ int ensure_work(vk_runtime* rt, size_t floats, const char* who) {
 
 int check_device(const vk_runtime* rt, const vk_tensor* t, const char* what) {
   VK_REQUIRE(t && t->rt && t->rt->device == rt->device, "%s: a tensor of another device", what);
+  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % dtype_size(t->dtype) == 0, "%s is misaligned",
+             what);
   return VK_OK;
 }
 

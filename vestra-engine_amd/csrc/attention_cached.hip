@@ -912,9 +912,17 @@ __device__ __forceinline__ f32x4 quotient(const f32x4& o, float l) {
   return f32x4{o[0] / l, o[1] / l, o[2] / l, o[3] / l};
 }
 
+// A lane's offset into a buffer, so that what a load adds to it is added there, as the
+// instruction's own offset, and not ahead of the loop in a register each.
+__device__ __forceinline__ int here(int offset) {
+  asm volatile("" : "+v"(offset));
+  return offset;
+}
+
 // Staging by all threads: eight codes of K (or V) a thread and row.  The block's
 // rows are a buffer of their own (its base and the bytes left of it in scalar registers), so
-// a load has no address arithmetic and keys past the end read zeros.
+// a load has no address arithmetic and keys past the end read zeros (every offset is part of
+// the lane's, a constant of it in the instruction: the uniform offset is left out of bounds checks).
 template <int FORMAT, int THREADS>
 struct StageRows {
   static constexpr int kPer = KB * 8 / THREADS;
@@ -925,10 +933,11 @@ struct StageRows {
     const int left = keys - k0 < KB ? keys - k0 : KB;
     const __amdgpu_buffer_rsrc_t r =
         vkd::buffer_rsrc(codes + (first + k0) * HD, static_cast<uint32_t>(left * HD));
+    const int at = here(8 * static_cast<int>(threadIdx.x));
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const i32x2_t x = __builtin_amdgcn_raw_buffer_load_b64(
-          r, static_cast<int>(8 * threadIdx.x), 8 * THREADS * i, 0);
+          r, at + 8 * THREADS * i, 0, 0);
       w[i] = make_uint2(static_cast<uint32_t>(x[0]), static_cast<uint32_t>(x[1]));
     }
   }
@@ -1143,29 +1152,29 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
         vkd::buffer_rsrc(a.cache.k + (first + k0) * HD, static_cast<uint32_t>(left * HD));
     const __amdgpu_buffer_rsrc_t vb =
         vkd::buffer_rsrc(a.cache.v + (first + k0) * HD, static_cast<uint32_t>(left * HD));
-    const int k_off = (lane & 31) * HD + 32 * half;
+    const int k_off = here((lane & 31) * HD + 32 * half), v_off = here(16 * lane);
 #pragma unroll
     for (int t = 0; t < 2; ++t)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        kr[t][x] = __builtin_amdgcn_raw_buffer_load_b128(kb, k_off, 32 * HD * t + 16 * x, 0);
+        kr[t][x] = __builtin_amdgcn_raw_buffer_load_b128(kb, k_off + 32 * HD * t + 16 * x, 0, 0);
 #pragma unroll
     for (int x = 0; x < 4; ++x)
-      vr[x] = __builtin_amdgcn_raw_buffer_load_b128(vb, 16 * lane, 1024 * x, 0);
+      vr[x] = __builtin_amdgcn_raw_buffer_load_b128(vb, v_off + 1024 * x, 0, 0);
     const __amdgpu_buffer_rsrc_t ksb = vkd::buffer_rsrc(a.cache.ks + first + k0, 4 * left);
     const __amdgpu_buffer_rsrc_t vsb = vkd::buffer_rsrc(a.cache.vs + first + k0, 4 * left);
-    const int at = 4 * (8 * ((lane & 15) >> 2) + 4 * half + (lane & 3));
+    const int at = here(4 * (8 * ((lane & 15) >> 2) + 4 * half + (lane & 3)));
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      kss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksb, at, 128 * t, 0));
-      vss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsb, at, 128 * t, 0));
+      kss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(ksb, at + 128 * t, 0, 0));
+      vss[t] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(vsb, at + 128 * t, 0, 0));
     }
     if (MASK && ru.q_docs) {
       const __amdgpu_buffer_rsrc_t db =
           vkd::buffer_rsrc(ru.k_docs + doc_first + k0, 4 * left);
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        docs[t] = static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(db, at, 128 * t, 0));
+        docs[t] = static_cast<int>(__builtin_amdgcn_raw_buffer_load_b32(db, at + 128 * t, 0, 0));
     }
   };
   char* vw = vl[wave];

@@ -474,8 +474,9 @@ __device__ __forceinline__ float f16_to_f32(uint16_t h) {
 
 // Raw buffer loads: a buffer resource (base address and byte size, held in
 // scalar registers) plus a 32-bit per-lane byte offset and a uniform byte
-// offset, with no 64-bit address arithmetic per load.  Reads at or past
-// `bytes` return zeros.  Third descriptor word: the gfx9-family raw-buffer
+// offset, with no 64-bit address arithmetic per load.  Reads whose lane offset is
+// at or past `bytes` return zeros; the uniform offset is added after that check,
+// so with one the caller stays inside.  Third descriptor word: the gfx9-family raw-buffer
 // format (32-bit data, no swizzle).
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void* base, uint32_t bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0,

@@ -136,12 +136,12 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const int blocks = (keys + 63) / 64;
   const int b0 = static_cast<int>(static_cast<long long>(split) * blocks / a.splits);
   const int b1 = static_cast<int>(static_cast<long long>(split + 1) * blocks / a.splits);
-  // The wave's blocks; whether q . code went past f32's range somewhere, which K's scale may
-  // bring it back into: `small` takes the codes times kDown.
+  // The wave's blocks; whether q . code of a key that is seen went past f32's range, which K's
+  // scale may bring it back into: `small` takes the codes times kDown.
   const auto run = [&](auto small) {
     constexpr bool kSmall = decltype(small)::value;
     constexpr float kDown = 0x1p-24f;
-    bool past = false;
+    uint32_t past = 0;
     m = -INFINITY;
     l = 0.0f;
 #pragma unroll
@@ -181,7 +181,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
       const float dot = (u[0] + u[1]) + (u[2] + u[3]);
       float t = dot * ks * ru.scale;
       if constexpr (kSmall) t *= 1.0f / kDown;
-      past = past || !(fabsf(dot) <= 3.4028235e38f);
+      // (a hidden code may be no number)
+      past = max(past, seen ? __float_as_uint(dot) & 0x7fffffffu : 0u);
       if (ru.cap > 0.0f) t = ru.cap * tanhf(t / ru.cap);
       if (ru.slopes) {
         const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
@@ -214,7 +215,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
         }
       }
     }
-    return past;
+    return past >= 0x7f800000u;
   };
   if (__builtin_expect(__builtin_amdgcn_ballot_w64(run(std::false_type{})) != 0, 0))
     run(std::true_type{});

@@ -28,3 +28,19 @@ def test_hidden_codes_change_no_bit_of_small_queries(rt, rng, n, keys, code):
     codes[:, :, hidden, ::7] = code
     c.cache.k.write(codes.reshape(-1))
     assert np.array_equal(c.run(docs), want)
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("qs,ks,rule", [
+    (1e27, 1e-27, {"scale": 0.125, "cap": 2e-13}),         # q scale / cap past f32's largest
+    (3e37, 1e-30, {"scale": 2.0 ** 30, "cap": 2.0 ** 32}),
+    (1e30, 1e-28, {"scale": 2.0 ** 39}),                   # q scale past it
+    (1e-36, 1e25, {"scale": 2.0 ** 39, "cap": 2.0 ** 79}),  # q scale / cap below its smallest
+    (1e-38, 3e37, {"scale": 2.0 ** -39}), (1e-42, 1e35, {"scale": 2.0 ** 25}),
+    (1e-38, 3e37, {"scale": -0.125}), (3e37, 1e-38, {"scale": 0.25, "cap": 1.0}),
+])
+def test_scaled_queries_outside_f32(rt, rng, fmt, n, qs, ks, rule):
+    """Scores in range, of a query times the scale (over the cap) that is not."""
+    c = Case(rt, rng, fmt, 1, 2, 2, 330, n, [330 - n], qs=qs, ks=ks).fill()
+    c.check(rule, label=f"{qs} {ks} {rule}")

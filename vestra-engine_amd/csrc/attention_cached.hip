@@ -458,7 +458,7 @@ __device__ __forceinline__ float tanh1(float x) {
 // A wave's 32 queries: lane l and lane l ^ 32 hold query l % 32.
 struct Queries {
   u32x4 q[4][2];         // two f16 parts of eight values, four steps of 16 d
-  float back;            // 1, or what the row's own scale has to be undone by
+  int undo;              // the power of two that undoes the row's own scale (usually 0)
   bool own_scale;        // uniform: some row has one
   bool far;              // uniform: some row has a base
   float slope, cap_up;   // per unit of distance and cap, in base 2
@@ -468,6 +468,16 @@ struct Queries {
   float m, l;            // running reference, this lane's denominators
 };
 
+// 2^x, -126 <= x <= 127.
+__device__ __forceinline__ float pow2(int x) {
+  return __uint_as_float(static_cast<uint32_t>(127 + x) << 23);
+}
+__device__ __forceinline__ int exponent(float v) {
+  return static_cast<int>(__float_as_uint(v) >> 23) - 127;
+}
+
+// q c, scaled by a power of two of its own where a row's largest is not of the usual size:
+// neither q c nor what undoes the scale has to be in f32's range (c is within 2^41 of 1).
 // The order of d: element j of step ks is d = DK ks + DH half + j.
 template <int DK, int DH>
 __device__ __forceinline__ void load_queries(Queries& w, const float* row, float c, int half) {
@@ -477,22 +487,23 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
   for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      x[ks][i] = *reinterpret_cast<const f32x4*>(row + DK * ks + DH * half + 4 * i) * c;
+      x[ks][i] = *reinterpret_cast<const f32x4*>(row + DK * ks + DH * half + 4 * i);
 #pragma unroll
       for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[ks][i][e]));
     }
   m = fmaxf(m, other_half(m));
-  const int e = static_cast<int>(__float_as_uint(m) >> 23) - 127;
+  const int eq = min(exponent(m), 126);
+  const float down = pow2(-eq);
+  const int e = eq + exponent(m * down * fabsf(c));  // of the largest |q c|
   const bool usual = m == 0.0f || (e >= -10 && e < 5);
-  int up = usual ? kQUp : 14 - e;
-  up = up > 127 ? 127 : up;
-  const float f = __uint_as_float(static_cast<uint32_t>(127 + up) << 23);
-  w.back = __uint_as_float(static_cast<uint32_t>(127 + kQUp - up) << 23);
+  const int up = usual ? kQUp : 14 - e;
+  const float f = c * pow2(eq + up);
+  w.undo = kQUp - up;
   w.own_scale = __builtin_amdgcn_ballot_w64(up != kQUp) != 0;
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) {
     uint32_t h[4], l[4];
-    const f32x4 a = x[ks][0] * f, b = x[ks][1] * f;
+    const f32x4 a = x[ks][0] * down * f, b = x[ks][1] * down * f;
     vks::split2_plain(a[0], a[1], &h[0], &l[0]);
     vks::split2_plain(a[2], a[3], &h[1], &l[1]);
     vks::split2_plain(b[0], b[1], &h[2], &l[2]);
@@ -550,11 +561,10 @@ __device__ __forceinline__ void clear(f32x16 (&s)[2]) {
     for (int r = 0; r < 16; ++r) s[t][r] = 0.0f;
 }
 
-// Half (the second half: `rest` 1) of the undoing of a row's own scale, a power of two.
-__device__ __forceinline__ void unscale(f32x16 (&s)[2], float back, int rest) {
-  asm volatile("" : "+v"(back));  // keeps the work in the branch around it
-  const int x = static_cast<int>(__float_as_uint(back) >> 23) - 127;
-  const float f = __uint_as_float(static_cast<uint32_t>(127 + ((x + rest) >> 1)) << 23);
+// Half (the second half: `rest` 1) of the undoing of a row's own scale.
+__device__ __forceinline__ void unscale(f32x16 (&s)[2], int undo, int rest) {
+  asm volatile("" : "+v"(undo));  // keeps the work in the branch around it
+  const float f = pow2((undo + rest) >> 1);
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -572,9 +582,9 @@ __device__ __forceinline__ void score_block(f32x16 (&s)[2], Queries& w, const Ru
                                             float* bases) {
   const int half = (threadIdx.x & 63) >> 5;
   // a row's own scale is undone in two steps about K's: either alone may leave f32's range
-  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.back, 0);
+  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.undo, 0);
   each<32>([&](auto i) { s[i / 16][i % 16] *= bcast<i % 16>(key.ks[i / 16]); });
-  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.back, 1);
+  if (__builtin_expect(w.own_scale, 0)) unscale(s, w.undo, 1);
   if constexpr (SCORE != 0) __builtin_amdgcn_sched_barrier(0);
   if constexpr ((SCORE & kCap) != 0) {
     // scores far below the cap, the usual case, are the series' alone (3 x 16 x 1,301 queries
@@ -1362,7 +1372,7 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   VK_REQUIRE(std::isfinite(ru.scale), "attention_cached: scale %g", static_cast<double>(ru.scale));
   VK_REQUIRE(std::isfinite(ru.cap) && ru.cap >= 0.0f, "attention_cached: cap %g",
              static_cast<double>(ru.cap));
-  // what a query is multiplied by keeps its values normal numbers
+  // so that what a query is multiplied by, and what undoes a row's own scale, are normal numbers
   const float scale = ru.scale == 0.0f ? 0.125f : ru.scale;
   const float by = std::fabs(ru.cap > 0.0f ? scale / ru.cap : scale);
   VK_UNSUPPORTED_IF(!(by >= 0x1p-40f && by <= 0x1p40f && std::fabs(scale) >= 0x1p-40f &&

@@ -44,3 +44,15 @@ def test_scaled_queries_outside_f32(rt, rng, fmt, n, qs, ks, rule):
     """Scores in range, of a query times the scale (over the cap) that is not."""
     c = Case(rt, rng, fmt, 1, 2, 2, 330, n, [330 - n], qs=qs, ks=ks).fill()
     c.check(rule, label=f"{qs} {ks} {rule}")
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("qs,ks", [(1e22, 1e22), (1e30, 1e10), (1e10, 1e30)])
+def test_products_that_a_small_scale_brings_back(rt, rng, n, qs, ks):
+    """q . k past f32's largest, the score far inside: one key has all the weight."""
+    c = Case(rt, rng, 0, 1, 2, 2, 330, n, [330 - n], qs=qs, ks=ks).fill()
+    got = c.check({"scale": 2.0 ** -40})
+    assert np.isfinite(got).all()
+    q, k = c.q.astype(np.float64), c.kh
+    best = np.argmax(np.einsum("shid,shjd->shij", q, k), -1)
+    assert np.allclose(got[0, 1, 0], c.vheld[0, 1, best[0, 1, 0]], rtol=1e-6, atol=1e-12)

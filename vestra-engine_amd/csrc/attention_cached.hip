@@ -121,6 +121,10 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
   const int d0 = PARTS > 1 ? static_cast<int>(blockIdx.x / all) * ND : 0;
   const uint32_t h = row % a.heads, s = row / a.heads;
   const Rules& ru = a.rules;
+  // a scale below 1 comes before K's, one above 1 after it: neither product leaves f32's
+  // range where the score is inside
+  const bool less = fabsf(ru.scale) < 1.0f;
+  const float before = less ? ru.scale : 1.0f, after = less ? 1.0f : ru.scale;
   // every scalar together: none waits for another
   const int count = vkc::count_of(a.rows, s), start = vkc::start_of(a.rows, s);
   const float slope = ru.slopes ? ru.slopes[h] : 0.0f;
@@ -179,7 +183,7 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
         }
       }
       const float dot = (u[0] + u[1]) + (u[2] + u[3]);
-      float t = dot * ks * ru.scale;
+      float t = dot * before * ks * after;
       if constexpr (kSmall) t *= 1.0f / kDown;
       // (a hidden code may be no number)
       past = max(past, seen ? __float_as_uint(dot) & 0x7fffffffu : 0u);

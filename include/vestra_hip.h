@@ -603,7 +603,8 @@ typedef struct vk_attention_rules {
  * counts[s] are left as they were.  A query that sees a key that reads back
  * as NaN gets NaN; keys that it does not see have no effect whatever they
  * hold, slots that nothing wrote too (codes 0x7f and 0xff of VK_CACHE_F8,
- * which the write never makes, count as zeros in V).  Scores, weights and
+ * which the write never makes, count as zeros in V).  A scale that is infinite,
+ * which the write never makes either, counts as a NaN.  Scores, weights and
  * sums are held as in f32: the values of the cache are exact in f16, queries
  * and weights are taken as two f16 parts (a query's value to 2^-25 of its
  * row's largest, a weight times V's scale to 2^-34 of the largest; one query:

@@ -56,3 +56,27 @@ def test_products_that_a_small_scale_brings_back(rt, rng, n, qs, ks):
     q, k = c.q.astype(np.float64), c.kh
     best = np.argmax(np.einsum("shid,shjd->shij", q, k), -1)
     assert np.allclose(got[0, 1, 0], c.vheld[0, 1, best[0, 1, 0]], rtol=1e-6, atol=1e-12)
+
+
+@pytest.mark.parametrize("n", ROWS)
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("which", ["k_scale", "v_scale"])
+@pytest.mark.parametrize("scale", [np.inf, -np.inf, np.nan])
+def test_scales_that_are_no_number(rt, rng, n, fmt, which, scale):
+    """An infinite or NaN scale, put there by hand: NaN to every query that sees the key, in
+    every column, whatever its codes and its score are."""
+    keys = 200
+    c = Case(rt, rng, fmt, 1, 2, 2, keys, n, [keys - n]).fill()
+    bad = 77
+    c.k[:, :, bad], c.v[:, :, bad, ::2] = 0.5 * c.k[:, :, bad], 0.0
+    c.fill()
+    want = c.run()
+    t = getattr(c.cache, which)
+    scales = t.numpy().reshape(1, 2, keys)
+    scales[0, 1, bad] = scale
+    t.write(scales.reshape(-1))
+    got = c.run()
+    assert np.array_equal(got[:, 0], want[:, 0]) and np.isnan(got[:, 1]).all()
+    # a score of -inf beside it
+    c.q[0, 1, 0] = -1e30 * np.sign(c.kh[0, 1, bad])
+    assert np.isnan(c.run()[0, 1, 0]).all()

@@ -192,7 +192,8 @@ __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const flo
         const long long far = p > j ? static_cast<long long>(p) - j : static_cast<long long>(j) - p;
         t -= slope * static_cast<float>(far);
       }
-      t *= kLog2e;
+      // (a scale that is infinite or a NaN, of K or of V, makes the score a NaN)
+      t = t * kLog2e + ((ks - ks) + (vs - vs));
       seen = seen && !(t == -INFINITY);
       if (seen && t > m + kRoom) {
         const float f = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - t);
@@ -403,7 +404,7 @@ __device__ __forceinline__ uint2 read_tr(const char* p) {
 // What a block's keys bring beside their codes, in LDS: 64 of each, key 32 t + 8
 // (r / 4) + 4 half + r % 4 at 32 t + 16 half + r.
 struct KeyData {
-  float ks[KB];   // K's scale / 2^kQUp (a NaN where V's scale is one, or infinite)
+  float ks[KB];   // K's scale / 2^kQUp (a NaN where a scale of the key is no finite number)
   float lsv[KB];  // log2 of V's scale, at least kLeastLsv
   float sv[KB];   // V's scale (0 there)
   int doc[KB];
@@ -430,9 +431,9 @@ __device__ __forceinline__ KeyRegs key_regs(const KeyData& kd, bool docs) {
 
 // ks, lsv and sv from the scales of a row of K and of V.
 __device__ __forceinline__ void key_values(float k, float v, float* ks, float* lsv, float* sv) {
-  const bool nan = !(fabsf(v) <= 3.4028235e38f);
-  *ks = nan ? NAN : k * (1.0f / (1 << kQUp));
-  *sv = nan ? 0.0f : v;
+  const float odd = (k - k) + (v - v);  // 0, or a NaN
+  *ks = __builtin_fmaf(k, 1.0f / (1 << kQUp), odd);
+  *sv = odd == 0.0f ? v : 0.0f;
   *lsv = fmaxf(__builtin_amdgcn_logf(fmaxf(*sv, vkc::kLeastScale)), kLeastLsv);
 }
 

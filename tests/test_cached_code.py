@@ -24,3 +24,15 @@ def test_every_offset_is_inside_the_bounds_check(kernel):
         for x in loads:
             scalar = x.split(", ")[3].split()[0]
             assert scalar == "0", (name, x)
+
+
+@pytest.mark.parametrize("kernel", ["attention_few_kernel", "attention_row_kernel",
+                                    "attention_join_kernel"])
+def test_short_chains_hold_nothing_in_scratch(kernel):
+    """Kernels that are bound by the latency of one chain: no spilled vector register and no
+    array or choice of addresses that lives in memory."""
+    found = code_objects.kernels(LIBRARY, kernel)
+    assert found
+    for name, (values, code) in found.items():
+        assert values["private_segment_fixed_size"] == 0 and values["vgpr_spill_count"] == 0, name
+        assert not [x for x in code if x.startswith(("scratch_", "flat_"))], name

@@ -531,8 +531,15 @@ __device__ __forceinline__ void load_queries(Queries& w, const float* row, float
 __device__ __forceinline__ float& base_of(float* bases) { return bases[threadIdx.x & 31]; }
 
 // The reference of a join: (reference, base) pairs by their exact difference.
-__device__ __forceinline__ float apart(const float2& a, const float2& b) {
+__device__ __forceinline__ float apart(float2 a, float2 b) {
   return (a.y - b.y) + (a.x - b.x);
+}
+
+// That of the two that stands higher, by value: a choice between an LDS element and a local
+// would be one of addresses, and the local be kept in scratch.
+__device__ __forceinline__ float2 larger(float2 a, float2 m) {
+  const bool more = apart(a, m) > 0.0f;
+  return make_float2(more ? a.x : m.x, more ? a.y : m.y);
 }
 
 // Two weights as f16 parts, packed: the remainder by one mixed-precision FMA each.
@@ -1270,7 +1277,7 @@ __global__ __launch_bounds__(64 * kFewWaves, 2) void attention_few_kernel(
     const int r = x >> 4, d = 4 * (x & 15);
     float2 m = sm[0][r];
 #pragma unroll
-    for (int y = 1; y < kFewWaves; ++y) m = apart(sm[y][r], m) > 0.0f ? sm[y][r] : m;
+    for (int y = 1; y < kFewWaves; ++y) m = larger(sm[y][r], m);
     float l = 0.0f;
     f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -1317,12 +1324,11 @@ __global__ __launch_bounds__(256) void attention_join_kernel(const float* __rest
     if (sp >= a.splits) x[j].z = 0.0f;
   }
   float2 m = make_float2(x[0].x, x[0].y);  // again the first past the last
-  const auto larger = [&](const float2& o) { m = apart(o, m) > 0.0f ? o : m; };
 #pragma unroll
-  for (int j = 1; j < PER; ++j) larger(make_float2(x[j].x, x[j].y));
+  for (int j = 1; j < PER; ++j) m = larger(make_float2(x[j].x, x[j].y), m);
 #pragma unroll
   for (int w = 16; w <= 32; w <<= 1)
-    larger(make_float2(__shfl_xor(m.x, w, 64), __shfl_xor(m.y, w, 64)));
+    m = larger(make_float2(__shfl_xor(m.x, w, 64), __shfl_xor(m.y, w, 64)), m);
   float l = 0.0f;
   f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll

@@ -86,3 +86,18 @@ def test_null_handles_are_answered():
                    lib.vk_qk_norm_rope_axes_f32(n, n, n, n, n, n, n, n, 1, 1, 1, 1, 64, n, 0, 1e-5,
                                                 n, n)):
         assert status == vh.VK_ERR_INVALID
+
+
+def test_the_tiles_model_counts_whole_parts(plan):
+    """Splits whose cost hangs on the parts' 68 floats a query (with 66 these were 13, 5 and 8),
+    from the model's own terms: steps of 1.3 us a workgroup of the fullest CU, 4 us and the parts
+    both ways at 4.5 TB/s for a join."""
+    for pairs, queries, keys, want in ((39, 161, 5789, 6), (19, 2567, 6921, 3), (23, 478, 6570, 5)):
+        tiles, blocks = pairs * -(-queries // 128), -(-keys // 64)
+
+        def us(sp):
+            load = -(-tiles * sp // 256)
+            t = -(-blocks // sp) * (1.3 * load if load > 1 else 1.5)
+            return t + (4 + 2 * 4 * (64 + 4) * sp * pairs * queries / 4.5e6 if sp > 1 else 0)
+        assert min(range(1, min(blocks // 4, 12 * 256 // tiles, 64) + 1), key=us) == want
+        assert plan(pairs, queries, keys) == (TILE, want)

@@ -1445,7 +1445,8 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache, const vk_t
   a.tiles = static_cast<uint32_t>(tiles);
   float* part = nullptr;
   if (splits > 1) {
-    VK_TRY(vk::ensure_work(rt, splits * rows * (HD + 4), "attention_cached"));
+    static_assert(vk::kCachedPart == HD + 4, "store_part's sums and store_ml's four");
+    VK_TRY(vk::ensure_work(rt, splits * rows * vk::kCachedPart, "attention_cached"));
     part = rt->work;
   }
   // 8 / share groups of `heads` pairs each

@@ -213,10 +213,11 @@ inline AttentionPlan attention_plan(int cus, size_t sequences, size_t n, int pro
 // Attention over the 8-bit cache (attention_cached.hip)
 // ---------------------------------------------------------------------------
 // Which kernel a call takes, and over how many workgroups the keys of a query are
-// shared out (each writes its part of 66 floats a query, and a second pass joins them).
+// shared out (each writes its part, kCachedPart floats a query, and a second pass joins them).
 // `pairs`: sequences x cache heads, `queries` of each, `rows` in all, `blocks` of 64 keys.
 enum CachedForm { kRow, kFew, kTile };
 constexpr int kTileRows = 128;
+constexpr int kCachedPart = 64 + 4;  // sums of V; reference, its base, denominator, unused
 struct CachedPlan {
   CachedForm form;
   int splits;
@@ -231,7 +232,7 @@ struct CachedPlan {
 // kTile (128 queries a workgroup, a block a step for all): a step takes 1.5 us with one
 // workgroup on the CU and 1.3 of the CU's time with two or three; a split adds its parts'
 // traffic and the join: 12 x 866 over 10,392 keys 236 us unsplit, 90 in 3, 79 in 6 and in 9.
-// Twelve workgroups a CU are the most: past that the parts (then 104 MB) grow for little.
+// Twelve workgroups a CU are the most: past that the parts (then 107 MB) grow for little.
 // One query: against the second kernel 16 x 124,704 46 us (64), 12 x 866 5.9 (9.2).
 inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t rows,
                               size_t blocks) {
@@ -255,7 +256,7 @@ inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t r
     const double load = static_cast<double>((tiles * sp + cus - 1) / cus);
     const double steps = static_cast<double>((blocks + sp - 1) / sp);
     double us = steps * (load > 1.0 ? 1.3 * load : 1.5);
-    if (sp > 1) us += 4.0 + 2.0 * 264.0 * sp * static_cast<double>(rows) / 4.5e6;
+    if (sp > 1) us += 4.0 + 2.0 * 4.0 * kCachedPart * sp * static_cast<double>(rows) / 4.5e6;
     if (best_us == 0.0 || us < best_us) {
       best = sp;
       best_us = us;

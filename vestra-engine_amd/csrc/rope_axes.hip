@@ -5,9 +5,9 @@
 // pairs lie in the row and which axis each takes is a table of 64 entries that
 // the host makes from vk_rope_axes, so one kernel serves every convention.
 //
-// A row is one float4 a lane of a 16-lane DPP row; a 16-lane group takes one
-// token and kHeads of its heads at a time, so the cosines and sines of the
-// token are worked out once for them.  A lane's partners of its four elements
+// A row is one float4 a lane of a 16-lane DPP row; a 16-lane group takes
+// kHeads heads of one token, so the cosines and sines of the token are worked
+// out once for them.  A lane's partners of its four elements
 // lie wherever the convention puts them: the normalised row goes through LDS (a
 // row is its group's alone: no barrier, the lanes of a wave are in step).
 //
@@ -26,7 +26,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kGroups = kThreads / 16;  // tokens of a workgroup
-// Rows of a group in flight.  866 tokens of 24 heads: 4.1 us; 4.7 with four rows (half the
+// Rows of a group.  866 tokens of 24 heads: 4.1 us; 4.7 with four rows (half the
 // workgroups), 5.3 with one (a token's angles for one row).  10,392: 24.2, 24.7, 34.
 constexpr int kHeads = 2;
 constexpr int kPitch = 68;              // floats of a row in LDS
@@ -40,10 +40,8 @@ struct alignas(16) AxesTable {
 
 struct AxesShape {
   uint32_t heads, kv_heads, n, axes, eps_bits;
-  uint32_t rows;      // sequences * n
-  uint32_t slice;     // rows (of Q, then K) of one workgroup
-  uint32_t sequences;
-  uint32_t outer;     // vk_qk_layout
+  uint32_t rows;   // sequences * n
+  uint32_t outer;  // vk_qk_layout
   vkd::FastDivU32 by_n;
 };
 
@@ -83,8 +81,7 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
   const uint32_t t = live ? token : sh.rows - 1;
   const uint32_t s = vkd::fdiv(t, sh.by_n), i = t - s * sh.n;
   const uint32_t all = sh.heads + sh.kv_heads;
-  const uint32_t h0 = blockIdx.y * sh.slice;
-  const uint32_t h1 = h0 + sh.slice < all ? h0 + sh.slice : all;
+  const uint32_t h = blockIdx.y * kHeads;  // the first head: of Q, then of K
   const float eps = __uint_as_float(sh.eps_bits);
   // first element of head h's row of this token
   auto row = [&](uint32_t h, uint32_t count) {
@@ -110,99 +107,93 @@ __global__ __launch_bounds__(kThreads) void qk_norm_rope_axes_kernel(
     at_axis[e] = static_cast<const POS*>(pos)[static_cast<size_t>(t) * sh.axes +
                                               (axis4 >> 8 * e & 0xff)];
   }
-  bool have = false;
-  for (uint32_t h = h0; h < h1; h += kHeads) {
-    float4 v[kHeads];
+  float4 v[kHeads];
 #pragma unroll
-    for (int j = 0; j < kHeads; ++j) {
-      const uint32_t hh = h + j < h1 ? h + j : h1 - 1;
-      v[j] = vkd::ld_stream(
-          reinterpret_cast<const float4*>((hh < sh.heads ? q : k) + at(hh)));
-    }
-    if (!have) {  // while the first rows are on their way
-      have = true;
+  for (int j = 0; j < kHeads; ++j) {
+    const uint32_t hh = h + j < all ? h + j : all - 1;
+    v[j] = vkd::ld_stream(
+        reinterpret_cast<const float4*>((hh < sh.heads ? q : k) + at(hh)));
+  }
+  // while the rows are on their way
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const double turns = static_cast<double>(at_axis[e]) * f[e];
-        const double quarter = rint(4.0 * turns);
-        const float r = static_cast<float>(turns - 0.25 * quarter);  // within 1/8
-        float sr, cr;
-        sincospif(2.0f * r, &sr, &cr);
-        const int quad = static_cast<int>(quarter - 4.0 * floor(0.25 * quarter));
-        float ca = quad & 1 ? sr : cr, sa = quad & 1 ? cr : sr;
-        if (quad == 1 || quad == 2) ca = -ca;
-        if (quad >= 2) sa = -sa;
-        c[e] = ca;
-        sn[e] = second4 >> 8 * e & 1 ? sa : -sa;
-      }
-    }
-    if constexpr (NORM) {
-      float mean[kHeads], inv[kHeads];
-      if constexpr (SEQ) {
+  for (int e = 0; e < 4; ++e) {
+    const double turns = static_cast<double>(at_axis[e]) * f[e];
+    const double quarter = rint(4.0 * turns);
+    const float r = static_cast<float>(turns - 0.25 * quarter);  // within 1/8
+    float sr, cr;
+    sincospif(2.0f * r, &sr, &cr);
+    const int quad = static_cast<int>(quarter - 4.0 * floor(0.25 * quarter));
+    float ca = quad & 1 ? sr : cr, sa = quad & 1 ? cr : sr;
+    if (quad == 1 || quad == 2) ca = -ca;
+    if (quad >= 2) sa = -sa;
+    c[e] = ca;
+    sn[e] = second4 >> 8 * e & 1 ? sa : -sa;
+  }
+  if constexpr (NORM) {
+    float mean[kHeads], inv[kHeads];
+    if constexpr (SEQ) {
 #pragma unroll
-        for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
-        vkd::wave_lds_fence();
-        float st = l < kHeads ? row_chain(mine + l * kPitch) / 64.0f : 0.0f;
-        vkd::wave_lds_fence();
-#pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-          mean[j] = __shfl(st, j, 16);
-          float4 d;
-          d.x = v[j].x - mean[j]; d.x = d.x * d.x;
-          d.y = v[j].y - mean[j]; d.y = d.y * d.y;
-          d.z = v[j].z - mean[j]; d.z = d.z * d.z;
-          d.w = v[j].w - mean[j]; d.w = d.w * d.w;
-          *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = d;
-        }
-        vkd::wave_lds_fence();
-        st = l < kHeads ? row_inv<true>(row_chain(mine + l * kPitch), eps) : 0.0f;
-        vkd::wave_lds_fence();
-#pragma unroll
-        for (int j = 0; j < kHeads; ++j) inv[j] = __shfl(st, j, 16);
-      } else {
-#pragma unroll
-        for (int j = 0; j < kHeads; ++j) {
-          float a = v[j].x;
-          a += v[j].y;
-          a += v[j].z;
-          a += v[j].w;
-          mean[j] = vkd::row16_sum(a) / 64.0f;
-          float d, sq;
-          d = v[j].x - mean[j]; sq = d * d;
-          d = v[j].y - mean[j]; sq += d * d;
-          d = v[j].z - mean[j]; sq += d * d;
-          d = v[j].w - mean[j]; sq += d * d;
-          inv[j] = row_inv<false>(vkd::row16_sum(sq), eps);
-        }
-      }
+      for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
+      vkd::wave_lds_fence();
+      float st = l < kHeads ? row_chain(mine + l * kPitch) / 64.0f : 0.0f;
+      vkd::wave_lds_fence();
 #pragma unroll
       for (int j = 0; j < kHeads; ++j) {
-        const bool is_q = (h + j < h1 ? h + j : h1 - 1) < sh.heads;
-        const float4 g = vkd::Param<PT>::load4(is_q ? qg : kg, l);
-        const float4 b = vkd::Param<PT>::load4(is_q ? qb : kb, l);
-        v[j] = vkd::ln_apply4(v[j], mean[j], inv[j], g, b);
+        mean[j] = __shfl(st, j, 16);
+        float4 d;
+        d.x = v[j].x - mean[j]; d.x = d.x * d.x;
+        d.y = v[j].y - mean[j]; d.y = d.y * d.y;
+        d.z = v[j].z - mean[j]; d.z = d.z * d.z;
+        d.w = v[j].w - mean[j]; d.w = d.w * d.w;
+        *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = d;
+      }
+      vkd::wave_lds_fence();
+      st = l < kHeads ? row_inv<true>(row_chain(mine + l * kPitch), eps) : 0.0f;
+      vkd::wave_lds_fence();
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j) inv[j] = __shfl(st, j, 16);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kHeads; ++j) {
+        float a = v[j].x;
+        a += v[j].y;
+        a += v[j].z;
+        a += v[j].w;
+        mean[j] = vkd::row16_sum(a) / 64.0f;
+        float d, sq;
+        d = v[j].x - mean[j]; sq = d * d;
+        d = v[j].y - mean[j]; sq += d * d;
+        d = v[j].z - mean[j]; sq += d * d;
+        d = v[j].w - mean[j]; sq += d * d;
+        inv[j] = row_inv<false>(vkd::row16_sum(sq), eps);
       }
     }
 #pragma unroll
-    for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
-    vkd::wave_lds_fence();
-#pragma unroll
     for (int j = 0; j < kHeads; ++j) {
-      const float* r = mine + j * kPitch;
-      float4 o;
-      o.x = v[j].x * c[0] + r[partner4 >> 0 & 0xff] * sn[0];
-      o.y = v[j].y * c[1] + r[partner4 >> 8 & 0xff] * sn[1];
-      o.z = v[j].z * c[2] + r[partner4 >> 16 & 0xff] * sn[2];
-      o.w = v[j].w * c[3] + r[partner4 >> 24 & 0xff] * sn[3];
-      v[j] = o;
+      const bool is_q = (h + j < all ? h + j : all - 1) < sh.heads;
+      const float4 g = vkd::Param<PT>::load4(is_q ? qg : kg, l);
+      const float4 b = vkd::Param<PT>::load4(is_q ? qb : kb, l);
+      v[j] = vkd::ln_apply4(v[j], mean[j], inv[j], g, b);
     }
-    vkd::wave_lds_fence();
-#pragma unroll
-    for (int j = 0; j < kHeads; ++j)
-      if (live && h + j < h1)
-        vkd::st_stream(reinterpret_cast<float4*>((h + j < sh.heads ? q_out : k_out) + at(h + j)),
-                       v[j]);
   }
+#pragma unroll
+  for (int j = 0; j < kHeads; ++j) *reinterpret_cast<float4*>(mine + j * kPitch + 4 * l) = v[j];
+  vkd::wave_lds_fence();
+#pragma unroll
+  for (int j = 0; j < kHeads; ++j) {
+    const float* r = mine + j * kPitch;
+    float4 o;
+    o.x = v[j].x * c[0] + r[partner4 >> 0 & 0xff] * sn[0];
+    o.y = v[j].y * c[1] + r[partner4 >> 8 & 0xff] * sn[1];
+    o.z = v[j].z * c[2] + r[partner4 >> 16 & 0xff] * sn[2];
+    o.w = v[j].w * c[3] + r[partner4 >> 24 & 0xff] * sn[3];
+    v[j] = o;
+  }
+#pragma unroll
+  for (int j = 0; j < kHeads; ++j)
+    if (live && h + j < all)
+      vkd::st_stream(reinterpret_cast<float4*>((h + j < sh.heads ? q_out : k_out) + at(h + j)),
+                     v[j]);
 }
 
 // The host's table: vk_rope_axes laid out element by element.
@@ -351,14 +342,12 @@ int vk_qk_norm_rope_axes_f32(vk_runtime* rt, const vk_tensor* q, const vk_tensor
   sh.n = static_cast<uint32_t>(n);
   sh.rows = static_cast<uint32_t>(rows);
   sh.axes = static_cast<uint32_t>(axes->count);
-  sh.sequences = static_cast<uint32_t>(sequences);
   sh.outer = static_cast<uint32_t>(layout);
   sh.by_n = vkd::make_fastdiv(static_cast<uint32_t>(n));
   memcpy(&sh.eps_bits, &eps, sizeof eps);
   const size_t all = heads + kv_heads;
-  sh.slice = kHeads;
   a.grid = dim3(static_cast<unsigned>((rows + kGroups - 1) / kGroups),
-                static_cast<unsigned>((all + sh.slice - 1) / sh.slice));
+                static_cast<unsigned>((all + kHeads - 1) / kHeads));
   switch (positions->dtype) {
     case VK_I32: return dispatch<int32_t>(a);
     case VK_I64: return dispatch<int64_t>(a);

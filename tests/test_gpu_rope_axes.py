@@ -189,6 +189,44 @@ def test_the_sequential_order_gives_the_cpu_sums(rt, rng):
                 assert np.array_equal(y[0, h, i], want.astype(f))
 
 
+@pytest.mark.parametrize("S,H,KV,n", [(2, 3, 2, 17), (1, 12, 12, 50), (3, 1, 0, 1)])
+@pytest.mark.parametrize("layout", [0, 1])
+@pytest.mark.parametrize("kind", [np.float32, np.float16])
+def test_the_sequential_order_at_real_positions(rt, rng, S, H, KV, n, layout, kind):
+    """The rotation of rows whose LayerNorm is the left-to-right sums in f32.  Beside those,
+    which are the kernel's own bits, cos and sin are off by 2 u and half a u of the reduced
+    angle, each product and the sum by u: 5 u of both values, and the angle's own error."""
+    f = np.float32
+    pairs, freq = (8, 12, 12), 100.0
+    q, k = normals(rng, S, H, n, 64, scale=3, shift=1), normals(rng, S, KV, n, 64) if KV else None
+    p = params_of(rng, kind)
+    if not KV:
+        p = p[:2] + [None, None]
+    pos = rng.integers(-30, 3000, (S * n, 3)).astype(np.int32)
+    spec = pairs_of(pairs, freq, False, False, False)
+    rt.set_layernorm_order(vh.VK_LN_ORDER_SEQUENTIAL)
+    try:
+        got = run(rt, q, k, p, pos, vh.RopeAxes(pairs, freq), sequences=S, layout=layout)
+    finally:
+        rt.set_layernorm_order(vh.VK_LN_ORDER_TREE)
+    for y, x, g, b in ((got[0], q, p[0], p[1]), (got[1], k, p[2], p[3])):
+        if x is None:
+            continue
+        mean = np.add.accumulate(x, -1, f)[..., -1:] / f(64)
+        d = x - mean
+        var = np.add.accumulate(d * d, -1, f)[..., -1:] / f(64)
+        x = (d * (f(1) / np.sqrt(var + f(1e-5)))) * g.astype(f) + b.astype(f)
+        assert x.dtype == f
+        for s in range(S):
+            at = pos[s * n:(s + 1) * n]
+            want, _ = reference(x[s], None, None, 0.0, at, spec)
+            for e0, e1, a, w in spec:
+                both = np.abs(x[s, ..., e0].astype(np.float64)) + np.abs(x[s, ..., e1])
+                tol = both * (5 * U + np.abs(at[:, a] * w) * 2.0 ** -50) + 1e-40
+                for e in (e0, e1):
+                    assert np.all(np.abs(y[s, ..., e] - want[..., e]) <= tol)
+
+
 def test_refusals(rt):
     n = 4
     q, k, o = (rt.alloc_f32(2 * n * 64) for _ in range(3))

@@ -520,7 +520,7 @@ typedef struct vk_rope_axes {
  * (VK_QK_HEADS_OUTER) or [sequences, heads, n, 64] (VK_QK_VIEWS_OUTER).
  * positions [sequences*n, count]: f32 (taken as they are, fractions
  * included), i32 or i64.  The angle is held in 64 bits, so far positions turn
- * exactly (to 1e-7 of a turn up to |p| = 2^31 where freq >= 1).  No table: nothing is
+ * exactly (to 2^-22 of a turn up to |p| = 2^31 where freq >= 1).  No table: nothing is
  * allocated.  q_out may be q (in place) or a tensor that overlaps no other;
  * k_out likewise.  head_dim 64.  No counterpart in the reference. */
 int vk_qk_norm_rope_axes_f32(vk_runtime* rt, const vk_tensor* q,

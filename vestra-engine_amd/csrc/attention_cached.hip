@@ -12,15 +12,17 @@
 // Three kernels (plans.h says which, and over how many workgroups the keys are split), and one
 // that joins the splits:
 //   attention_row_kernel   one query: a lane a key, f32 on the vector units.  Bound by memory (16 x
-//                          124,704 keys: 45.9 us, 5.9 TB/s); a short cache by its CUs'
-//                          vector units (12 x 866 keys: 5.9 us).
+//                          124,704 keys: 53.3 us called back to back, 47 in a graph, 5.1 and
+//                          5.8 TB/s); a short cache by its CUs' vector units (12 x 866 keys:
+//                          5.9 us).  It reads every key whatever the masks leave: 12 x 124,704
+//                          keys 38 us, of which one document of 866 is seen 39.
 //   attention_few_kernel   up to 32 queries of a cache head: a wave a block of 64 keys.  Bound
 //                          by the latency of a block's chain (12 x 10,392 keys, 32 queries:
-//                          13.7 us).
+//                          14.2 us, 13.4 in a graph).
 //   attention_tile_kernel  128 queries a workgroup, the blocks through LDS.  Bound by the vector
-//                          units beside the matrix cores (softmax and the splitting of weights: 64% and
-//                          42% of the time; 12 x 10,392 rows over the frames before theirs: 407 us,
-//                          883 TFLOP/s of f16 products where a large library product reaches
+//                          units beside the matrix cores (softmax and the splitting of weights: 63% and
+//                          41% of the time; 12 x 10,392 rows over the frames before theirs: 405 us,
+//                          887 TFLOP/s of f16 products where a large library product reaches
 //                          1,080).
 // No atomics and no order that depends on timing: the same call gives the same bits, and a
 // row's do not depend on the values of other queries.
@@ -101,8 +103,8 @@ constexpr int kRowWaves = 8;
 constexpr float kRoom = 4.0f;  // a lane's maximum follows scores that pass it by 2^kRoom
 
 // One query a sequence and cache head: a workgroup a query and key split, a lane a key.  The
-// lane's 64 products are F32 FMAs with the query in scalar registers (four running sums), and
-// it keeps a softmax of its own (maximum, sum and 64 sums of values) over the keys that it
+// lane's 64 products are F32 FMAs with the query uniform (scalar registers, and what they do not
+// hold read back out of lanes of a vector register; four running sums), and it keeps a softmax of its own (maximum, sum and 64 sums of values) over the keys that it
 // meets; the lanes are joined once, at the end, halving: lane d is left with d.  A short cache's
 // few rows have four workgroups each (PARTS), which share V's columns and all take the scores: a
 // CU has 60% of the vector work (12 x 866 keys 5.9 us, 7.1 in one).
@@ -1009,7 +1011,8 @@ struct StageKeys {
 };
 
 // Three workgroups a CU; two with a cap, whose work a score wants the registers (in 168 of
-// them it spills: 122 us for 110).
+// them it spills: 122 us for 110).  A masked bias spills 8 to 11 of the 168, a plain mask one at
+// most; two workgroups are slower there (12 x 10,392 queries, documents of 866: 173 us for 109).
 template <int FORMAT, int SCORE, bool MASK, int QW>
 __global__ __launch_bounds__(64 * QW, SCORE & kCap ? 2 : 3) void attention_tile_kernel(const float* __restrict__ q,
                                                                     float* __restrict__ out,

@@ -224,16 +224,21 @@ struct CachedPlan {
 };
 
 // kRow (one query a pair, a lane a key): a workgroup a CU, four blocks of keys at
-// least; up to 24 blocks (three a wave) its keys unsplit and no join: 12 x 1,536 keys 6.9 us
-// unsplit; 12 x 2,000 7.7 and 7.3 split; 12 x 4,000 11.2 and 8.7; 16 x 124,704 348 and 46.
+// least; up to 24 blocks (three a wave) its keys unsplit and no join (in a graph): 12 x 1,536
+// keys 7.1 us unsplit, 7.7 in six; 12 x 2,000 8.1 and 7.7 split; 12 x 4,000 12.2 and 9.0;
+// 16 x 124,704 262 and 47.
 // kFew (up to 32 queries a pair, a wave a block): a workgroup a CU, six blocks at least; two
-// a CU where each still has 16 blocks: 12 x 10,392 keys and 32 queries 80 us unsplit, 20 in
-// 8, 15 in 16, 20 in 64; 4 x 30,000 231, 36, 22, 13.
+// a CU where each still has 16 blocks: 12 x 10,392 keys and 32 queries 83 us unsplit, 20 in
+// 8, 15 in 16, 14 in 21, 21 in 64; 4 x 30,000 and 2 243, 36 in 8, 22 in 16, 12.5 in 64.
 // kTile (128 queries a workgroup, a block a step for all): a step takes 1.5 us with one
 // workgroup on the CU and 1.3 of the CU's time with two or three; a split adds its parts'
-// traffic and the join: 12 x 866 over 10,392 keys 236 us unsplit, 90 in 3, 79 in 6 and in 9.
+// traffic and the join: 12 x 866 over 10,392 keys 239 us unsplit, 93 in 3, 75 in 6, 77 in 9.
+// The model counts every block and one workgroup a tile: what masks hide and the second
+// workgroups of documents' tiles, which the host does not know, are left out.  A tile's waves
+// without rows still stage: 12 x 10,392 keys and 33 queries 19.7 us, 64 21.0, 128 24.6 (32, as
+// kFew, 13.4).
 // Twelve workgroups a CU are the most: past that the parts (then 107 MB) grow for little.
-// One query: against the second kernel 16 x 124,704 46 us (64), 12 x 866 5.9 (9.2).
+// One query: against the second kernel 16 x 124,704 46 us (62), 12 x 866 5.6 (10.4).
 inline CachedPlan cached_plan(size_t cus, size_t pairs, size_t queries, size_t rows,
                               size_t blocks) {
   const auto between = [](size_t v, size_t most) { return v < 1 ? size_t{1} : v > most ? most : v; };

@@ -608,7 +608,9 @@ typedef struct vk_attention_rules {
  * sums are held as in f32: the values of the cache are exact in f16, queries
  * and weights are taken as two f16 parts (a query's value to 2^-25 of its
  * row's largest, a weight times V's scale to 2^-34 of the largest; one query:
- * f32 throughout).  Positions past 2^31 - 2 count as 2^31 - 2.  The same call
+ * f32 throughout).  That holds for V's scales of 2^-88 to 2^99 (values of some
+ * 1e-25 to 1e31); a row whose keys are all below loses bits as f16's smallest
+ * numbers do, one with a key above its weights below 2^-126.  Positions past 2^31 - 2 count as 2^31 - 2.  The same call
  * gives the same bits.  A large call splits its keys and keeps partial
  * results in the runtime's work buffer (run it once before a capture, which
  * cannot grow it).  No counterpart in the reference. */

@@ -610,10 +610,11 @@ typedef struct vk_attention_rules {
  * row's largest, a weight times V's scale to 2^-34 of the largest; one query:
  * f32 throughout).  That holds for V's scales of 2^-88 to 2^99 (values of some
  * 1e-25 to 1e31); a row whose keys are all below loses bits as f16's smallest
- * numbers do, one with a key above its weights below 2^-126.  Positions past 2^31 - 2 count as 2^31 - 2.  The same call
- * gives the same bits.  A large call splits its keys and keeps partial
- * results in the runtime's work buffer (run it once before a capture, which
- * cannot grow it).  No counterpart in the reference. */
+ * numbers do, one with a key above its weights below 2^-126.  Positions past
+ * 2^31 - 2 count as 2^31 - 2.  The same call gives the same bits.  A large call
+ * splits its keys and keeps partial results in the runtime's work buffer (run
+ * it once before a capture, which cannot grow it).  No counterpart in the
+ * reference. */
 int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache,
                             const vk_tensor* q, size_t heads, size_t n,
                             const vk_tensor* starts, const vk_tensor* counts,

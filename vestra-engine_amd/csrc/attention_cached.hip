@@ -104,10 +104,11 @@ constexpr float kRoom = 4.0f;  // a lane's maximum follows scores that pass it b
 
 // One query a sequence and cache head: a workgroup a query and key split, a lane a key.  The
 // lane's 64 products are F32 FMAs with the query uniform (scalar registers, and what they do not
-// hold read back out of lanes of a vector register; four running sums), and it keeps a softmax of its own (maximum, sum and 64 sums of values) over the keys that it
-// meets; the lanes are joined once, at the end, halving: lane d is left with d.  A short cache's
-// few rows have four workgroups each (PARTS), which share V's columns and all take the scores: a
-// CU has 60% of the vector work (12 x 866 keys 5.9 us, 7.1 in one).
+// hold read back out of lanes of a vector register; four running sums), and it keeps a softmax
+// of its own (maximum, sum and 64 sums of values) over the keys that it meets; the lanes are
+// joined once, at the end, halving: lane d is left with d.  A short cache's few rows have four
+// workgroups each (PARTS), which share V's columns and all take the scores: a CU has 60% of the
+// vector work (12 x 866 keys 5.9 us, 7.1 in one).
 template <int FORMAT, int PARTS>
 __global__ __launch_bounds__(64 * kRowWaves) void attention_row_kernel(const float* __restrict__ q,
                                                                        float* __restrict__ out,
@@ -947,7 +948,7 @@ __device__ __forceinline__ int here(int offset) {
 // Staging by all threads: eight codes of K (or V) a thread and row.  The block's
 // rows are a buffer of their own (its base and the bytes left of it in scalar registers), so
 // a load has no address arithmetic and keys past the end read zeros (every offset is part of
-// the lane's, a constant of it in the instruction: the uniform offset is left out of bounds checks).
+// the lane's, constants in the instruction: the uniform offset is left out of bounds checks).
 template <int FORMAT, int THREADS>
 struct StageRows {
   static constexpr int kPer = KB * 8 / THREADS;

@@ -23,7 +23,7 @@
  *    threads at once without external locking; separate runtimes are
  *    independent.
  *  - Tensors are flat, contiguous, typed device buffers (f32, f16, u8, or
- *    i32 / i64 for RoPE positions).
+ *    i32 / i64 for RoPE positions; bf16 where a call says so).
  *    Creators allocate; every creator has a matching destroy.  In-place
  *    operations take the tensor handle they modify; the reference's
  *    "consume and return the token tensor" (vit_block.rs:489-499,563) is
@@ -60,12 +60,14 @@ typedef enum vk_dtype {
   VK_F16 = 1,
   VK_U8 = 2,
   VK_I32 = 3,
-  VK_I64 = 4
+  VK_I64 = 4,
+  VK_BF16 = 5
 } vk_dtype;
 
 typedef struct vk_runtime vk_runtime;
 typedef struct vk_tensor vk_tensor;
 typedef struct vk_linear vk_linear;
+typedef struct vk_linear_i8 vk_linear_i8;
 typedef struct vk_event vk_event;
 typedef struct vk_graph vk_graph;
 
@@ -141,6 +143,8 @@ void* vk_tensor_device_ptr(const vk_tensor* t);
 /* CudaRuntime::upload_f32 (vit_block.rs:161-184, 335). Synchronous. */
 int vk_upload_f32(vk_runtime* rt, const float* host, size_t len, vk_tensor** out);
 int vk_upload_f16(vk_runtime* rt, const uint16_t* host, size_t len, vk_tensor** out);
+/* The bits of bf16 values. */
+int vk_upload_bf16(vk_runtime* rt, const uint16_t* host, size_t len, vk_tensor** out);
 int vk_upload_u8(vk_runtime* rt, const uint8_t* host, size_t len, vk_tensor** out);
 /* Integer RoPE positions [rows*2] (y, x) for vk_qk_norm_rope_mode_f32 and
  * vk_rope2d_f32.  Synchronous. */
@@ -153,6 +157,8 @@ int vk_write_u8(vk_runtime* rt, vk_tensor* t, const uint8_t* host, size_t len);
 int vk_download_f32(vk_runtime* rt, const vk_tensor* t, float* host, size_t len);
 /* The same for u8 tensors (images). Blocks. */
 int vk_download_u8(vk_runtime* rt, const vk_tensor* t, uint8_t* host, size_t len);
+/* The bits of an f16 or bf16 tensor. Blocks. */
+int vk_download_16(vk_runtime* rt, const vk_tensor* t, uint16_t* host, size_t len);
 /* CudaRuntime::copy_f32 (backbone.rs:991-1027). New tensor. */
 int vk_copy_f32(vk_runtime* rt, const vk_tensor* src, vk_tensor** out);
 /* CudaRuntime::copy_segment_f32: new tensor = src[offset .. offset+len]. */
@@ -620,6 +626,80 @@ int vk_attention_cached_f32(vk_runtime* rt, const vk_kv_cache* cache,
                             const vk_tensor* starts, const vk_tensor* counts,
                             size_t max_length, const vk_attention_rules* rules,
                             vk_qk_layout layout, vk_tensor* out);
+
+/* ------------------------------------------------------------------ */
+/* the feed-forward in fewer bits                                       */
+/* ------------------------------------------------------------------ */
+
+/* A linear in 8-bit integers: weights as int8 codes with an f32 scale for each
+ * output channel, rows of x quantised as they come with a scale for each token:
+ *   y[m, n] = (sum_k c[m, k] q[n, k]) * t[n] * s[m] + b[n]
+ * s[m] is the row's largest |x| / 127 rounded to f32; c = x / s rounded to f32
+ * and then to the nearest whole number (ties to even); the sum is exact.  A row
+ * whose scale would be below 2^-100 counts as zeros; one that holds an
+ * infinity or a NaN gives NaN throughout (other rows are untouched).
+ *
+ * Host pointers, synchronous.  codes_out_in int8 [out, in], scale f32 [out],
+ * bias and ls_gamma f32 [out] or NULL.  in_features at most 131,072 (the sum is
+ * an int32), any out_features.  No counterpart in the reference. */
+int vk_linear_i8_prepare(vk_runtime* rt, size_t in_features,
+                         size_t out_features, const int8_t* codes_out_in,
+                         const float* scale, const float* bias,
+                         const float* ls_gamma, vk_linear_i8** out);
+/* The same from f32 weights [in, out] (the layout of vk_linear_prepare_f32),
+ * each channel quantised by the rule for rows of x. */
+int vk_linear_i8_prepare_f32(vk_runtime* rt, size_t in_features,
+                             size_t out_features, const float* weight_in_out,
+                             const float* bias, const float* ls_gamma,
+                             vk_linear_i8** out);
+int vk_linear_i8_destroy(vk_linear_i8* lin);
+size_t vk_linear_i8_input_features(const vk_linear_i8* lin);
+/* out [rows, out_features] = y [* gamma].  x and out are f32, f16 or bf16, each
+ * of its own type; 16-bit results are rounded once.  out must not overlap x. */
+int vk_linear_i8_run_into(vk_runtime* rt, const vk_linear_i8* lin,
+                          const vk_tensor* x, size_t rows, vk_tensor* out);
+/* out = GELU(y), the erf of vk_gelu_f32_inplace.  No LayerScale. */
+int vk_linear_i8_run_gelu(vk_runtime* rt, const vk_linear_i8* lin,
+                          const vk_tensor* x, size_t rows, vk_tensor* out);
+/* residual += y [* gamma]; residual f32 [rows, out_features]. */
+int vk_linear_i8_run_residual(vk_runtime* rt, const vk_linear_i8* lin,
+                              const vk_tensor* x, size_t rows,
+                              vk_tensor* residual);
+
+/* The activation of a gated feed-forward. */
+#define VK_GATE_SILU 0 /* g / (1 + e^-g)                        */
+#define VK_GATE_GELU 1 /* 0.5 g (1 + erf(g / sqrt 2))           */
+/* The gated form: of the linear's out_features = 2 hidden columns the first
+ * half are gates, the second their partners, and out [rows, hidden] =
+ * act(y[:, h]) * y[:, hidden + h].  No LayerScale.  (A gated block is refused by
+ * the reference, vit_block.rs:1455-1465.) */
+int vk_linear_i8_run_gated(vk_runtime* rt, const vk_linear_i8* lin,
+                           const vk_tensor* x, size_t rows, int activation,
+                           vk_tensor* out);
+
+/* The gated feed-forward in 16 bits: g = x Wg^T + bg, u = x Wu^T + bu,
+ * out = act(g) * u, in one kernel.  All tensors f16, or all bf16: x [rows,
+ * in_features], w [2 hidden, in_features] (Wg's rows, then Wu's), bias
+ * [2 hidden] or NULL, out [rows, hidden], overlapping no input.  Sums are f32,
+ * out is rounded once.  in_features of a multiple of 8 are read where they lie;
+ * any others are copied to the runtime's work buffer first (run such a call
+ * once before a capture, which cannot grow it). */
+int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
+                     const vk_tensor* bias, size_t rows, size_t in_features,
+                     size_t hidden, int activation, vk_tensor* out);
+/* Its gradients, from the forward's inputs and grad = d loss / d out [rows,
+ * hidden]; nothing is kept from the forward.  dx [rows, in_features], dw
+ * [2 hidden, in_features], dbias [2 hidden] of x's type are overwritten; each may
+ * be NULL (not computed), and overlaps no other tensor.  The gradients of g and u
+ * are f32 up to one rounding to x's type, as operands of the products; dbias sums
+ * them before that rounding.  The same call gives the same bits.  Intermediate
+ * values (some 4 (rows + in_features) hidden values) go to the runtime's work
+ * buffer: run it once before a capture.  At most 2,097,152 rows. */
+int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
+                      const vk_tensor* bias, const vk_tensor* grad,
+                      size_t rows, size_t in_features, size_t hidden,
+                      int activation, vk_tensor* dx, vk_tensor* dw,
+                      vk_tensor* dbias);
 
 /* CudaRuntime::prepend_cls_add_pos_f32(patches, cls, pos, n_patches, embed)
  * (patch_embed.rs:234-240): row 0 = cls + pos[0]; row 1+p = patch_p + pos[1+p]. */

@@ -1,0 +1,487 @@
+// A gated feed-forward's first half in 16 bits (f16 or bf16) for gfx950, forward and
+// backward.
+//
+//   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u          (w = [Wg; Wu])
+//
+// Forward is one kernel: a workgroup's tile holds the gates and their partners of the
+// same hidden columns, so both products, the activation and the product of the two
+// meet in registers; h is rounded once.
+//
+// Backward, from x, w, b and the gradient dh, with nothing kept from the forward:
+//   1. g and u again, and in the same kernel dg = dh u act'(g), du = dh act(g), in
+//      f32 up to one rounding to x's type: the two products below take 16-bit
+//      operands.  Written as [rows, 2 H] and as its transpose, with the f32 column
+//      sums of each tile;
+//   2. dx = [dg du] [Wg; Wu]   (against w transposed);
+//   3. dw = [dg du]^T x        (transposes of both);
+//   4. db: the tiles' column sums added in order.
+#include "product_nt.h"
+#include "product_plan.h"
+
+namespace {
+
+using vkp::Kind;
+using vkp::kBF16;
+using vkp::kF16;
+using vkp::Operand;
+
+struct Args {
+  Operand a, b;
+  int k_bytes;
+  const void* bias;  // 2 N values of the type, or null
+  const void* grad;  // [M, N]
+  void* out;         // [M, N]; null in the backward
+  void* d;           // dg | du [M, 2 N], rows of d_pitch values, or null
+  void* dt;          // its transpose [2 N, M], rows of dt_pitch values, or null
+  float* sums;       // [gm * WM, 2 N], or null
+  uint32_t d_pitch, dt_pitch;
+  int M, N;
+  int act;
+  int gm, gn, group;
+};
+
+template <Kind KIND>
+__device__ __forceinline__ float bias_at(const Args& g, int n) {
+  typedef typename vkp::Value<KIND>::type V;
+  return g.bias ? vkp::widen(static_cast<const V*>(g.bias)[n]) : 0.0f;
+}
+
+__device__ __forceinline__ float gate_any(int act, float g) {
+  return act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(g) : vkp::gate<VK_GATE_GELU>(g);
+}
+
+__device__ __forceinline__ void slope_any(int act, float g, float* a, float* s) {
+  if (act == VK_GATE_SILU)
+    vkp::gate_slope<VK_GATE_SILU>(g, a, s);
+  else
+    vkp::gate_slope<VK_GATE_GELU>(g, a, s);
+}
+
+template <Kind KIND, typename T>
+__global__ __launch_bounds__(T::kThreads, 2) void gated_kernel(Args g) {
+  typedef typename vkp::Value<KIND>::type V;
+  __shared__ __align__(16) char s0[T::kBytes];
+  __shared__ __align__(16) char s1[T::kBytes];
+  int mt, nt;
+  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  const int m0 = mt * T::TM, n0 = nt * T::kHeld;
+  vkp::f32x16 acc[T::MT][T::NT];
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int kCols = T::NT / 2;
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    const int n = n0 + T::b_row(wn, j) + (lane & 31);
+    if (n >= g.N) continue;
+    const float bg = bias_at<KIND>(g, n), bu = bias_at<KIND>(g, g.N + n);
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
+        if (m >= g.M) continue;
+        static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] =
+            static_cast<V>(gate_any(g.act, acc[i][j][r] + bg) * (acc[i][j + kCols][r] + bu));
+      }
+  }
+}
+
+// Step 1 of the backward.
+template <Kind KIND, typename T>
+__global__ __launch_bounds__(T::kThreads, 2) void gated_grad_kernel(Args g) {
+  typedef typename vkp::Value<KIND>::type V;
+  typedef V V4 __attribute__((ext_vector_type(4)));
+  __shared__ __align__(16) char s0[T::kBytes];
+  __shared__ __align__(16) char s1[T::kBytes];
+  int mt, nt;
+  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  const int m0 = mt * T::TM, n0 = nt * T::kHeld;
+  vkp::f32x16 acc[T::MT][T::NT];
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int kCols = T::NT / 2;
+  const V* grad = static_cast<const V*>(g.grad);
+  const int rows8 = (g.M + 7) & ~7, cols8 = (2 * g.N + 7) & ~7;
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    const int n = n0 + T::b_row(wn, j) + (lane & 31);
+    const bool in = n < g.N;
+    const float bg = in ? bias_at<KIND>(g, n) : 0.0f, bu = in ? bias_at<KIND>(g, g.N + n) : 0.0f;
+    float sg = 0.0f, su = 0.0f;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int m4 = m0 + (wm * T::MT + i) * 32 + 8 * q + 4 * (lane >> 5);
+        V4 dg{}, du{};
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int m = m4 + r;
+          if (!in || m >= g.M) continue;
+          float a, s;
+          slope_any(g.act, acc[i][j][4 * q + r] + bg, &a, &s);
+          const float dh = vkp::widen(grad[static_cast<size_t>(m) * g.N + n]);
+          const float fg = dh * (acc[i][j + kCols][4 * q + r] + bu) * s, fu = dh * a;
+          sg += fg;
+          su += fu;
+          dg[r] = static_cast<V>(fg);
+          du[r] = static_cast<V>(fu);
+          if (g.d) {
+            V* d = static_cast<V*>(g.d) + static_cast<size_t>(m) * g.d_pitch;
+            d[n] = dg[r];
+            d[g.N + n] = du[r];
+            // zeros up to the next multiple of 16 bytes
+            if (n == g.N - 1)
+              for (int z = 2 * g.N; z < cols8; ++z) d[z] = static_cast<V>(0.0f);
+          }
+        }
+        if (g.dt && in && m4 < rows8) {
+          V* dt = static_cast<V*>(g.dt);
+          *reinterpret_cast<V4*>(dt + static_cast<size_t>(n) * g.dt_pitch + m4) = dg;
+          *reinterpret_cast<V4*>(dt + static_cast<size_t>(g.N + n) * g.dt_pitch + m4) = du;
+        }
+      }
+    if (g.sums) {
+      sg += __shfl_xor(sg, 32, 64);
+      su += __shfl_xor(su, 32, 64);
+      if (in && lane < 32) {
+        float* to = g.sums + static_cast<size_t>(mt * T::WM + wm) * 2 * g.N;
+        to[n] = sg;
+        to[g.N + n] = su;
+      }
+    }
+  }
+}
+
+// out[m, n] = sum_k a[m, k] b[n, k], rounded to the type.
+template <Kind KIND, typename T>
+__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(Args g) {
+  typedef typename vkp::Value<KIND>::type V;
+  __shared__ __align__(16) char s0[T::kBytes];
+  __shared__ __align__(16) char s1[T::kBytes];
+  int mt, nt;
+  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  const int m0 = mt * T::TM, n0 = nt * T::TN;
+  vkp::f32x16 acc[T::MT][T::NT];
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wm = wave / T::WN, wn = wave % T::WN;
+#pragma unroll
+  for (int j = 0; j < T::NT; ++j) {
+    const int n = n0 + T::b_row(wn, j) + (lane & 31);
+    if (n >= g.N) continue;
+#pragma unroll
+    for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
+        if (m < g.M)
+          static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(acc[i][j][r]);
+      }
+  }
+}
+
+// Forward of at most 16 RT rows.
+template <Kind KIND, int RT>
+__global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
+  typedef typename vkp::Value<KIND>::type V;
+  __shared__ __align__(16) char smem[vkp::few_bytes<KIND, RT, true>()];
+  const int n0 = blockIdx.x * 16;
+  vkp::few_product<KIND, RT, true>(g.a, g.b, g.k_bytes, n0, smem);
+  for (int e = threadIdx.x; e < 256 * RT; e += vkp::kFewThreads) {
+    const int m = e >> 4, n = n0 + (e & 15);
+    if (m >= g.M || n >= g.N) continue;
+    const float gate = vkp::few_sum<KIND, RT, true>(smem, 0, m, e & 15) + bias_at<KIND>(g, n);
+    const float up = vkp::few_sum<KIND, RT, true>(smem, 1, m, e & 15) + bias_at<KIND>(g, g.N + n);
+    static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(gate_any(g.act, gate) * up);
+  }
+}
+
+// ---------------------------------------------------------------- layouts
+// to[c, r] = from[r, c] of 16-bit values, zeros from row `rows` to the next multiple of 8.
+__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* __restrict__ from, int rows,
+                                                          int cols, uint16_t* __restrict__ to,
+                                                          size_t pitch) {
+  __shared__ uint16_t tile[64][66];
+  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
+  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int r = r0 + ty + 8 * i, c = c0 + tx + 32 * h;
+      tile[ty + 8 * i][tx + 32 * h] =
+          r < rows && c < cols ? from[static_cast<size_t>(r) * cols + c] : uint16_t{0};
+    }
+  __syncthreads();
+  const int rows8 = (rows + 7) & ~7;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int c = c0 + ty + 8 * i, r = r0 + 2 * tx;
+    if (c < cols && r < rows8) {
+      const uint32_t lo = tile[2 * tx][ty + 8 * i], hi = tile[2 * tx + 1][ty + 8 * i];
+      *reinterpret_cast<uint32_t*>(to + static_cast<size_t>(c) * pitch + r) = lo | hi << 16;
+    }
+  }
+}
+
+// Rows of `cols` 16-bit values into rows of `pitch` (a multiple of 8), zeros behind.
+__global__ __launch_bounds__(256) void pad16_kernel(const uint16_t* __restrict__ from, int cols,
+                                                    uint16_t* __restrict__ to, int pitch) {
+  const size_t r = blockIdx.x;
+  for (int c = threadIdx.x; c < pitch; c += 256)
+    to[r * pitch + c] = c < cols ? from[r * cols + c] : uint16_t{0};
+}
+
+__global__ __launch_bounds__(256) void zero16_kernel(uint16_t* to, size_t n) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i < n) to[i] = 0;
+}
+
+void zero16(const vk_runtime* rt, void* p, size_t n) {
+  hipLaunchKernelGGL(zero16_kernel, dim3((n + 255) / 256), dim3(256), 0, rt->stream,
+                     static_cast<uint16_t*>(p), n);
+}
+
+// dbias[c] = sum over the tiles' sums, in order.
+template <Kind KIND>
+__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int parts,
+                                                        int cols, void* out) {
+  const int c = blockIdx.x * 256 + threadIdx.x;
+  if (c >= cols) return;
+  float s = 0.0f;
+  for (int p = 0; p < parts; ++p) s += sums[static_cast<size_t>(p) * cols + c];
+  static_cast<typename vkp::Value<KIND>::type*>(out)[c] =
+      static_cast<typename vkp::Value<KIND>::type>(s);
+}
+
+// ---------------------------------------------------------------- launches
+constexpr size_t kPitchValues = 64;  // rows of workspace start on 128-byte lines
+size_t padded(size_t n) { return (n + kPitchValues - 1) / kPitchValues * kPitchValues; }
+
+template <bool PAIRED, typename F>
+void with_tile(vkp::TileSize size, Args& g, F go) {
+  const auto set = [&](auto tile) {
+    typedef decltype(tile) T;
+    g.gm = (g.M + T::TM - 1) / T::TM;
+    g.gn = (g.N + T::kHeld - 1) / T::kHeld;
+    g.group = vkp::kGroupRows / T::TM;
+    go(tile);
+  };
+  if (size == vkp::kTile256) set(vkp::Tile<2, 4, 4, 2, PAIRED>{});
+  else if (size == vkp::kTile128) set(vkp::Tile<2, 2, 2, 2, PAIRED>{});
+  else set(vkp::Tile<2, 1, 1, 2, PAIRED>{});
+}
+
+template <Kind KIND>
+int launch_forward(vk_runtime* rt, Args& g) {
+  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, 2LL * g.N, g.k_bytes);
+  if (p.few) {
+    const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
+    if (g.M <= 16)
+      hipLaunchKernelGGL((gated_few_kernel<KIND, 1>), grid, block, 0, rt->stream, g);
+    else
+      hipLaunchKernelGGL((gated_few_kernel<KIND, 2>), grid, block, 0, rt->stream, g);
+    return vk::check_launch("gated_few_kernel");
+  }
+  with_tile<true>(p.tile, g, [&](auto tile) {
+    typedef decltype(tile) T;
+    hipLaunchKernelGGL((gated_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream, g);
+  });
+  return vk::check_launch("gated_kernel");
+}
+
+template <Kind KIND>
+int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k, void* out) {
+  Args g{};
+  g.a = a;
+  g.b = b;
+  g.k_bytes = static_cast<int>(2 * k);
+  g.out = out;
+  g.M = a.rows;
+  g.N = b.rows;
+  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, g.N, g.k_bytes);
+  with_tile<false>(p.tile, g, [&](auto tile) {
+    typedef decltype(tile) T;
+    hipLaunchKernelGGL((product_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream,
+                       g);
+  });
+  return vk::check_launch("product_kernel");
+}
+
+void transpose(const vk_runtime* rt, const void* from, size_t rows, size_t cols, void* to,
+               size_t pitch) {
+  hipLaunchKernelGGL(transpose16_kernel, dim3((cols + 63) / 64, (rows + 63) / 64), dim3(256), 0,
+                     rt->stream, static_cast<const uint16_t*>(from), static_cast<int>(rows),
+                     static_cast<int>(cols), static_cast<uint16_t*>(to), pitch);
+}
+
+// A tensor's rows as an operand: as they are, or where a row is no multiple of 16
+// bytes, copied into `room` with zeros behind (room null: says how many bytes that takes).
+size_t operand_room(size_t rows, size_t cols) { return cols % 8 == 0 ? 0 : rows * padded(cols) * 2; }
+
+Operand as_operand(const vk_runtime* rt, const void* p, size_t rows, size_t cols, char* room) {
+  if (cols % 8 == 0)
+    return Operand{static_cast<const char*>(p), static_cast<int>(rows), static_cast<uint32_t>(2 * cols)};
+  hipLaunchKernelGGL(pad16_kernel, dim3(rows), dim3(256), 0, rt->stream,
+                     static_cast<const uint16_t*>(p), static_cast<int>(cols),
+                     reinterpret_cast<uint16_t*>(room), static_cast<int>(padded(cols)));
+  return Operand{room, static_cast<int>(rows), static_cast<uint32_t>(2 * padded(cols))};
+}
+
+template <Kind KIND>
+int backward(vk_runtime* rt, Args& g, const void* x, const void* w, size_t rows, size_t in,
+             size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
+  const size_t dp = padded(2 * hidden), rp = padded(rows);
+  const auto take = [&](size_t bytes) {
+    char* at = room;
+    room += (bytes + 255) / 256 * 256;
+    return at;
+  };
+  if (dx) {
+    g.d = take(rows * dp * 2);
+    g.d_pitch = static_cast<uint32_t>(dp);
+  }
+  if (dw) {
+    g.dt = take(2 * hidden * rp * 2);
+    g.dt_pitch = static_cast<uint32_t>(rp);
+  }
+  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, 2LL * g.N, g.k_bytes);
+  int parts = 0;
+  with_tile<true>(p.tile, g, [&](auto tile) {
+    typedef decltype(tile) T;
+    parts = g.gm * T::WM;
+    if (dbias) g.sums = reinterpret_cast<float*>(take(static_cast<size_t>(parts) * 2 * hidden * 4));
+    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
+                       rt->stream, g);
+  });
+  VK_TRY(vk::check_launch("gated_grad_kernel"));
+  const int R = static_cast<int>(rows), D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden);
+  if (dx) {
+    char* wt = take(in * dp * 2);
+    transpose(rt, w, 2 * hidden, in, wt, dp);
+    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.d), R, static_cast<uint32_t>(2 * dp)},
+                                Operand{wt, D, static_cast<uint32_t>(2 * dp)}, 2 * hidden, dx->ptr));
+  }
+  if (dw) {
+    char* xt = take(in * rp * 2);
+    transpose(rt, x, rows, in, xt, rp);
+    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.dt), H2, static_cast<uint32_t>(2 * rp)},
+                                Operand{xt, D, static_cast<uint32_t>(2 * rp)}, rows, dw->ptr));
+  }
+  if (dbias) {
+    hipLaunchKernelGGL(bias_grad_kernel<KIND>, dim3((2 * hidden + 255) / 256), dim3(256), 0, rt->stream,
+                       g.sums, parts, static_cast<int>(2 * hidden), dbias->ptr);
+    VK_TRY(vk::check_launch("bias_grad_kernel"));
+  }
+  return VK_OK;
+}
+
+// ---------------------------------------------------------------- arguments
+int check16(const vk_runtime* rt, const vk_tensor* t, vk_dtype dtype, size_t len, const char* what) {
+  VK_REQUIRE(t && t->dtype == dtype && t->len == len,
+             "gated: %s must hold %zu values of x's type (holds %zu)", what, len, t ? t->len : 0);
+  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0, "gated: %s must be 16-byte aligned", what);
+  return vk::check_device(rt, t, what);
+}
+
+int check_inputs(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
+                 size_t rows, size_t in, size_t hidden, int act) {
+  VK_REQUIRE(x && w, "gated: null argument");
+  VK_REQUIRE(x->dtype == VK_F16 || x->dtype == VK_BF16, "gated: x must be f16 or bf16");
+  VK_REQUIRE(in > 0 && hidden > 0, "gated: empty weights");
+  VK_REQUIRE(act == VK_GATE_SILU || act == VK_GATE_GELU, "gated: unknown activation %d", act);
+  // a tile addresses its rows of an operand by 31 bits
+  VK_UNSUPPORTED_IF(in > 0x100000 || hidden > 0x100000 || rows > 0x1000000, "gated: %zu x %zu -> %zu",
+                    rows, in, hidden);
+  VK_UNSUPPORTED_IF(2 * hidden * padded(in) * 2 > 0x7fffff00ULL, "gated: weights of %zu x %zu", 2 * hidden,
+                    in);
+  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((hidden + 31) / 32) > 0x7fffffULL, "gated: %zu x %zu outputs",
+                    rows, hidden);
+  VK_TRY(check16(rt, x, x->dtype, rows * in, "x"));
+  VK_TRY(check16(rt, w, x->dtype, 2 * hidden * in, "w"));
+  if (bias) VK_TRY(check16(rt, bias, x->dtype, 2 * hidden, "bias"));
+  return VK_OK;
+}
+
+Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
+                  size_t rows, size_t in, size_t hidden, int act, char** room) {
+  Args g{};
+  g.a = as_operand(rt, x->ptr, rows, in, *room);
+  *room += operand_room(rows, in);
+  g.b = as_operand(rt, w->ptr, 2 * hidden, in, *room);
+  *room += operand_room(2 * hidden, in);
+  g.k_bytes = static_cast<int>(2 * in);
+  g.bias = bias ? bias->ptr : nullptr;
+  g.M = static_cast<int>(rows);
+  g.N = static_cast<int>(hidden);
+  g.act = act;
+  return g;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
+                     size_t rows, size_t in_features, size_t hidden, int activation, vk_tensor* out) {
+  VK_TRY(vk::bind(rt));
+  VK_TRY(check_inputs(rt, x, w, bias, rows, in_features, hidden, activation));
+  VK_TRY(check16(rt, out, x->dtype, rows * hidden, "out"));
+  for (const vk_tensor* t : {x, w, bias}) VK_REQUIRE(!vk::overlap(out, t), "gated: out overlaps an input");
+  if (rows == 0) return VK_OK;
+  const size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features);
+  if (need > 0) VK_TRY(vk::ensure_work(rt, need / 4, "gated_forward"));
+  char* room = reinterpret_cast<char*>(rt->work);
+  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation, &room);
+  VK_TRY(vk::check_launch("pad16_kernel"));
+  g.out = out->ptr;
+  return x->dtype == VK_F16 ? launch_forward<kF16>(rt, g) : launch_forward<kBF16>(rt, g);
+}
+
+int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
+                      const vk_tensor* grad, size_t rows, size_t in_features, size_t hidden,
+                      int activation, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
+  VK_TRY(vk::bind(rt));
+  VK_TRY(check_inputs(rt, x, w, bias, rows, in_features, hidden, activation));
+  VK_TRY(check16(rt, grad, x->dtype, rows * hidden, "grad"));
+  VK_REQUIRE(dx || dw || dbias, "gated: no gradient to compute");
+  if (dx) VK_TRY(check16(rt, dx, x->dtype, rows * in_features, "dx"));
+  if (dw) VK_TRY(check16(rt, dw, x->dtype, 2 * hidden * in_features, "dw"));
+  if (dbias) VK_TRY(check16(rt, dbias, x->dtype, 2 * hidden, "dbias"));
+  const vk_tensor* outs[] = {dx, dw, dbias};
+  for (int i = 0; i < 3; ++i) {
+    for (const vk_tensor* t : {x, w, bias, grad})
+      VK_REQUIRE(!vk::overlap(outs[i], t), "gated: a gradient overlaps an input");
+    for (int j = 0; j < i; ++j) VK_REQUIRE(!vk::overlap(outs[i], outs[j]), "gated: gradients overlap");
+  }
+  VK_UNSUPPORTED_IF(rows > 0x200000, "gated: the gradients of %zu rows", rows);
+  if (rows == 0) {  // sums of nothing
+    if (dw) zero16(rt, dw->ptr, dw->len);
+    if (dbias) zero16(rt, dbias->ptr, dbias->len);
+    return vk::check_launch("zero16_kernel");
+  }
+  const size_t dp = padded(2 * hidden), rp = padded(rows);
+  size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features) + 8 * 256;
+  if (dx) need += (rows + in_features) * dp * 2;
+  if (dw) need += (2 * hidden + in_features) * rp * 2;
+  if (dbias) need += ((rows + 63) / 64 * 2) * 2 * hidden * 4;
+  VK_TRY(vk::ensure_work(rt, (need + 3) / 4, "gated_backward"));
+  char* room = reinterpret_cast<char*>(rt->work);
+  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation, &room);
+  VK_TRY(vk::check_launch("pad16_kernel"));
+  g.grad = grad->ptr;
+  return x->dtype == VK_F16
+             ? backward<kF16>(rt, g, x->ptr, w->ptr, rows, in_features, hidden, room, dx, dw, dbias)
+             : backward<kBF16>(rt, g, x->ptr, w->ptr, rows, in_features, hidden, room, dx, dw, dbias);
+}
+
+}  // extern "C"

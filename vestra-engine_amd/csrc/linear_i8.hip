@@ -1,0 +1,508 @@
+// The linear in 8-bit integers for gfx950: weights as int8 codes with an f32 scale for
+// each output channel, rows of x quantised as they come, with a scale for each token.
+//
+//   y[m, n] = (sum_k c[m, k] q[n, k]) * t[n] * s[m] + b[n]
+//
+// s[m] is the row's largest |x| / 127 rounded to f32 and c = x / s rounded to f32 and
+// then to the nearest whole number (ties to even).  The sum is exact in int32.  Then
+// the epilogues of the F32 linear (LayerScale, GELU, residual), or the gate: of out =
+// 2 H columns, column h of the result is act(y[m, h]) * y[m, H + h].
+#include <cmath>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "product_nt.h"
+#include "product_plan.h"
+
+struct vk_linear_i8 {
+  vk_runtime* rt = nullptr;
+  size_t in_features = 0, out_features = 0;
+  size_t pitch = 0;          // bytes of a row of codes: in_features rounded up to 128
+  int8_t* codes = nullptr;   // [out, pitch], zeros past in_features
+  float* scale = nullptr;    // [out]
+  float* bias = nullptr;     // [out] or null
+  float* ls_gamma = nullptr; // [out] or null
+};
+
+namespace {
+
+using vkp::Kind;
+using vkp::kBF16;
+using vkp::kF16;
+using vkp::kI8;
+using vkp::Operand;
+
+constexpr float kTop = 127.0f;
+constexpr float kLeastScale = 0x1p-100f;  // below, a row is held as zeros (as the cache does)
+constexpr size_t kMostK = 1 << 17;        // 127 * 128 * 2^17 < 2^31: the sum fits
+
+enum End { kStore = 0, kGelu = 1, kResidual = 2, kGated = 3 };
+
+struct Args {
+  Operand a, b;  // codes of x and of the weights
+  const float* sx;
+  const float* sw;
+  const float* bias;
+  const float* ls;
+  void* out;
+  int M, N;  // N: columns of out
+  int k_bytes;
+  int act, type;  // VK_GATE_*, vk_dtype of out
+  int gm, gn, group;
+};
+
+// ---------------------------------------------------------------- rows to codes
+__device__ __forceinline__ uint32_t bits_abs(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) {
+    const uint32_t o = static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), d, 64));
+    v = o > v ? o : v;
+  }
+  return v;
+}
+
+// A row's scale from the bits of its largest |x| (a NaN is above an infinity is above
+// every number), what to divide by, and whether all codes are 0.
+struct RowScale {
+  float scale, by;
+  bool none;
+};
+__device__ __forceinline__ RowScale row_scale(uint32_t top) {
+  const float d = __uint_as_float(top) / kTop;
+  const bool odd = top >= 0x7f800000u;
+  const bool none = odd || d < kLeastScale;
+  return RowScale{odd ? __uint_as_float(0x7fc00000u) : (none ? 0.0f : d), none ? 1.0f : d, none};
+}
+
+__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
+  return s.none ? 0u : static_cast<uint32_t>(static_cast<int>(rintf(x / s.by))) & 0xffu;
+}
+
+template <typename XT>
+__device__ __forceinline__ float x_at(const XT* x, size_t i) {
+  return vkp::widen(x[i]);
+}
+
+// Eight values from x[i]; VEC: x + i is 16-byte aligned.
+template <typename XT, bool VEC>
+__device__ __forceinline__ void load8(const XT* x, size_t i, int left, float (&v)[8]) {
+  if constexpr (VEC) {
+    if (left > 0) {
+      struct alignas(16) Eight {
+        XT e[8];
+      };
+      const Eight t = *reinterpret_cast<const Eight*>(x + i);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = vkp::widen(t.e[j]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? x_at(x, i + j) : 0.0f;
+  }
+}
+
+// A wave a row: NV steps of 8 values a lane stay in registers between the maximum and
+// the codes; NV 0: any length, read twice.
+template <typename XT, bool VEC, int NV>
+__global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict__ x, int M, int K,
+                                                            uint32_t pitch, char* codes,
+                                                            float* scales) {
+  const int lane = threadIdx.x & 63;
+  const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (m >= M) return;
+  const XT* row = x + static_cast<size_t>(m) * K;
+  char* to = codes + static_cast<size_t>(m) * pitch;
+  auto store = [&](int at, const float (&v)[8], const RowScale& s) {
+    if (at >= static_cast<int>(pitch)) return;
+    uint2 w;
+    w.x = code_of(v[0], s) | code_of(v[1], s) << 8 | code_of(v[2], s) << 16 | code_of(v[3], s) << 24;
+    w.y = code_of(v[4], s) | code_of(v[5], s) << 8 | code_of(v[6], s) << 16 | code_of(v[7], s) << 24;
+    *reinterpret_cast<uint2*>(to + at) = w;
+  };
+  uint32_t top = 0;
+  if constexpr (NV > 0) {
+    float v[NV][8];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int at = (i * 64 + lane) * 8;
+      load8<XT, VEC>(row, at, K - at, v[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, bits_abs(v[i][j]));
+    const RowScale s = row_scale(wave_umax(top));
+#pragma unroll
+    for (int i = 0; i < NV; ++i) store((i * 64 + lane) * 8, v[i], s);
+    if (lane == 0) scales[m] = s.scale;
+  } else {
+    float v[8];
+    for (int at = lane * 8; at < K; at += 512) {
+      load8<XT, VEC>(row, at, K - at, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) top = max(top, bits_abs(v[j]));
+    }
+    const RowScale s = row_scale(wave_umax(top));
+    for (int at = lane * 8; at < static_cast<int>(pitch); at += 512) {
+      load8<XT, VEC>(row, at, K - at, v);
+      store(at, v, s);
+    }
+    if (lane == 0) scales[m] = s.scale;
+  }
+}
+
+// ---------------------------------------------------------------- what leaves
+__device__ __forceinline__ void put(const Args& g, size_t at, float v) {
+  if (g.type == VK_F32)
+    static_cast<float*>(g.out)[at] = v;
+  else if (g.type == VK_F16)
+    static_cast<_Float16*>(g.out)[at] = static_cast<_Float16>(v);
+  else
+    static_cast<__bf16*>(g.out)[at] = static_cast<__bf16>(v);
+}
+
+struct Column {
+  float scale, bias, ls;
+};
+__device__ __forceinline__ Column column(const Args& g, int n) {
+  return Column{g.sw[n], g.bias ? g.bias[n] : 0.0f, g.ls ? g.ls[n] : 1.0f};
+}
+
+// The channel's scale first: a row's largest scale then overflows only where the result
+// does.
+__device__ __forceinline__ float linear_of(int acc, const Column& c, float row) {
+  return static_cast<float>(acc) * c.scale * row + c.bias;
+}
+
+template <int END>
+__device__ __forceinline__ void finish(const Args& g, size_t at, float v, const Column& c) {
+  if (g.ls) v = v * c.ls;
+  if constexpr (END == kGelu) v = vkd::gelu1<0>(v);
+  if constexpr (END == kResidual) v = static_cast<const float*>(g.out)[at] + v;
+  put(g, at, v);
+}
+
+__device__ __forceinline__ float gated_of(const Args& g, float gate, float up) {
+  return (g.act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(gate) : vkp::gate<VK_GATE_GELU>(gate)) * up;
+}
+
+template <int END, typename T>
+__global__ __launch_bounds__(T::kThreads, 2) void linear_i8_kernel(Args g) {
+  __shared__ __align__(16) char s0[T::kBytes];
+  __shared__ __align__(16) char s1[T::kBytes];
+  int mt, nt;
+  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  const int m0 = mt * T::TM, n0 = nt * T::kHeld;
+  vkp::i32x16 acc[T::MT][T::NT];
+  vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
+
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
+  const int wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
+  int n[kCols];
+  Column c[kCols], u[kCols];
+#pragma unroll
+  for (int j = 0; j < kCols; ++j) {
+    n[j] = n0 + T::b_row(wn, j) + (lane & 31);
+    const int at = n[j] < g.N ? n[j] : g.N - 1;
+    c[j] = column(g, at);
+    if constexpr (T::PAIRED) u[j] = column(g, g.N + at);
+  }
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
+      if (m >= g.M) continue;
+      const float row = g.sx[m];
+#pragma unroll
+      for (int j = 0; j < kCols; ++j) {
+        if (n[j] >= g.N) continue;
+        const size_t at = static_cast<size_t>(m) * g.N + n[j];
+        if constexpr (T::PAIRED)
+          put(g, at, gated_of(g, linear_of(acc[i][j][r], c[j], row),
+                              linear_of(acc[i][j + kCols][r], u[j], row)));
+        else
+          finish<END>(g, at, linear_of(acc[i][j][r], c[j], row), c[j]);
+      }
+    }
+}
+
+// At most 16 RT rows, their codes in memory.
+template <int END, int RT>
+__global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g) {
+  constexpr bool kPaired = END == kGated;
+  __shared__ __align__(16) char smem[vkp::few_bytes<kI8, RT, kPaired>()];
+  const int n0 = blockIdx.x * 16;
+  vkp::few_product<kI8, RT, kPaired>(g.a, g.b, g.k_bytes, n0, smem);
+  for (int e = threadIdx.x; e < 256 * RT; e += vkp::kFewThreads) {
+    const int m = e >> 4, n = n0 + (e & 15);
+    if (m >= g.M || n >= g.N) continue;
+    const float row = g.sx[m];
+    const size_t at = static_cast<size_t>(m) * g.N + n;
+    const Column c = column(g, n);
+    const float v = linear_of(vkp::few_sum<kI8, RT, kPaired>(smem, 0, m, e & 15), c, row);
+    if constexpr (kPaired)
+      put(g, at, gated_of(g, v, linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15),
+                                          column(g, g.N + n), row)));
+    else
+      finish<END>(g, at, v, c);
+  }
+}
+
+// ---------------------------------------------------------------- launches
+template <typename XT, bool VEC>
+void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, char* codes,
+              float* scales) {
+  const dim3 grid((M + 3) / 4), block(256);
+  const auto p = static_cast<uint32_t>(pitch);
+#define VK_LAUNCH(NV)                                                                            \
+  hipLaunchKernelGGL((quantise_rows_kernel<XT, VEC, NV>), grid, block, 0, rt->stream, x, M, K, p, \
+                     codes, scales)
+  if (pitch <= 512) VK_LAUNCH(1);
+  else if (pitch <= 1024) VK_LAUNCH(2);
+  else if (pitch <= 2048) VK_LAUNCH(4);
+  else if (pitch <= 4096) VK_LAUNCH(8);
+  else VK_LAUNCH(0);
+#undef VK_LAUNCH
+}
+
+template <typename XT>
+void quantise_any(const vk_runtime* rt, const vk_tensor* x, int M, int K, size_t pitch, char* codes,
+                  float* scales) {
+  const auto* p = static_cast<const XT*>(x->ptr);
+  if (K % 8 == 0)
+    quantise<XT, true>(rt, p, M, K, pitch, codes, scales);
+  else
+    quantise<XT, false>(rt, p, M, K, pitch, codes, scales);
+}
+
+template <int END, bool PAIRED>
+int launch_tiles(vk_runtime* rt, Args& g, vkp::TileSize size) {
+  const auto go = [&](auto tile) {
+    typedef decltype(tile) T;
+    g.gm = (g.M + T::TM - 1) / T::TM;
+    g.gn = (g.N + T::kHeld - 1) / T::kHeld;
+    g.group = vkp::kGroupRows / T::TM;
+    hipLaunchKernelGGL((linear_i8_kernel<END, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream,
+                       g);
+  };
+  if (size == vkp::kTile256) go(vkp::Tile<2, 4, 4, 2, PAIRED>{});
+  else if (size == vkp::kTile128) go(vkp::Tile<2, 2, 2, 2, PAIRED>{});
+  else go(vkp::Tile<2, 1, 1, 2, PAIRED>{});
+  return vk::check_launch("linear_i8_kernel");
+}
+
+template <int END>
+int launch(vk_runtime* rt, Args& g) {
+  constexpr bool kPaired = END == kGated;
+  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, kPaired ? 2LL * g.N : g.N, g.k_bytes);
+  if (!p.few) return launch_tiles<END, kPaired>(rt, g, p.tile);
+  const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
+  if (g.M <= 16)
+    hipLaunchKernelGGL((linear_i8_few_kernel<END, 1>), grid, block, 0, rt->stream, g);
+  else
+    hipLaunchKernelGGL((linear_i8_few_kernel<END, 2>), grid, block, 0, rt->stream, g);
+  return vk::check_launch("linear_i8_few_kernel");
+}
+
+bool is_float(const vk_tensor* t) {
+  return t->dtype == VK_F32 || t->dtype == VK_F16 || t->dtype == VK_BF16;
+}
+
+int check_tensor(const vk_runtime* rt, const vk_tensor* t, size_t rows, size_t cols,
+                 const char* what) {
+  VK_REQUIRE(t, "linear_i8: null %s", what);
+  VK_REQUIRE(is_float(t) && t->len == rows * cols,
+             "linear_i8: %s must be f32, f16 or bf16 [%zu x %zu] (holds %zu)", what, rows, cols,
+             t->len);
+  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0, "linear_i8: %s must be 16-byte aligned",
+             what);
+  return vk::check_device(rt, t, what);
+}
+
+int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows, vk_tensor* out,
+        End end, int act) {
+  VK_TRY(vk::bind(rt));
+  VK_REQUIRE(lin, "linear_i8: null linear");
+  VK_REQUIRE(lin->rt->device == rt->device, "linear_i8: a linear of another device");
+  VK_UNSUPPORTED_IF(rows > 0x7fffff00ULL, "linear_i8: %zu rows", rows);
+  const size_t K = lin->in_features;
+  if (end == kGated) {
+    VK_REQUIRE(lin->out_features % 2 == 0, "linear_i8: gated over %zu columns", lin->out_features);
+    VK_REQUIRE(act == VK_GATE_SILU || act == VK_GATE_GELU, "linear_i8: unknown activation %d", act);
+  }
+  VK_REQUIRE(!lin->ls_gamma || end == kStore || end == kResidual,
+             "linear_i8: this call's linear carries no LayerScale");
+  const size_t N = end == kGated ? lin->out_features / 2 : lin->out_features;
+  VK_TRY(check_tensor(rt, x, rows, K, "x"));
+  VK_TRY(check_tensor(rt, out, rows, N, end == kResidual ? "residual" : "out"));
+  VK_REQUIRE(end != kResidual || out->dtype == VK_F32, "linear_i8: residual must be f32");
+  VK_REQUIRE(!vk::overlap(x, out), "linear_i8: the output overlaps x");
+  if (rows == 0) return VK_OK;
+  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((N + 31) / 32) > 0x7fffffULL, "linear_i8: %zu x %zu outputs",
+                    rows, N);
+
+  const size_t code_bytes = rows * lin->pitch;  // a multiple of 128
+  VK_TRY(vk::ensure_work(rt, code_bytes / 4 + rows, "linear_i8"));
+  char* codes = reinterpret_cast<char*>(rt->work);
+  float* scales = reinterpret_cast<float*>(codes + code_bytes);
+  const int M = static_cast<int>(rows);
+  if (x->dtype == VK_F32)
+    quantise_any<float>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+  else if (x->dtype == VK_F16)
+    quantise_any<_Float16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+  else
+    quantise_any<__bf16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+  VK_TRY(vk::check_launch("quantise_rows_kernel"));
+
+  Args g{};
+  g.a = Operand{codes, M, static_cast<uint32_t>(lin->pitch)};
+  g.b = Operand{reinterpret_cast<const char*>(lin->codes), static_cast<int>(lin->out_features),
+                static_cast<uint32_t>(lin->pitch)};
+  g.sx = scales;
+  g.sw = lin->scale;
+  g.bias = lin->bias;
+  g.ls = lin->ls_gamma;
+  g.out = out->ptr;
+  g.M = M;
+  g.N = static_cast<int>(N);
+  g.k_bytes = static_cast<int>(lin->pitch);
+  g.act = act;
+  g.type = out->dtype;
+  switch (end) {
+    case kStore: return launch<kStore>(rt, g);
+    case kGelu: return launch<kGelu>(rt, g);
+    case kResidual: return launch<kResidual>(rt, g);
+    default: return launch<kGated>(rt, g);
+  }
+}
+
+// ---------------------------------------------------------------- weights
+int check_prepare(size_t in, size_t out) {
+  VK_REQUIRE(in > 0 && out > 0, "linear_i8: empty");
+  VK_UNSUPPORTED_IF(in > kMostK, "linear_i8: in_features=%zu (at most %zu: the int32 sum)", in, kMostK);
+  VK_UNSUPPORTED_IF(out > 0x7fffff00ULL / ((in + 127) / 128 * 128), "linear_i8: %zu x %zu weights", in,
+                    out);
+  return VK_OK;
+}
+
+int upload(void** dev, const void* host, size_t bytes) {
+  VK_HIP(hipMalloc(dev, bytes));
+  VK_HIP(hipMemcpy(*dev, host, bytes, hipMemcpyHostToDevice));
+  return VK_OK;
+}
+
+// codes [out, pitch]
+int make(vk_runtime* rt, size_t in, size_t out, const std::vector<int8_t>& codes, const float* scale,
+         const float* bias, const float* ls, vk_linear_i8** res) {
+  auto* lin = new (std::nothrow) vk_linear_i8;
+  if (!lin) return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
+  lin->rt = rt;
+  vk::retain(rt);
+  lin->in_features = in;
+  lin->out_features = out;
+  lin->pitch = codes.size() / out;
+  int s = upload(reinterpret_cast<void**>(&lin->codes), codes.data(), codes.size());
+  if (s == VK_OK) s = upload(reinterpret_cast<void**>(&lin->scale), scale, out * 4);
+  if (s == VK_OK && bias) s = upload(reinterpret_cast<void**>(&lin->bias), bias, out * 4);
+  if (s == VK_OK && ls) s = upload(reinterpret_cast<void**>(&lin->ls_gamma), ls, out * 4);
+  if (s != VK_OK) {
+    vk_linear_i8_destroy(lin);
+    return s;
+  }
+  *res = lin;
+  return VK_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int vk_linear_i8_prepare(vk_runtime* rt, size_t in_features, size_t out_features,
+                         const int8_t* codes_out_in, const float* scale, const float* bias,
+                         const float* ls_gamma, vk_linear_i8** out) try {
+  VK_TRY(vk::bind(rt));
+  VK_REQUIRE(out && codes_out_in && scale, "null argument");
+  VK_TRY(check_prepare(in_features, out_features));
+  const size_t pitch = (in_features + 127) / 128 * 128;
+  std::vector<int8_t> w(pitch * out_features, 0);
+  for (size_t o = 0; o < out_features; ++o)
+    std::memcpy(&w[o * pitch], codes_out_in + o * in_features, in_features);
+  return make(rt, in_features, out_features, w, scale, bias, ls_gamma, out);
+} catch (const std::bad_alloc&) {
+  return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
+}
+
+int vk_linear_i8_prepare_f32(vk_runtime* rt, size_t in_features, size_t out_features,
+                             const float* weight_in_out, const float* bias, const float* ls_gamma,
+                             vk_linear_i8** out) try {
+  VK_TRY(vk::bind(rt));
+  VK_REQUIRE(out && weight_in_out, "null argument");
+  VK_TRY(check_prepare(in_features, out_features));
+  const size_t pitch = (in_features + 127) / 128 * 128;
+  std::vector<int8_t> w(pitch * out_features, 0);
+  std::vector<float> scale(out_features, 0.0f);  // first each channel's largest |w|
+  std::vector<char> odd(out_features, 0);
+  for (size_t i = 0; i < in_features; ++i)
+    for (size_t o = 0; o < out_features; ++o) {
+      const float a = std::fabs(weight_in_out[i * out_features + o]);
+      if (!std::isfinite(a)) odd[o] = 1;
+      if (a > scale[o]) scale[o] = a;
+    }
+  for (size_t o = 0; o < out_features; ++o) {
+    const float d = scale[o] / kTop;
+    scale[o] = odd[o] ? std::nanf("") : (d < kLeastScale ? 0.0f : d);
+  }
+  for (size_t i = 0; i < in_features; ++i)
+    for (size_t o = 0; o < out_features; ++o)
+      if (scale[o] > 0.0f)
+        w[o * pitch + i] = static_cast<int8_t>(std::nearbyint(weight_in_out[i * out_features + o] / scale[o]));
+  return make(rt, in_features, out_features, w, scale.data(), bias, ls_gamma, out);
+} catch (const std::bad_alloc&) {
+  return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
+}
+
+int vk_linear_i8_destroy(vk_linear_i8* lin) {
+  if (!lin) return VK_OK;
+  vk_runtime* rt = lin->rt;
+  (void)vk::bind_device(rt);
+  (void)hipStreamSynchronize(rt->stream);
+  for (void* p : {static_cast<void*>(lin->codes), static_cast<void*>(lin->scale),
+                  static_cast<void*>(lin->bias), static_cast<void*>(lin->ls_gamma)})
+    if (p) (void)hipFree(p);
+  delete lin;
+  vk::release(rt);
+  return VK_OK;
+}
+
+size_t vk_linear_i8_input_features(const vk_linear_i8* lin) { return lin ? lin->in_features : 0; }
+
+int vk_linear_i8_run_into(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows,
+                          vk_tensor* out) {
+  return run(rt, lin, x, rows, out, kStore, 0);
+}
+
+int vk_linear_i8_run_gelu(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows,
+                          vk_tensor* out) {
+  return run(rt, lin, x, rows, out, kGelu, 0);
+}
+
+int vk_linear_i8_run_residual(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x,
+                              size_t rows, vk_tensor* residual) {
+  return run(rt, lin, x, rows, residual, kResidual, 0);
+}
+
+int vk_linear_i8_run_gated(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows,
+                           int activation, vk_tensor* out) {
+  return run(rt, lin, x, rows, out, kGated, activation);
+}
+
+}  // extern "C"

@@ -40,6 +40,7 @@ size_t dtype_size(vk_dtype d) {
     case VK_U8: return 1;
     case VK_I32: return 4;
     case VK_I64: return 8;
+    case VK_BF16: return 2;
   }
   return 0;
 }
@@ -441,6 +442,10 @@ int vk_upload_f16(vk_runtime* rt, const uint16_t* host, size_t len, vk_tensor** 
   return upload(rt, VK_F16, host, len, out);
 }
 
+int vk_upload_bf16(vk_runtime* rt, const uint16_t* host, size_t len, vk_tensor** out) {
+  return upload(rt, VK_BF16, host, len, out);
+}
+
 int vk_upload_u8(vk_runtime* rt, const uint8_t* host, size_t len, vk_tensor** out) {
   return upload(rt, VK_U8, host, len, out);
 }
@@ -492,6 +497,16 @@ int vk_download_u8(vk_runtime* rt, const vk_tensor* t, uint8_t* host, size_t len
   VK_REQUIRE(t->len == len, "length mismatch: tensor %zu, host %zu", t->len, len);
   VK_TRY(bind(rt));
   if (len > 0) VK_HIP(hipMemcpyAsync(host, t->ptr, len, hipMemcpyDeviceToHost, rt->stream));
+  VK_HIP(hipStreamSynchronize(rt->stream));
+  return VK_OK;
+}
+
+int vk_download_16(vk_runtime* rt, const vk_tensor* t, uint16_t* host, size_t len) {
+  VK_REQUIRE(t != nullptr && (host != nullptr || len == 0), "null tensor or host pointer");
+  VK_REQUIRE(t->dtype == VK_F16 || t->dtype == VK_BF16, "download_16 of a tensor of other values");
+  VK_REQUIRE(t->len == len, "length mismatch: tensor %zu, host %zu", t->len, len);
+  VK_TRY(bind(rt));
+  if (len > 0) VK_HIP(hipMemcpyAsync(host, t->ptr, len * 2, hipMemcpyDeviceToHost, rt->stream));
   VK_HIP(hipStreamSynchronize(rt->stream));
   return VK_OK;
 }

@@ -29,13 +29,15 @@ VK_ERR_UNSUPPORTED = -2
 VK_ERR_HIP = -3
 VK_ERR_OOM = -4
 
-VK_F32, VK_F16, VK_U8, VK_I32, VK_I64 = 0, 1, 2, 3, 4
+VK_F32, VK_F16, VK_U8, VK_I32, VK_I64, VK_BF16 = 0, 1, 2, 3, 4, 5
 # 2D RoPE convention flags (pairing | exponent); 0 is the default
 VK_ROPE_ROTATE_HALF, VK_ROPE_INTERLEAVED = 0, 1
 VK_ROPE_EXP_HALF, VK_ROPE_EXP_HEAD = 0, 2
 VK_ROPE_DEFAULT = 0
 VK_ROPE_SECTIONS, VK_ROPE_MAX_AXES = 4, 4
 VK_CACHE_Q8, VK_CACHE_F8 = 0, 1
+# activation of a gated feed-forward
+VK_GATE_SILU, VK_GATE_GELU = 0, 1
 VK_QK_HEADS_OUTER, VK_QK_VIEWS_OUTER = 0, 1
 # LayerNorm summation order of a runtime (vk_runtime_set_layernorm_order)
 VK_LN_ORDER_TREE, VK_LN_ORDER_SEQUENTIAL = 0, 1
@@ -138,6 +140,8 @@ _SIGS = {
     "vk_tensor_device_ptr": ([_vp], _vp),
     "vk_upload_f32": ([_vp, _vp, _sz, _pp], _i),
     "vk_upload_f16": ([_vp, _vp, _sz, _pp], _i),
+    "vk_upload_bf16": ([_vp, _vp, _sz, _pp], _i),
+    "vk_download_16": ([_vp, _vp, _vp, _sz], _i),
     "vk_upload_u8": ([_vp, _vp, _sz, _pp], _i),
     "vk_upload_i32": ([_vp, _vp, _sz, _pp], _i),
     "vk_upload_i64": ([_vp, _vp, _sz, _pp], _i),
@@ -217,6 +221,16 @@ _SIGS = {
     "vk_attention_cached_f32": (
         [_vp, C.POINTER(_KvCache), _vp, _sz, _sz, _vp, _vp, _sz, C.POINTER(_AttentionRules), _i,
          _vp], _i),
+    "vk_linear_i8_prepare": ([_vp, _sz, _sz, _vp, _vp, _vp, _vp, _pp], _i),
+    "vk_linear_i8_prepare_f32": ([_vp, _sz, _sz, _vp, _vp, _vp, _pp], _i),
+    "vk_linear_i8_destroy": ([_vp], _i),
+    "vk_linear_i8_input_features": ([_vp], _sz),
+    "vk_linear_i8_run_into": ([_vp, _vp, _vp, _sz, _vp], _i),
+    "vk_linear_i8_run_gelu": ([_vp, _vp, _vp, _sz, _vp], _i),
+    "vk_linear_i8_run_residual": ([_vp, _vp, _vp, _sz, _vp], _i),
+    "vk_linear_i8_run_gated": ([_vp, _vp, _vp, _sz, _i, _vp], _i),
+    "vk_gated_forward": ([_vp, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp], _i),
+    "vk_gated_backward": ([_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, _i, _vp, _vp, _vp], _i),
     "vk_prepend_cls_add_pos_f32": ([_vp, _vp, _vp, _vp, _sz, _sz, _pp], _i),
     "vk_pos_embed_bicubic_f32": ([_vp, _vp, _sz, _sz, _sz, _sz, _f, _pp], _i),
     "vk_patch_embed_u8": ([_vp, _vp, _sz, _sz, _sz, _vp, _vp, _vp, _vp, _vp, _sz, _vp, _vp], _i),
@@ -284,7 +298,7 @@ class Tensor:
         if offset < 0 or length < 0 or offset + length > len(self):
             raise VestraError(VK_ERR_INVALID, "view out of range")
         dt = self.dtype
-        size = {VK_F32: 4, VK_F16: 2, VK_U8: 1, VK_I32: 4, VK_I64: 8}[dt]
+        size = {VK_F32: 4, VK_F16: 2, VK_U8: 1, VK_I32: 4, VK_I64: 8, VK_BF16: 2}[dt]
         out = C.c_void_p()
         _check(lib.vk_tensor_wrap(self.rt.handle, dt, self.device_ptr + size * offset, length,
                                   C.byref(out)))
@@ -393,6 +407,46 @@ class Linear:
         try:
             if self.handle:
                 lib.vk_linear_destroy(self.handle)
+                self.handle = None
+        except Exception:
+            pass
+
+
+class LinearI8:
+    """A linear in 8-bit integers (``vk_linear_i8``): codes with a scale for each
+    output channel, rows of x quantised as they come.  x and out are f32, f16 or
+    bf16."""
+
+    def __init__(self, rt: "Runtime", handle: C.c_void_p):
+        self.rt = rt
+        self.handle = handle
+
+    def input_features(self) -> int:
+        return int(lib.vk_linear_i8_input_features(self.handle))
+
+    def run_into(self, x: Tensor, rows: int, out: Tensor) -> None:
+        """out = x W + b [* gamma]."""
+        _check(lib.vk_linear_i8_run_into(self.rt.handle, self.handle, x.handle, rows, out.handle))
+
+    def run_gelu(self, x: Tensor, rows: int, out: Tensor) -> None:
+        """out = GELU(x W + b), A&S erf."""
+        _check(lib.vk_linear_i8_run_gelu(self.rt.handle, self.handle, x.handle, rows, out.handle))
+
+    def run_residual(self, x: Tensor, rows: int, residual: Tensor) -> None:
+        """residual += (x W + b) [* gamma]."""
+        _check(lib.vk_linear_i8_run_residual(self.rt.handle, self.handle, x.handle, rows,
+                                             residual.handle))
+
+    def run_gated(self, x: Tensor, rows: int, out: Tensor,
+                  activation: int = VK_GATE_SILU) -> None:
+        """out = act(first half of the columns) * second half."""
+        _check(lib.vk_linear_i8_run_gated(self.rt.handle, self.handle, x.handle, rows, activation,
+                                          out.handle))
+
+    def __del__(self):
+        try:
+            if self.handle:
+                lib.vk_linear_i8_destroy(self.handle)
                 self.handle = None
         except Exception:
             pass
@@ -526,6 +580,28 @@ class Runtime:
         out = C.c_void_p()
         _check(lib.vk_upload_f16(self.handle, _ptr(h), h.size, C.byref(out)))
         return Tensor(self, out)
+
+    def upload_bf16(self, host: np.ndarray) -> Tensor:
+        """f32 values rounded to bf16 (nearest, ties to even; a NaN stays one)."""
+        b = np.ascontiguousarray(host, dtype=np.float32).reshape(-1).view(np.uint32)
+        r = (b + (0x7fff + ((b >> 16) & 1))) >> 16
+        h = np.where((b & 0x7fffffff) > 0x7f800000, (b >> 16) | 0x40, r).astype(np.uint16)
+        out = C.c_void_p()
+        _check(lib.vk_upload_bf16(self.handle, _ptr(h), h.size, C.byref(out)))
+        return Tensor(self, out)
+
+    def alloc(self, dtype: int, n: int) -> Tensor:
+        out = C.c_void_p()
+        _check(lib.vk_tensor_alloc(self.handle, dtype, n, C.byref(out)))
+        return Tensor(self, out)
+
+    def download_16(self, t: Tensor) -> np.ndarray:
+        """An f16 or bf16 tensor's values, widened to f32."""
+        host = np.empty(len(t), dtype=np.uint16)
+        _check(lib.vk_download_16(self.handle, t.handle, _ptr(host), host.size))
+        if t.dtype == VK_F16:
+            return host.view(np.float16).astype(np.float32)
+        return (host.astype(np.uint32) << 16).view(np.float32)
 
     def upload_i32(self, host: np.ndarray) -> Tensor:
         h = np.ascontiguousarray(host, dtype=np.int32).reshape(-1)
@@ -857,6 +933,53 @@ class Runtime:
         _check(lib.vk_linear_prepare_oihw_w16(self.handle, in_features, out_features, _ptr(w),
                                               _ptr(b), C.byref(out)))
         return Linear(self, out)
+
+    def prepare_linear_i8(self, in_features: int, out_features: int, codes_out_in: np.ndarray,
+                          scale: np.ndarray, bias: Optional[np.ndarray] = None,
+                          ls_gamma: Optional[np.ndarray] = None) -> LinearI8:
+        """A linear from int8 codes [out, in] and a scale for each output channel."""
+        w = np.ascontiguousarray(codes_out_in, dtype=np.int8).reshape(-1)
+        v = [None if a is None else np.ascontiguousarray(a, dtype=np.float32).reshape(-1)
+             for a in (scale, bias, ls_gamma)]
+        if w.size != in_features * out_features or any(
+                a is not None and a.size != out_features for a in v):
+            raise VestraError(VK_ERR_INVALID, "linear_i8: sizes do not match")
+        out = C.c_void_p()
+        _check(lib.vk_linear_i8_prepare(self.handle, in_features, out_features, _ptr(w),
+                                        *(None if a is None else _ptr(a) for a in v),
+                                        C.byref(out)))
+        return LinearI8(self, out)
+
+    def prepare_linear_i8_f32(self, in_features: int, out_features: int,
+                              weight_in_out: np.ndarray, bias: Optional[np.ndarray] = None,
+                              ls_gamma: Optional[np.ndarray] = None) -> LinearI8:
+        """The same from f32 weights [in, out], quantised channel by channel."""
+        w = np.ascontiguousarray(weight_in_out, dtype=np.float32).reshape(-1)
+        v = [None if a is None else np.ascontiguousarray(a, dtype=np.float32).reshape(-1)
+             for a in (bias, ls_gamma)]
+        if w.size != in_features * out_features or any(
+                a is not None and a.size != out_features for a in v):
+            raise VestraError(VK_ERR_INVALID, "linear_i8: sizes do not match")
+        out = C.c_void_p()
+        _check(lib.vk_linear_i8_prepare_f32(self.handle, in_features, out_features, _ptr(w),
+                                            *(None if a is None else _ptr(a) for a in v),
+                                            C.byref(out)))
+        return LinearI8(self, out)
+
+    def gated_forward(self, x: Tensor, w: Tensor, bias: Optional[Tensor], rows: int,
+                      in_features: int, hidden: int, out: Tensor,
+                      activation: int = VK_GATE_SILU) -> None:
+        """out = act(x Wg^T + bg) * (x Wu^T + bu), all f16 or all bf16, w [2 hidden, in]."""
+        _check(lib.vk_gated_forward(self.handle, x.handle, w.handle, _h(bias), rows, in_features,
+                                    hidden, activation, out.handle))
+
+    def gated_backward(self, x: Tensor, w: Tensor, bias: Optional[Tensor], grad: Tensor,
+                       rows: int, in_features: int, hidden: int, dx: Optional[Tensor],
+                       dw: Optional[Tensor], dbias: Optional[Tensor],
+                       activation: int = VK_GATE_SILU) -> None:
+        """The gradients of gated_forward from its inputs and out's gradient."""
+        _check(lib.vk_gated_backward(self.handle, x.handle, w.handle, _h(bias), grad.handle, rows,
+                                     in_features, hidden, activation, _h(dx), _h(dw), _h(dbias)))
 
     def widen_f16_f32(self, src: Tensor, dst: Tensor) -> None:
         _check(lib.vk_widen_f16_f32(self.handle, src.handle, dst.handle))

@@ -16,7 +16,6 @@
 //   3. dw = [dg du]^T x        (transposes of both);
 //   4. db: the tiles' column sums added in order.
 #include "product_nt.h"
-#include "product_plan.h"
 
 namespace {
 
@@ -31,12 +30,12 @@ struct Args {
   const void* bias;  // 2 N values of the type, or null
   const void* grad;  // [M, N]
   void* out;         // [M, N]; null in the backward
-  void* d;           // dg | du [M, 2 N], rows of d_pitch values, or null
-  void* dt;          // its transpose [2 N, M], rows of dt_pitch values, or null
+  void* d;           // dg | du, rows of 2 d_half values, zeros from N to d_half of each half
   float* sums;       // [gm * WM, 2 N], or null
-  uint32_t d_pitch, dt_pitch;
+  int d_half;
   int M, N;
   int act;
+  bool vec;          // rows of N values are whole 16-byte pieces
   int gm, gn, group;
 };
 
@@ -44,6 +43,15 @@ template <Kind KIND>
 __device__ __forceinline__ float bias_at(const Args& g, int n) {
   typedef typename vkp::Value<KIND>::type V;
   return g.bias ? vkp::widen(static_cast<const V*>(g.bias)[n]) : 0.0f;
+}
+
+// The tile's biases, gates then partners.
+template <Kind KIND, typename T>
+__device__ __forceinline__ void load_bias(const Args& g, int n0, float* to) {
+  for (int c = threadIdx.x; c < T::TN; c += T::kThreads) {
+    const int n = n0 + c % T::kHeld;
+    to[c] = bias_at<KIND>(g, (n < g.N ? n : g.N - 1) + (c < T::kHeld ? 0 : g.N));
+  }
 }
 
 __device__ __forceinline__ float gate_any(int act, float g) {
@@ -58,134 +66,165 @@ __device__ __forceinline__ void slope_any(int act, float g, float* a, float* s) 
 }
 
 template <Kind KIND, typename T>
-__global__ __launch_bounds__(T::kThreads, 2) void gated_kernel(Args g) {
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args g) {
   typedef typename vkp::Value<KIND>::type V;
-  __shared__ __align__(16) char s0[T::kBytes];
-  __shared__ __align__(16) char s1[T::kBytes];
+  VK_STAGES(T);
+  __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
   vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
+  load_bias<KIND, T>(g, n0, bias);
+  const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave / T::WN, wn = wave % T::WN;
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
+  if (place.group > 0) return;
+  const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
+  typedef vkp::Chunk<V, kCols> C;
+  char* chunk = stages_[0] + wave * C::kBytes;
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    const int n = n0 + T::b_row(wn, j) + (lane & 31);
-    if (n >= g.N) continue;
-    const float bg = bias_at<KIND>(g, n), bu = bias_at<KIND>(g, g.N + n);
+  for (int i = 0; i < T::MT; ++i) {
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int j = 0; j < kCols; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
-        if (m >= g.M) continue;
-        static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] =
-            static_cast<V>(gate_any(g.act, acc[i][j][r] + bg) * (acc[i][j + kCols][r] + bu));
+      for (int q = 0; q < 4; ++q) {
+        const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+        const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
+        const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
+        typename C::V4 h;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          h[e] = static_cast<V>(gate_any(g.act, acc[i][j][4 * q + e] + bg[e]) *
+                                (acc[i][j + kCols][4 * q + e] + bu[e]));
+        *C::at(chunk, lane, j, q) = h;
       }
+    vkd::wave_lds_fence();
+    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
+                             n0 + T::b_row(wn, 0), g.N, g.vec);
+    vkd::wave_lds_fence();
   }
 }
 
 // Step 1 of the backward.
 template <Kind KIND, typename T>
-__global__ __launch_bounds__(T::kThreads, 2) void gated_grad_kernel(Args g) {
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel(Args g) {
   typedef typename vkp::Value<KIND>::type V;
-  typedef V V4 __attribute__((ext_vector_type(4)));
-  __shared__ __align__(16) char s0[T::kBytes];
-  __shared__ __align__(16) char s1[T::kBytes];
+  VK_STAGES(T);
+  __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
   vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
+  load_bias<KIND, T>(g, n0, bias);
+  const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave / T::WN, wn = wave % T::WN;
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
+  if (place.group > 0) return;
+  const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
+  typedef vkp::Chunk<V, kCols> C;
+  char* chunk = stages_[0] + wave * C::kBytes;
   const V* grad = static_cast<const V*>(g.grad);
-  const int rows8 = (g.M + 7) & ~7, cols8 = (2 * g.N + 7) & ~7;
+  V* d = static_cast<V*>(g.d);
+  const size_t pitch = 2 * static_cast<size_t>(g.d_half);
+  const int nb = n0 + T::b_row(wn, 0);
+  vkp::i32x4 dh[C::kFetch];
+  C::fetch(dh, lane, grad, g.N, m0 + wm * T::MT * 32, g.M, nb, g.N, g.vec);
+  float sum[kCols] = {};
 #pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    const int n = n0 + T::b_row(wn, j) + (lane & 31);
-    const bool in = n < g.N;
-    const float bg = in ? bias_at<KIND>(g, n) : 0.0f, bu = in ? bias_at<KIND>(g, g.N + n) : 0.0f;
-    float sg = 0.0f, su = 0.0f;
+  for (int i = 0; i < T::MT; ++i) {
+    const int mb = m0 + (wm * T::MT + i) * 32;
+    C::fill(chunk, lane, dh);
+    if (i + 1 < T::MT) C::fetch(dh, lane, grad, g.N, mb + 32, g.M, nb, g.N, g.vec);
+    vkd::wave_lds_fence();
+    // rows past M and columns past N have dh of 0; what their g and u are is finite only where
+    // the others' are
+    const bool in = mb + (lane & 31) < g.M;
+    typename C::V4 du[kCols][4];
+    float v[kCols * 32];
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int j = 0; j < kCols; ++j)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int m4 = m0 + (wm * T::MT + i) * 32 + 8 * q + 4 * (lane >> 5);
-        V4 dg{}, du{};
+        const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+        const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
+        const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
+        typename C::V4* at = C::at(chunk, lane, j, q);
+        const typename C::V4 h4 = *at;
+        typename C::V4 dg;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int m = m4 + r;
-          if (!in || m >= g.M) continue;
+        for (int e = 0; e < 4; ++e) {
           float a, s;
-          slope_any(g.act, acc[i][j][4 * q + r] + bg, &a, &s);
-          const float dh = vkp::widen(grad[static_cast<size_t>(m) * g.N + n]);
-          const float fg = dh * (acc[i][j + kCols][4 * q + r] + bu) * s, fu = dh * a;
-          sg += fg;
-          su += fu;
-          dg[r] = static_cast<V>(fg);
-          du[r] = static_cast<V>(fu);
-          if (g.d) {
-            V* d = static_cast<V*>(g.d) + static_cast<size_t>(m) * g.d_pitch;
-            d[n] = dg[r];
-            d[g.N + n] = du[r];
-            // zeros up to the next multiple of 16 bytes
-            if (n == g.N - 1)
-              for (int z = 2 * g.N; z < cols8; ++z) d[z] = static_cast<V>(0.0f);
-          }
+          slope_any(g.act, acc[i][j][4 * q + e] + bg[e], &a, &s);
+          const float h = vkp::widen(h4[e]);
+          const bool held = in && n0 + c + e < g.N;
+          const float fg = held ? h * (acc[i][j + kCols][4 * q + e] + bu[e]) * s : 0.0f;
+          const float fu = held ? h * a : 0.0f;
+          v[j * 16 + 4 * q + e] = fg;
+          v[kCols * 16 + j * 16 + 4 * q + e] = fu;
+          dg[e] = static_cast<V>(fg);
+          du[j][q][e] = static_cast<V>(fu);
         }
-        if (g.dt && in && m4 < rows8) {
-          V* dt = static_cast<V*>(g.dt);
-          *reinterpret_cast<V4*>(dt + static_cast<size_t>(n) * g.dt_pitch + m4) = dg;
-          *reinterpret_cast<V4*>(dt + static_cast<size_t>(g.N + n) * g.dt_pitch + m4) = du;
-        }
+        *at = dg;
       }
     if (g.sums) {
-      sg += __shfl_xor(sg, 32, 64);
-      su += __shfl_xor(su, 32, 64);
-      if (in && lane < 32) {
-        float* to = g.sums + static_cast<size_t>(mt * T::WM + wm) * 2 * g.N;
-        to[n] = sg;
-        to[g.N + n] = su;
-      }
+      vkp::sum_rows<kCols>(v, lane);
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) sum[k] += v[k];
+    }
+    if (d) {
+      vkd::wave_lds_fence();
+      C::template store<false>(chunk, lane, d, pitch, mb, g.M, nb, g.d_half, true);
+      vkd::wave_lds_fence();
+#pragma unroll
+      for (int j = 0; j < kCols; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *C::at(chunk, lane, j, q) = du[j][q];
+      vkd::wave_lds_fence();
+      C::template store<false>(chunk, lane, d + g.d_half, pitch, mb, g.M, nb, g.d_half, true);
+    }
+    vkd::wave_lds_fence();
+  }
+  if (g.sums) {
+    // value k of lane l: columns of dg, then of du, by j, q, e
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+      const int at = kCols * (lane & 31) + k, part = at / (kCols * 16), j = at / 16 % kCols;
+      const int n = n0 + T::b_row(wn, 0) + 32 * j + 8 * (at / 4 % 4) + 4 * (lane >> 5) + at % 4;
+      if (n < g.N) g.sums[(static_cast<size_t>(mt * T::WM + wm) * 2 + part) * g.N + n] = sum[k];
     }
   }
 }
 
 // out[m, n] = sum_k a[m, k] b[n, k], rounded to the type.
 template <Kind KIND, typename T>
-__global__ __launch_bounds__(T::kThreads, 2) void product_kernel(Args g) {
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Args g) {
   typedef typename vkp::Value<KIND>::type V;
-  __shared__ __align__(16) char s0[T::kBytes];
-  __shared__ __align__(16) char s1[T::kBytes];
+  VK_STAGES(T);
   int mt, nt;
   vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::TN;
+  const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave / T::WN, wn = wave % T::WN;
+  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
+  if (place.group > 0) return;
+  const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
+  typedef vkp::Chunk<V, T::NT> C;
+  char* chunk = stages_[0] + wave * C::kBytes;
 #pragma unroll
-  for (int j = 0; j < T::NT; ++j) {
-    const int n = n0 + T::b_row(wn, j) + (lane & 31);
-    if (n >= g.N) continue;
+  for (int i = 0; i < T::MT; ++i) {
 #pragma unroll
-    for (int i = 0; i < T::MT; ++i)
+    for (int j = 0; j < T::NT; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
-        if (m < g.M)
-          static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(acc[i][j][r]);
+      for (int q = 0; q < 4; ++q) {
+        typename C::V4 w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(acc[i][j][4 * q + e]);
+        *C::at(chunk, lane, j, q) = w;
       }
+    vkd::wave_lds_fence();
+    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
+                             n0 + T::b_row(wn, 0), g.N, g.vec);
+    vkd::wave_lds_fence();
   }
 }
 
@@ -206,10 +245,10 @@ __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
 }
 
 // ---------------------------------------------------------------- layouts
-// to[c, r] = from[r, c] of 16-bit values, zeros from row `rows` to the next multiple of 8.
-__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* __restrict__ from, int rows,
-                                                          int cols, uint16_t* __restrict__ to,
-                                                          size_t pitch) {
+// to[c, r] = from[r, c] of 16-bit values, zeros from row `rows` to the next multiple of 64.
+__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* __restrict__ from,
+                                                          size_t from_pitch, int rows, int cols,
+                                                          uint16_t* __restrict__ to, size_t pitch) {
   __shared__ uint16_t tile[64][66];
   const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
@@ -219,14 +258,13 @@ __global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* __rest
     for (int h = 0; h < 2; ++h) {
       const int r = r0 + ty + 8 * i, c = c0 + tx + 32 * h;
       tile[ty + 8 * i][tx + 32 * h] =
-          r < rows && c < cols ? from[static_cast<size_t>(r) * cols + c] : uint16_t{0};
+          r < rows && c < cols ? from[r * from_pitch + c] : uint16_t{0};
     }
   __syncthreads();
-  const int rows8 = (rows + 7) & ~7;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int c = c0 + ty + 8 * i, r = r0 + 2 * tx;
-    if (c < cols && r < rows8) {
+    if (c < cols) {
       const uint32_t lo = tile[2 * tx][ty + 8 * i], hi = tile[2 * tx + 1][ty + 8 * i];
       *reinterpret_cast<uint32_t*>(to + static_cast<size_t>(c) * pitch + r) = lo | hi << 16;
     }
@@ -251,14 +289,24 @@ void zero16(const vk_runtime* rt, void* p, size_t n) {
                      static_cast<uint16_t*>(p), n);
 }
 
-// dbias[c] = sum over the tiles' sums, in order.
+// dbias[c] = sum over the tiles' sums: sixteen runs of parts a column, each in order, then the
+// runs in order.
 template <Kind KIND>
 __global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int parts,
                                                         int cols, void* out) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= cols) return;
+  __shared__ float run[16][16];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
+  const int from = parts * y / 16, to = parts * (y + 1) / 16;
   float s = 0.0f;
-  for (int p = 0; p < parts; ++p) s += sums[static_cast<size_t>(p) * cols + c];
+  if (c < cols)
+#pragma unroll 8
+    for (int p = from; p < to; ++p) s += sums[static_cast<size_t>(p) * cols + c];
+  run[y][x] = s;
+  __syncthreads();
+  if (y > 0 || c >= cols) return;
+  s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) s += run[i][x];
   static_cast<typename vkp::Value<KIND>::type*>(out)[c] =
       static_cast<typename vkp::Value<KIND>::type>(s);
 }
@@ -269,16 +317,13 @@ size_t padded(size_t n) { return (n + kPitchValues - 1) / kPitchValues * kPitchV
 
 template <bool PAIRED, typename F>
 void with_tile(vkp::TileSize size, Args& g, F go) {
-  const auto set = [&](auto tile) {
+  vkp::with_tile<PAIRED>(size, [&](auto tile) {
     typedef decltype(tile) T;
     g.gm = (g.M + T::TM - 1) / T::TM;
     g.gn = (g.N + T::kHeld - 1) / T::kHeld;
     g.group = vkp::kGroupRows / T::TM;
     go(tile);
-  };
-  if (size == vkp::kTile256) set(vkp::Tile<2, 4, 4, 2, PAIRED>{});
-  else if (size == vkp::kTile128) set(vkp::Tile<2, 2, 2, 2, PAIRED>{});
-  else set(vkp::Tile<2, 1, 1, 2, PAIRED>{});
+  });
 }
 
 template <Kind KIND>
@@ -308,6 +353,7 @@ int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k,
   g.out = out;
   g.M = a.rows;
   g.N = b.rows;
+  g.vec = g.N % 8 == 0;
   const vkp::Plan p = vkp::plan(rt->cu_count, g.M, g.N, g.k_bytes);
   with_tile<false>(p.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
@@ -317,10 +363,10 @@ int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k,
   return vk::check_launch("product_kernel");
 }
 
-void transpose(const vk_runtime* rt, const void* from, size_t rows, size_t cols, void* to,
-               size_t pitch) {
+void transpose(const vk_runtime* rt, const void* from, size_t from_pitch, size_t rows, size_t cols,
+               void* to, size_t pitch) {
   hipLaunchKernelGGL(transpose16_kernel, dim3((cols + 63) / 64, (rows + 63) / 64), dim3(256), 0,
-                     rt->stream, static_cast<const uint16_t*>(from), static_cast<int>(rows),
+                     rt->stream, static_cast<const uint16_t*>(from), from_pitch, static_cast<int>(rows),
                      static_cast<int>(cols), static_cast<uint16_t*>(to), pitch);
 }
 
@@ -340,25 +386,22 @@ Operand as_operand(const vk_runtime* rt, const void* p, size_t rows, size_t cols
 template <Kind KIND>
 int backward(vk_runtime* rt, Args& g, const void* x, const void* w, size_t rows, size_t in,
              size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
-  const size_t dp = padded(2 * hidden), rp = padded(rows);
+  const size_t half = padded(hidden), rp = padded(rows);
   const auto take = [&](size_t bytes) {
     char* at = room;
     room += (bytes + 255) / 256 * 256;
     return at;
   };
-  if (dx) {
-    g.d = take(rows * dp * 2);
-    g.d_pitch = static_cast<uint32_t>(dp);
-  }
-  if (dw) {
-    g.dt = take(2 * hidden * rp * 2);
-    g.dt_pitch = static_cast<uint32_t>(rp);
+  if (dx || dw) {
+    g.d = take(rows * 2 * half * 2);
+    g.d_half = static_cast<int>(half);
   }
   const vkp::Plan p = vkp::plan(rt->cu_count, g.M, 2LL * g.N, g.k_bytes);
   int parts = 0;
   with_tile<true>(p.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
     parts = g.gm * T::WM;
+    g.gn = (static_cast<int>(half) + T::kHeld - 1) / T::kHeld;  // the zeros up to d_half too
     if (dbias) g.sums = reinterpret_cast<float*>(take(static_cast<size_t>(parts) * 2 * hidden * 4));
     hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
                        rt->stream, g);
@@ -366,19 +409,24 @@ int backward(vk_runtime* rt, Args& g, const void* x, const void* w, size_t rows,
   VK_TRY(vk::check_launch("gated_grad_kernel"));
   const int R = static_cast<int>(rows), D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden);
   if (dx) {
-    char* wt = take(in * dp * 2);
-    transpose(rt, w, 2 * hidden, in, wt, dp);
-    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.d), R, static_cast<uint32_t>(2 * dp)},
-                                Operand{wt, D, static_cast<uint32_t>(2 * dp)}, 2 * hidden, dx->ptr));
+    const uint32_t pitch = static_cast<uint32_t>(4 * half);
+    char* wt = take(in * 2 * half * 2);
+    transpose(rt, w, in, hidden, in, wt, 2 * half);
+    transpose(rt, static_cast<const char*>(w) + hidden * in * 2, in, hidden, in, wt + half * 2, 2 * half);
+    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.d), R, pitch}, Operand{wt, D, pitch},
+                                2 * half, dx->ptr));
   }
   if (dw) {
+    char* dt = take(2 * hidden * rp * 2);
     char* xt = take(in * rp * 2);
-    transpose(rt, x, rows, in, xt, rp);
-    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.dt), H2, static_cast<uint32_t>(2 * rp)},
+    transpose(rt, g.d, 2 * half, rows, hidden, dt, rp);
+    transpose(rt, static_cast<char*>(g.d) + half * 2, 2 * half, rows, hidden, dt + hidden * rp * 2, rp);
+    transpose(rt, x, in, rows, in, xt, rp);
+    VK_TRY(launch_product<KIND>(rt, Operand{dt, H2, static_cast<uint32_t>(2 * rp)},
                                 Operand{xt, D, static_cast<uint32_t>(2 * rp)}, rows, dw->ptr));
   }
   if (dbias) {
-    hipLaunchKernelGGL(bias_grad_kernel<KIND>, dim3((2 * hidden + 255) / 256), dim3(256), 0, rt->stream,
+    hipLaunchKernelGGL(bias_grad_kernel<KIND>, dim3((2 * hidden + 15) / 16), dim3(256), 0, rt->stream,
                        g.sums, parts, static_cast<int>(2 * hidden), dbias->ptr);
     VK_TRY(vk::check_launch("bias_grad_kernel"));
   }
@@ -424,6 +472,7 @@ Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, 
   g.M = static_cast<int>(rows);
   g.N = static_cast<int>(hidden);
   g.act = act;
+  g.vec = hidden % 8 == 0;
   return g;
 }
 
@@ -469,9 +518,10 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
     if (dbias) zero16(rt, dbias->ptr, dbias->len);
     return vk::check_launch("zero16_kernel");
   }
-  const size_t dp = padded(2 * hidden), rp = padded(rows);
+  const size_t half = padded(hidden), rp = padded(rows);
   size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features) + 8 * 256;
-  if (dx) need += (rows + in_features) * dp * 2;
+  if (dx || dw) need += rows * 4 * half;
+  if (dx) need += in_features * 4 * half;
   if (dw) need += (2 * hidden + in_features) * rp * 2;
   if (dbias) need += ((rows + 63) / 64 * 2) * 2 * hidden * 4;
   VK_TRY(vk::ensure_work(rt, (need + 3) / 4, "gated_backward"));

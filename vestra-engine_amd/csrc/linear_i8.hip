@@ -13,7 +13,6 @@
 #include <vector>
 
 #include "product_nt.h"
-#include "product_plan.h"
 
 struct vk_linear_i8 {
   vk_runtime* rt = nullptr;
@@ -48,7 +47,8 @@ struct Args {
   void* out;
   int M, N;  // N: columns of out
   int k_bytes;
-  int act, type;  // VK_GATE_*, vk_dtype of out
+  int act;  // VK_GATE_*
+  bool vec; // out's rows are whole 16-byte pieces
   int gm, gn, group;
 };
 
@@ -158,85 +158,92 @@ __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict
 }
 
 // ---------------------------------------------------------------- what leaves
-__device__ __forceinline__ void put(const Args& g, size_t at, float v) {
-  if (g.type == VK_F32)
-    static_cast<float*>(g.out)[at] = v;
-  else if (g.type == VK_F16)
-    static_cast<_Float16*>(g.out)[at] = static_cast<_Float16>(v);
-  else
-    static_cast<__bf16*>(g.out)[at] = static_cast<__bf16>(v);
-}
-
-struct Column {
-  float scale, bias, ls;
-};
-__device__ __forceinline__ Column column(const Args& g, int n) {
-  return Column{g.sw[n], g.bias ? g.bias[n] : 0.0f, g.ls ? g.ls[n] : 1.0f};
-}
-
 // The channel's scale first: a row's largest scale then overflows only where the result
 // does.
-__device__ __forceinline__ float linear_of(int acc, const Column& c, float row) {
-  return static_cast<float>(acc) * c.scale * row + c.bias;
+__device__ __forceinline__ float linear_of(int acc, float channel, float row, float bias) {
+  return static_cast<float>(acc) * channel * row + bias;
+}
+
+__device__ __forceinline__ float gated_of(int act, float gate, float up) {
+  return (act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(gate) : vkp::gate<VK_GATE_GELU>(gate)) * up;
 }
 
 template <int END>
-__device__ __forceinline__ void finish(const Args& g, size_t at, float v, const Column& c) {
-  if (g.ls) v = v * c.ls;
+__device__ __forceinline__ float finish(float v, float ls) {
+  if constexpr (END == kStore || END == kResidual) v = v * ls;  // 1 where there is none
   if constexpr (END == kGelu) v = vkd::gelu1<0>(v);
-  if constexpr (END == kResidual) v = static_cast<const float*>(g.out)[at] + v;
-  put(g, at, v);
+  return v;
 }
 
-__device__ __forceinline__ float gated_of(const Args& g, float gate, float up) {
-  return (g.act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(gate) : vkp::gate<VK_GATE_GELU>(gate)) * up;
-}
-
-template <int END, typename T>
-__global__ __launch_bounds__(T::kThreads, 2) void linear_i8_kernel(Args g) {
-  __shared__ __align__(16) char s0[T::kBytes];
-  __shared__ __align__(16) char s1[T::kBytes];
+template <int END, typename V, typename T>
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(Args g) {
+  VK_STAGES(T);
+  __shared__ __align__(16) float cols[3][T::TN];  // scale, bias, LayerScale of the tile's columns
   int mt, nt;
   vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
-  vkp::i32x16 acc[T::MT][T::NT];
-  vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, s0, s1, acc);
-
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
-  const int wm = wave / T::WN, wn = wave % T::WN;
-  constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
-  int n[kCols];
-  Column c[kCols], u[kCols];
-#pragma unroll
-  for (int j = 0; j < kCols; ++j) {
-    n[j] = n0 + T::b_row(wn, j) + (lane & 31);
-    const int at = n[j] < g.N ? n[j] : g.N - 1;
-    c[j] = column(g, at);
-    if constexpr (T::PAIRED) u[j] = column(g, g.N + at);
+  for (int c = threadIdx.x; c < T::TN; c += T::kThreads) {
+    const int n = n0 + c % T::kHeld;
+    const int at = (n < g.N ? n : g.N - 1) + (c < T::kHeld ? 0 : g.N);
+    cols[0][c] = g.sw[at];
+    cols[1][c] = g.bias ? g.bias[at] : 0.0f;
+    cols[2][c] = g.ls ? g.ls[at] : 1.0f;
   }
+  const vkp::Place<T> place;
+  vkp::i32x16 acc[T::MT][T::NT];
+  vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
+  if (place.group > 0) return;
+  const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
+  constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
+  constexpr int J = sizeof(V) == 4 ? 1 : (kCols < 2 ? kCols : 2);
+  typedef vkp::Chunk<V, J> C;
+  static_assert(T::kWaves * C::kBytes <= T::kBytes, "the chunks fit a stage buffer");
+  char* chunk = stages_[0] + wave * C::kBytes;
+  V* out = static_cast<V*>(g.out);
 #pragma unroll
-  for (int i = 0; i < T::MT; ++i)
+  for (int i = 0; i < T::MT; ++i) {
+    const int mb = m0 + (wm * T::MT + i) * 32, m = mb + (lane & 31);
+    const float row = g.sx[m < g.M ? m : g.M - 1];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int m = m0 + (wm * T::MT + i) * 32 + vkp::acc_row(lane, r);
-      if (m >= g.M) continue;
-      const float row = g.sx[m];
+    for (int jg = 0; jg < kCols; jg += J) {
 #pragma unroll
-      for (int j = 0; j < kCols; ++j) {
-        if (n[j] >= g.N) continue;
-        const size_t at = static_cast<size_t>(m) * g.N + n[j];
-        if constexpr (T::PAIRED)
-          put(g, at, gated_of(g, linear_of(acc[i][j][r], c[j], row),
-                              linear_of(acc[i][j + kCols][r], u[j], row)));
-        else
-          finish<END>(g, at, linear_of(acc[i][j][r], c[j], row), c[j]);
-      }
+      for (int jj = 0; jj < J; ++jj)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int j = jg + jj, c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+          const float4 s = *reinterpret_cast<const float4*>(&cols[0][c]);
+          const float4 b = *reinterpret_cast<const float4*>(&cols[1][c]);
+          const float4 l = *reinterpret_cast<const float4*>(&cols[2][c]);
+          float v[4] = {linear_of(acc[i][j][4 * q], s.x, row, b.x),
+                        linear_of(acc[i][j][4 * q + 1], s.y, row, b.y),
+                        linear_of(acc[i][j][4 * q + 2], s.z, row, b.z),
+                        linear_of(acc[i][j][4 * q + 3], s.w, row, b.w)};
+          const float ls[4] = {l.x, l.y, l.z, l.w};
+          if constexpr (T::PAIRED) {
+            const float4 us = *reinterpret_cast<const float4*>(&cols[0][c + T::kHeld]);
+            const float4 ub = *reinterpret_cast<const float4*>(&cols[1][c + T::kHeld]);
+            const float u[4] = {linear_of(acc[i][j + kCols][4 * q], us.x, row, ub.x),
+                                linear_of(acc[i][j + kCols][4 * q + 1], us.y, row, ub.y),
+                                linear_of(acc[i][j + kCols][4 * q + 2], us.z, row, ub.z),
+                                linear_of(acc[i][j + kCols][4 * q + 3], us.w, row, ub.w)};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = gated_of(g.act, v[e], u[e]);
+          }
+          typename C::V4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(finish<END>(v[e], ls[e]));
+          *C::at(chunk, lane, jj, q) = w;
+        }
+      vkd::wave_lds_fence();
+      C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N,
+                                          g.vec);
+      vkd::wave_lds_fence();
     }
+  }
 }
 
 // At most 16 RT rows, their codes in memory.
-template <int END, int RT>
+template <int END, typename V, int RT>
 __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g) {
   constexpr bool kPaired = END == kGated;
   __shared__ __align__(16) char smem[vkp::few_bytes<kI8, RT, kPaired>()];
@@ -246,14 +253,17 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g)
     const int m = e >> 4, n = n0 + (e & 15);
     if (m >= g.M || n >= g.N) continue;
     const float row = g.sx[m];
-    const size_t at = static_cast<size_t>(m) * g.N + n;
-    const Column c = column(g, n);
-    const float v = linear_of(vkp::few_sum<kI8, RT, kPaired>(smem, 0, m, e & 15), c, row);
-    if constexpr (kPaired)
-      put(g, at, gated_of(g, v, linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15),
-                                          column(g, g.N + n), row)));
-    else
-      finish<END>(g, at, v, c);
+    V* to = static_cast<V*>(g.out) + static_cast<size_t>(m) * g.N + n;
+    const float bias = g.bias ? g.bias[n] : 0.0f;
+    float v = linear_of(vkp::few_sum<kI8, RT, kPaired>(smem, 0, m, e & 15), g.sw[n], row, bias);
+    if constexpr (kPaired) {
+      const int p = g.N + n;
+      v = gated_of(g.act, v, linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15), g.sw[p], row,
+                                       g.bias ? g.bias[p] : 0.0f));
+    }
+    v = finish<END>(v, g.ls ? g.ls[n] : 1.0f);
+    if constexpr (END == kResidual) v = *to + v;
+    *to = static_cast<V>(v);
   }
 }
 
@@ -284,33 +294,34 @@ void quantise_any(const vk_runtime* rt, const vk_tensor* x, int M, int K, size_t
     quantise<XT, false>(rt, p, M, K, pitch, codes, scales);
 }
 
-template <int END, bool PAIRED>
-int launch_tiles(vk_runtime* rt, Args& g, vkp::TileSize size) {
-  const auto go = [&](auto tile) {
+template <int END, typename V>
+int launch(vk_runtime* rt, Args& g) {
+  constexpr bool kPaired = END == kGated;
+  g.vec = static_cast<size_t>(g.N) * sizeof(V) % 16 == 0;
+  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, kPaired ? 2LL * g.N : g.N, g.k_bytes);
+  if (p.few) {
+    const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
+    if (g.M <= 16)
+      hipLaunchKernelGGL((linear_i8_few_kernel<END, V, 1>), grid, block, 0, rt->stream, g);
+    else
+      hipLaunchKernelGGL((linear_i8_few_kernel<END, V, 2>), grid, block, 0, rt->stream, g);
+    return vk::check_launch("linear_i8_few_kernel");
+  }
+  vkp::with_tile<kPaired>(p.tile, [&](auto tile) {
     typedef decltype(tile) T;
     g.gm = (g.M + T::TM - 1) / T::TM;
     g.gn = (g.N + T::kHeld - 1) / T::kHeld;
     g.group = vkp::kGroupRows / T::TM;
-    hipLaunchKernelGGL((linear_i8_kernel<END, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream,
-                       g);
-  };
-  if (size == vkp::kTile256) go(vkp::Tile<2, 4, 4, 2, PAIRED>{});
-  else if (size == vkp::kTile128) go(vkp::Tile<2, 2, 2, 2, PAIRED>{});
-  else go(vkp::Tile<2, 1, 1, 2, PAIRED>{});
+    hipLaunchKernelGGL((linear_i8_kernel<END, V, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
+                       rt->stream, g);
+  });
   return vk::check_launch("linear_i8_kernel");
 }
 
 template <int END>
-int launch(vk_runtime* rt, Args& g) {
-  constexpr bool kPaired = END == kGated;
-  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, kPaired ? 2LL * g.N : g.N, g.k_bytes);
-  if (!p.few) return launch_tiles<END, kPaired>(rt, g, p.tile);
-  const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
-  if (g.M <= 16)
-    hipLaunchKernelGGL((linear_i8_few_kernel<END, 1>), grid, block, 0, rt->stream, g);
-  else
-    hipLaunchKernelGGL((linear_i8_few_kernel<END, 2>), grid, block, 0, rt->stream, g);
-  return vk::check_launch("linear_i8_few_kernel");
+int launch_type(vk_runtime* rt, Args& g, vk_dtype type) {
+  if (type == VK_F32) return launch<END, float>(rt, g);
+  return type == VK_F16 ? launch<END, _Float16>(rt, g) : launch<END, __bf16>(rt, g);
 }
 
 bool is_float(const vk_tensor* t) {
@@ -376,12 +387,11 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
   g.N = static_cast<int>(N);
   g.k_bytes = static_cast<int>(lin->pitch);
   g.act = act;
-  g.type = out->dtype;
   switch (end) {
-    case kStore: return launch<kStore>(rt, g);
-    case kGelu: return launch<kGelu>(rt, g);
-    case kResidual: return launch<kResidual>(rt, g);
-    default: return launch<kGated>(rt, g);
+    case kStore: return launch_type<kStore>(rt, g, out->dtype);
+    case kGelu: return launch_type<kGelu>(rt, g, out->dtype);
+    case kResidual: return launch<kResidual, float>(rt, g);
+    default: return launch_type<kGated>(rt, g, out->dtype);
   }
 }
 

@@ -11,12 +11,16 @@
 // both operands go from memory straight into LDS (16 bytes a lane, no
 // registers), two stage buffers, one barrier a stage -- a stage's loads run
 // while the stage before it is multiplied.  In LDS a row is 128 bytes, its
-// 16-byte pieces permuted by (piece ^ row % 8): a fragment read, whose eight
-// neighbouring lanes read the same piece of eight rows, then touches all banks
-// once.  The permutation is applied to the addresses that the loads read from.
+// 16-byte pieces permuted by (piece ^ row / 2 % 8): a fragment read, whose lanes read the
+// same piece of 32 rows, then touches all 64 banks once with any 16 lanes that it takes
+// together (0-3, 12-15, 20-23 and 24-27 among them).  The permutation is applied to the
+// addresses that the loads read from.
 #pragma once
 
+#include <type_traits>
+
 #include "common.h"
+#include "product_plan.h"
 
 namespace vkp {
 
@@ -79,16 +83,25 @@ constexpr uint32_t kMostBytes = 0x7ffffff0u;
 // columns are TN / 2 gates and the TN / 2 partners of the same hidden columns, b
 // rows h and hidden + h; a wave's first NT / 2 column tiles are gates, the others
 // the partners.
-template <int WM_, int WN_, int MT_, int NT_, bool PAIRED_>
+// KG groups of waves share k out by stages and are added in their order at the end: for
+// grids of few tiles.
+template <int WM_, int WN_, int MT_, int NT_, bool PAIRED_, int S_, int R_, int KG_>
 struct Tile {
-  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_;
+  static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, KG = KG_;
+  static constexpr int S = S_, R = R_;  // bytes of k of a stage, stage buffers
   static constexpr bool PAIRED = PAIRED_;
-  static constexpr int kWaves = WM * WN, kThreads = 64 * kWaves;
+  static constexpr int kWaves = WM * WN;  // of a group
+  static constexpr int kThreads = 64 * kWaves * KG;
   static constexpr int TM = 32 * WM * MT, TN = 32 * WN * NT;
   static constexpr int kHeld = PAIRED ? TN / 2 : TN;  // columns of the result
-  static constexpr int kALoads = TM / 8 / kWaves, kBLoads = TN / 8 / kWaves;
-  static constexpr int kBytes = (TM + TN) * kStage;
-  static_assert(kALoads * kWaves * 8 == TM && kBLoads * kWaves * 8 == TN, "loads divide evenly");
+  static constexpr int kRows = 1024 / S;  // rows of a wave's load
+  static constexpr int kALoads = TM / kRows / kWaves, kBLoads = TN / kRows / kWaves;
+  static constexpr int kGroupBytes = (TM + TN) * S, kBytes = KG * kGroupBytes;
+  static_assert((KG - 1) * TM * TN * 4 <= kBytes, "a group's sums fit a stage buffer");
+  static constexpr int kWavesASimd = MT * NT > 8 ? 1 : 2;  // by the registers of the sums
+  static_assert(S == 128 || S == 64, "a row's stage");
+  static_assert(kALoads * kWaves * kRows == TM && kBLoads * kWaves * kRows == TN,
+                "loads divide evenly");
   static_assert(!PAIRED || NT % 2 == 0, "gates and partners");
   // First row of b, within the tile, of a wave's column tile.
   static __device__ __forceinline__ constexpr int b_row(int wn, int nt) {
@@ -100,31 +113,89 @@ struct Tile {
   }
 };
 
-typedef __attribute__((address_space(3))) void* lds_ptr;
-
-// Every load into LDS of the wave has landed, then all waves': the barrier's own fence does
-// not count loads that go past the registers.
-__device__ __forceinline__ void stage_barrier() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+// The tile of a plan's size.  Gates and partners of the largest: a wave's 64 hidden columns are
+// one line of 16-bit results.
+template <bool PAIRED, typename F>
+void with_tile(TileSize size, F go) {
+  if (size == kTile256) {
+    if constexpr (PAIRED) go(Tile<4, 2, 2, 4, true, 128, 2, 1>{});
+    else go(Tile<2, 4, 4, 2, false, 128, 2, 1>{});
+  } else if (size == kTile128) {
+    go(Tile<2, 2, 2, 2, PAIRED, 128, 2, 1>{});
+  } else if (size == kTile64K) {
+    go(Tile<2, 1, 1, 2, PAIRED, 128, 2, 4>{});
+  } else {
+    go(Tile<2, 1, 1, 2, PAIRED, 128, 2, 1>{});
+  }
 }
 
+typedef __attribute__((address_space(3))) void* lds_ptr;
+
+constexpr int kReadsDone = 0xc07f;  // s_waitcnt lgkmcnt(0)
+
+// All but the wave's last COUNT loads into LDS have landed, then all waves'.
+template <int COUNT>
+__device__ __forceinline__ void stage_barrier() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COUNT) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// Everyone is done with the stage buffers.
+__device__ __forceinline__ void tile_done() {
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// The stage buffers of a kernel: arrays of their own, so that the compiler sees that a load
+// into one and a read of another do not meet.
+#define VK_STAGES(T)                                                     \
+  __shared__ __align__(16) char s0_[T::kBytes];                          \
+  __shared__ __align__(16) char s1_[T::kBytes];                          \
+  __shared__ __align__(16) char s2_[T::R > 2 ? T::kBytes : 16];          \
+  __shared__ __align__(16) char s3_[T::R > 3 ? T::kBytes : 16];          \
+  __shared__ __align__(16) char s4_[T::R > 4 ? T::kBytes : 16];          \
+  char* const stages_[5] = {s0_, s1_, s2_, s3_, s4_}
+
+// Where a wave stands: in group `group` of those that share k, wave `wave`, with the rows
+// and columns of (wm, wn).
+template <typename T>
+struct Place {
+  int lane, group, wave, wm, wn;
+  __device__ __forceinline__ Place() {
+    const int tid = threadIdx.x;
+    __builtin_assume(tid < T::kThreads);
+    lane = tid & 63;
+    const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    group = w / T::kWaves;
+    wave = w % T::kWaves;
+    wm = wave / T::WN;
+    wn = wave % T::WN;
+  }
+};
+
 // acc[mt][nt] of this wave: the tile's rows from m0, columns from n0 (of the
-// hidden ones, where PAIRED), over all of k.
+// hidden ones, where PAIRED), over all of k; with KG > 1 group 0 has them, the others are done.
 template <Kind KIND, typename T>
 __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int k_bytes,
-                                             int m0, int n0, char* s0, char* s1,
+                                             int m0, int n0, const Place<T>& at,
+                                             char* const (&stages_)[5],
                                              typename Ops<KIND>::Acc16 (&acc)[T::MT][T::NT]) {
-  const int tid = threadIdx.x;
-  __builtin_assume(tid < T::kThreads);
-  const int lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / T::WN, wn = wave % T::WN;
+  constexpr int S = T::S, R = T::R, KG = T::KG, KS = S / 32;
+  const int lane = at.lane, wave = at.wave, wm = at.wm, wn = at.wn;
+  char* buf[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) buf[i] = stages_[i] + at.group * T::kGroupBytes;
 
-  // Loads: eight rows of 128 bytes an instruction, lane l row l / 8, piece
-  // (l % 8) ^ (l / 8).
-  const int lr = lane >> 3;
-  const uint32_t piece = static_cast<uint32_t>((lane & 7) ^ lr) * 16u;
+  // Loads: 1 KiB of rows an instruction, a lane 16 bytes.  With 128-byte rows bit 3 of a
+  // row is the lowest of the wave (rows from 8 (wave + i kWaves)).
+  static_assert(T::kWaves % 2 == 0, "the permutation of a lane's rows is one");
+  const int lr = S == 128 ? lane >> 3 : lane >> 2;
+  const uint32_t piece =
+      16u * static_cast<uint32_t>(S == 128 ? (lane & 7) ^ (4 * (wave & 1) + (lr >> 1))
+                                           : (lane & 3) ^ (lr >> 2));
   const size_t a_at = static_cast<size_t>(m0) * a.pitch, b_at = static_cast<size_t>(n0) * b.pitch;
   const size_t a_left = static_cast<size_t>(a.rows) * a.pitch - a_at;
   const size_t b_left = static_cast<size_t>(b.rows) * b.pitch - b_at;
@@ -133,91 +204,237 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
   uint32_t av[T::kALoads], bv[T::kBLoads];
 #pragma unroll
   for (int i = 0; i < T::kALoads; ++i) {
-    const int r = (wave + i * T::kWaves) * 8 + lr;
+    const int r = (wave + i * T::kWaves) * T::kRows + lr;
     av[i] = m0 + r < a.rows ? static_cast<uint32_t>(r) * a.pitch + piece : kOutside;
   }
 #pragma unroll
   for (int i = 0; i < T::kBLoads; ++i) {
-    const int r = (wave + i * T::kWaves) * 8 + lr;
+    const int r = (wave + i * T::kWaves) * T::kRows + lr;
     if constexpr (T::PAIRED) {
       const int hidden = b.rows / 2, j = r % T::kHeld;
-      const uint32_t at = static_cast<uint32_t>(r < T::kHeld ? j : hidden + j);
-      bv[i] = n0 + j < hidden ? at * b.pitch + piece : kOutside;
+      const uint32_t row = static_cast<uint32_t>(r < T::kHeld ? j : hidden + j);
+      bv[i] = n0 + j < hidden ? row * b.pitch + piece : kOutside;
     } else {
       bv[i] = n0 + r < b.rows ? static_cast<uint32_t>(r) * b.pitch + piece : kOutside;
     }
   }
-  const int stages = (k_bytes + kStage - 1) / kStage;
-  const bool whole = (stages - 1) * kStage + static_cast<int>(piece) < k_bytes;
-  auto issue = [&](char* to, int t) {
-    const bool in = t < stages - 1 || whole;
-    const int k = t * kStage;
-#pragma unroll
-    for (int i = 0; i < T::kALoads; ++i)
+  const int stages = (k_bytes + S * KG - 1) / (S * KG);  // of a group
+  const int last = k_bytes - static_cast<int>(piece);  // the lane's bytes of stage t: t S < last
+  // Load i of stage t (past the last stage they read zeros: their number stays the same).
+  constexpr int kLoads = T::kALoads + T::kBLoads;
+  auto load = [&](char* to, int t, int i) {
+    const int k = (t * KG + at.group) * S;
+    const bool in = k < last;
+    if (i < T::kALoads)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
           ra, (lds_ptr)(to + (wave + i * T::kWaves) * 1024), 16,
           static_cast<int>(in ? av[i] : kOutside), k, 0, 0);
-#pragma unroll
-    for (int i = 0; i < T::kBLoads; ++i)
+    else
       __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rb, (lds_ptr)(to + T::TM * kStage + (wave + i * T::kWaves) * 1024), 16,
-          static_cast<int>(in ? bv[i] : kOutside), k, 0, 0);
-    __builtin_amdgcn_sched_barrier(0);  // not behind the stage that is multiplied meanwhile
+          rb, (lds_ptr)(to + T::TM * S + (wave + (i - T::kALoads) * T::kWaves) * 1024), 16,
+          static_cast<int>(in ? bv[i - T::kALoads] : kOutside), k, 0, 0);
   };
 
   // Fragment reads: step ks of a stage is pieces 2 ks + lane / 32.
   const int fr = lane & 31;
-  const int at0 = fr * kStage + (((lane >> 5) ^ (fr & 7)) << 4);
-  const int a0 = at0 + wm * T::MT * 32 * kStage;
-  auto compute = [&](const char* from) {
-    i32x4 fa[2][T::MT], fb[2][T::NT];
-    auto read = [&](int ks) {
+  const int at0 = fr * S + (((lane >> 5) ^ (S == 128 ? (fr >> 1) & 7 : (fr >> 2) & 3)) << 4);
+  const int a0 = at0 + wm * T::MT * 32 * S;
+  i32x4 fa[2][T::MT], fb[2][T::NT];
+  constexpr int kReads = T::MT + T::NT;
+  auto read = [&](const char* from, int ks, int i) {
+    if (i < T::NT)
+      fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(from + T::TM * S + (at0 ^ (ks << 5)) +
+                                                      T::b_row(wn, i) * S);
+    else
+      fa[ks & 1][i - T::NT] =
+          *reinterpret_cast<const i32x4*>(from + (a0 ^ (ks << 5)) + (i - T::NT) * 32 * S);
+  };
+  // The products of a step, and between them the reads of the step after it (`next`, step
+  // nks) and the loads of stage t into `to`: one at a time, so that neither LDS nor the
+  // load path holds the matrix pipe up.
+  auto step = [&](auto reads, auto loads, int ks, const char* next, int nks, char* to, int t) {
+    constexpr int kTiles = T::MT * T::NT;
+    constexpr int kReadsEach = (kReads + kTiles - 1) / kTiles, kLoadsEach = (kLoads + kTiles - 1) / kTiles;
 #pragma unroll
-      for (int i = 0; i < T::NT; ++i)
-        fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(
-            from + T::TM * kStage + (at0 ^ (ks << 5)) + T::b_row(wn, i) * kStage);
+    for (int e = 0; e < kTiles; ++e) {
+      const int i = e / T::NT, j = e % T::NT;
+      acc[i][j] = Ops<KIND>::mma32(fb[ks & 1][j], fa[ks & 1][i], acc[i][j]);
+      __builtin_amdgcn_sched_barrier(0);
+      if constexpr (reads.value)
 #pragma unroll
-      for (int i = 0; i < T::MT; ++i)
-        fa[ks & 1][i] =
-            *reinterpret_cast<const i32x4*>(from + (a0 ^ (ks << 5)) + i * 32 * kStage);
-    };
-    read(0);
+        for (int r = e * kReadsEach; r < (e + 1) * kReadsEach && r < kReads; ++r) read(next, nks, r);
+      if constexpr (loads.value)
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      if (ks < 3) read(ks + 1);
-      __builtin_amdgcn_sched_barrier(0);  // the next step's reads before this one's products
-#pragma unroll
-      for (int i = 0; i < T::MT; ++i)
-#pragma unroll
-        for (int j = 0; j < T::NT; ++j)
-          acc[i][j] = Ops<KIND>::mma32(fa[ks & 1][i], fb[ks & 1][j], acc[i][j]);
+        for (int l = e * kLoadsEach; l < (e + 1) * kLoadsEach && l < kLoads; ++l) load(to, t, l);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-
+  constexpr int kFlying = (R - 2) * kLoads;
+  constexpr std::true_type kYes{};
+  constexpr std::false_type kNo{};
+  // Stage t from `cur`: its last step's products run behind the barrier.
+  auto stage = [&](char* cur, const char* next, int t) {
+#pragma unroll
+    for (int ks = 0; ks + 1 < KS; ++ks) step(kYes, kNo, ks, cur, ks + 1, nullptr, 0);
+    __builtin_amdgcn_s_waitcnt(kReadsDone);
+    stage_barrier<kFlying>();  // the next stage has landed, and nobody reads this one any more
+    step(kYes, kYes, KS - 1, next, 0, cur, t + R);
+  };
 #pragma unroll
   for (int i = 0; i < T::MT; ++i)
 #pragma unroll
     for (int j = 0; j < T::NT; ++j) acc[i][j] = typename Ops<KIND>::Acc16{};
-  issue(s0, 0);
-  int t = 0;
-  for (; t + 1 < stages; t += 2) {
-    stage_barrier();  // stage t has landed; everyone is done with the other buffer
-    issue(s1, t + 1);
-    compute(s0);
-    stage_barrier();
-    if (t + 2 < stages) issue(s0, t + 2);
-    compute(s1);
-  }
-  if (t < stages) {
-    stage_barrier();
-    compute(s0);
+#pragma unroll
+  for (int i = 0; i < R; ++i)
+#pragma unroll
+    for (int l = 0; l < kLoads; ++l) load(buf[i], i, l);
+  stage_barrier<kFlying + kLoads>();
+#pragma unroll
+  for (int i = 0; i < kReads; ++i) read(buf[0], 0, i);
+  // To a multiple of R: stages past the last one are zeros, and a loop that does not branch
+  // keeps the sums in one place.
+  for (int t = 0; t < stages; t += R)
+#pragma unroll
+    for (int i = 0; i < R; ++i) stage(buf[i], buf[(i + 1) % R], t + i);
+  tile_done();
+  if constexpr (KG > 1) {
+    typedef typename Ops<KIND>::Acc4 Acc4;
+    constexpr int kTiles = T::MT * T::NT, kWaveSums = kTiles * 4 * 64;
+    Acc4* sums = reinterpret_cast<Acc4*>(stages_[1]) + wave * kWaveSums + lane;
+#pragma unroll
+    for (int e = 0; e < kTiles * 4; ++e) {
+      const auto& v = acc[e / 4 / T::NT][e / 4 % T::NT];
+      const int r = e % 4 * 4;
+      if (at.group > 0)
+        sums[(at.group - 1) * T::kWaves * kWaveSums + e * 64] = Acc4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+    }
+    tile_done();
+    if (at.group > 0) return;
+#pragma unroll
+    for (int e = 0; e < kTiles * 4; ++e) {
+      auto& v = acc[e / 4 / T::NT][e / 4 % T::NT];
+#pragma unroll
+      for (int o = 0; o < KG - 1; ++o) {
+        const Acc4 w = sums[o * T::kWaves * kWaveSums + e * 64];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[e % 4 * 4 + i] += w[i];
+      }
+    }
   }
 }
 
-// Row of acc register r of a 32 x 32 tile (its column is lane % 32).
-__device__ __forceinline__ int acc_row(int lane, int r) {
-  return 8 * (r >> 2) + 4 * (lane >> 5) + (r & 3);
+// A wave's sums lie with a row of a in each lane (lane % 32) and 16 columns in its registers:
+// register 4 q + e is column 8 q + 4 (lane / 32) + e of its 32.  Results leave through LDS, 32
+// rows at a time, so that a row's columns go to memory as whole lines: a Chunk is a wave's own
+// 32 rows of 32 J columns, in the stage buffers that the products are done with, its 16-byte
+// pieces permuted as the stages' are.
+template <typename V, int J>
+struct Chunk {
+  typedef V V4 __attribute__((ext_vector_type(4)));
+  static constexpr int kRowBytes = 32 * J * static_cast<int>(sizeof(V));
+  static constexpr int kPieces = kRowBytes / 16, kPer = 16 / static_cast<int>(sizeof(V));
+  static constexpr int kBytes = 32 * kRowBytes;
+  static_assert(kRowBytes == 128 || kRowBytes == 64, "rows of a line or half of one");
+  static __device__ __forceinline__ int slot(int row, int piece) {
+    return row * kRowBytes + ((piece ^ (kPieces == 8 ? (row >> 1) & 7 : (row >> 2) & 3)) << 4);
+  }
+  // The four columns 32 j + 8 q + 4 (lane / 32) .. of the lane's row.
+  static __device__ __forceinline__ V4* at(char* c, int lane, int j, int q) {
+    const int byte = (32 * j + 8 * q + 4 * (lane >> 5)) * static_cast<int>(sizeof(V));
+    return reinterpret_cast<V4*>(c + slot(lane & 31, byte >> 4) + (byte & 15));
+  }
+  static __device__ __forceinline__ V* element(char* c, int row, int col) {
+    const int byte = col * static_cast<int>(sizeof(V));
+    return reinterpret_cast<V*>(c + slot(row, byte >> 4) + (byte & 15));
+  }
+  // From rows m0 .., columns n0 .. of a matrix (zeros outside), through registers, so that the
+  // loads of the next rows can be under way: fetch, then fill.  As store.
+  static constexpr int kFetch = kBytes / 1024;
+  static __device__ __forceinline__ void fetch(i32x4 (&v)[kFetch], int lane, const V* from,
+                                               size_t pitch, int m0, int M, int n0, int N, bool vec) {
+#pragma unroll
+    for (int p = 0; p < kFetch; ++p) {
+      v[p] = i32x4{};
+      const int m = m0 + p * (64 / kPieces) + lane / kPieces, n = n0 + lane % kPieces * kPer;
+      if (m >= M || n >= N) continue;
+      const V* at = from + static_cast<size_t>(m) * pitch + n;
+      if (vec) {
+        v[p] = *reinterpret_cast<const i32x4*>(at);
+      } else {
+        V e[kPer];
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) e[i] = n + i < N ? at[i] : static_cast<V>(0.0f);
+        __builtin_memcpy(&v[p], e, 16);
+      }
+    }
+  }
+  static __device__ __forceinline__ void fill(char* c, int lane, const i32x4 (&v)[kFetch]) {
+#pragma unroll
+    for (int p = 0; p < kFetch; ++p)
+      *reinterpret_cast<i32x4*>(c + slot(p * (64 / kPieces) + lane / kPieces, lane % kPieces)) = v[p];
+  }
+  // To rows m0 .. of `out` (pitch values a row), columns n0 .., of those below M and N.  vec:
+  // every row starts on 16 bytes and N is whole pieces.  ADD: added to what is there.
+  template <bool ADD>
+  static __device__ __forceinline__ void store(char* c, int lane, V* out, size_t pitch, int m0,
+                                               int M, int n0, int N, bool vec) {
+    if (vec) {
+#pragma unroll
+      for (int p = 0; p < kBytes / 1024; ++p) {
+        const int row = p * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+        const int m = m0 + row, n = n0 + piece * kPer;
+        i32x4 v = *reinterpret_cast<const i32x4*>(c + slot(row, piece));
+        if (m >= M || n >= N) continue;
+        i32x4* to = reinterpret_cast<i32x4*>(out + static_cast<size_t>(m) * pitch + n);
+        if constexpr (ADD)
+          v = __builtin_bit_cast(i32x4, __builtin_bit_cast(f32x4, *to) + __builtin_bit_cast(f32x4, v));
+        *to = v;
+      }
+    } else {
+      constexpr int kCols = 32 * J;
+#pragma unroll 4
+      for (int p = 0; p < 32 * kCols / 64; ++p) {
+        const int row = p * (64 / kCols) + lane / kCols, col = lane % kCols;
+        const int m = m0 + row, n = n0 + col;
+        const V v = *element(c, row, col);
+        if (m >= M || n >= N) continue;
+        V* to = out + static_cast<size_t>(m) * pitch + n;
+        if constexpr (ADD)
+          *to = *to + v;
+        else
+          *to = v;
+      }
+    }
+  }
+};
+
+// Sums over lanes 0 .. 31 and over lanes 32 .. 63 of N = 32 R values a lane: lane l is left with the
+// sums of values R (l % 32) .. + R.  A step adds half of the values of two lanes that
+// differ in one more bit (lanes l and l ^ 16, 15, 7, 3, 1), in a fixed order.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+template <int N, int CTRL>
+__device__ __forceinline__ void halve(float* v, bool upper) {
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float keep = upper ? v[k + N] : v[k], send = upper ? v[k] : v[k + N];
+    v[k] = keep + dpp<CTRL>(send);
+  }
+}
+template <int R>
+__device__ __forceinline__ void sum_rows(float* v, int lane) {
+#pragma unroll
+  for (int k = 0; k < 16 * R; ++k) {  // lanes l and l ^ 16
+    const bool upper = lane & 16;
+    const float keep = upper ? v[k + 16 * R] : v[k], send = upper ? v[k] : v[k + 16 * R];
+    v[k] = keep + __shfl_xor(send, 16, 64);
+  }
+  halve<8 * R, 0x140>(v, lane & 8);  // row_mirror
+  halve<4 * R, 0x141>(v, lane & 4);  // row_half_mirror
+  halve<2 * R, 0x1b>(v, lane & 2);   // quad_perm 3, 2, 1, 0
+  halve<R, 0xb1>(v, lane & 1);       // quad_perm 1, 0, 3, 2
 }
 
 // The tile of workgroup t, XCD-major in groups of rows that a 4 MiB L2 holds together
@@ -232,15 +449,16 @@ __device__ __forceinline__ void tile_at(int gm, int gn, int group, int* mt, int*
 }
 
 // ---------------------------------------------------------------- activations
-// act(g): SiLU g / (1 + e^-g), GELU g Phi(g) with the device erff.  The exponential is
-// v_exp_f32 of g log2(e) and the quotient v_rcp_f32: some 2 ulp each, against
-// results that are then multiplied and, but for f32 outputs, rounded to 16 bits.
+// act(g): SiLU g / (1 + e^-g), GELU g Phi(g) by the GELU stream's erf (error below 1.5e-7: half
+// the instructions of erff, which a tile's end would wait for).  The exponential is v_exp_f32 of
+// g log2(e) and the quotient v_rcp_f32: some 2 ulp each, against results that are then
+// multiplied and, but for f32 outputs, rounded to 16 bits.
 template <int ACT>
 __device__ __forceinline__ float gate(float g) {
   if constexpr (ACT == VK_GATE_SILU)
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
   else
-    return vkd::gelu1<1>(g);
+    return vkd::gelu1<0>(g);
 }
 
 // act(g) and its derivative: SiLU's is s (1 + g (1 - s)), s = 1 / (1 + e^-g); GELU's
@@ -252,7 +470,7 @@ __device__ __forceinline__ void gate_slope(float g, float* act, float* slope) {
     *act = g * s;
     *slope = s * __builtin_fmaf(g, 1.0f - s, 1.0f);
   } else {
-    const float phi = 0.5f + 0.5f * erff(g * 0.70710678f);
+    const float phi = 0.5f + 0.5f * vkd::erf_as7126(g * 0.70710678f);
     *act = g * phi;
     *slope = __builtin_fmaf(g * 0.39894228f, __builtin_amdgcn_exp2f(g * g * -0.72134752f), phi);
   }

@@ -693,8 +693,8 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
  * be NULL (not computed), and overlaps no other tensor.  The gradients of g and u
  * are f32 up to one rounding to x's type, as operands of the products; dbias sums
  * them before that rounding.  The same call gives the same bits.  Intermediate
- * values (some 4 (rows + in_features) hidden values) go to the runtime's work
- * buffer: run it once before a capture.  At most 2,097,152 rows. */
+ * values (2 rows x hidden and some) go to the runtime's work buffer: run it once
+ * before a capture. */
 int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
                       const vk_tensor* bias, const vk_tensor* grad,
                       size_t rows, size_t in_features, size_t hidden,

@@ -10,10 +10,9 @@
 // Backward, from x, w, b and the gradient dh, with nothing kept from the forward:
 //   1. g and u again, and in the same kernel dg = dh u act'(g), du = dh act(g), in
 //      f32 up to one rounding to x's type: the two products below take 16-bit
-//      operands.  Written as [rows, 2 H] and as its transpose, with the f32 column
-//      sums of each tile;
-//   2. dx = [dg du] [Wg; Wu]   (against w transposed);
-//   3. dw = [dg du]^T x        (transposes of both);
+//      operands.  Written as rows dg | du, with the f32 column sums of each tile;
+//   2. dx = [dg du] [Wg; Wu], w's lines being k;
+//   3. dw = [dg du]^T x, the lines of both being k;
 //   4. db: the tiles' column sums added in order.
 #include "product_nt.h"
 
@@ -32,7 +31,7 @@ struct Args {
   void* out;         // [M, N]; null in the backward
   void* d;           // dg | du, rows of 2 d_half values, zeros from N to d_half of each half
   float* sums;       // [gm * WM, 2 N], or null
-  int d_half;
+  int d_half, m_half;
   int M, N;
   int act;
   bool vec;          // rows of N values are whole 16-byte pieces
@@ -195,8 +194,10 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   }
 }
 
-// out[m, n] = sum_k a[m, k] b[n, k], rounded to the type.
-template <Kind KIND, typename T>
+// out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a as rows or columns, b as columns.  With
+// m_half > 0 a's rows come in two halves: row m < m_half is out's m where that is below M / 2, row m
+// >= m_half out's M / 2 + m - m_half where that is below M.
+template <Kind KIND, typename T, bool AC>
 __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Args g) {
   typedef typename vkp::Value<KIND>::type V;
   VK_STAGES(T);
@@ -205,7 +206,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Ar
   const int m0 = mt * T::TM, n0 = nt * T::TN;
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
+  vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
   if (place.group > 0) return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   typedef vkp::Chunk<V, T::NT> C;
@@ -222,8 +223,16 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Ar
         *C::at(chunk, lane, j, q) = w;
       }
     vkd::wave_lds_fence();
-    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
-                             n0 + T::b_row(wn, 0), g.N, g.vec);
+    int mb = m0 + (wm * T::MT + i) * 32, end = g.M;
+    if (g.m_half > 0) {  // 32 rows lie in one half: m_half is a multiple of 64
+      end = g.M / 2;
+      if (mb >= g.m_half) {
+        mb += end - g.m_half;
+        end = g.M;
+      }
+    }
+    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end, n0 + T::b_row(wn, 0),
+                             g.N, g.vec);
     vkd::wave_lds_fence();
   }
 }
@@ -245,32 +254,6 @@ __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
 }
 
 // ---------------------------------------------------------------- layouts
-// to[c, r] = from[r, c] of 16-bit values, zeros from row `rows` to the next multiple of 64.
-__global__ __launch_bounds__(256) void transpose16_kernel(const uint16_t* __restrict__ from,
-                                                          size_t from_pitch, int rows, int cols,
-                                                          uint16_t* __restrict__ to, size_t pitch) {
-  __shared__ uint16_t tile[64][66];
-  const int c0 = blockIdx.x * 64, r0 = blockIdx.y * 64;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int r = r0 + ty + 8 * i, c = c0 + tx + 32 * h;
-      tile[ty + 8 * i][tx + 32 * h] =
-          r < rows && c < cols ? from[r * from_pitch + c] : uint16_t{0};
-    }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int c = c0 + ty + 8 * i, r = r0 + 2 * tx;
-    if (c < cols) {
-      const uint32_t lo = tile[2 * tx][ty + 8 * i], hi = tile[2 * tx + 1][ty + 8 * i];
-      *reinterpret_cast<uint32_t*>(to + static_cast<size_t>(c) * pitch + r) = lo | hi << 16;
-    }
-  }
-}
-
 // Rows of `cols` 16-bit values into rows of `pitch` (a multiple of 8), zeros behind.
 __global__ __launch_bounds__(256) void pad16_kernel(const uint16_t* __restrict__ from, int cols,
                                                     uint16_t* __restrict__ to, int pitch) {
@@ -344,30 +327,27 @@ int launch_forward(vk_runtime* rt, Args& g) {
   return vk::check_launch("gated_kernel");
 }
 
-template <Kind KIND>
-int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k, void* out) {
+// out [M, N] from a.rows rows of a (in halves, where m_half > 0) and b's columns.
+template <Kind KIND, bool AC>
+int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k, size_t M, size_t N,
+                   size_t m_half, void* out) {
   Args g{};
   g.a = a;
   g.b = b;
   g.k_bytes = static_cast<int>(2 * k);
   g.out = out;
-  g.M = a.rows;
-  g.N = b.rows;
-  g.vec = g.N % 8 == 0;
-  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, g.N, g.k_bytes);
+  g.M = static_cast<int>(M);
+  g.N = static_cast<int>(N);
+  g.m_half = static_cast<int>(m_half);
+  g.vec = N % 8 == 0;
+  const vkp::Plan p = vkp::plan(rt->cu_count, a.rows, g.N, g.k_bytes);
   with_tile<false>(p.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
-    hipLaunchKernelGGL((product_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream,
-                       g);
+    g.gm = (a.rows + T::TM - 1) / T::TM;
+    hipLaunchKernelGGL((product_kernel<KIND, T, AC>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
+                       rt->stream, g);
   });
   return vk::check_launch("product_kernel");
-}
-
-void transpose(const vk_runtime* rt, const void* from, size_t from_pitch, size_t rows, size_t cols,
-               void* to, size_t pitch) {
-  hipLaunchKernelGGL(transpose16_kernel, dim3((cols + 63) / 64, (rows + 63) / 64), dim3(256), 0,
-                     rt->stream, static_cast<const uint16_t*>(from), from_pitch, static_cast<int>(rows),
-                     static_cast<int>(cols), static_cast<uint16_t*>(to), pitch);
 }
 
 // A tensor's rows as an operand: as they are, or where a row is no multiple of 16
@@ -384,9 +364,8 @@ Operand as_operand(const vk_runtime* rt, const void* p, size_t rows, size_t cols
 }
 
 template <Kind KIND>
-int backward(vk_runtime* rt, Args& g, const void* x, const void* w, size_t rows, size_t in,
-             size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
-  const size_t half = padded(hidden), rp = padded(rows);
+int backward(vk_runtime* rt, Args& g, size_t rows, size_t in, size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
+  const size_t half = padded(hidden);
   const auto take = [&](size_t bytes) {
     char* at = room;
     room += (bytes + 255) / 256 * 256;
@@ -407,23 +386,22 @@ int backward(vk_runtime* rt, Args& g, const void* x, const void* w, size_t rows,
                        rt->stream, g);
   });
   VK_TRY(vk::check_launch("gated_grad_kernel"));
-  const int R = static_cast<int>(rows), D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden);
+  const char* d = static_cast<char*>(g.d);
+  const auto pitch = static_cast<uint32_t>(4 * half);
+  const int R = static_cast<int>(rows), values = static_cast<int>((in + 7) / 8 * 8);
   if (dx) {
-    const uint32_t pitch = static_cast<uint32_t>(4 * half);
-    char* wt = take(in * 2 * half * 2);
-    transpose(rt, w, in, hidden, in, wt, 2 * half);
-    transpose(rt, static_cast<const char*>(w) + hidden * in * 2, in, hidden, in, wt + half * 2, 2 * half);
-    VK_TRY(launch_product<KIND>(rt, Operand{static_cast<char*>(g.d), R, pitch}, Operand{wt, D, pitch},
-                                2 * half, dx->ptr));
+    Operand lines = g.b;  // w's lines are k
+    lines.rows = values;
+    lines.ks = static_cast<int>(2 * hidden);
+    lines.k_half = static_cast<int>(half);
+    VK_TRY((launch_product<KIND, false>(rt, Operand{d, R, pitch}, lines, 2 * half, rows, in, 0, dx->ptr)));
   }
   if (dw) {
-    char* dt = take(2 * hidden * rp * 2);
-    char* xt = take(in * rp * 2);
-    transpose(rt, g.d, 2 * half, rows, hidden, dt, rp);
-    transpose(rt, static_cast<char*>(g.d) + half * 2, 2 * half, rows, hidden, dt + hidden * rp * 2, rp);
-    transpose(rt, x, in, rows, in, xt, rp);
-    VK_TRY(launch_product<KIND>(rt, Operand{dt, H2, static_cast<uint32_t>(2 * rp)},
-                                Operand{xt, D, static_cast<uint32_t>(2 * rp)}, rows, dw->ptr));
+    Operand lines = g.a;
+    lines.rows = values;
+    lines.ks = R;
+    VK_TRY((launch_product<KIND, true>(rt, Operand{d, static_cast<int>(2 * half), pitch, R}, lines, rows,
+                                       2 * hidden, in, half, dw->ptr)));
   }
   if (dbias) {
     hipLaunchKernelGGL(bias_grad_kernel<KIND>, dim3((2 * hidden + 15) / 16), dim3(256), 0, rt->stream,
@@ -512,17 +490,13 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
       VK_REQUIRE(!vk::overlap(outs[i], t), "gated: a gradient overlaps an input");
     for (int j = 0; j < i; ++j) VK_REQUIRE(!vk::overlap(outs[i], outs[j]), "gated: gradients overlap");
   }
-  VK_UNSUPPORTED_IF(rows > 0x200000, "gated: the gradients of %zu rows", rows);
   if (rows == 0) {  // sums of nothing
     if (dw) zero16(rt, dw->ptr, dw->len);
     if (dbias) zero16(rt, dbias->ptr, dbias->len);
     return vk::check_launch("zero16_kernel");
   }
-  const size_t half = padded(hidden), rp = padded(rows);
-  size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features) + 8 * 256;
-  if (dx || dw) need += rows * 4 * half;
-  if (dx) need += in_features * 4 * half;
-  if (dw) need += (2 * hidden + in_features) * rp * 2;
+  size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features) + 2 * 256;
+  if (dx || dw) need += rows * padded(hidden) * 4;
   if (dbias) need += ((rows + 63) / 64 * 2) * 2 * hidden * 4;
   VK_TRY(vk::ensure_work(rt, (need + 3) / 4, "gated_backward"));
   char* room = reinterpret_cast<char*>(rt->work);
@@ -530,8 +504,8 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
   VK_TRY(vk::check_launch("pad16_kernel"));
   g.grad = grad->ptr;
   return x->dtype == VK_F16
-             ? backward<kF16>(rt, g, x->ptr, w->ptr, rows, in_features, hidden, room, dx, dw, dbias)
-             : backward<kBF16>(rt, g, x->ptr, w->ptr, rows, in_features, hidden, room, dx, dw, dbias);
+             ? backward<kF16>(rt, g, rows, in_features, hidden, room, dx, dw, dbias)
+             : backward<kBF16>(rt, g, rows, in_features, hidden, room, dx, dw, dbias);
 }
 
 }  // extern "C"

@@ -1,6 +1,7 @@
-// Products out[m, n] = sum_k a[m, k] b[n, k] of two operands whose rows are
-// contiguous in k, on the gfx950 matrix cores: int8 with int32 sums, f16 and
-// bf16 with f32 sums.
+// Products out[m, n] = sum_k a[m, k] b[n, k] on the gfx950 matrix cores: int8 with
+// int32 sums, f16 and bf16 with f32 sums.  An operand's rows are contiguous in k, or (16-bit
+// types) its columns are: then a stage lies in LDS as it lies in memory, and fragments are read
+// with the transposing LDS reads.
 //
 // All three types share one kernel, because they share one layout in bytes: an
 // operand of v_mfma_*_32x32x{32 int8, 16 f16/bf16} is 16 bytes a lane, lane l
@@ -66,13 +67,18 @@ struct Ops<kI8> {
   }
 };
 
-// Rows of an operand: row r is `bytes` bytes at base + r * pitch; pitch and base are
-// multiples of 16, what is read past `bytes` counts as zeros (in pieces of 16:
-// between `bytes` and the next multiple of 16 the row holds zeros).
+// An operand in memory; base and pitch are multiples of 16 bytes.
+//   Rows (k contiguous): row r at base + r * pitch, k_bytes of k; what lies between k_bytes and
+//     the next multiple of 16 is zeros.
+//   Columns (16-bit types): k's values at base + k * pitch, `rows` of them, a multiple of
+//     8; `ks` of k.  With k_half > 0 (a multiple of 64) k comes in two halves: k < k_half is line k where
+//     that is below ks / 2, k >= k_half line ks / 2 + k - k_half where that is below ks; zeros
+//     otherwise.
 struct Operand {
   const char* base;
   int rows;
   uint32_t pitch;
+  int ks = 0, k_half = 0;
 };
 
 constexpr int kStage = 128;            // bytes of k of a stage
@@ -159,6 +165,92 @@ __device__ __forceinline__ void tile_done() {
   __shared__ __align__(16) char s4_[T::R > 4 ? T::kBytes : 16];          \
   char* const stages_[5] = {s0_, s1_, s2_, s3_, s4_}
 
+// A buffer resource's parts.
+struct Source {
+  const char* base;
+  uint32_t bytes;
+};
+
+// Rows r0 .. of an operand.
+__device__ __forceinline__ Source rows_of(const Operand& o, int r0) {
+  const size_t from = static_cast<size_t>(r0) * o.pitch;
+  const size_t left = static_cast<size_t>(o.rows) * o.pitch - from;
+  return Source{o.base + from, left < kMostBytes ? static_cast<uint32_t>(left) : kMostBytes};
+}
+
+// 16 bytes a lane from source + lane offset (zeros past its bytes) + k into LDS.  BY_HAND: the
+// instruction itself, which the compiler does not count: it would wait for every load under way before
+// a transposing read, whose buffer it does not see.  No register is written, and what has to be
+// waited for is waited for by stage_barrier and tile_done.  (The s_nop covers scalar operands that a
+// vector instruction may just have written.)
+template <bool BY_HAND>
+__device__ __forceinline__ void load_lds(const Source& s, char* to, uint32_t lane_off, int k) {
+  if constexpr (BY_HAND) {
+    const uint64_t base = reinterpret_cast<uint64_t>(s.base);
+    const i32x4 r = {static_cast<int>(base), static_cast<int>((base >> 32) & 0xffff),
+                     static_cast<int>(s.bytes), 0x00020000};
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
+                 :
+                 : "s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(to)))), "v"(lane_off),
+                   "s"(r), "s"(k)
+                 : "memory", "m0");
+  } else {
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(vkd::buffer_rsrc(s.base, s.bytes), (lds_ptr)(to), 16,
+                                             static_cast<int>(lane_off), k, 0, 0);
+  }
+}
+
+// Columns: a stage is 64 lines of W values.  In LDS a line's 16-byte pieces are permuted by
+// piece ^ 4 (k % 4) (two 64-value lines to the 64 banks: by 4 (k / 2 % 2)): the 32 lanes of a
+// transposing read take 64 bytes each of four neighbouring lines, all banks once.
+template <int W>
+__device__ __forceinline__ constexpr int column_turn(int k) {
+  return W == 64 ? ((k >> 1) & 1) * 4 : (k & 3) * 4;
+}
+
+// The lines of stage st, up to the last.
+__device__ __forceinline__ Source columns_of(const Operand& o, int st) {
+  int line = st * 64, end = o.ks;
+  if (o.k_half > 0) {
+    end = o.ks / 2;
+    if (line >= o.k_half) {
+      line += end - o.k_half;
+      end = o.ks;
+    }
+  }
+  const int lines = line < end ? (end - line < 64 ? end - line : 64) : 0;
+  return Source{o.base + static_cast<size_t>(line) * o.pitch, static_cast<uint32_t>(lines) * o.pitch};
+}
+
+// A lane's offsets in a stage's lines, of values c0 ...
+template <int W, int WAVES, int N>
+__device__ __forceinline__ void columns_at(const Operand& o, int c0, int lane, int wave,
+                                           uint32_t (&v)[N]) {
+  constexpr int kPieces = W / 8, kLines = 64 / kPieces;  // of a line; lines a load
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int line = (wave + i * WAVES) * kLines + lane / kPieces;
+    const int piece = (lane % kPieces) ^ column_turn<W>(line);
+    const int c = c0 + piece * 8;
+    v[i] = c < o.rows ? static_cast<uint32_t>(line) * o.pitch + 2u * static_cast<uint32_t>(c) : kOutside;
+  }
+}
+
+// The fragment of step ks, rows r0 .. of the tile: sixteen lanes read four lines of sixteen
+// values and get a value's four k each; two reads make eight.
+template <int W>
+__device__ __forceinline__ i32x4 read_columns(const char* from, int lane, int ks, int r0) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) s16x4* lds_s4;
+  const int line = 16 * ks + 8 * (lane >> 5) + ((lane >> 2) & 3);  // and 4 more: the same turn
+  const int piece = (r0 >> 3) + 2 * ((lane >> 4) & 1) + ((lane >> 1) & 1);
+  const char* p = from + line * 2 * W + ((piece ^ column_turn<W>(line)) << 4) + 8 * (lane & 1);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4)(p + 8 * W));
+  const int2 a = __builtin_bit_cast(int2, lo), b = __builtin_bit_cast(int2, hi);
+  return i32x4{a.x, a.y, b.x, b.y};
+}
+
 // Where a wave stands: in group `group` of those that share k, wave `wave`, with the rows
 // and columns of (wm, wn).
 template <typename T>
@@ -178,7 +270,8 @@ struct Place {
 
 // acc[mt][nt] of this wave: the tile's rows from m0, columns from n0 (of the
 // hidden ones, where PAIRED), over all of k; with KG > 1 group 0 has them, the others are done.
-template <Kind KIND, typename T>
+// AC, BC: a, b as columns.
+template <Kind KIND, typename T, bool AC = false, bool BC = false>
 __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int k_bytes,
                                              int m0, int n0, const Place<T>& at,
                                              char* const (&stages_)[5],
@@ -189,33 +282,41 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
 #pragma unroll
   for (int i = 0; i < R; ++i) buf[i] = stages_[i] + at.group * T::kGroupBytes;
 
-  // Loads: 1 KiB of rows an instruction, a lane 16 bytes.  With 128-byte rows bit 3 of a
+  // Loads of rows: 1 KiB an instruction, a lane 16 bytes.  With 128-byte rows bit 3 of a
   // row is the lowest of the wave (rows from 8 (wave + i kWaves)).
   static_assert(T::kWaves % 2 == 0, "the permutation of a lane's rows is one");
+  static_assert(S == 128 || !(AC || BC), "columns in stages of 64 k");
   const int lr = S == 128 ? lane >> 3 : lane >> 2;
   const uint32_t piece =
       16u * static_cast<uint32_t>(S == 128 ? (lane & 7) ^ (4 * (wave & 1) + (lr >> 1))
                                            : (lane & 3) ^ (lr >> 2));
-  const size_t a_at = static_cast<size_t>(m0) * a.pitch, b_at = static_cast<size_t>(n0) * b.pitch;
-  const size_t a_left = static_cast<size_t>(a.rows) * a.pitch - a_at;
-  const size_t b_left = static_cast<size_t>(b.rows) * b.pitch - b_at;
-  const auto ra = vkd::buffer_rsrc(a.base + a_at, a_left < kMostBytes ? static_cast<uint32_t>(a_left) : kMostBytes);
-  const auto rb = vkd::buffer_rsrc(b.base + b_at, b_left < kMostBytes ? static_cast<uint32_t>(b_left) : kMostBytes);
   uint32_t av[T::kALoads], bv[T::kBLoads];
+  Source sa{}, sb{};
+  if constexpr (!AC) sa = rows_of(a, m0);
+  if constexpr (!BC) sb = rows_of(b, n0);
+  if constexpr (AC) {
+    columns_at<T::TM, T::kWaves>(a, m0, lane, wave, av);
+  } else {
 #pragma unroll
-  for (int i = 0; i < T::kALoads; ++i) {
-    const int r = (wave + i * T::kWaves) * T::kRows + lr;
-    av[i] = m0 + r < a.rows ? static_cast<uint32_t>(r) * a.pitch + piece : kOutside;
+    for (int i = 0; i < T::kALoads; ++i) {
+      const int r = (wave + i * T::kWaves) * T::kRows + lr;
+      av[i] = m0 + r < a.rows ? static_cast<uint32_t>(r) * a.pitch + piece : kOutside;
+    }
   }
+  if constexpr (BC) {
+    static_assert(!T::PAIRED, "gates and partners come as rows");
+    columns_at<T::TN, T::kWaves>(b, n0, lane, wave, bv);
+  } else {
 #pragma unroll
-  for (int i = 0; i < T::kBLoads; ++i) {
-    const int r = (wave + i * T::kWaves) * T::kRows + lr;
-    if constexpr (T::PAIRED) {
-      const int hidden = b.rows / 2, j = r % T::kHeld;
-      const uint32_t row = static_cast<uint32_t>(r < T::kHeld ? j : hidden + j);
-      bv[i] = n0 + j < hidden ? row * b.pitch + piece : kOutside;
-    } else {
-      bv[i] = n0 + r < b.rows ? static_cast<uint32_t>(r) * b.pitch + piece : kOutside;
+    for (int i = 0; i < T::kBLoads; ++i) {
+      const int r = (wave + i * T::kWaves) * T::kRows + lr;
+      if constexpr (T::PAIRED) {
+        const int hidden = b.rows / 2, j = r % T::kHeld;
+        const uint32_t row = static_cast<uint32_t>(r < T::kHeld ? j : hidden + j);
+        bv[i] = n0 + j < hidden ? row * b.pitch + piece : kOutside;
+      } else {
+        bv[i] = n0 + r < b.rows ? static_cast<uint32_t>(r) * b.pitch + piece : kOutside;
+      }
     }
   }
   const int stages = (k_bytes + S * KG - 1) / (S * KG);  // of a group
@@ -223,16 +324,23 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
   // Load i of stage t (past the last stage they read zeros: their number stays the same).
   constexpr int kLoads = T::kALoads + T::kBLoads;
   auto load = [&](char* to, int t, int i) {
-    const int k = (t * KG + at.group) * S;
+    const int st = t * KG + at.group, k = st * S;
     const bool in = k < last;
-    if (i < T::kALoads)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          ra, (lds_ptr)(to + (wave + i * T::kWaves) * 1024), 16,
-          static_cast<int>(in ? av[i] : kOutside), k, 0, 0);
-    else
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rb, (lds_ptr)(to + T::TM * S + (wave + (i - T::kALoads) * T::kWaves) * 1024), 16,
-          static_cast<int>(in ? bv[i - T::kALoads] : kOutside), k, 0, 0);
+    constexpr bool kByHand = AC || BC;
+    if (i < T::kALoads) {
+      char* lds = to + (wave + i * T::kWaves) * 1024;
+      if constexpr (AC)
+        load_lds<kByHand>(columns_of(a, st), lds, av[i], 0);
+      else
+        load_lds<kByHand>(sa, lds, in ? av[i] : kOutside, k);
+    } else {
+      const int j = i - T::kALoads;
+      char* lds = to + T::TM * S + (wave + j * T::kWaves) * 1024;
+      if constexpr (BC)
+        load_lds<kByHand>(columns_of(b, st), lds, bv[j], 0);
+      else
+        load_lds<kByHand>(sb, lds, in ? bv[j] : kOutside, k);
+    }
   };
 
   // Fragment reads: step ks of a stage is pieces 2 ks + lane / 32.
@@ -242,12 +350,19 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
   i32x4 fa[2][T::MT], fb[2][T::NT];
   constexpr int kReads = T::MT + T::NT;
   auto read = [&](const char* from, int ks, int i) {
-    if (i < T::NT)
-      fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(from + T::TM * S + (at0 ^ (ks << 5)) +
-                                                      T::b_row(wn, i) * S);
-    else
-      fa[ks & 1][i - T::NT] =
-          *reinterpret_cast<const i32x4*>(from + (a0 ^ (ks << 5)) + (i - T::NT) * 32 * S);
+    if (i < T::NT) {
+      const char* fb_at = from + T::TM * S;
+      if constexpr (BC)
+        fb[ks & 1][i] = read_columns<T::TN>(fb_at, lane, ks, T::b_row(wn, i));
+      else
+        fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(fb_at + (at0 ^ (ks << 5)) + T::b_row(wn, i) * S);
+    } else {
+      const int r = i - T::NT;
+      if constexpr (AC)
+        fa[ks & 1][r] = read_columns<T::TM>(from, lane, ks, (wm * T::MT + r) * 32);
+      else
+        fa[ks & 1][r] = *reinterpret_cast<const i32x4*>(from + (a0 ^ (ks << 5)) + r * 32 * S);
+    }
   };
   // The products of a step, and between them the reads of the step after it (`next`, step
   // nks) and the loads of stage t into `to`: one at a time, so that neither LDS nor the

@@ -49,6 +49,8 @@ struct Args {
   int k_bytes;
   int act;  // VK_GATE_*
   bool vec; // out's rows are whole 16-byte pieces
+  const void* x;  // for workgroups that quantise for themselves: [M, K] of vk_dtype x_type
+  int K, x_type;
   int gm, gn, group;
 };
 
@@ -65,28 +67,39 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 }
 
 // A row's scale from the bits of its largest |x| (a NaN is above an infinity is above
-// every number), what to divide by, and whether all codes are 0.
+// every number), what to divide by and its reciprocal (0 where all codes are 0).
 struct RowScale {
-  float scale, by;
-  bool none;
+  float scale, by, inverse;
 };
 __device__ __forceinline__ RowScale row_scale(uint32_t top) {
   const float d = __uint_as_float(top) / kTop;
   const bool odd = top >= 0x7f800000u;
   const bool none = odd || d < kLeastScale;
-  return RowScale{odd ? __uint_as_float(0x7fc00000u) : (none ? 0.0f : d), none ? 1.0f : d, none};
+  return RowScale{odd ? __uint_as_float(0x7fc00000u) : (none ? 0.0f : d), none ? 1.0f : d,
+                  none ? 0.0f : 1.0f / d};
 }
 
-__device__ __forceinline__ uint32_t code_of(float x, const RowScale& s) {
-  return s.none ? 0u : static_cast<uint32_t>(static_cast<int>(rintf(x / s.by))) & 0xffu;
+// Four codes.  x / by rounded to f32 without a division each: with the correctly rounded
+// reciprocal r and q = x r, q + (x - q by) r in two fused steps is the correctly rounded quotient
+// (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000
+// processor", 1990; by is 2^-100 to 2^122 here, and a quotient that could leave the normal
+// numbers rounds to 0 either way).  Adding 1.5 x 2^23 then rounds it to a whole number, ties to
+// even, whose lowest byte is the code.
+__device__ __forceinline__ uint32_t codes_of(const float* x, const RowScale& s) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float v = s.inverse == 0.0f ? 0.0f : x[i];  // (an infinity times 0 is none)
+    const float q = v * s.inverse;
+    const float y = __builtin_fmaf(__builtin_fmaf(-q, s.by, v), s.inverse, q);
+    c[i] = __float_as_uint(y + 12582912.0f);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u);
+  const uint32_t hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+  return lo | hi;
 }
 
-template <typename XT>
-__device__ __forceinline__ float x_at(const XT* x, size_t i) {
-  return vkp::widen(x[i]);
-}
-
-// Eight values from x[i]; VEC: x + i is 16-byte aligned.
+// Eight values from x[i]; VEC: x + i is 16-byte aligned, and all eight are in or none is.
 template <typename XT, bool VEC>
 __device__ __forceinline__ void load8(const XT* x, size_t i, int left, float (&v)[8]) {
   if constexpr (VEC) {
@@ -103,57 +116,70 @@ __device__ __forceinline__ void load8(const XT* x, size_t i, int left, float (&v
     }
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? x_at(x, i + j) : 0.0f;
+    for (int j = 0; j < 8; ++j) v[j] = j < left ? vkp::widen(x[i + j]) : 0.0f;
   }
 }
 
-// A wave a row: NV steps of 8 values a lane stay in registers between the maximum and
-// the codes; NV 0: any length, read twice.
-template <typename XT, bool VEC, int NV>
+__device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) top = max(top, bits_abs(v[j]));
+  return top;
+}
+
+// WPR waves a row (4 of them are a workgroup's, otherwise it has 4 rows).  NV steps of 8
+// values a lane stay in registers between the maximum and the codes; NV 0: any length, read
+// twice.
+template <typename XT, bool VEC, int NV, int WPR>
 __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict__ x, int M, int K,
                                                             uint32_t pitch, char* codes,
                                                             float* scales) {
-  const int lane = threadIdx.x & 63;
-  const int m = blockIdx.x * 4 + (threadIdx.x >> 6);
+  constexpr int kStep = 512 * WPR;
+  const int lane = threadIdx.x & (64 * WPR - 1);
+  const int m = WPR == 4 ? blockIdx.x : blockIdx.x * 4 + (threadIdx.x >> 6);
   if (m >= M) return;
   const XT* row = x + static_cast<size_t>(m) * K;
   char* to = codes + static_cast<size_t>(m) * pitch;
-  auto store = [&](int at, const float (&v)[8], const RowScale& s) {
-    if (at >= static_cast<int>(pitch)) return;
-    uint2 w;
-    w.x = code_of(v[0], s) | code_of(v[1], s) << 8 | code_of(v[2], s) << 16 | code_of(v[3], s) << 24;
-    w.y = code_of(v[4], s) | code_of(v[5], s) << 8 | code_of(v[6], s) << 16 | code_of(v[7], s) << 24;
-    *reinterpret_cast<uint2*>(to + at) = w;
+  const auto scale_of = [&](uint32_t top) {
+    top = wave_umax(top);
+    if constexpr (WPR == 4) {
+      __shared__ uint32_t tops[4];
+      if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+      __syncthreads();
+      top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+    }
+    const RowScale s = row_scale(top);
+    if (lane == 0) scales[m] = s.scale;
+    return s;
   };
-  uint32_t top = 0;
+  const auto store = [&](int at, const float (&v)[8], const RowScale& s) {
+    if (at < static_cast<int>(pitch))
+      *reinterpret_cast<uint2*>(to + at) = make_uint2(codes_of(v, s), codes_of(v + 4, s));
+  };
   if constexpr (NV > 0) {
     float v[NV][8];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-      const int at = (i * 64 + lane) * 8;
+      const int at = i * kStep + lane * 8;
       load8<XT, VEC>(row, at, K - at, v[i]);
     }
+    uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < NV; ++i)
+    for (int i = 0; i < NV; ++i) top = top_of(v[i], top);
+    const RowScale s = scale_of(top);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, bits_abs(v[i][j]));
-    const RowScale s = row_scale(wave_umax(top));
-#pragma unroll
-    for (int i = 0; i < NV; ++i) store((i * 64 + lane) * 8, v[i], s);
-    if (lane == 0) scales[m] = s.scale;
+    for (int i = 0; i < NV; ++i) store(i * kStep + lane * 8, v[i], s);
   } else {
     float v[8];
-    for (int at = lane * 8; at < K; at += 512) {
+    uint32_t top = 0;
+    for (int at = lane * 8; at < K; at += kStep) {
       load8<XT, VEC>(row, at, K - at, v);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) top = max(top, bits_abs(v[j]));
+      top = top_of(v, top);
     }
-    const RowScale s = row_scale(wave_umax(top));
-    for (int at = lane * 8; at < static_cast<int>(pitch); at += 512) {
+    const RowScale s = scale_of(top);
+    for (int at = lane * 8; at < static_cast<int>(pitch); at += kStep) {
       load8<XT, VEC>(row, at, K - at, v);
       store(at, v, s);
     }
-    if (lane == 0) scales[m] = s.scale;
   }
 }
 
@@ -242,20 +268,17 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   }
 }
 
-// At most 16 RT rows, their codes in memory.
+// What leaves after the waves' sums are joined: thread by thread.
 template <int END, typename V, int RT>
-__global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g) {
+__device__ __forceinline__ void few_finish(const Args& g, const char* smem, int n0, const float* scales) {
   constexpr bool kPaired = END == kGated;
-  __shared__ __align__(16) char smem[vkp::few_bytes<kI8, RT, kPaired>()];
-  const int n0 = blockIdx.x * 16;
-  vkp::few_product<kI8, RT, kPaired>(g.a, g.b, g.k_bytes, n0, smem);
   for (int e = threadIdx.x; e < 256 * RT; e += vkp::kFewThreads) {
     const int m = e >> 4, n = n0 + (e & 15);
     if (m >= g.M || n >= g.N) continue;
-    const float row = g.sx[m];
+    const float row = scales[m];
     V* to = static_cast<V*>(g.out) + static_cast<size_t>(m) * g.N + n;
-    const float bias = g.bias ? g.bias[n] : 0.0f;
-    float v = linear_of(vkp::few_sum<kI8, RT, kPaired>(smem, 0, m, e & 15), g.sw[n], row, bias);
+    float v = linear_of(vkp::few_sum<kI8, RT, kPaired>(smem, 0, m, e & 15), g.sw[n], row,
+                        g.bias ? g.bias[n] : 0.0f);
     if constexpr (kPaired) {
       const int p = g.N + n;
       v = gated_of(g.act, v, linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15), g.sw[p], row,
@@ -267,20 +290,99 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g)
   }
 }
 
+// At most 16 RT rows, their codes in memory.
+template <int END, typename V, int RT>
+__global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g) {
+  constexpr bool kPaired = END == kGated;
+  __shared__ __align__(16) char smem[vkp::few_bytes<kI8, RT, kPaired>()];
+  const int n0 = blockIdx.x * 16;
+  vkp::few_product<kI8, RT, kPaired>(g.a, g.b, g.k_bytes, n0, smem);
+  few_finish<END, V, RT>(g, smem, n0, g.sx);
+}
+
+// A row or a few, of at most kRowBytes of codes: every workgroup quantises them for itself, in one
+// launch, while its weights are on their way.
+template <typename XT>
+__device__ __forceinline__ void load8_any(const Args& g, int m, int at, float (&v)[8]) {
+  const XT* row = static_cast<const XT*>(g.x) + static_cast<size_t>(m) * g.K;
+  if (g.K % 8 == 0)
+    load8<XT, true>(row, at, g.K - at, v);
+  else
+    load8<XT, false>(row, at, g.K - at, v);
+}
+
+template <int END, typename V>
+__global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g) {
+  constexpr bool kPaired = END == kGated;
+  constexpr int kPitch = vkp::kOwnBytes + 16;  // rows start in different banks
+  __shared__ __align__(16) char smem[vkp::few_bytes<kI8, 1, kPaired>()];
+  __shared__ __align__(16) char codes[vkp::kOwnRows * kPitch];
+  __shared__ uint32_t tops[vkp::kOwnRows][vkp::kFewWaves];
+  __shared__ float scales[vkp::kOwnRows];
+  const int n0 = blockIdx.x * 16, tid = threadIdx.x, c = tid & 15;
+  static_assert(vkp::kOwnBytes <= 8 * vkp::kFewThreads, "eight values a thread");
+  vkp::few_product<kI8, 1, kPaired>(
+      g.b, g.k_bytes, n0, smem,
+      [&] {
+        float v[vkp::kOwnRows][8];
+#pragma unroll
+        for (int m = 0; m < vkp::kOwnRows; ++m)
+          if (m < g.M) {
+            if (g.x_type == VK_F32) load8_any<float>(g, m, 8 * tid, v[m]);
+            else if (g.x_type == VK_F16) load8_any<_Float16>(g, m, 8 * tid, v[m]);
+            else load8_any<__bf16>(g, m, 8 * tid, v[m]);
+          }
+#pragma unroll
+        for (int m = 0; m < vkp::kOwnRows; ++m)
+          if (m < g.M) {
+            const uint32_t top = wave_umax(top_of(v[m], 0));
+            if ((tid & 63) == 0) tops[m][tid >> 6] = top;
+          }
+        __syncthreads();
+#pragma unroll
+        for (int m = 0; m < vkp::kOwnRows; ++m)
+          if (m < g.M) {
+            uint32_t top = tops[m][0];
+#pragma unroll
+            for (int w = 1; w < vkp::kFewWaves; ++w) top = max(top, tops[m][w]);
+            const RowScale s = row_scale(top);
+            if (8 * tid < g.k_bytes)
+              *reinterpret_cast<uint2*>(codes + m * kPitch + 8 * tid) =
+                  make_uint2(codes_of(v[m], s), codes_of(v[m] + 4, s));
+            if (tid == 0) scales[m] = s.scale;
+          }
+        __syncthreads();
+      },
+      [&](int, int k) {
+        vkp::i32x4 a = {0, 0, 0, 0};
+        if (c < g.M && k < g.k_bytes) a = *reinterpret_cast<const vkp::i32x4*>(codes + c * kPitch + k);
+        return a;
+      });
+  few_finish<END, V, 1>(g, smem, n0, scales);
+}
+
 // ---------------------------------------------------------------- launches
+// Four waves a row where a wave each would leave the card half empty.
 template <typename XT, bool VEC>
 void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, char* codes,
               float* scales) {
-  const dim3 grid((M + 3) / 4), block(256);
+  const bool wide = pitch > 512 && M < 16 * (rt->cu_count > 0 ? rt->cu_count : 256);
+  const dim3 grid(wide ? M : (M + 3) / 4), block(256);
   const auto p = static_cast<uint32_t>(pitch);
-#define VK_LAUNCH(NV)                                                                            \
-  hipLaunchKernelGGL((quantise_rows_kernel<XT, VEC, NV>), grid, block, 0, rt->stream, x, M, K, p, \
-                     codes, scales)
-  if (pitch <= 512) VK_LAUNCH(1);
-  else if (pitch <= 1024) VK_LAUNCH(2);
-  else if (pitch <= 2048) VK_LAUNCH(4);
-  else if (pitch <= 4096) VK_LAUNCH(8);
-  else VK_LAUNCH(0);
+#define VK_LAUNCH(NV, WPR)                                                                          \
+  hipLaunchKernelGGL((quantise_rows_kernel<XT, VEC, NV, WPR>), grid, block, 0, rt->stream, x, M, K, \
+                     p, codes, scales)
+  if (wide) {
+    if (pitch <= 2048) VK_LAUNCH(1, 4);
+    else if (pitch <= 4096) VK_LAUNCH(2, 4);
+    else VK_LAUNCH(0, 4);
+  } else {
+    if (pitch <= 512) VK_LAUNCH(1, 1);
+    else if (pitch <= 1024) VK_LAUNCH(2, 1);
+    else if (pitch <= 2048) VK_LAUNCH(4, 1);
+    else if (pitch <= 4096) VK_LAUNCH(8, 1);
+    else VK_LAUNCH(0, 1);
+  }
 #undef VK_LAUNCH
 }
 
@@ -298,6 +400,11 @@ template <int END, typename V>
 int launch(vk_runtime* rt, Args& g) {
   constexpr bool kPaired = END == kGated;
   g.vec = static_cast<size_t>(g.N) * sizeof(V) % 16 == 0;
+  if (g.x) {
+    hipLaunchKernelGGL((linear_i8_rows_kernel<END, V>), dim3((g.N + 15) / 16), dim3(vkp::kFewThreads), 0,
+                       rt->stream, g);
+    return vk::check_launch("linear_i8_rows_kernel");
+  }
   const vkp::Plan p = vkp::plan(rt->cu_count, g.M, kPaired ? 2LL * g.N : g.N, g.k_bytes);
   if (p.few) {
     const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
@@ -361,24 +468,29 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
   VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((N + 31) / 32) > 0x7fffffULL, "linear_i8: %zu x %zu outputs",
                     rows, N);
 
-  const size_t code_bytes = rows * lin->pitch;  // a multiple of 128
-  VK_TRY(vk::ensure_work(rt, code_bytes / 4 + rows, "linear_i8"));
-  char* codes = reinterpret_cast<char*>(rt->work);
-  float* scales = reinterpret_cast<float*>(codes + code_bytes);
   const int M = static_cast<int>(rows);
-  if (x->dtype == VK_F32)
-    quantise_any<float>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
-  else if (x->dtype == VK_F16)
-    quantise_any<_Float16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
-  else
-    quantise_any<__bf16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
-  VK_TRY(vk::check_launch("quantise_rows_kernel"));
-
   Args g{};
-  g.a = Operand{codes, M, static_cast<uint32_t>(lin->pitch)};
+  if (vkp::own_rows(rows, lin->pitch)) {
+    g.x = x->ptr;
+    g.K = static_cast<int>(K);
+    g.x_type = x->dtype;
+  } else {
+    const size_t code_bytes = rows * lin->pitch;  // a multiple of 128
+    VK_TRY(vk::ensure_work(rt, code_bytes / 4 + rows, "linear_i8"));
+    char* codes = reinterpret_cast<char*>(rt->work);
+    float* scales = reinterpret_cast<float*>(codes + code_bytes);
+    if (x->dtype == VK_F32)
+      quantise_any<float>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+    else if (x->dtype == VK_F16)
+      quantise_any<_Float16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+    else
+      quantise_any<__bf16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+    VK_TRY(vk::check_launch("quantise_rows_kernel"));
+    g.a = Operand{codes, M, static_cast<uint32_t>(lin->pitch)};
+    g.sx = scales;
+  }
   g.b = Operand{reinterpret_cast<const char*>(lin->codes), static_cast<int>(lin->out_features),
                 static_cast<uint32_t>(lin->pitch)};
-  g.sx = scales;
   g.sw = lin->scale;
   g.bias = lin->bias;
   g.ls = lin->ls_gamma;

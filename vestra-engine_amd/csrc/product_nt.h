@@ -684,36 +684,32 @@ constexpr int few_bytes() {
   return kFewWaves * (PAIRED ? 2 : 1) * RT * 64 * 16;
 }
 
-// The product of rows 0 .. a.rows of a, read from memory.
-template <Kind KIND, int RT, bool PAIRED>
-__device__ __forceinline__ void few_product(const Operand& a, const Operand& b, int k_bytes, int n0,
-                                            char* smem) {
+// The product of the columns n0 .. with at most 16 RT rows: a_at(r, k) is the lane's 16 bytes from k
+// of row 16 r + lane % 16, zeros outside.  The first columns are on their way before `first()` runs,
+// the next ones while a stage's products do.
+template <Kind KIND, int RT, bool PAIRED, typename A, typename F>
+__device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n0, char* smem, F first,
+                                            A a_at) {
   constexpr int U = 2;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  uint32_t at[2], aat[RT];
+  uint32_t at[2];
   const auto rb = few_rows_of<PAIRED>(b, n0, c, at);
-  const size_t a_bytes = static_cast<size_t>(a.rows) * a.pitch;
-  const auto ra = vkd::buffer_rsrc(a.base, a_bytes < kMostBytes ? static_cast<uint32_t>(a_bytes) : kMostBytes);
-#pragma unroll
-  for (int r = 0; r < RT; ++r)
-    aat[r] = r * 16 + c < a.rows ? static_cast<uint32_t>(r * 16 + c) * a.pitch : kOutside;
   FewSums<KIND, RT, PAIRED> s{};
   const int stages = (k_bytes + kStage - 1) / kStage;
+  FewColumns<PAIRED, U> fb;
+  fb.load(rb, at, q, wave, k_bytes);
+  first();
   for (int t = wave; t < stages; t += U * kFewWaves) {
-    FewColumns<PAIRED, U> fb;
-    fb.load(rb, at, q, t, k_bytes);
+    const FewColumns<PAIRED, U> now = fb;
     i32x4 fa[U][RT][2];
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = (t + u * kFewWaves) * kStage + q * 32 + h * 16;
-          fa[u][r][h] = __builtin_bit_cast(
-              i32x4, vkd::buffer_load4(ra, k < k_bytes && aat[r] != kOutside ? aat[r] + static_cast<uint32_t>(k) : kOutside, 0));
-        }
+        for (int h = 0; h < 2; ++h) fa[u][r][h] = a_at(r, (t + u * kFewWaves) * kStage + q * 32 + h * 16);
+    if (t + U * kFewWaves < stages) fb.load(rb, at, q, t + U * kFewWaves, k_bytes);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
@@ -722,9 +718,26 @@ __device__ __forceinline__ void few_product(const Operand& a, const Operand& b, 
         for (int p = 0; p < (PAIRED ? 2 : 1); ++p)
 #pragma unroll
           for (int r = 0; r < RT; ++r)
-            s.v[p][r] = Ops<KIND>::mma16(fa[u][r][h], fb.v[u][p][h], s.v[p][r]);
+            s.v[p][r] = Ops<KIND>::mma16(fa[u][r][h], now.v[u][p][h], s.v[p][r]);
   }
   few_join<KIND, RT, PAIRED>(s, smem, wave, lane);
+}
+
+// Rows 0 .. a.rows of a in memory.
+template <Kind KIND, int RT, bool PAIRED>
+__device__ __forceinline__ void few_product(const Operand& a, const Operand& b, int k_bytes, int n0,
+                                            char* smem) {
+  const int c = threadIdx.x & 15;
+  const size_t a_bytes = static_cast<size_t>(a.rows) * a.pitch;
+  const auto ra = vkd::buffer_rsrc(a.base, a_bytes < kMostBytes ? static_cast<uint32_t>(a_bytes) : kMostBytes);
+  few_product<KIND, RT, PAIRED>(
+      b, k_bytes, n0, smem, [] {},
+      [&](int r, int k) {
+        const uint32_t row = static_cast<uint32_t>(r * 16 + c);
+        const bool in = k < k_bytes && static_cast<int>(row) < a.rows;
+        return __builtin_bit_cast(
+            i32x4, vkd::buffer_load4(ra, in ? row * a.pitch + static_cast<uint32_t>(k) : kOutside, 0));
+      });
 }
 
 }  // namespace vkp

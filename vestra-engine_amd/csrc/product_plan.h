@@ -2,10 +2,16 @@
 // that a host without a GPU evaluates the same rules.
 #pragma once
 
+#include <cstddef>
+
 namespace vkp {
 
 constexpr int kGroupRows = 1024;  // rows of a that an XCD walks the columns with
 constexpr int kFewRows = 32;      // most rows of the few-row kernels
+// Rows of x that every workgroup of the 8-bit linear quantises for itself: a launch less, against
+// reading them that many times.
+constexpr int kOwnRows = 4, kOwnBytes = 4096;
+inline bool own_rows(size_t rows, size_t bytes) { return rows <= kOwnRows && bytes <= kOwnBytes; }
 
 // Tiles of 64 x 64 by one group of two waves or by four groups that share k, of 128 x 128 and
 // of 256 x 256.

@@ -34,7 +34,6 @@ struct Args {
   int d_half, m_half;
   int M, N;
   int act;
-  bool vec;          // rows of N values are whole 16-byte pieces
   int gm, gn, group;
 };
 
@@ -99,7 +98,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
       }
     vkd::wave_lds_fence();
     C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
-                             n0 + T::b_row(wn, 0), g.N, g.vec);
+                             n0 + T::b_row(wn, 0), g.N);
     vkd::wave_lds_fence();
   }
 }
@@ -127,13 +126,13 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   const size_t pitch = 2 * static_cast<size_t>(g.d_half);
   const int nb = n0 + T::b_row(wn, 0);
   vkp::i32x4 dh[C::kFetch];
-  C::fetch(dh, lane, grad, g.N, m0 + wm * T::MT * 32, g.M, nb, g.N, g.vec);
+  C::fetch(dh, lane, grad, g.N, m0 + wm * T::MT * 32, g.M, nb, g.N);
   float sum[kCols] = {};
 #pragma unroll
   for (int i = 0; i < T::MT; ++i) {
     const int mb = m0 + (wm * T::MT + i) * 32;
     C::fill(chunk, lane, dh);
-    if (i + 1 < T::MT) C::fetch(dh, lane, grad, g.N, mb + 32, g.M, nb, g.N, g.vec);
+    if (i + 1 < T::MT) C::fetch(dh, lane, grad, g.N, mb + 32, g.M, nb, g.N);
     vkd::wave_lds_fence();
     // rows past M and columns past N have dh of 0; what their g and u are is finite only where
     // the others' are
@@ -172,14 +171,14 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
     }
     if (d) {
       vkd::wave_lds_fence();
-      C::template store<false>(chunk, lane, d, pitch, mb, g.M, nb, g.d_half, true);
+      C::template store<false>(chunk, lane, d, pitch, mb, g.M, nb, g.d_half);
       vkd::wave_lds_fence();
 #pragma unroll
       for (int j = 0; j < kCols; ++j)
 #pragma unroll
         for (int q = 0; q < 4; ++q) *C::at(chunk, lane, j, q) = du[j][q];
       vkd::wave_lds_fence();
-      C::template store<false>(chunk, lane, d + g.d_half, pitch, mb, g.M, nb, g.d_half, true);
+      C::template store<false>(chunk, lane, d + g.d_half, pitch, mb, g.M, nb, g.d_half);
     }
     vkd::wave_lds_fence();
   }
@@ -232,7 +231,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Ar
       }
     }
     C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end, n0 + T::b_row(wn, 0),
-                             g.N, g.vec);
+                             g.N);
     vkd::wave_lds_fence();
   }
 }
@@ -339,7 +338,6 @@ int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k,
   g.M = static_cast<int>(M);
   g.N = static_cast<int>(N);
   g.m_half = static_cast<int>(m_half);
-  g.vec = N % 8 == 0;
   const vkp::Plan p = vkp::plan(rt->cu_count, a.rows, g.N, g.k_bytes);
   with_tile<false>(p.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
@@ -450,7 +448,6 @@ Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, 
   g.M = static_cast<int>(rows);
   g.N = static_cast<int>(hidden);
   g.act = act;
-  g.vec = hidden % 8 == 0;
   return g;
 }
 

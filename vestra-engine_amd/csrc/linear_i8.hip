@@ -48,7 +48,6 @@ struct Args {
   int M, N;  // N: columns of out
   int k_bytes;
   int act;  // VK_GATE_*
-  bool vec; // out's rows are whole 16-byte pieces
   const void* x;  // for workgroups that quantise for themselves: [M, K] of vk_dtype x_type
   int K, x_type;
   int gm, gn, group;
@@ -99,25 +98,18 @@ __device__ __forceinline__ uint32_t codes_of(const float* x, const RowScale& s) 
   return lo | hi;
 }
 
-// Eight values from x[i]; VEC: x + i is 16-byte aligned, and all eight are in or none is.
-template <typename XT, bool VEC>
+// Eight values from x[i], zeros from the left-th on; x + i may lie anywhere.
+template <typename XT>
 __device__ __forceinline__ void load8(const XT* x, size_t i, int left, float (&v)[8]) {
-  if constexpr (VEC) {
-    if (left > 0) {
-      struct alignas(16) Eight {
-        XT e[8];
-      };
-      const Eight t = *reinterpret_cast<const Eight*>(x + i);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = vkp::widen(t.e[j]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] = 0.0f;
-    }
+  XT e[8];
+  if (left >= 8) {
+    __builtin_memcpy(e, x + i, sizeof(e));
   } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = j < left ? vkp::widen(x[i + j]) : 0.0f;
+    for (int j = 0; j < 8; ++j) e[j] = j < left ? x[i + j] : static_cast<XT>(0.0f);
   }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = vkp::widen(e[j]);
 }
 
 __device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
@@ -129,7 +121,7 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
 // WPR waves a row (4 of them are a workgroup's, otherwise it has 4 rows).  NV steps of 8
 // values a lane stay in registers between the maximum and the codes; NV 0: any length, read
 // twice.
-template <typename XT, bool VEC, int NV, int WPR>
+template <typename XT, int NV, int WPR>
 __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict__ x, int M, int K,
                                                             uint32_t pitch, char* codes,
                                                             float* scales) {
@@ -160,7 +152,7 @@ __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int at = i * kStep + lane * 8;
-      load8<XT, VEC>(row, at, K - at, v[i]);
+      load8(row, at, K - at, v[i]);
     }
     uint32_t top = 0;
 #pragma unroll
@@ -172,12 +164,12 @@ __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict
     float v[8];
     uint32_t top = 0;
     for (int at = lane * 8; at < K; at += kStep) {
-      load8<XT, VEC>(row, at, K - at, v);
+      load8(row, at, K - at, v);
       top = top_of(v, top);
     }
     const RowScale s = scale_of(top);
     for (int at = lane * 8; at < static_cast<int>(pitch); at += kStep) {
-      load8<XT, VEC>(row, at, K - at, v);
+      load8(row, at, K - at, v);
       store(at, v, s);
     }
   }
@@ -261,8 +253,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
           *C::at(chunk, lane, jj, q) = w;
         }
       vkd::wave_lds_fence();
-      C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N,
-                                          g.vec);
+      C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N);
       vkd::wave_lds_fence();
     }
   }
@@ -303,12 +294,8 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g)
 // A row or a few, of at most kRowBytes of codes: every workgroup quantises them for itself, in one
 // launch, while its weights are on their way.
 template <typename XT>
-__device__ __forceinline__ void load8_any(const Args& g, int m, int at, float (&v)[8]) {
-  const XT* row = static_cast<const XT*>(g.x) + static_cast<size_t>(m) * g.K;
-  if (g.K % 8 == 0)
-    load8<XT, true>(row, at, g.K - at, v);
-  else
-    load8<XT, false>(row, at, g.K - at, v);
+__device__ __forceinline__ void load8_of(const Args& g, int m, int at, float (&v)[8]) {
+  load8(static_cast<const XT*>(g.x) + static_cast<size_t>(m) * g.K, at, g.K - at, v);
 }
 
 template <int END, typename V>
@@ -328,9 +315,9 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g
 #pragma unroll
         for (int m = 0; m < vkp::kOwnRows; ++m)
           if (m < g.M) {
-            if (g.x_type == VK_F32) load8_any<float>(g, m, 8 * tid, v[m]);
-            else if (g.x_type == VK_F16) load8_any<_Float16>(g, m, 8 * tid, v[m]);
-            else load8_any<__bf16>(g, m, 8 * tid, v[m]);
+            if (g.x_type == VK_F32) load8_of<float>(g, m, 8 * tid, v[m]);
+            else if (g.x_type == VK_F16) load8_of<_Float16>(g, m, 8 * tid, v[m]);
+            else load8_of<__bf16>(g, m, 8 * tid, v[m]);
           }
 #pragma unroll
         for (int m = 0; m < vkp::kOwnRows; ++m)
@@ -363,14 +350,14 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g
 
 // ---------------------------------------------------------------- launches
 // Four waves a row where a wave each would leave the card half empty.
-template <typename XT, bool VEC>
+template <typename XT>
 void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, char* codes,
               float* scales) {
   const bool wide = pitch > 512 && M < 16 * (rt->cu_count > 0 ? rt->cu_count : 256);
   const dim3 grid(wide ? M : (M + 3) / 4), block(256);
   const auto p = static_cast<uint32_t>(pitch);
 #define VK_LAUNCH(NV, WPR)                                                                          \
-  hipLaunchKernelGGL((quantise_rows_kernel<XT, VEC, NV, WPR>), grid, block, 0, rt->stream, x, M, K, \
+  hipLaunchKernelGGL((quantise_rows_kernel<XT, NV, WPR>), grid, block, 0, rt->stream, x, M, K, \
                      p, codes, scales)
   if (wide) {
     if (pitch <= 2048) VK_LAUNCH(1, 4);
@@ -386,20 +373,9 @@ void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, cha
 #undef VK_LAUNCH
 }
 
-template <typename XT>
-void quantise_any(const vk_runtime* rt, const vk_tensor* x, int M, int K, size_t pitch, char* codes,
-                  float* scales) {
-  const auto* p = static_cast<const XT*>(x->ptr);
-  if (K % 8 == 0)
-    quantise<XT, true>(rt, p, M, K, pitch, codes, scales);
-  else
-    quantise<XT, false>(rt, p, M, K, pitch, codes, scales);
-}
-
 template <int END, typename V>
 int launch(vk_runtime* rt, Args& g) {
   constexpr bool kPaired = END == kGated;
-  g.vec = static_cast<size_t>(g.N) * sizeof(V) % 16 == 0;
   if (g.x) {
     hipLaunchKernelGGL((linear_i8_rows_kernel<END, V>), dim3((g.N + 15) / 16), dim3(vkp::kFewThreads), 0,
                        rt->stream, g);
@@ -480,11 +456,14 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
     char* codes = reinterpret_cast<char*>(rt->work);
     float* scales = reinterpret_cast<float*>(codes + code_bytes);
     if (x->dtype == VK_F32)
-      quantise_any<float>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+      quantise(rt, static_cast<const float*>(x->ptr), M, static_cast<int>(K), lin->pitch, codes,
+               scales);
     else if (x->dtype == VK_F16)
-      quantise_any<_Float16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+      quantise(rt, static_cast<const _Float16*>(x->ptr), M, static_cast<int>(K), lin->pitch, codes,
+               scales);
     else
-      quantise_any<__bf16>(rt, x, M, static_cast<int>(K), lin->pitch, codes, scales);
+      quantise(rt, static_cast<const __bf16*>(x->ptr), M, static_cast<int>(K), lin->pitch, codes,
+               scales);
     VK_TRY(vk::check_launch("quantise_rows_kernel"));
     g.a = Operand{codes, M, static_cast<uint32_t>(lin->pitch)};
     g.sx = scales;

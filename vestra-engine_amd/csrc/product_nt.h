@@ -129,7 +129,7 @@ void with_tile(TileSize size, F go) {
   } else if (size == kTile128) {
     go(Tile<2, 2, 2, 2, PAIRED, 128, 2, 1>{});
   } else if (size == kTile64K) {
-    go(Tile<2, 1, 1, 2, PAIRED, 128, 2, 4>{});
+    go(Tile<2, 1, 1, 2, PAIRED, 128, 4, 2>{});
   } else {
     go(Tile<2, 1, 1, 2, PAIRED, 128, 2, 1>{});
   }
@@ -415,7 +415,7 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
   if constexpr (KG > 1) {
     typedef typename Ops<KIND>::Acc4 Acc4;
     constexpr int kTiles = T::MT * T::NT, kWaveSums = kTiles * 4 * 64;
-    Acc4* sums = reinterpret_cast<Acc4*>(stages_[1]) + wave * kWaveSums + lane;
+    Acc4* sums = reinterpret_cast<Acc4*>(stages_[R - 1]) + wave * kWaveSums + lane;
 #pragma unroll
     for (int e = 0; e < kTiles * 4; ++e) {
       const auto& v = acc[e / 4 / T::NT][e / 4 % T::NT];
@@ -458,23 +458,20 @@ struct Chunk {
     const int byte = (32 * j + 8 * q + 4 * (lane >> 5)) * static_cast<int>(sizeof(V));
     return reinterpret_cast<V4*>(c + slot(lane & 31, byte >> 4) + (byte & 15));
   }
-  static __device__ __forceinline__ V* element(char* c, int row, int col) {
-    const int byte = col * static_cast<int>(sizeof(V));
-    return reinterpret_cast<V*>(c + slot(row, byte >> 4) + (byte & 15));
-  }
   // From rows m0 .., columns n0 .. of a matrix (zeros outside), through registers, so that the
-  // loads of the next rows can be under way: fetch, then fill.  As store.
+  // loads of the next rows can be under way: fetch, then fill.  Rows may start anywhere: 16 bytes
+  // go to and from any address, and only a row's last piece goes value by value.
   static constexpr int kFetch = kBytes / 1024;
   static __device__ __forceinline__ void fetch(i32x4 (&v)[kFetch], int lane, const V* from,
-                                               size_t pitch, int m0, int M, int n0, int N, bool vec) {
+                                               size_t pitch, int m0, int M, int n0, int N) {
 #pragma unroll
     for (int p = 0; p < kFetch; ++p) {
       v[p] = i32x4{};
       const int m = m0 + p * (64 / kPieces) + lane / kPieces, n = n0 + lane % kPieces * kPer;
       if (m >= M || n >= N) continue;
       const V* at = from + static_cast<size_t>(m) * pitch + n;
-      if (vec) {
-        v[p] = *reinterpret_cast<const i32x4*>(at);
+      if (n + kPer <= N) {
+        __builtin_memcpy(&v[p], at, 16);
       } else {
         V e[kPer];
 #pragma unroll
@@ -488,36 +485,36 @@ struct Chunk {
     for (int p = 0; p < kFetch; ++p)
       *reinterpret_cast<i32x4*>(c + slot(p * (64 / kPieces) + lane / kPieces, lane % kPieces)) = v[p];
   }
-  // To rows m0 .. of `out` (pitch values a row), columns n0 .., of those below M and N.  vec:
-  // every row starts on 16 bytes and N is whole pieces.  ADD: added to what is there.
+  // To rows m0 .. of `out` (pitch values a row), columns n0 .., of those below M and N.  ADD: added
+  // to what is there (f32).
   template <bool ADD>
   static __device__ __forceinline__ void store(char* c, int lane, V* out, size_t pitch, int m0,
-                                               int M, int n0, int N, bool vec) {
-    if (vec) {
+                                               int M, int n0, int N) {
 #pragma unroll
-      for (int p = 0; p < kBytes / 1024; ++p) {
-        const int row = p * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
-        const int m = m0 + row, n = n0 + piece * kPer;
-        i32x4 v = *reinterpret_cast<const i32x4*>(c + slot(row, piece));
-        if (m >= M || n >= N) continue;
-        i32x4* to = reinterpret_cast<i32x4*>(out + static_cast<size_t>(m) * pitch + n);
-        if constexpr (ADD)
-          v = __builtin_bit_cast(i32x4, __builtin_bit_cast(f32x4, *to) + __builtin_bit_cast(f32x4, v));
-        *to = v;
-      }
-    } else {
-      constexpr int kCols = 32 * J;
-#pragma unroll 4
-      for (int p = 0; p < 32 * kCols / 64; ++p) {
-        const int row = p * (64 / kCols) + lane / kCols, col = lane % kCols;
-        const int m = m0 + row, n = n0 + col;
-        const V v = *element(c, row, col);
-        if (m >= M || n >= N) continue;
-        V* to = out + static_cast<size_t>(m) * pitch + n;
-        if constexpr (ADD)
-          *to = *to + v;
-        else
-          *to = v;
+    for (int p = 0; p < kFetch; ++p) {
+      const int row = p * (64 / kPieces) + lane / kPieces, piece = lane % kPieces;
+      const int m = m0 + row, n = n0 + piece * kPer;
+      i32x4 v = *reinterpret_cast<const i32x4*>(c + slot(row, piece));
+      if (m >= M || n >= N) continue;
+      V* to = out + static_cast<size_t>(m) * pitch + n;
+      if (n + kPer <= N) {
+        if constexpr (ADD) {
+          f32x4 old;
+          __builtin_memcpy(&old, to, 16);
+          v = __builtin_bit_cast(i32x4, old + __builtin_bit_cast(f32x4, v));
+        }
+        __builtin_memcpy(to, &v, 16);
+      } else {
+        V e[kPer];
+        __builtin_memcpy(e, &v, 16);
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          if (n + i >= N) continue;
+          if constexpr (ADD)
+            to[i] = to[i] + e[i];
+          else
+            to[i] = e[i];
+        }
       }
     }
   }

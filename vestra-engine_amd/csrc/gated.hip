@@ -52,17 +52,6 @@ __device__ __forceinline__ void load_bias(const Args& g, int n0, float* to) {
   }
 }
 
-__device__ __forceinline__ float gate_any(int act, float g) {
-  return act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(g) : vkp::gate<VK_GATE_GELU>(g);
-}
-
-__device__ __forceinline__ void slope_any(int act, float g, float* a, float* s) {
-  if (act == VK_GATE_SILU)
-    vkp::gate_slope<VK_GATE_SILU>(g, a, s);
-  else
-    vkp::gate_slope<VK_GATE_GELU>(g, a, s);
-}
-
 template <Kind KIND, typename T>
 __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args g) {
   typedef typename vkp::Value<KIND>::type V;
@@ -80,27 +69,29 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
   constexpr int kCols = T::NT / 2;
   typedef vkp::Chunk<V, kCols> C;
   char* chunk = stages_[0] + wave * C::kBytes;
+  vkp::with_act(g.act, [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < T::MT; ++i) {
+    for (int i = 0; i < T::MT; ++i) {
 #pragma unroll
-    for (int j = 0; j < kCols; ++j)
+      for (int j = 0; j < kCols; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
-        const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
-        const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
-        typename C::V4 h;
+        for (int q = 0; q < 4; ++q) {
+          const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+          const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
+          const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
+          typename C::V4 h;
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          h[e] = static_cast<V>(gate_any(g.act, acc[i][j][4 * q + e] + bg[e]) *
-                                (acc[i][j + kCols][4 * q + e] + bu[e]));
-        *C::at(chunk, lane, j, q) = h;
-      }
-    vkd::wave_lds_fence();
-    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
-                             n0 + T::b_row(wn, 0), g.N);
-    vkd::wave_lds_fence();
-  }
+          for (int e = 0; e < 4; ++e)
+            h[e] = static_cast<V>(vkp::gate<act.value>(acc[i][j][4 * q + e] + bg[e]) *
+                                  (acc[i][j + kCols][4 * q + e] + bu[e]));
+          *C::at(chunk, lane, j, q) = h;
+        }
+      vkd::wave_lds_fence();
+      C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
+                               n0 + T::b_row(wn, 0), g.N);
+      vkd::wave_lds_fence();
+    }
+  });
 }
 
 // Step 1 of the backward.
@@ -125,63 +116,65 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   V* d = static_cast<V*>(g.d);
   const size_t pitch = 2 * static_cast<size_t>(g.d_half);
   const int nb = n0 + T::b_row(wn, 0);
-  vkp::i32x4 dh[C::kFetch];
-  C::fetch(dh, lane, grad, g.N, m0 + wm * T::MT * 32, g.M, nb, g.N);
   float sum[kCols] = {};
+  vkp::with_act(g.act, [&](auto act) {
+    vkp::i32x4 dh[C::kFetch];
+    C::fetch(dh, lane, grad, g.N, m0 + wm * T::MT * 32, g.M, nb, g.N);
 #pragma unroll
-  for (int i = 0; i < T::MT; ++i) {
-    const int mb = m0 + (wm * T::MT + i) * 32;
-    C::fill(chunk, lane, dh);
-    if (i + 1 < T::MT) C::fetch(dh, lane, grad, g.N, mb + 32, g.M, nb, g.N);
-    vkd::wave_lds_fence();
-    // rows past M and columns past N have dh of 0; what their g and u are is finite only where
-    // the others' are
-    const bool in = mb + (lane & 31) < g.M;
-    typename C::V4 du[kCols][4];
-    float v[kCols * 32];
-#pragma unroll
-    for (int j = 0; j < kCols; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
-        const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
-        const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
-        typename C::V4* at = C::at(chunk, lane, j, q);
-        const typename C::V4 h4 = *at;
-        typename C::V4 dg;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          float a, s;
-          slope_any(g.act, acc[i][j][4 * q + e] + bg[e], &a, &s);
-          const float h = vkp::widen(h4[e]);
-          const bool held = in && n0 + c + e < g.N;
-          const float fg = held ? h * (acc[i][j + kCols][4 * q + e] + bu[e]) * s : 0.0f;
-          const float fu = held ? h * a : 0.0f;
-          v[j * 16 + 4 * q + e] = fg;
-          v[kCols * 16 + j * 16 + 4 * q + e] = fu;
-          dg[e] = static_cast<V>(fg);
-          du[j][q][e] = static_cast<V>(fu);
-        }
-        *at = dg;
-      }
-    if (g.sums) {
-      vkp::sum_rows<kCols>(v, lane);
-#pragma unroll
-      for (int k = 0; k < kCols; ++k) sum[k] += v[k];
-    }
-    if (d) {
+    for (int i = 0; i < T::MT; ++i) {
+      const int mb = m0 + (wm * T::MT + i) * 32;
+      C::fill(chunk, lane, dh);
+      if (i + 1 < T::MT) C::fetch(dh, lane, grad, g.N, mb + 32, g.M, nb, g.N);
       vkd::wave_lds_fence();
-      C::template store<false>(chunk, lane, d, pitch, mb, g.M, nb, g.d_half);
-      vkd::wave_lds_fence();
+      // rows past M and columns past N have dh of 0; what their g and u are is finite only where
+      // the others' are
+      const bool in = mb + (lane & 31) < g.M;
+      typename C::V4 du[kCols][4];
+      float v[kCols * 32];
 #pragma unroll
       for (int j = 0; j < kCols; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) *C::at(chunk, lane, j, q) = du[j][q];
+        for (int q = 0; q < 4; ++q) {
+          const int c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+          const vkp::f32x4 bg = *reinterpret_cast<const vkp::f32x4*>(bias + c);
+          const vkp::f32x4 bu = *reinterpret_cast<const vkp::f32x4*>(bias + T::kHeld + c);
+          typename C::V4* at = C::at(chunk, lane, j, q);
+          const typename C::V4 h4 = *at;
+          typename C::V4 dg;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            float a, s;
+            vkp::gate_slope<act.value>(acc[i][j][4 * q + e] + bg[e], &a, &s);
+            const float h = vkp::widen(h4[e]);
+            const bool held = in && n0 + c + e < g.N;
+            const float fg = held ? h * (acc[i][j + kCols][4 * q + e] + bu[e]) * s : 0.0f;
+            const float fu = held ? h * a : 0.0f;
+            v[j * 16 + 4 * q + e] = fg;
+            v[kCols * 16 + j * 16 + 4 * q + e] = fu;
+            dg[e] = static_cast<V>(fg);
+            du[j][q][e] = static_cast<V>(fu);
+          }
+          *at = dg;
+        }
+      if (g.sums) {
+        vkp::sum_rows<kCols>(v, lane);
+#pragma unroll
+        for (int k = 0; k < kCols; ++k) sum[k] += v[k];
+      }
+      if (d) {
+        vkd::wave_lds_fence();
+        C::template store<false>(chunk, lane, d, pitch, mb, g.M, nb, g.d_half);
+        vkd::wave_lds_fence();
+#pragma unroll
+        for (int j = 0; j < kCols; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) *C::at(chunk, lane, j, q) = du[j][q];
+        vkd::wave_lds_fence();
+        C::template store<false>(chunk, lane, d + g.d_half, pitch, mb, g.M, nb, g.d_half);
+      }
       vkd::wave_lds_fence();
-      C::template store<false>(chunk, lane, d + g.d_half, pitch, mb, g.M, nb, g.d_half);
     }
-    vkd::wave_lds_fence();
-  }
+  });
   if (g.sums) {
     // value k of lane l: columns of dg, then of du, by j, q, e
 #pragma unroll
@@ -248,7 +241,9 @@ __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
     if (m >= g.M || n >= g.N) continue;
     const float gate = vkp::few_sum<KIND, RT, true>(smem, 0, m, e & 15) + bias_at<KIND>(g, n);
     const float up = vkp::few_sum<KIND, RT, true>(smem, 1, m, e & 15) + bias_at<KIND>(g, g.N + n);
-    static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(gate_any(g.act, gate) * up);
+    vkp::with_act(g.act, [&](auto act) {
+      static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(vkp::gate<act.value>(gate) * up);
+    });
   }
 }
 

@@ -179,11 +179,7 @@ __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict
 // The channel's scale first: a row's largest scale then overflows only where the result
 // does.
 __device__ __forceinline__ float linear_of(int acc, float channel, float row, float bias) {
-  return static_cast<float>(acc) * channel * row + bias;
-}
-
-__device__ __forceinline__ float gated_of(int act, float gate, float up) {
-  return (act == VK_GATE_SILU ? vkp::gate<VK_GATE_SILU>(gate) : vkp::gate<VK_GATE_GELU>(gate)) * up;
+  return __builtin_fmaf(static_cast<float>(acc) * channel, row, bias);
 }
 
 template <int END>
@@ -218,45 +214,49 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   static_assert(T::kWaves * C::kBytes <= T::kBytes, "the chunks fit a stage buffer");
   char* chunk = stages_[0] + wave * C::kBytes;
   V* out = static_cast<V*>(g.out);
+  const auto leave = [&](auto act) {
 #pragma unroll
-  for (int i = 0; i < T::MT; ++i) {
-    const int mb = m0 + (wm * T::MT + i) * 32, m = mb + (lane & 31);
-    const float row = g.sx[m < g.M ? m : g.M - 1];
+    for (int i = 0; i < T::MT; ++i) {
+      const int mb = m0 + (wm * T::MT + i) * 32, m = mb + (lane & 31);
+      const float row = g.sx[m < g.M ? m : g.M - 1];
 #pragma unroll
-    for (int jg = 0; jg < kCols; jg += J) {
+      for (int jg = 0; jg < kCols; jg += J) {
 #pragma unroll
-      for (int jj = 0; jj < J; ++jj)
+        for (int jj = 0; jj < J; ++jj)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int j = jg + jj, c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
-          const float4 s = *reinterpret_cast<const float4*>(&cols[0][c]);
-          const float4 b = *reinterpret_cast<const float4*>(&cols[1][c]);
-          const float4 l = *reinterpret_cast<const float4*>(&cols[2][c]);
-          float v[4] = {linear_of(acc[i][j][4 * q], s.x, row, b.x),
-                        linear_of(acc[i][j][4 * q + 1], s.y, row, b.y),
-                        linear_of(acc[i][j][4 * q + 2], s.z, row, b.z),
-                        linear_of(acc[i][j][4 * q + 3], s.w, row, b.w)};
-          const float ls[4] = {l.x, l.y, l.z, l.w};
-          if constexpr (T::PAIRED) {
-            const float4 us = *reinterpret_cast<const float4*>(&cols[0][c + T::kHeld]);
-            const float4 ub = *reinterpret_cast<const float4*>(&cols[1][c + T::kHeld]);
-            const float u[4] = {linear_of(acc[i][j + kCols][4 * q], us.x, row, ub.x),
-                                linear_of(acc[i][j + kCols][4 * q + 1], us.y, row, ub.y),
-                                linear_of(acc[i][j + kCols][4 * q + 2], us.z, row, ub.z),
-                                linear_of(acc[i][j + kCols][4 * q + 3], us.w, row, ub.w)};
+          for (int q = 0; q < 4; ++q) {
+            const int j = jg + jj, c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
+            const auto at = [&](int p, int c_) { return *reinterpret_cast<const vkp::f32x4*>(&cols[p][c_]); };
+            const vkp::f32x4 s = at(0, c), b = at(1, c);
+            vkp::f32x4 v;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = gated_of(g.act, v[e], u[e]);
+            for (int e = 0; e < 4; ++e) v[e] = linear_of(acc[i][j][4 * q + e], s[e], row, b[e]);
+            if constexpr (T::PAIRED) {
+              const vkp::f32x4 us = at(0, c + T::kHeld), ub = at(1, c + T::kHeld);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                v[e] = vkp::gate<act.value>(v[e]) *
+                       linear_of(acc[i][j + kCols][4 * q + e], us[e], row, ub[e]);
+            } else {
+              const vkp::f32x4 l = at(2, c);
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = finish<END>(v[e], l[e]);
+            }
+            typename C::V4 w;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(v[e]);
+            *C::at(chunk, lane, jj, q) = w;
           }
-          typename C::V4 w;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(finish<END>(v[e], ls[e]));
-          *C::at(chunk, lane, jj, q) = w;
-        }
-      vkd::wave_lds_fence();
-      C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N);
-      vkd::wave_lds_fence();
+        vkd::wave_lds_fence();
+        C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N);
+        vkd::wave_lds_fence();
+      }
     }
-  }
+  };
+  if constexpr (END == kGated)
+    vkp::with_act(g.act, leave);
+  else
+    leave(std::integral_constant<int, 0>{});
 }
 
 // What leaves after the waves' sums are joined: thread by thread.
@@ -272,10 +272,11 @@ __device__ __forceinline__ void few_finish(const Args& g, const char* smem, int 
                         g.bias ? g.bias[n] : 0.0f);
     if constexpr (kPaired) {
       const int p = g.N + n;
-      v = gated_of(g.act, v, linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15), g.sw[p], row,
-                                       g.bias ? g.bias[p] : 0.0f));
+      const float u = linear_of(vkp::few_sum<kI8, RT, true>(smem, 1, m, e & 15), g.sw[p], row,
+                                g.bias ? g.bias[p] : 0.0f);
+      vkp::with_act(g.act, [&](auto act) { v = vkp::gate<act.value>(v) * u; });
     }
-    v = finish<END>(v, g.ls ? g.ls[n] : 1.0f);
+    if constexpr (!kPaired) v = finish<END>(v, g.ls ? g.ls[n] : 1.0f);
     if constexpr (END == kResidual) v = *to + v;
     *to = static_cast<V>(v);
   }

@@ -588,6 +588,16 @@ __device__ __forceinline__ void gate_slope(float g, float* act, float* slope) {
   }
 }
 
+// f(std::integral_constant<int, ACT>) for the activation of a launch: one branch, so that the values of a
+// tile's end overlap one another's latencies.
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F f) {
+  if (act == VK_GATE_SILU)
+    f(std::integral_constant<int, VK_GATE_SILU>{});
+  else
+    f(std::integral_constant<int, VK_GATE_GELU>{});
+}
+
 // ---------------------------------------------------------------- 16-bit values
 __device__ __forceinline__ float widen(float v) { return v; }
 __device__ __forceinline__ float widen(_Float16 v) { return static_cast<float>(v); }

@@ -13,7 +13,8 @@
 //      operands.  Written as rows dg | du, with the f32 column sums of each tile;
 //   2. dx = [dg du] [Wg; Wu], w's lines being k;
 //   3. dw = [dg du]^T x, the lines of both being k;
-//   4. db: the tiles' column sums added in order.
+//   4. db: the tiles' column sums added in order;
+// the last three in one launch.
 #include "product_nt.h"
 
 namespace {
@@ -31,7 +32,7 @@ struct Args {
   void* out;         // [M, N]; null in the backward
   void* d;           // dg | du, rows of 2 d_half values, zeros from N to d_half of each half
   float* sums;       // [gm * WM, 2 N], or null
-  int d_half, m_half;
+  int d_half;
   int M, N;
   int act;
   int gm, gn, group;
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
   VK_STAGES(T);
   __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
-  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
@@ -101,7 +102,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   VK_STAGES(T);
   __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
-  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
@@ -186,15 +187,22 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   }
 }
 
-// out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a as rows or columns, b as columns.  With
-// m_half > 0 a's rows come in two halves: row m < m_half is out's m where that is below M / 2, row m
-// >= m_half out's M / 2 + m - m_half where that is below M.
+// One of the products of steps 2 and 3: out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a as
+// rows or columns, b as columns.  With m_half > 0 a's rows come in two halves: row m < m_half is out's
+// m where that is below M / 2, row m >= m_half out's M / 2 + m - m_half where that is below M.
+struct Product {
+  Operand a, b;
+  int k_bytes;
+  void* out;
+  int M, N, m_half;
+  int gm, gn, group;
+};
+
 template <Kind KIND, typename T, bool AC>
-__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Args g) {
+__device__ __forceinline__ void product(const Product& g, int tile, char* const (&stages_)[5]) {
   typedef typename vkp::Value<KIND>::type V;
-  VK_STAGES(T);
   int mt, nt;
-  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::TN;
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
@@ -229,6 +237,50 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void product_kernel(Ar
   }
 }
 
+// dbias: the tiles' sums of sixteen columns, eight runs of parts each in order, then the runs in order.
+struct BiasSums {
+  const float* sums;  // [parts, cols]
+  int parts, cols;
+  void* out;
+};
+
+template <Kind KIND>
+__device__ __forceinline__ void bias_gradient(const BiasSums& g, int block, char* smem) {
+  float(*run)[16] = reinterpret_cast<float(*)[16]>(smem);
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = block * 16 + x;
+  if (y < 8) {
+    const int from = g.parts * y / 8, to = g.parts * (y + 1) / 8;
+    float s = 0.0f;
+    if (c < g.cols)
+#pragma unroll 8
+      for (int p = from; p < to; ++p) s += g.sums[static_cast<size_t>(p) * g.cols + c];
+    run[y][x] = s;
+  }
+  __syncthreads();
+  if (y > 0 || c >= g.cols) return;
+  float s = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s += run[i][x];
+  static_cast<typename vkp::Value<KIND>::type*>(g.out)[c] =
+      static_cast<typename vkp::Value<KIND>::type>(s);
+}
+
+// Steps 2 to 4 in one launch: they need the same step before them, and few rows leave the card
+// half empty one after another.  Workgroups 0 .. n_bias are dbias, the next n_dx dx, the others dw.
+template <Kind KIND, typename T>
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gradients_kernel(Product dx, Product dw,
+                                                                              BiasSums bias, int n_bias,
+                                                                              int n_dx) {
+  VK_STAGES(T);
+  const int wg = blockIdx.x;
+  if (wg < n_bias)
+    bias_gradient<KIND>(bias, wg, stages_[0]);
+  else if (wg < n_bias + n_dx)
+    product<KIND, T, false>(dx, wg - n_bias, stages_);
+  else
+    product<KIND, T, true>(dw, wg - n_bias - n_dx, stages_);
+}
+
 // Forward of at most 16 RT rows.
 template <Kind KIND, int RT>
 __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
@@ -248,12 +300,21 @@ __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
 }
 
 // ---------------------------------------------------------------- layouts
-// Rows of `cols` 16-bit values into rows of `pitch` (a multiple of 8), zeros behind.
-__global__ __launch_bounds__(256) void pad16_kernel(const uint16_t* __restrict__ from, int cols,
-                                                    uint16_t* __restrict__ to, int pitch) {
-  const size_t r = blockIdx.x;
-  for (int c = threadIdx.x; c < pitch; c += 256)
-    to[r * pitch + c] = c < cols ? from[r * cols + c] : uint16_t{0};
+// Rows of x, then of w, of `cols` 16-bit values into rows of 8 `pieces`, zeros behind.
+__global__ __launch_bounds__(256) void pad16_kernel(const char* __restrict__ x, const char* __restrict__ w,
+                                                    size_t x_rows, size_t rows, int cols, int pieces,
+                                                    char* __restrict__ to) {
+  const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
+  const size_t row = i / static_cast<unsigned>(pieces);
+  if (row >= rows) return;
+  const int piece = static_cast<int>(i - row * static_cast<unsigned>(pieces));
+  const char* from = row < x_rows ? x + row * 2 * cols : w + (row - x_rows) * 2 * cols;
+  vkp::i32x4 v = {0, 0, 0, 0};
+  if (16 * piece + 16 <= 2 * cols)
+    __builtin_memcpy(&v, from + 16 * piece, 16);
+  else if (16 * piece < 2 * cols)
+    v = vkp::row_rest(from, 2 * cols);
+  *reinterpret_cast<vkp::i32x4*>(to + i * 16) = v;
 }
 
 __global__ __launch_bounds__(256) void zero16_kernel(uint16_t* to, size_t n) {
@@ -264,28 +325,6 @@ __global__ __launch_bounds__(256) void zero16_kernel(uint16_t* to, size_t n) {
 void zero16(const vk_runtime* rt, void* p, size_t n) {
   hipLaunchKernelGGL(zero16_kernel, dim3((n + 255) / 256), dim3(256), 0, rt->stream,
                      static_cast<uint16_t*>(p), n);
-}
-
-// dbias[c] = sum over the tiles' sums: sixteen runs of parts a column, each in order, then the
-// runs in order.
-template <Kind KIND>
-__global__ __launch_bounds__(256) void bias_grad_kernel(const float* __restrict__ sums, int parts,
-                                                        int cols, void* out) {
-  __shared__ float run[16][16];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
-  const int from = parts * y / 16, to = parts * (y + 1) / 16;
-  float s = 0.0f;
-  if (c < cols)
-#pragma unroll 8
-    for (int p = from; p < to; ++p) s += sums[static_cast<size_t>(p) * cols + c];
-  run[y][x] = s;
-  __syncthreads();
-  if (y > 0 || c >= cols) return;
-  s = 0.0f;
-#pragma unroll
-  for (int i = 0; i < 16; ++i) s += run[i][x];
-  static_cast<typename vkp::Value<KIND>::type*>(out)[c] =
-      static_cast<typename vkp::Value<KIND>::type>(s);
 }
 
 // ---------------------------------------------------------------- launches
@@ -321,39 +360,10 @@ int launch_forward(vk_runtime* rt, Args& g) {
   return vk::check_launch("gated_kernel");
 }
 
-// out [M, N] from a.rows rows of a (in halves, where m_half > 0) and b's columns.
-template <Kind KIND, bool AC>
-int launch_product(vk_runtime* rt, const Operand& a, const Operand& b, size_t k, size_t M, size_t N,
-                   size_t m_half, void* out) {
-  Args g{};
-  g.a = a;
-  g.b = b;
-  g.k_bytes = static_cast<int>(2 * k);
-  g.out = out;
-  g.M = static_cast<int>(M);
-  g.N = static_cast<int>(N);
-  g.m_half = static_cast<int>(m_half);
-  const vkp::Plan p = vkp::plan(rt->cu_count, a.rows, g.N, g.k_bytes);
-  with_tile<false>(p.tile, g, [&](auto tile) {
-    typedef decltype(tile) T;
-    g.gm = (a.rows + T::TM - 1) / T::TM;
-    hipLaunchKernelGGL((product_kernel<KIND, T, AC>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
-                       rt->stream, g);
-  });
-  return vk::check_launch("product_kernel");
-}
-
-// A tensor's rows as an operand: as they are, or where a row is no multiple of 16
-// bytes, copied into `room` with zeros behind (room null: says how many bytes that takes).
-size_t operand_room(size_t rows, size_t cols) { return cols % 8 == 0 ? 0 : rows * padded(cols) * 2; }
-
-Operand as_operand(const vk_runtime* rt, const void* p, size_t rows, size_t cols, char* room) {
-  if (cols % 8 == 0)
-    return Operand{static_cast<const char*>(p), static_cast<int>(rows), static_cast<uint32_t>(2 * cols)};
-  hipLaunchKernelGGL(pad16_kernel, dim3(rows), dim3(256), 0, rt->stream,
-                     static_cast<const uint16_t*>(p), static_cast<int>(cols),
-                     reinterpret_cast<uint16_t*>(room), static_cast<int>(padded(cols)));
-  return Operand{room, static_cast<int>(rows), static_cast<uint32_t>(2 * padded(cols))};
+// x's and w's rows as operands: as they are, or where a row is no multiple of 16 bytes, copied into the
+// work buffer with zeros behind.
+size_t operands_room(size_t rows, size_t in, size_t hidden) {
+  return in % 8 == 0 ? 0 : (rows + 2 * hidden) * padded(in) * 2;
 }
 
 template <Kind KIND>
@@ -382,24 +392,50 @@ int backward(vk_runtime* rt, Args& g, size_t rows, size_t in, size_t hidden, cha
   const char* d = static_cast<char*>(g.d);
   const auto pitch = static_cast<uint32_t>(4 * half);
   const int R = static_cast<int>(rows), values = static_cast<int>((in + 7) / 8 * 8);
+  const int D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden), both = static_cast<int>(2 * half);
+  Product x{}, w{};
   if (dx) {
-    Operand lines = g.b;  // w's lines are k
-    lines.rows = values;
-    lines.ks = static_cast<int>(2 * hidden);
-    lines.k_half = static_cast<int>(half);
-    VK_TRY((launch_product<KIND, false>(rt, Operand{d, R, pitch}, lines, 2 * half, rows, in, 0, dx->ptr)));
+    x.a = Operand{d, R, pitch};
+    x.b = g.b;  // w's lines are k
+    x.b.rows = values;
+    x.b.ks = H2;
+    x.b.k_half = static_cast<int>(half);
+    x.k_bytes = 2 * both;
+    x.out = dx->ptr;
+    x.M = R;
+    x.N = D;
   }
   if (dw) {
-    Operand lines = g.a;
-    lines.rows = values;
-    lines.ks = R;
-    VK_TRY((launch_product<KIND, true>(rt, Operand{d, static_cast<int>(2 * half), pitch, R}, lines, rows,
-                                       2 * hidden, in, half, dw->ptr)));
+    w.a = Operand{d, both, pitch, R};
+    w.b = g.a;  // x's lines are k
+    w.b.rows = values;
+    w.b.ks = R;
+    w.k_bytes = 2 * R;
+    w.out = dw->ptr;
+    w.M = H2;
+    w.N = D;
+    w.m_half = static_cast<int>(half);
   }
-  if (dbias) {
-    hipLaunchKernelGGL(bias_grad_kernel<KIND>, dim3((2 * hidden + 15) / 16), dim3(256), 0, rt->stream,
-                       g.sums, parts, static_cast<int>(2 * hidden), dbias->ptr);
-    VK_TRY(vk::check_launch("bias_grad_kernel"));
+  BiasSums sums{g.sums, parts, H2, dbias ? dbias->ptr : nullptr};
+  const int n_bias = dbias ? (H2 + 15) / 16 : 0;
+  const vkp::PlanTwo plan = vkp::plan_two(rt->cu_count, vkp::Shape{dx ? R : 0, D, x.k_bytes},
+                                          vkp::Shape{dw ? both : 0, D, w.k_bytes});
+  // one launch, or dx in one of its own
+  for (int part = plan.together ? 1 : 0; part < 2; ++part) {
+    vkp::with_tile<false>(part == 0 ? plan.first : plan.second, [&](auto tile) {
+      typedef decltype(tile) T;
+      for (Product* p : {&x, &w}) {
+        p->gm = (p->a.rows + T::TM - 1) / T::TM;
+        p->gn = (p->N + T::TN - 1) / T::TN;
+        p->group = vkp::kGroupRows / T::TM;
+      }
+      const int n_dx = part == 0 || plan.together ? x.gm * x.gn : 0;
+      const int biases = part == 0 ? 0 : n_bias, grid = biases + n_dx + (part == 0 ? 0 : w.gm * w.gn);
+      if (grid > 0)
+        hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(grid), dim3(T::kThreads), 0, rt->stream, x, w,
+                           sums, biases, n_dx);
+    });
+    VK_TRY(vk::check_launch("gradients_kernel"));
   }
   return VK_OK;
 }
@@ -432,18 +468,32 @@ int check_inputs(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const v
 }
 
 Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
-                  size_t rows, size_t in, size_t hidden, int act, char** room) {
+                  size_t rows, size_t in, size_t hidden, int act) {
   Args g{};
-  g.a = as_operand(rt, x->ptr, rows, in, *room);
-  *room += operand_room(rows, in);
-  g.b = as_operand(rt, w->ptr, 2 * hidden, in, *room);
-  *room += operand_room(2 * hidden, in);
+  const char* xp = static_cast<const char*>(x->ptr);
+  const char* wp = static_cast<const char*>(w->ptr);
+  const auto pitch = static_cast<uint32_t>(2 * in);
+  g.a = Operand{xp, static_cast<int>(rows), pitch};
+  g.b = Operand{wp, static_cast<int>(2 * hidden), pitch};
   g.k_bytes = static_cast<int>(2 * in);
   g.bias = bias ? bias->ptr : nullptr;
   g.M = static_cast<int>(rows);
   g.N = static_cast<int>(hidden);
   g.act = act;
   return g;
+}
+
+// The tiles' operands: 16-byte aligned rows.
+int align_operands(const vk_runtime* rt, Args& g, size_t in, char* room) {
+  if (in % 8 == 0) return VK_OK;
+  const size_t rows = g.a.rows, all = rows + g.b.rows, pieces = padded(in) / 8;
+  VK_UNSUPPORTED_IF(all * pieces > 0x7fffffULL * 256, "gated: %zu rows of %zu", all, in);
+  hipLaunchKernelGGL(pad16_kernel, dim3((all * pieces + 255) / 256), dim3(256), 0, rt->stream, g.a.base,
+                     g.b.base, rows, all, static_cast<int>(in), static_cast<int>(pieces), room);
+  g.a.pitch = g.b.pitch = static_cast<uint32_t>(2 * padded(in));
+  g.a.base = room;
+  g.b.base = room + rows * g.a.pitch;
+  return vk::check_launch("pad16_kernel");
 }
 
 }  // namespace
@@ -457,12 +507,12 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, con
   VK_TRY(check16(rt, out, x->dtype, rows * hidden, "out"));
   for (const vk_tensor* t : {x, w, bias}) VK_REQUIRE(!vk::overlap(out, t), "gated: out overlaps an input");
   if (rows == 0) return VK_OK;
-  const size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features);
-  if (need > 0) VK_TRY(vk::ensure_work(rt, need / 4, "gated_forward"));
-  char* room = reinterpret_cast<char*>(rt->work);
-  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation, &room);
-  VK_TRY(vk::check_launch("pad16_kernel"));
+  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
   g.out = out->ptr;
+  if (rows > vkp::kFewRows && in_features % 8 != 0) {
+    VK_TRY(vk::ensure_work(rt, operands_room(rows, in_features, hidden) / 4, "gated_forward"));
+    VK_TRY(align_operands(rt, g, in_features, reinterpret_cast<char*>(rt->work)));
+  }
   return x->dtype == VK_F16 ? launch_forward<kF16>(rt, g) : launch_forward<kBF16>(rt, g);
 }
 
@@ -487,17 +537,19 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
     if (dbias) zero16(rt, dbias->ptr, dbias->len);
     return vk::check_launch("zero16_kernel");
   }
-  size_t need = operand_room(rows, in_features) + operand_room(2 * hidden, in_features) + 2 * 256;
+  const size_t room = operands_room(rows, in_features, hidden);
+  size_t need = room + 2 * 256;
   if (dx || dw) need += rows * padded(hidden) * 4;
   if (dbias) need += ((rows + 63) / 64 * 2) * 2 * hidden * 4;
   VK_TRY(vk::ensure_work(rt, (need + 3) / 4, "gated_backward"));
-  char* room = reinterpret_cast<char*>(rt->work);
-  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation, &room);
-  VK_TRY(vk::check_launch("pad16_kernel"));
+  char* work = reinterpret_cast<char*>(rt->work);
+  Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
+  VK_TRY(align_operands(rt, g, in_features, work));
+  work += room;
   g.grad = grad->ptr;
   return x->dtype == VK_F16
-             ? backward<kF16>(rt, g, rows, in_features, hidden, room, dx, dw, dbias)
-             : backward<kBF16>(rt, g, rows, in_features, hidden, room, dx, dw, dbias);
+             ? backward<kF16>(rt, g, rows, in_features, hidden, work, dx, dw, dbias)
+             : backward<kBF16>(rt, g, rows, in_features, hidden, work, dx, dw, dbias);
 }
 
 }  // extern "C"

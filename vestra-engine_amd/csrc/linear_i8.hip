@@ -194,7 +194,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   VK_STAGES(T);
   __shared__ __align__(16) float cols[3][T::TN];  // scale, bias, LayerScale of the tile's columns
   int mt, nt;
-  vkp::tile_at(g.gm, g.gn, g.group, &mt, &nt);
+  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   for (int c = threadIdx.x; c < T::TN; c += T::kThreads) {
     const int n = n0 + c % T::kHeld;
@@ -292,8 +292,9 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g)
   few_finish<END, V, RT>(g, smem, n0, g.sx);
 }
 
-// A row or a few, of at most kRowBytes of codes: every workgroup quantises them for itself, in one
-// launch, while its weights are on their way.
+// Rows of at most kOwnBytes of codes in all: every workgroup quantises them for itself, in one
+// launch, while its weights are on their way.  Thread by thread eight values; sixteen lanes are of one
+// row, whose maximum meets in LDS.
 template <typename XT>
 __device__ __forceinline__ void load8_of(const Args& g, int m, int at, float (&v)[8]) {
   load8(static_cast<const XT*>(g.x) + static_cast<size_t>(m) * g.K, at, g.K - at, v);
@@ -302,50 +303,59 @@ __device__ __forceinline__ void load8_of(const Args& g, int m, int at, float (&v
 template <int END, typename V>
 __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g) {
   constexpr bool kPaired = END == kGated;
-  constexpr int kPitch = vkp::kOwnBytes + 16;  // rows start in different banks
+  constexpr int kEights = vkp::kOwnBytes / 8 / vkp::kFewThreads;  // of a thread
   __shared__ __align__(16) char smem[vkp::few_bytes<kI8, 1, kPaired>()];
-  __shared__ __align__(16) char codes[vkp::kOwnRows * kPitch];
-  __shared__ uint32_t tops[vkp::kOwnRows][vkp::kFewWaves];
+  __shared__ __align__(16) char codes[vkp::kOwnBytes + 16 * vkp::kOwnRows];
+  __shared__ uint32_t tops[vkp::kOwnRows];
   __shared__ float scales[vkp::kOwnRows];
   const int n0 = blockIdx.x * 16, tid = threadIdx.x, c = tid & 15;
-  static_assert(vkp::kOwnBytes <= 8 * vkp::kFewThreads, "eight values a thread");
+  const int pitch = g.k_bytes + 16;  // rows start in different banks
+  if (tid < vkp::kOwnRows) tops[tid] = 0;
   vkp::few_product<kI8, 1, kPaired>(
       g.b, g.k_bytes, n0, smem,
       [&] {
-        float v[vkp::kOwnRows][8];
+        float v[kEights][8];
+        int m[kEights], at[kEights];
+        const int eights = g.k_bytes / 8;
 #pragma unroll
-        for (int m = 0; m < vkp::kOwnRows; ++m)
-          if (m < g.M) {
-            if (g.x_type == VK_F32) load8_of<float>(g, m, 8 * tid, v[m]);
-            else if (g.x_type == VK_F16) load8_of<_Float16>(g, m, 8 * tid, v[m]);
-            else load8_of<__bf16>(g, m, 8 * tid, v[m]);
-          }
+        for (int i = 0; i < kEights; ++i) {
+          const int e = tid + i * vkp::kFewThreads;
+          m[i] = e / eights;
+          at[i] = (e - m[i] * eights) * 8;
+          if (m[i] >= g.M) continue;
+          if (g.x_type == VK_F32) load8_of<float>(g, m[i], at[i], v[i]);
+          else if (g.x_type == VK_F16) load8_of<_Float16>(g, m[i], at[i], v[i]);
+          else load8_of<__bf16>(g, m[i], at[i], v[i]);
+        }
+        __syncthreads();  // the maxima are cleared
 #pragma unroll
-        for (int m = 0; m < vkp::kOwnRows; ++m)
-          if (m < g.M) {
-            const uint32_t top = wave_umax(top_of(v[m], 0));
-            if ((tid & 63) == 0) tops[m][tid >> 6] = top;
+        for (int i = 0; i < kEights; ++i) {
+          if (m[i] >= g.M) continue;
+          uint32_t top = top_of(v[i], 0);
+#pragma unroll
+          for (int d = 8; d > 0; d >>= 1) {
+            const uint32_t o = static_cast<uint32_t>(__shfl_xor(static_cast<int>(top), d, 16));
+            top = o > top ? o : top;
           }
+          if (c == 0) atomicMax(&tops[m[i]], top);
+        }
         __syncthreads();
 #pragma unroll
-        for (int m = 0; m < vkp::kOwnRows; ++m)
-          if (m < g.M) {
-            uint32_t top = tops[m][0];
-#pragma unroll
-            for (int w = 1; w < vkp::kFewWaves; ++w) top = max(top, tops[m][w]);
-            const RowScale s = row_scale(top);
-            if (8 * tid < g.k_bytes)
-              *reinterpret_cast<uint2*>(codes + m * kPitch + 8 * tid) =
-                  make_uint2(codes_of(v[m], s), codes_of(v[m] + 4, s));
-            if (tid == 0) scales[m] = s.scale;
-          }
+        for (int i = 0; i < kEights; ++i) {
+          if (m[i] >= g.M) continue;
+          const RowScale s = row_scale(tops[m[i]]);
+          *reinterpret_cast<uint2*>(codes + m[i] * pitch + at[i]) =
+              make_uint2(codes_of(v[i], s), codes_of(v[i] + 4, s));
+          if (at[i] == 0) scales[m[i]] = s.scale;
+        }
         __syncthreads();
       },
       [&](int, int k) {
         vkp::i32x4 a = {0, 0, 0, 0};
-        if (c < g.M && k < g.k_bytes) a = *reinterpret_cast<const vkp::i32x4*>(codes + c * kPitch + k);
+        if (c < g.M && k < g.k_bytes) a = *reinterpret_cast<const vkp::i32x4*>(codes + c * pitch + k);
         return a;
-      });
+      },
+      [](int) { return vkp::i32x4{0, 0, 0, 0}; });
   few_finish<END, V, 1>(g, smem, n0, scales);
 }
 

@@ -549,10 +549,10 @@ __device__ __forceinline__ void sum_rows(float* v, int lane) {
   halve<R, 0xb1>(v, lane & 1);       // quad_perm 1, 0, 3, 2
 }
 
-// The tile of workgroup t, XCD-major in groups of rows that a 4 MiB L2 holds together
+// Tile `tile` of a product, XCD-major in groups of rows that a 4 MiB L2 holds together
 // with the columns being walked: in a group, rows fastest.
-__device__ __forceinline__ void tile_at(int gm, int gn, int group, int* mt, int* nt) {
-  const int t = vkd::xcd_tile(blockIdx.x, gridDim.x);
+__device__ __forceinline__ void tile_at(int tile, int gm, int gn, int group, int* mt, int* nt) {
+  const int t = vkd::xcd_tile(tile, gm * gn);
   const int per = group * gn;
   const int g = t / per, r = t - g * per;
   const int left = gm - g * group, rows = left < group ? left : group;
@@ -627,38 +627,44 @@ struct FewSums {
   typename Ops<KIND>::Acc4 v[PAIRED ? 2 : 1][RT];
 };
 
+// The 16 bytes of a row from byte k, zeros where they are not all below `whole`, the row's whole pieces (one
+// at least).  The row may lie at any address.  No branch: a load in one would be waited for there.
+__device__ __forceinline__ i32x4 row_piece(const char* row, int k, int whole) {
+  i32x4 v;
+  const bool in = k < whole;
+  __builtin_memcpy(&v, row + (in ? k : 0), 16);
+  return in ? v : i32x4{0, 0, 0, 0};
+}
+
+// The 16-bit values behind a row's whole pieces, zeros from its end on.
+__device__ __forceinline__ i32x4 row_rest(const char* row, int k_bytes) {
+  uint16_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = (k_bytes & ~15) + 2 * i;
+    uint16_t v;
+    __builtin_memcpy(&v, row + (k < k_bytes ? k : 0), 2);
+    e[i] = k < k_bytes ? v : uint16_t{0};
+  }
+  i32x4 v;
+  __builtin_memcpy(&v, e, 16);
+  return v;
+}
+
 // Loads of b for U stages t, t + 8, ...: zeros past k and past the last stage.
 template <bool PAIRED, int U>
 struct FewColumns {
   i32x4 v[U][PAIRED ? 2 : 1][2];
-  __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t rb, const uint32_t (&at)[2], int q,
-                                       int t, int k_bytes) {
+  __device__ __forceinline__ void load(const char* const (&row)[2], int q, int t, int whole) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int p = 0; p < (PAIRED ? 2 : 1); ++p)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int k = (t + u * kFewWaves) * kStage + q * 32 + h * 16;
-          v[u][p][h] = __builtin_bit_cast(
-              i32x4, vkd::buffer_load4(rb, k < k_bytes ? at[p] + static_cast<uint32_t>(k) : kOutside, 0));
-        }
+        for (int h = 0; h < 2; ++h)
+          v[u][p][h] = row_piece(row[p], (t + u * kFewWaves) * kStage + q * 32 + h * 16, whole);
   }
 };
-
-// The resource and the lane's row offsets of the columns n0 .. n0 + 16.  Columns past
-// the last one read the last one.
-template <bool PAIRED>
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t few_rows_of(const Operand& b, int n0, int c,
-                                                              uint32_t (&at)[2]) {
-  const int held = PAIRED ? b.rows / 2 : b.rows;
-  const int n = n0 + c < held ? c : held - 1 - n0;
-  at[0] = static_cast<uint32_t>(n) * b.pitch;
-  at[1] = static_cast<uint32_t>(n + (PAIRED ? held : 0)) * b.pitch;
-  const size_t from = static_cast<size_t>(n0) * b.pitch;
-  const size_t left = static_cast<size_t>(b.rows) * b.pitch - from;
-  return vkd::buffer_rsrc(b.base + from, left < kMostBytes ? static_cast<uint32_t>(left) : kMostBytes);
-}
 
 // The sums of all waves: thread i < 256 RT has (p, row, column) element i of each p.
 template <Kind KIND, int RT, bool PAIRED>
@@ -692,20 +698,23 @@ constexpr int few_bytes() {
 }
 
 // The product of the columns n0 .. with at most 16 RT rows: a_at(r, k) is the lane's 16 bytes from k
-// of row 16 r + lane % 16, zeros outside.  The first columns are on their way before `first()` runs,
-// the next ones while a stage's products do.
-template <Kind KIND, int RT, bool PAIRED, typename A, typename F>
+// of row 16 r + lane % 16, zeros outside, a_rest(r) the values behind the whole pieces of a row of 16-bit
+// ones.  The first columns are on their way before `first()` runs, the next ones while a stage's
+// products do.
+template <Kind KIND, int RT, bool PAIRED, typename A, typename R, typename F>
 __device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n0, char* smem, F first,
-                                            A a_at) {
-  constexpr int U = 2;
+                                            A a_at, R a_rest) {
+  constexpr int U = 2, P = PAIRED ? 2 : 1;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
-  uint32_t at[2];
-  const auto rb = few_rows_of<PAIRED>(b, n0, c, at);
+  // (columns past the last one read the last one)
+  const int held = b.rows / P, n = n0 + c < held ? n0 + c : held - 1;
+  const char* const rows[2] = {b.base + static_cast<size_t>(n) * b.pitch,
+                               b.base + static_cast<size_t>(n + (PAIRED ? held : 0)) * b.pitch};
   FewSums<KIND, RT, PAIRED> s{};
-  const int stages = (k_bytes + kStage - 1) / kStage;
+  const int whole = k_bytes & ~15, stages = (whole + kStage - 1) / kStage;
   FewColumns<PAIRED, U> fb;
-  fb.load(rb, at, q, wave, k_bytes);
+  if (stages > 0) fb.load(rows, q, wave, whole);
   first();
   for (int t = wave; t < stages; t += U * kFewWaves) {
     const FewColumns<PAIRED, U> now = fb;
@@ -716,35 +725,48 @@ __device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n
       for (int r = 0; r < RT; ++r)
 #pragma unroll
         for (int h = 0; h < 2; ++h) fa[u][r][h] = a_at(r, (t + u * kFewWaves) * kStage + q * 32 + h * 16);
-    if (t + U * kFewWaves < stages) fb.load(rb, at, q, t + U * kFewWaves, k_bytes);
+    if (t + U * kFewWaves < stages) fb.load(rows, q, t + U * kFewWaves, whole);
 #pragma unroll
     for (int u = 0; u < U; ++u)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int p = 0; p < (PAIRED ? 2 : 1); ++p)
+        for (int p = 0; p < P; ++p)
 #pragma unroll
           for (int r = 0; r < RT; ++r)
             s.v[p][r] = Ops<KIND>::mma16(fa[u][r][h], now.v[u][p][h], s.v[p][r]);
   }
+  if constexpr (KIND != kI8) {
+    if (k_bytes > whole && wave == kFewWaves - 1) {
+      const i32x4 none = {0, 0, 0, 0};
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const i32x4 w = row_rest(rows[p], k_bytes);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const i32x4 x = a_rest(r);
+          s.v[p][r] = Ops<KIND>::mma16(q == 0 ? x : none, q == 0 ? w : none, s.v[p][r]);
+        }
+      }
+    }
+  }
   few_join<KIND, RT, PAIRED>(s, smem, wave, lane);
 }
 
-// Rows 0 .. a.rows of a in memory.
+// Rows 0 .. a.rows of a in memory (rows past the last one read the last one: their sums go nowhere).
 template <Kind KIND, int RT, bool PAIRED>
 __device__ __forceinline__ void few_product(const Operand& a, const Operand& b, int k_bytes, int n0,
                                             char* smem) {
   const int c = threadIdx.x & 15;
-  const size_t a_bytes = static_cast<size_t>(a.rows) * a.pitch;
-  const auto ra = vkd::buffer_rsrc(a.base, a_bytes < kMostBytes ? static_cast<uint32_t>(a_bytes) : kMostBytes);
+  const char* rows[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const int row = r * 16 + c;
+    rows[r] = a.base + static_cast<size_t>(row < a.rows ? row : a.rows - 1) * a.pitch;
+  }
   few_product<KIND, RT, PAIRED>(
-      b, k_bytes, n0, smem, [] {},
-      [&](int r, int k) {
-        const uint32_t row = static_cast<uint32_t>(r * 16 + c);
-        const bool in = k < k_bytes && static_cast<int>(row) < a.rows;
-        return __builtin_bit_cast(
-            i32x4, vkd::buffer_load4(ra, in ? row * a.pitch + static_cast<uint32_t>(k) : kOutside, 0));
-      });
+      b, k_bytes, n0, smem, [] {}, [&](int r, int k) { return row_piece(rows[r], k, k_bytes & ~15); },
+      [&](int r) { return row_rest(rows[r], k_bytes); });
 }
 
 }  // namespace vkp

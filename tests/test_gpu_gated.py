@@ -21,7 +21,7 @@ def up(rt, t, *arrays):
     return [None if a is None else ff.upload(rt, a, t) for a in arrays]
 
 
-SIZES = [(1, 64, 64), (1, 8, 1), (2, 136, 33), (5, 1024, 300), (16, 7, 40), (17, 513, 70),
+SIZES = [(1, 64, 64), (1, 8, 1), (48, 2881, 173), (70, 4000, 64), (33, 2000, 7), (2, 136, 33), (5, 1024, 300), (16, 7, 40), (17, 513, 70),
          (32, 384, 96), (33, 100, 31), (64, 64, 32), (70, 257, 65), (257, 384, 1023),
          (866, 768, 700), (1300, 96, 2050), (2100, 130, 1030)]
 
@@ -38,7 +38,7 @@ def test_forward(rt, rng, m, k, h, t):
         ff.assert_within(rt.download_16(out), want, tol, (m, k, h, act))
 
 
-BACK = [(1, 64, 64), (1, 8, 1), (3, 17, 5), (31, 136, 33), (64, 64, 32), (65, 96, 63), (70, 257, 65),
+BACK = [(1, 64, 64), (1, 8, 1), (2, 1344, 688), (8651, 64, 64), (40, 2881, 65), (281, 241, 3330), (3, 17, 5), (31, 136, 33), (64, 64, 32), (65, 96, 63), (70, 257, 65),
         (130, 384, 129), (257, 384, 1023), (866, 256, 300), (1300, 96, 2050), (2100, 520, 130)]
 
 

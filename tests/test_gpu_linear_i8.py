@@ -32,7 +32,7 @@ def run(rt, lin, x, t, n, out, call, start=None):
 SIZES = [(1, 64, 64), (1, 1024, 4096), (2, 130, 33), (3, 5000, 40), (4, 4096, 20), (4, 4097, 17), (5, 900, 70),
          (7, 1, 5), (16, 257, 96), (17, 512, 48),
          (31, 1031, 200), (32, 4096, 64), (33, 127, 65), (64, 128, 64), (65, 129, 127),
-         (130, 768, 300), (257, 384, 257), (866, 768, 640), (1301, 770, 1999), (300, 5000, 96),
+         (130, 768, 300), (257, 384, 257), (866, 768, 640), (1301, 770, 1999), (300, 5000, 96), (40, 20000, 70), (129, 9000, 33),
          (2600, 512, 2304)]
 
 

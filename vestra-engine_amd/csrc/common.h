@@ -43,6 +43,9 @@ struct vk_runtime {
   // capture.
   float* work = nullptr;
   size_t work_len = 0;
+  // Counters of the workgroups that have left their part of a tile whose k is shared out over
+  // several (product_nt.h): zeros between launches, since the last one to arrive clears its tile's.
+  unsigned* arrivals = nullptr;
   // Replaced device buffers (work buffers, smaller RoPE tables): graphs
   // captured earlier may still name them, so they live until the runtime
   // is destroyed.
@@ -129,6 +132,8 @@ __host__ __device__ inline FastDivU32 make_fastdiv(uint32_t d) {
 }  // namespace vkd
 
 namespace vk {
+
+constexpr int kArrivals = 4096;  // counters of vk_runtime::arrivals
 
 int set_error(int code, const char* fmt, ...);
 void clear_error();

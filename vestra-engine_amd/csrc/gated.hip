@@ -36,6 +36,7 @@ struct Args {
   int M, N;
   int act;
   int gm, gn, group;
+  vkp::Split split;
 };
 
 template <Kind KIND>
@@ -59,13 +60,14 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
   VK_STAGES(T);
   __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
-  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
+  const int tiles = g.gm * g.gn, tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+  vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
-  if (place.group > 0) return;
+  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+    return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
   typedef vkp::Chunk<V, kCols> C;
@@ -102,13 +104,14 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   VK_STAGES(T);
   __shared__ __align__(16) float bias[T::TN];
   int mt, nt;
-  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
+  const int tiles = g.gm * g.gn, tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+  vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
-  if (place.group > 0) return;
+  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+    return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
   typedef vkp::Chunk<V, kCols> C;
@@ -196,18 +199,20 @@ struct Product {
   void* out;
   int M, N, m_half;
   int gm, gn, group;
+  vkp::Split split;
 };
 
 template <Kind KIND, typename T, bool AC>
-__device__ __forceinline__ void product(const Product& g, int tile, char* const (&stages_)[5]) {
+__device__ __forceinline__ void product(const Product& g, int wg, char* const (&stages_)[5]) {
   typedef typename vkp::Value<KIND>::type V;
+  const int tiles = g.gm * g.gn, tile = wg % tiles, part = wg / tiles;
   int mt, nt;
   vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::TN;
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
-  if (place.group > 0) return;
+  if (!vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+    return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   typedef vkp::Chunk<V, T::NT> C;
   char* chunk = stages_[0] + wave * C::kBytes;
@@ -342,9 +347,10 @@ void with_tile(vkp::TileSize size, Args& g, F go) {
   });
 }
 
+vkp::Shape forward_shape(const Args& g) { return vkp::Shape{g.M, 2LL * g.N, g.k_bytes}; }
+
 template <Kind KIND>
-int launch_forward(vk_runtime* rt, Args& g) {
-  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, 2LL * g.N, g.k_bytes);
+int launch_forward(vk_runtime* rt, Args& g, const vkp::Plan& p) {
   if (p.few) {
     const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
     if (g.M <= 16)
@@ -353,9 +359,12 @@ int launch_forward(vk_runtime* rt, Args& g) {
       hipLaunchKernelGGL((gated_few_kernel<KIND, 2>), grid, block, 0, rt->stream, g);
     return vk::check_launch("gated_few_kernel");
   }
+  g.split.count = p.splits;
+  g.split.arrivals = rt->arrivals;
   with_tile<true>(p.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
-    hipLaunchKernelGGL((gated_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0, rt->stream, g);
+    hipLaunchKernelGGL((gated_kernel<KIND, T>), dim3(g.gm * g.gn * p.splits), dim3(T::kThreads), 0,
+                       rt->stream, g);
   });
   return vk::check_launch("gated_kernel");
 }
@@ -366,26 +375,49 @@ size_t operands_room(size_t rows, size_t in, size_t hidden) {
   return in % 8 == 0 ? 0 : (rows + 2 * hidden) * padded(in) * 2;
 }
 
+// What the backward's launches are and what they keep in the work buffer: d, the biases' sums, then
+// split tiles' sums, of the first step and after it of the products.
+struct BackwardPlan {
+  vkp::Plan first;
+  vkp::PlanTwo second;
+  size_t work, dx_sums, bytes;
+};
+BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, bool dbias) {
+  BackwardPlan p{};
+  double us = 0;
+  const size_t rows = g.M, half = padded(g.N);
+  const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes};  // the zeros up to d_half too
+  p.first = vkp::plan(cus, step, &us);
+  const auto D = static_cast<long long>(in);
+  const vkp::Shape x{dx ? g.M : 0, D, static_cast<long long>(4 * half)};
+  const vkp::Shape w{dw ? static_cast<long long>(2 * half) : 0, D, 2LL * g.M};
+  p.second = vkp::plan_two(cus, x, w);
+  const auto round = [](size_t n) { return (n + 255) / 256 * 256; };
+  if (dx || dw) p.work += round(rows * 4 * half);
+  // (a tile of 64 or 128 rows has two waves' sums, one of 256 four)
+  if (dbias) p.work += round(((rows + 63) / 64 * 2 + 4) * 2 * g.N * 4);
+  p.dx_sums = vkp::split_bytes(p.second.tile[0], vkp::Job{x, p.second.splits[0]});
+  const size_t after = p.dx_sums + vkp::split_bytes(p.second.tile[1], vkp::Job{w, p.second.splits[1]});
+  const size_t before = vkp::split_bytes(p.first.tile, vkp::Job{step, p.first.splits});
+  p.bytes = p.work + (before > after ? before : after);
+  return p;
+}
+
 template <Kind KIND>
-int backward(vk_runtime* rt, Args& g, size_t rows, size_t in, size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
-  const size_t half = padded(hidden);
-  const auto take = [&](size_t bytes) {
-    char* at = room;
-    room += (bytes + 255) / 256 * 256;
-    return at;
-  };
+int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, size_t in, size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
+  const size_t half = padded(hidden), d_bytes = dx || dw ? (rows * 4 * half + 255) / 256 * 256 : 0;
   if (dx || dw) {
-    g.d = take(rows * 2 * half * 2);
+    g.d = room;
     g.d_half = static_cast<int>(half);
   }
-  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, 2LL * g.N, g.k_bytes);
+  if (dbias) g.sums = reinterpret_cast<float*>(room + d_bytes);
+  g.split = vkp::Split{plan.first.splits, room + plan.work, rt->arrivals};
   int parts = 0;
-  with_tile<true>(p.tile, g, [&](auto tile) {
+  with_tile<true>(plan.first.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
     parts = g.gm * T::WM;
     g.gn = (static_cast<int>(half) + T::kHeld - 1) / T::kHeld;  // the zeros up to d_half too
-    if (dbias) g.sums = reinterpret_cast<float*>(take(static_cast<size_t>(parts) * 2 * hidden * 4));
-    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
+    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn * g.split.count), dim3(T::kThreads), 0,
                        rt->stream, g);
   });
   VK_TRY(vk::check_launch("gated_grad_kernel"));
@@ -418,22 +450,24 @@ int backward(vk_runtime* rt, Args& g, size_t rows, size_t in, size_t hidden, cha
   }
   BiasSums sums{g.sums, parts, H2, dbias ? dbias->ptr : nullptr};
   const int n_bias = dbias ? (H2 + 15) / 16 : 0;
-  const vkp::PlanTwo plan = vkp::plan_two(rt->cu_count, vkp::Shape{dx ? R : 0, D, x.k_bytes},
-                                          vkp::Shape{dw ? both : 0, D, w.k_bytes});
+  // (the first step's split sums are done with)
+  const vkp::PlanTwo& two = plan.second;
+  x.split = vkp::Split{two.splits[0], room + plan.work, rt->arrivals};
+  w.split = vkp::Split{two.splits[1], room + plan.work + plan.dx_sums, rt->arrivals + vkp::kMostTilesSplit};
   // one launch, or dx in one of its own
-  for (int part = plan.together ? 1 : 0; part < 2; ++part) {
-    vkp::with_tile<false>(part == 0 ? plan.first : plan.second, [&](auto tile) {
+  for (int part = two.together ? 1 : 0; part < 2; ++part) {
+    vkp::with_tile<false>(two.tile[part], [&](auto tile) {
       typedef decltype(tile) T;
       for (Product* p : {&x, &w}) {
         p->gm = (p->a.rows + T::TM - 1) / T::TM;
         p->gn = (p->N + T::TN - 1) / T::TN;
         p->group = vkp::kGroupRows / T::TM;
       }
-      const int n_dx = part == 0 || plan.together ? x.gm * x.gn : 0;
-      const int biases = part == 0 ? 0 : n_bias, grid = biases + n_dx + (part == 0 ? 0 : w.gm * w.gn);
-      if (grid > 0)
-        hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(grid), dim3(T::kThreads), 0, rt->stream, x, w,
-                           sums, biases, n_dx);
+      const int n_dx = part == 0 || two.together ? x.gm * x.gn * x.split.count : 0;
+      const int n_dw = part == 0 ? 0 : w.gm * w.gn * w.split.count, biases = part == 0 ? 0 : n_bias;
+      if (biases + n_dx + n_dw > 0)
+        hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(biases + n_dx + n_dw), dim3(T::kThreads), 0,
+                           rt->stream, x, w, sums, biases, n_dx);
     });
     VK_TRY(vk::check_launch("gradients_kernel"));
   }
@@ -509,11 +543,17 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, con
   if (rows == 0) return VK_OK;
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
   g.out = out->ptr;
-  if (rows > vkp::kFewRows && in_features % 8 != 0) {
-    VK_TRY(vk::ensure_work(rt, operands_room(rows, in_features, hidden) / 4, "gated_forward"));
-    VK_TRY(align_operands(rt, g, in_features, reinterpret_cast<char*>(rt->work)));
+  const vkp::Shape shape = forward_shape(g);
+  const vkp::Plan p = vkp::plan(rt->cu_count, shape.m, shape.n, shape.k_bytes);
+  if (!p.few) {
+    const size_t room = operands_room(rows, in_features, hidden);
+    const size_t sums = vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});
+    if (room + sums > 0) VK_TRY(vk::ensure_work(rt, (room + sums) / 4, "gated_forward"));
+    char* work = reinterpret_cast<char*>(rt->work);
+    VK_TRY(align_operands(rt, g, in_features, work));
+    g.split.partial = work + room;
   }
-  return x->dtype == VK_F16 ? launch_forward<kF16>(rt, g) : launch_forward<kBF16>(rt, g);
+  return x->dtype == VK_F16 ? launch_forward<kF16>(rt, g, p) : launch_forward<kBF16>(rt, g, p);
 }
 
 int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
@@ -538,18 +578,16 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
     return vk::check_launch("zero16_kernel");
   }
   const size_t room = operands_room(rows, in_features, hidden);
-  size_t need = room + 2 * 256;
-  if (dx || dw) need += rows * padded(hidden) * 4;
-  if (dbias) need += ((rows + 63) / 64 * 2) * 2 * hidden * 4;
-  VK_TRY(vk::ensure_work(rt, (need + 3) / 4, "gated_backward"));
-  char* work = reinterpret_cast<char*>(rt->work);
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
+  const BackwardPlan plan = plan_backward(rt->cu_count, g, in_features, dx, dw, dbias);
+  VK_TRY(vk::ensure_work(rt, (room + plan.bytes + 3) / 4, "gated_backward"));
+  char* work = reinterpret_cast<char*>(rt->work);
   VK_TRY(align_operands(rt, g, in_features, work));
   work += room;
   g.grad = grad->ptr;
   return x->dtype == VK_F16
-             ? backward<kF16>(rt, g, rows, in_features, hidden, work, dx, dw, dbias)
-             : backward<kBF16>(rt, g, rows, in_features, hidden, work, dx, dw, dbias);
+             ? backward<kF16>(rt, g, plan, rows, in_features, hidden, work, dx, dw, dbias)
+             : backward<kBF16>(rt, g, plan, rows, in_features, hidden, work, dx, dw, dbias);
 }
 
 }  // extern "C"

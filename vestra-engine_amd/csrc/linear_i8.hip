@@ -51,6 +51,7 @@ struct Args {
   const void* x;  // for workgroups that quantise for themselves: [M, K] of vk_dtype x_type
   int K, x_type;
   int gm, gn, group;
+  vkp::Split split;
 };
 
 // ---------------------------------------------------------------- rows to codes
@@ -194,7 +195,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   VK_STAGES(T);
   __shared__ __align__(16) float cols[3][T::TN];  // scale, bias, LayerScale of the tile's columns
   int mt, nt;
-  vkp::tile_at(blockIdx.x, g.gm, g.gn, g.group, &mt, &nt);
+  const int tiles = g.gm * g.gn, tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
+  vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::kHeld;
   for (int c = threadIdx.x; c < T::TN; c += T::kThreads) {
     const int n = n0 + c % T::kHeld;
@@ -205,8 +207,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   }
   const vkp::Place<T> place;
   vkp::i32x16 acc[T::MT][T::NT];
-  vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, place, stages_, acc);
-  if (place.group > 0) return;
+  if (!vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+    return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
   constexpr int J = sizeof(V) == 4 ? 1 : (kCols < 2 ? kCols : 2);
@@ -385,14 +387,13 @@ void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, cha
 }
 
 template <int END, typename V>
-int launch(vk_runtime* rt, Args& g) {
+int launch(vk_runtime* rt, Args& g, const vkp::Plan& p) {
   constexpr bool kPaired = END == kGated;
   if (g.x) {
     hipLaunchKernelGGL((linear_i8_rows_kernel<END, V>), dim3((g.N + 15) / 16), dim3(vkp::kFewThreads), 0,
                        rt->stream, g);
     return vk::check_launch("linear_i8_rows_kernel");
   }
-  const vkp::Plan p = vkp::plan(rt->cu_count, g.M, kPaired ? 2LL * g.N : g.N, g.k_bytes);
   if (p.few) {
     const dim3 grid((g.N + 15) / 16), block(vkp::kFewThreads);
     if (g.M <= 16)
@@ -406,16 +407,18 @@ int launch(vk_runtime* rt, Args& g) {
     g.gm = (g.M + T::TM - 1) / T::TM;
     g.gn = (g.N + T::kHeld - 1) / T::kHeld;
     g.group = vkp::kGroupRows / T::TM;
-    hipLaunchKernelGGL((linear_i8_kernel<END, V, T>), dim3(g.gm * g.gn), dim3(T::kThreads), 0,
+    g.split.count = p.splits;
+    g.split.arrivals = rt->arrivals;
+    hipLaunchKernelGGL((linear_i8_kernel<END, V, T>), dim3(g.gm * g.gn * p.splits), dim3(T::kThreads), 0,
                        rt->stream, g);
   });
   return vk::check_launch("linear_i8_kernel");
 }
 
 template <int END>
-int launch_type(vk_runtime* rt, Args& g, vk_dtype type) {
-  if (type == VK_F32) return launch<END, float>(rt, g);
-  return type == VK_F16 ? launch<END, _Float16>(rt, g) : launch<END, __bf16>(rt, g);
+int launch_type(vk_runtime* rt, Args& g, const vkp::Plan& p, vk_dtype type) {
+  if (type == VK_F32) return launch<END, float>(rt, g, p);
+  return type == VK_F16 ? launch<END, _Float16>(rt, g, p) : launch<END, __bf16>(rt, g, p);
 }
 
 bool is_float(const vk_tensor* t) {
@@ -456,16 +459,21 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
                     rows, N);
 
   const int M = static_cast<int>(rows);
+  const vkp::Plan p = vkp::plan(rt->cu_count, M, static_cast<long long>(lin->out_features),
+                                static_cast<long long>(lin->pitch));
   Args g{};
   if (vkp::own_rows(rows, lin->pitch)) {
     g.x = x->ptr;
     g.K = static_cast<int>(K);
     g.x_type = x->dtype;
   } else {
-    const size_t code_bytes = rows * lin->pitch;  // a multiple of 128
-    VK_TRY(vk::ensure_work(rt, code_bytes / 4 + rows, "linear_i8"));
-    char* codes = reinterpret_cast<char*>(rt->work);
+    const size_t code_bytes = rows * lin->pitch, scale_bytes = (rows * 4 + 255) / 256 * 256;
+    const vkp::Shape shape{M, static_cast<long long>(lin->out_features), static_cast<long long>(lin->pitch)};
+    const size_t sums = p.few ? 0 : vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});
+    VK_TRY(vk::ensure_work(rt, (code_bytes + scale_bytes + sums) / 4, "linear_i8"));
+    char* codes = reinterpret_cast<char*>(rt->work);  // (code_bytes: a multiple of 128)
     float* scales = reinterpret_cast<float*>(codes + code_bytes);
+    g.split.partial = codes + code_bytes + scale_bytes;
     if (x->dtype == VK_F32)
       quantise(rt, static_cast<const float*>(x->ptr), M, static_cast<int>(K), lin->pitch, codes,
                scales);
@@ -490,10 +498,10 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
   g.k_bytes = static_cast<int>(lin->pitch);
   g.act = act;
   switch (end) {
-    case kStore: return launch_type<kStore>(rt, g, out->dtype);
-    case kGelu: return launch_type<kGelu>(rt, g, out->dtype);
-    case kResidual: return launch<kResidual, float>(rt, g);
-    default: return launch_type<kGated>(rt, g, out->dtype);
+    case kStore: return launch_type<kStore>(rt, g, p, out->dtype);
+    case kGelu: return launch_type<kGelu>(rt, g, p, out->dtype);
+    case kResidual: return launch<kResidual, float>(rt, g, p);
+    default: return launch_type<kGated>(rt, g, p, out->dtype);
   }
 }
 

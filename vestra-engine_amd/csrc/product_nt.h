@@ -208,8 +208,8 @@ __device__ __forceinline__ constexpr int column_turn(int k) {
   return W == 64 ? ((k >> 1) & 1) * 4 : (k & 3) * 4;
 }
 
-// The lines of stage st, up to the last.
-__device__ __forceinline__ Source columns_of(const Operand& o, int st) {
+// The lines of stage st, up to the last; none from stage `stop` on.
+__device__ __forceinline__ Source columns_of(const Operand& o, int st, int stop) {
   int line = st * 64, end = o.ks;
   if (o.k_half > 0) {
     end = o.ks / 2;
@@ -218,7 +218,7 @@ __device__ __forceinline__ Source columns_of(const Operand& o, int st) {
       end = o.ks;
     }
   }
-  const int lines = line < end ? (end - line < 64 ? end - line : 64) : 0;
+  const int lines = line < end && st < stop ? (end - line < 64 ? end - line : 64) : 0;
   return Source{o.base + static_cast<size_t>(line) * o.pitch, static_cast<uint32_t>(lines) * o.pitch};
 }
 
@@ -268,12 +268,82 @@ struct Place {
   }
 };
 
+// A launch may share a tile's k out over `count` workgroups: each leaves its sums in `partial`, and the
+// one that arrives last adds all of them, in their order whoever it is, and goes on.  For few tiles of
+// a long k.
+struct Split {
+  int count;
+  char* partial;       // [count][tiles][a tile's sums]
+  unsigned* arrivals;  // [tiles], zeros before and after a launch
+};
+
+// Leaves a wave's sums; whether its workgroup is its tile's last one, whose acc is then the sum of all
+// parts'.  Nobody waits for anybody.  The sums go past the L2 of the XCD, 8 bytes at a time, in both
+// directions (agent scope), so that they are where every XCD sees them once the wave's stores have
+// returned, and a fence, which would write back and drop the whole L2, is not needed: with fences a
+// launch of this kind took 44 us in place of 11.
+template <Kind KIND, typename T>
+__device__ __forceinline__ bool last_of_split(const Split& split, int part, int tile, int tiles,
+                                              const Place<T>& at,
+                                              typename Ops<KIND>::Acc16 (&acc)[T::MT][T::NT]) {
+  typedef decltype(typename Ops<KIND>::Acc4{}[0] + 0) S;
+  typedef S S2 __attribute__((ext_vector_type(2)));
+  constexpr int kPairs = T::MT * T::NT * 8, kSums = T::kWaves * kPairs * 64;  // pairs of a lane, a tile
+  __shared__ unsigned arrived;
+  uint64_t* mine = reinterpret_cast<uint64_t*>(split.partial) + static_cast<size_t>(tile) * kSums +
+                   at.wave * kPairs * 64 + at.lane;
+  const size_t part_sums = static_cast<size_t>(tiles) * kSums;
+#pragma unroll
+  for (int e = 0; e < kPairs; ++e) {
+    const auto& v = acc[e / 8 / T::NT][e / 8 % T::NT];
+    const S2 pair = {v[e % 8 * 2], v[e % 8 * 2 + 1]};
+    __hip_atomic_store(mine + part * part_sums + e * 64, __builtin_bit_cast(uint64_t, pair),
+                       __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have arrived, then the count
+  __syncthreads();
+  if (threadIdx.x == 0)
+    arrived = __hip_atomic_fetch_add(&split.arrivals[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (arrived + 1 != static_cast<unsigned>(split.count)) return false;
+  if (threadIdx.x == 0)
+    __hip_atomic_store(&split.arrivals[tile], 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+  for (int i = 0; i < T::MT; ++i)
+#pragma unroll
+    for (int j = 0; j < T::NT; ++j) acc[i][j] = typename Ops<KIND>::Acc16{};
+  // (a round trip for several parts together, as many as the registers hold)
+  constexpr int kAtOnce = kPairs <= 16 ? 4 : 2;
+  for (int p = 0; p < split.count; p += kAtOnce) {
+    uint64_t w[kAtOnce][kPairs];
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u)
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e)
+        w[u][e] = __hip_atomic_load(mine + (p + u < split.count ? p + u : p) * part_sums + e * 64,
+                                    __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (int u = 0; u < kAtOnce; ++u) {
+      if (p + u >= split.count) break;
+#pragma unroll
+      for (int e = 0; e < kPairs; ++e) {
+        auto& v = acc[e / 8 / T::NT][e / 8 % T::NT];
+        const S2 pair = __builtin_bit_cast(S2, w[u][e]);
+        v[e % 8 * 2] += pair[0];
+        v[e % 8 * 2 + 1] += pair[1];
+      }
+    }
+  }
+  return true;
+}
+
 // acc[mt][nt] of this wave: the tile's rows from m0, columns from n0 (of the
-// hidden ones, where PAIRED), over all of k; with KG > 1 group 0 has them, the others are done.
-// AC, BC: a, b as columns.
+// hidden ones, where PAIRED), over all of k, where the wave is to go on with them: with KG > 1 those of
+// group 0, with a split those of the tile's last workgroup.  AC, BC: a, b as columns.
 template <Kind KIND, typename T, bool AC = false, bool BC = false>
-__device__ __forceinline__ void product_tile(const Operand& a, const Operand& b, int k_bytes,
-                                             int m0, int n0, const Place<T>& at,
+__device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b, int k_bytes,
+                                             int m0, int n0, const Split& split, int part, int tile,
+                                             int tiles, const Place<T>& at,
                                              char* const (&stages_)[5],
                                              typename Ops<KIND>::Acc16 (&acc)[T::MT][T::NT]) {
   constexpr int S = T::S, R = T::R, KG = T::KG, KS = S / 32;
@@ -319,25 +389,28 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
       }
     }
   }
-  const int stages = (k_bytes + S * KG - 1) / (S * KG);  // of a group
-  const int last = k_bytes - static_cast<int>(piece);  // the lane's bytes of stage t: t S < last
+  const int every = (k_bytes + S - 1) / S, mine = (every + split.count - 1) / split.count;
+  const int start = part * mine, stop = start + mine < every ? start + mine : every;
+  const int stages = (mine + KG - 1) / KG;  // of a group
+  // the lane's bytes of stage t: t S < last
+  const int last = (stop < every ? stop * S : k_bytes) - static_cast<int>(piece);
   // Load i of stage t (past the last stage they read zeros: their number stays the same).
   constexpr int kLoads = T::kALoads + T::kBLoads;
   auto load = [&](char* to, int t, int i) {
-    const int st = t * KG + at.group, k = st * S;
+    const int st = start + t * KG + at.group, k = st * S;
     const bool in = k < last;
     constexpr bool kByHand = AC || BC;
     if (i < T::kALoads) {
       char* lds = to + (wave + i * T::kWaves) * 1024;
       if constexpr (AC)
-        load_lds<kByHand>(columns_of(a, st), lds, av[i], 0);
+        load_lds<kByHand>(columns_of(a, st, stop), lds, av[i], 0);
       else
         load_lds<kByHand>(sa, lds, in ? av[i] : kOutside, k);
     } else {
       const int j = i - T::kALoads;
       char* lds = to + T::TM * S + (wave + j * T::kWaves) * 1024;
       if constexpr (BC)
-        load_lds<kByHand>(columns_of(b, st), lds, bv[j], 0);
+        load_lds<kByHand>(columns_of(b, st, stop), lds, bv[j], 0);
       else
         load_lds<kByHand>(sb, lds, in ? bv[j] : kOutside, k);
     }
@@ -424,7 +497,7 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
         sums[(at.group - 1) * T::kWaves * kWaveSums + e * 64] = Acc4{v[r], v[r + 1], v[r + 2], v[r + 3]};
     }
     tile_done();
-    if (at.group > 0) return;
+    if (at.group > 0) return false;
 #pragma unroll
     for (int e = 0; e < kTiles * 4; ++e) {
       auto& v = acc[e / 4 / T::NT][e / 4 % T::NT];
@@ -436,6 +509,10 @@ __device__ __forceinline__ void product_tile(const Operand& a, const Operand& b,
       }
     }
   }
+  // (not for the largest tiles: 256 KiB of sums a workgroup cost more than they save)
+  if constexpr (T::TM < 256)
+    if (split.count > 1) return last_of_split<KIND, T>(split, part, tile, tiles, at, acc);
+  return true;
 }
 
 // A wave's sums lie with a row of a in each lane (lane % 32) and 16 columns in its registers:

@@ -150,6 +150,7 @@ void release(vk_runtime* rt) {
   (void)hipStreamSynchronize(rt->stream);
   for (auto& kv : rt->rope_tables) (void)hipFree(kv.second.first);
   if (rt->work) (void)hipFree(rt->work);
+  if (rt->arrivals) (void)hipFree(rt->arrivals);
   for (void* p : rt->retired) (void)hipFree(p);
   (void)hipStreamDestroy(rt->stream);
   delete rt;
@@ -353,6 +354,15 @@ int vk_runtime_create(int device, vk_runtime** out) {
   if (e != hipSuccess) {
     delete rt;
     return hip_fail(e, "hipStreamCreateWithFlags");
+  }
+  e = hipMalloc(reinterpret_cast<void**>(&rt->arrivals), kArrivals * sizeof(unsigned));
+  if (e == hipSuccess) e = hipMemsetAsync(rt->arrivals, 0, kArrivals * sizeof(unsigned), rt->stream);
+  if (e == hipSuccess) e = hipStreamSynchronize(rt->stream);
+  if (e != hipSuccess) {
+    if (rt->arrivals) (void)hipFree(rt->arrivals);
+    (void)hipStreamDestroy(rt->stream);
+    delete rt;
+    return hip_fail(e, "hipMalloc(arrival counters)");
   }
   *out = rt;
   return VK_OK;

@@ -131,6 +131,16 @@ def backward(x, w, bias, grad, act, t):
     return {k: (v, held(v, e, t)) for k, (v, e) in out.items()}
 
 
+def slope(f, step=2.0 ** -7):
+    """f'(0) of f(s) by differences of the fourth order, and a bound on their error: halving the
+    step takes it to a sixteenth, so that what the two differ by is above it; and f's own
+    rounding, 2^-50 of its size, over the step."""
+    def difference(e):
+        return (8 * (f(e) - f(-e)) - (f(2 * e) - f(-2 * e))) / (12 * e)
+    a, b = difference(step), difference(step / 2)
+    return b, abs(a - b) + abs(f(0.0)) * 2.0 ** -40
+
+
 def assert_within(got, want, tol, label):
     got = np.asarray(got, np.float64).reshape(want.shape)
     odd = np.isnan(want)
@@ -139,4 +149,5 @@ def assert_within(got, want, tol, label):
     off[odd] = 0
     if off.size and off.max() > 0:
         at = np.unravel_index(int(np.argmax(off)), want.shape)
-        raise AssertionError(f"{label}: at {at} got {got[at]!r}, want {want[at]!r} +- {tol[at]:.3e}")
+        raise AssertionError(f"{label}: at {at} got {got[at]!r}, want {want[at]!r} "
+                             f"+- {tol[at]:.3e}")

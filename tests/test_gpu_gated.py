@@ -21,9 +21,9 @@ def up(rt, t, *arrays):
     return [None if a is None else ff.upload(rt, a, t) for a in arrays]
 
 
-SIZES = [(1, 64, 64), (1, 8, 1), (48, 2881, 173), (70, 4000, 64), (33, 2000, 7), (2, 136, 33), (5, 1024, 300), (16, 7, 40), (17, 513, 70),
-         (32, 384, 96), (33, 100, 31), (64, 64, 32), (70, 257, 65), (257, 384, 1023),
-         (866, 768, 700), (1300, 96, 2050), (2100, 130, 1030)]
+SIZES = [(1, 64, 64), (1, 8, 1), (48, 2881, 173), (70, 4000, 64), (33, 2000, 7), (2, 136, 33),
+         (5, 1024, 300), (16, 7, 40), (17, 513, 70), (32, 384, 96), (33, 100, 31),
+         (64, 64, 32), (70, 257, 65), (257, 384, 1023), (866, 768, 700), (1300, 96, 2050), (2100, 130, 1030)]
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])
@@ -38,7 +38,8 @@ def test_forward(rt, rng, m, k, h, t):
         ff.assert_within(rt.download_16(out), want, tol, (m, k, h, act))
 
 
-BACK = [(1, 64, 64), (1, 8, 1), (2, 1344, 688), (8651, 64, 64), (40, 2881, 65), (281, 241, 3330), (3, 17, 5), (31, 136, 33), (64, 64, 32), (65, 96, 63), (70, 257, 65),
+BACK = [(1, 64, 64), (1, 8, 1), (2, 1344, 688), (8651, 64, 64), (40, 2881, 65), (281, 241, 3330),
+        (3, 17, 5), (31, 136, 33), (64, 64, 32), (65, 96, 63), (70, 257, 65),
         (130, 384, 129), (257, 384, 1023), (866, 256, 300), (1300, 96, 2050), (2100, 520, 130)]
 
 
@@ -54,6 +55,118 @@ def test_backward(rt, rng, m, k, h, t):
         rt.gated_backward(dx, dw, db, dg, m, k, h, out["dx"], out["dw"], out["dbias"], act)
         for n, (want, tol) in ff.backward(x, w, b, grad, act, t).items():
             ff.assert_within(rt.download_16(out[n]), want, tol, (n, m, k, h, act))
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("m,k,h,t", [(3, 24, 9, "f16"), (90, 40, 50, "bf16"), (65, 2100, 3, "f16")])
+def test_gradients_are_slopes(rt, rng, m, k, h, t, act):
+    """Against differences of the 64-bit forward, value by value of each input."""
+    x, w, b = inputs(rng, m, k, h, t)
+    grad = ff.rounded(rng.standard_normal((m, h)), t)
+    o = {"dx": rt.alloc(ff.DTYPE[t], m * k), "dw": rt.alloc(ff.DTYPE[t], 2 * h * k),
+         "dbias": rt.alloc(ff.DTYPE[t], 2 * h)}
+    rt.gated_backward(*up(rt, t, x, w, b, grad), m, k, h, o["dx"], o["dw"], o["dbias"], act)
+    tol = {n: e for n, (_, e) in ff.backward(x, w, b, grad, act, t).items()}
+    at = {"dx": x, "dw": w, "dbias": b}
+    for name, got in o.items():
+        got = rt.download_16(got).reshape(at[name].shape)
+        for i in rng.choice(got.size, min(got.size, 12), replace=False):
+            def loss(s):
+                v = {n: a.astype(np.float64) for n, a in at.items()}
+                v[name].flat[i] += s
+                y = v["dx"] @ v["dw"].T + v["dbias"]
+                return float((grad * ff.activation(y[:, :h], act)[0] * y[:, h:]).sum())
+
+            want, off = ff.slope(loss)
+            assert abs(got.flat[i] - want) <= tol[name].flat[i] + off, (name, i)
+
+
+def steps(rt, rng, sizes, t="bf16"):
+    """Forward and backward of each size: [(what enqueues it, its outputs)]; step(True) takes other
+    inputs, for outputs that hold something else."""
+    out = []
+    for m, k, h in sizes:
+        a, other = (up(rt, t, *inputs(rng, m, k, h, t),
+                       ff.rounded(rng.standard_normal((m, h)), t)) for _ in "ab")
+        o = [rt.alloc(ff.DTYPE[t], s) for s in (m * h, m * k, 2 * h * k, 2 * h)]
+
+        def step(dirty=False, a=a, other=other, o=o, m=m, k=k, h=h):
+            v = other if dirty else a
+            rt.gated_forward(*v[:3], m, k, h, o[0])
+            rt.gated_backward(*v, m, k, h, *o[1:])
+        out.append((step, o))
+    return out
+
+
+def bits(rt, o):
+    rt.synchronize()
+    return [rt.download_16(v) for v in o]
+
+
+# products whose k several workgroups share, among others
+SHARED = [(70, 4000, 64), (2048, 72, 40), (40, 2881, 65), (130, 384, 129)]
+
+
+def test_the_same_bits_from_shared_products(rt, rng):
+    """Whoever arrives last adds the parts in their order, and leaves the counters as they were."""
+    calls = steps(rt, rng, SHARED)
+    for step, _ in calls:
+        step()
+    want = [bits(rt, o) for _, o in calls]
+    for i in range(12):
+        for step, _ in calls[i % 2::2] if i % 3 else calls:
+            step(True)
+            step()
+        for (_, o), w in zip(calls, want):
+            for p, q in zip(bits(rt, o), w):
+                np.testing.assert_array_equal(p, q)
+
+
+def test_two_runtimes_side_by_side(rng):
+    """Each its stream, work buffer and counters; their calls queued together."""
+    a, b = vh.Runtime(0), vh.Runtime(0)
+    calls = [(r, *c) for pair in zip(steps(a, rng, SHARED), steps(b, rng, SHARED))
+             for r, c in zip((a, b), pair)]
+    for _, step, _ in calls:
+        step()
+    want = [bits(r, o) for r, _, o in calls]
+    for _ in range(4):
+        for _, step, _ in calls:
+            step()
+    for (r, _, o), w in zip(calls, want):
+        for p, q in zip(bits(r, o), w):
+            np.testing.assert_array_equal(p, q)
+
+
+def test_graphs_outlive_a_larger_work_buffer(rng):
+    """A capture that would have to grow the work buffer is refused; captured after an eager call,
+    graphs give the same bits while eager calls grow and fill the buffer."""
+    rt = vh.Runtime(0)
+    calls = steps(rt, rng, SHARED)
+    big, out = steps(rt, rng, [(4000, 1031, 2048)])[0]  # more than the first buffer's 32 MiB
+
+    def refused():
+        with pytest.raises(vh.VestraError):
+            big()
+
+    for step, _ in calls:
+        step()
+    want = [bits(rt, o) for _, o in calls]
+    graphs = [cached.captured(rt, step) for step, _ in calls]
+    cached.captured(rt, refused)
+    big()
+    first = bits(rt, out)
+    for _ in range(3):
+        for step, _ in calls:
+            step(True)
+        for g in graphs:
+            g.launch()
+        big()
+        for (_, o), w in zip(calls, want):
+            for p, q in zip(bits(rt, o), w):
+                np.testing.assert_array_equal(p, q)
+        for p, q in zip(bits(rt, out), first):
+            np.testing.assert_array_equal(p, q)
 
 
 def test_gradients_one_at_a_time(rt, rng):
@@ -144,7 +257,8 @@ def test_guard_values_stay(rt, rng):
         x, w, b = inputs(rng, m, k, h, "bf16")
         grad = ff.rounded(rng.standard_normal((m, h)), "bf16")
         a = up(rt, "bf16", x, w, b, grad)
-        rooms = [ff.upload(rt, np.full(s + 512, 7.0), "bf16") for s in (m * h, m * k, 2 * h * k, 2 * h)]
+        rooms = [ff.upload(rt, np.full(s + 512, 7.0), "bf16")
+                 for s in (m * h, m * k, 2 * h * k, 2 * h)]
         o = [r.view(256, len(r) - 512) for r in rooms]
         rt.gated_forward(*a[:3], m, k, h, o[0])
         rt.gated_backward(*a, m, k, h, *o[1:])
@@ -199,8 +313,8 @@ def test_refusals(rt, rng):
     refused(rt.gated_backward, x, w, b, grad, m, k, h, rt.alloc(vh.VK_BF16, 1), None, None)
     refused(rt.gated_backward, x, w, b, grad, m, k, h, None, None, room.view(0, 2 * h + 1))
     refused(rt.gated_backward, x, w, b, grad, m, k, h, x, None, None)
-    refused(rt.gated_backward, x, w, b, grad, m, k, h, room.view(0, m * k), room.view(32, 2 * h * k),
-            None)
+    refused(rt.gated_backward, x, w, b, grad, m, k, h, room.view(0, m * k),
+            room.view(32, 2 * h * k), None)
     rt.gated_forward(x, w, b, m, k, h, out)  # and still runs
     rt.synchronize()
 
@@ -213,7 +327,8 @@ def test_the_feed_forward_of_a_block(rt, rng, act):
     tok = rng.standard_normal((m, d)).astype(np.float32)
     w12 = rng.standard_normal((2 * h, d)).astype(np.float32) * np.float32(1.5 * d ** -0.5)
     w3 = rng.standard_normal((d, h)).astype(np.float32) * np.float32(h ** -0.5)
-    b12, b3, ls = (rng.standard_normal(n).astype(np.float32) * np.float32(0.1) for n in (2 * h, d, d))
+    b12, b3, ls = (rng.standard_normal(n).astype(np.float32) * np.float32(0.1)
+                   for n in (2 * h, d, d))
     gamma, beta = np.ones(d, np.float32), np.zeros(d, np.float32)
     tokens, ln = rt.upload_f32(tok), rt.alloc_f32(m * d)
     rt.layernorm_into_f32(tokens, rt.upload_f32(gamma), rt.upload_f32(beta), m, d, 1e-6, ln)

@@ -29,10 +29,11 @@ def run(rt, lin, x, t, n, out, call, start=None):
     return ff.download(rt, y).reshape(m, n)
 
 
-SIZES = [(1, 64, 64), (1, 1024, 4096), (2, 130, 33), (3, 5000, 40), (4, 4096, 20), (4, 4097, 17), (5, 900, 70),
-         (7, 1, 5), (16, 257, 96), (17, 512, 48),
+SIZES = [(1, 64, 64), (1, 1024, 4096), (2, 130, 33), (3, 5000, 40), (4, 4096, 20), (4, 4097, 17),
+         (5, 900, 70), (7, 1, 5), (16, 257, 96), (17, 512, 48),
          (31, 1031, 200), (32, 4096, 64), (33, 127, 65), (64, 128, 64), (65, 129, 127),
-         (130, 768, 300), (257, 384, 257), (866, 768, 640), (1301, 770, 1999), (300, 5000, 96), (40, 20000, 70), (129, 9000, 33),
+         (130, 768, 300), (257, 384, 257), (866, 768, 640), (1301, 770, 1999), (300, 5000, 96),
+         (40, 20000, 70), (129, 9000, 33),
          (2600, 512, 2304)]
 
 
@@ -79,8 +80,8 @@ def test_epilogues(rt, rng, m, k, n):
 
 
 @pytest.mark.parametrize("act", [vh.VK_GATE_SILU, vh.VK_GATE_GELU])
-@pytest.mark.parametrize("m,k,h,out", [(1, 1536, 4096, "f32"), (1, 7, 1, "f32"), (15, 130, 31, "bf16"),
-                                       (32, 384, 96, "f16"), (33, 384, 33, "f32"),
+@pytest.mark.parametrize("m,k,h,out", [(1, 1536, 4096, "f32"), (1, 7, 1, "f32"),
+                                       (15, 130, 31, "bf16"), (32, 384, 96, "f16"), (33, 384, 33, "f32"),
                                        (130, 257, 191, "f32"), (866, 256, 683, "bf16"),
                                        (2700, 200, 1365, "f32")])
 def test_gated(rt, rng, m, k, h, out, act):
@@ -153,7 +154,8 @@ def test_weights_quantised_here(rt, rng):
     x = rows_of(rng, 70, k)
     codes, s = ff.quantised(w.T.copy())
     got = [run(rt, lin, x, "f32", n, "f32", lambda lin, *a: lin.run_into(*a)) for lin in
-           (rt.prepare_linear_i8_f32(k, n, w), rt.prepare_linear_i8(k, n, codes.astype(np.int8), s))]
+           (rt.prepare_linear_i8_f32(k, n, w),
+            rt.prepare_linear_i8(k, n, codes.astype(np.int8), s))]
     np.testing.assert_array_equal(*got)
     assert np.isnan(got[0][:, 4]).all() and (got[0][:, 3] == 0).all()
 
@@ -173,7 +175,8 @@ def test_guard_values_stay(rt, rng):
         room = rt.upload_f32(np.full(m * n + 512, 7.0, np.float32))
         lin.run_into(rt.upload_f32(rows_of(rng, m, 96)), m, room.view(256, m * n))
         got = room.numpy()
-        assert (got[:256] == 7).all() and (got[256 + m * n:] == 7).all() and (got[256:-256] != 7).all()
+        assert (got[:256] == 7).all() and (got[256 + m * n:] == 7).all()
+        assert (got[256:-256] != 7).all()
 
 
 @pytest.mark.parametrize("m", [1, 40, 1000])
@@ -193,6 +196,24 @@ def test_captured(rt, rng, m):
         np.testing.assert_array_equal(got, y.numpy().reshape(m, n))
         want, tol = ff.linear(h, w, s, None, None)
         ff.assert_within(got, want, tol, m)
+
+
+def test_two_runtimes_share_a_linear(rng):
+    """Queued together, each with its own codes of x, sums and counters; few tiles of a long k."""
+    a, b = vh.Runtime(0), vh.Runtime(0)
+    calls = []
+    for m, k, n in ((40, 20000, 70), (866, 768, 640), (8, 300, 90)):
+        w, s = weights(rng, k, n)
+        lin = a.prepare_linear_i8(k, n, w, s)
+        for r in (a, b):
+            x, y = rows_of(rng, m, k), r.alloc_f32(m * n)
+            calls.append((r, lin, r.upload_f32(x), m, y, ff.linear(x, w, s, None, None)))
+    for _ in range(4):
+        for r, lin, x, m, y, _ in calls:
+            assert vh.lib.vk_linear_i8_run_into(r.handle, lin.handle, x.handle, m, y.handle) == 0
+    for r, _, _, m, y, (want, tol) in calls:
+        r.synchronize()
+        ff.assert_within(y.numpy(), want, tol, m)
 
 
 def test_refusals(rt, rng):

@@ -66,7 +66,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place,
+                                  stages_, acc))
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
@@ -90,8 +91,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
           *C::at(chunk, lane, j, q) = h;
         }
       vkd::wave_lds_fence();
-      C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32, g.M,
-                               n0 + T::b_row(wn, 0), g.N);
+      C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, m0 + (wm * T::MT + i) * 32,
+                               g.M, n0 + T::b_row(wn, 0), g.N);
       vkd::wave_lds_fence();
     }
   });
@@ -110,7 +111,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   load_bias<KIND, T>(g, n0, bias);
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+  if (!vkp::product_tile<KIND, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place,
+                                  stages_, acc))
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::NT / 2;
@@ -190,9 +192,10 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   }
 }
 
-// One of the products of steps 2 and 3: out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a as
-// rows or columns, b as columns.  With m_half > 0 a's rows come in two halves: row m < m_half is out's
-// m where that is below M / 2, row m >= m_half out's M / 2 + m - m_half where that is below M.
+// One of the products of steps 2 and 3: out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a
+// as rows or columns, b as columns.  With m_half > 0 a's rows come in two halves: row m < m_half is
+// out's m where that is below M / 2, row m >= m_half out's M / 2 + m - m_half where that is below
+// M.
 struct Product {
   Operand a, b;
   int k_bytes;
@@ -203,7 +206,7 @@ struct Product {
 };
 
 template <Kind KIND, typename T, bool AC>
-__device__ __forceinline__ void product(const Product& g, int wg, char* const (&stages_)[5]) {
+__device__ __forceinline__ void product(const Product& g, int wg, char* const (&stages_)[4]) {
   typedef typename vkp::Value<KIND>::type V;
   const int tiles = g.gm * g.gn, tile = wg % tiles, part = wg / tiles;
   int mt, nt;
@@ -211,7 +214,8 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
   const int m0 = mt * T::TM, n0 = nt * T::TN;
   const vkp::Place<T> place;
   vkp::f32x16 acc[T::MT][T::NT];
-  if (!vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+  if (!vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles,
+                                            place, stages_, acc))
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   typedef vkp::Chunk<V, T::NT> C;
@@ -236,13 +240,14 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
         end = g.M;
       }
     }
-    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end, n0 + T::b_row(wn, 0),
-                             g.N);
+    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end,
+                             n0 + T::b_row(wn, 0), g.N);
     vkd::wave_lds_fence();
   }
 }
 
-// dbias: the tiles' sums of sixteen columns, eight runs of parts each in order, then the runs in order.
+// dbias: the tiles' sums of sixteen columns, eight runs of parts each in order, then the runs in
+// order.
 struct BiasSums {
   const float* sums;  // [parts, cols]
   int parts, cols;
@@ -273,9 +278,8 @@ __device__ __forceinline__ void bias_gradient(const BiasSums& g, int block, char
 // Steps 2 to 4 in one launch: they need the same step before them, and few rows leave the card
 // half empty one after another.  Workgroups 0 .. n_bias are dbias, the next n_dx dx, the others dw.
 template <Kind KIND, typename T>
-__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gradients_kernel(Product dx, Product dw,
-                                                                              BiasSums bias, int n_bias,
-                                                                              int n_dx) {
+__global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gradients_kernel(
+    Product dx, Product dw, BiasSums bias, int n_bias, int n_dx) {
   VK_STAGES(T);
   const int wg = blockIdx.x;
   if (wg < n_bias)
@@ -299,15 +303,17 @@ __global__ __launch_bounds__(vkp::kFewThreads) void gated_few_kernel(Args g) {
     const float gate = vkp::few_sum<KIND, RT, true>(smem, 0, m, e & 15) + bias_at<KIND>(g, n);
     const float up = vkp::few_sum<KIND, RT, true>(smem, 1, m, e & 15) + bias_at<KIND>(g, g.N + n);
     vkp::with_act(g.act, [&](auto act) {
-      static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] = static_cast<V>(vkp::gate<act.value>(gate) * up);
+      static_cast<V*>(g.out)[static_cast<size_t>(m) * g.N + n] =
+          static_cast<V>(vkp::gate<act.value>(gate) * up);
     });
   }
 }
 
 // ---------------------------------------------------------------- layouts
 // Rows of x, then of w, of `cols` 16-bit values into rows of 8 `pieces`, zeros behind.
-__global__ __launch_bounds__(256) void pad16_kernel(const char* __restrict__ x, const char* __restrict__ w,
-                                                    size_t x_rows, size_t rows, int cols, int pieces,
+__global__ __launch_bounds__(256) void pad16_kernel(const char* __restrict__ x,
+                                                    const char* __restrict__ w, size_t x_rows,
+                                                    size_t rows, int cols, int pieces,
                                                     char* __restrict__ to) {
   const size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x;
   const size_t row = i / static_cast<unsigned>(pieces);
@@ -369,8 +375,8 @@ int launch_forward(vk_runtime* rt, Args& g, const vkp::Plan& p) {
   return vk::check_launch("gated_kernel");
 }
 
-// x's and w's rows as operands: as they are, or where a row is no multiple of 16 bytes, copied into the
-// work buffer with zeros behind.
+// x's and w's rows as operands: as they are, or where a row is no multiple of 16 bytes, copied into
+// the work buffer with zeros behind.
 size_t operands_room(size_t rows, size_t in, size_t hidden) {
   return in % 8 == 0 ? 0 : (rows + 2 * hidden) * padded(in) * 2;
 }
@@ -386,7 +392,8 @@ BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, 
   BackwardPlan p{};
   double us = 0;
   const size_t rows = g.M, half = padded(g.N);
-  const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes};  // the zeros up to d_half too
+  // the zeros up to d_half too
+  const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes};
   p.first = vkp::plan(cus, step, &us);
   const auto D = static_cast<long long>(in);
   const vkp::Shape x{dx ? g.M : 0, D, static_cast<long long>(4 * half)};
@@ -397,14 +404,16 @@ BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, 
   // (a tile of 64 or 128 rows has two waves' sums, one of 256 four)
   if (dbias) p.work += round(((rows + 63) / 64 * 2 + 4) * 2 * g.N * 4);
   p.dx_sums = vkp::split_bytes(p.second.tile[0], vkp::Job{x, p.second.splits[0]});
-  const size_t after = p.dx_sums + vkp::split_bytes(p.second.tile[1], vkp::Job{w, p.second.splits[1]});
+  const size_t after =
+      p.dx_sums + vkp::split_bytes(p.second.tile[1], vkp::Job{w, p.second.splits[1]});
   const size_t before = vkp::split_bytes(p.first.tile, vkp::Job{step, p.first.splits});
   p.bytes = p.work + (before > after ? before : after);
   return p;
 }
 
 template <Kind KIND>
-int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, size_t in, size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
+int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, size_t in,
+             size_t hidden, char* room, vk_tensor* dx, vk_tensor* dw, vk_tensor* dbias) {
   const size_t half = padded(hidden), d_bytes = dx || dw ? (rows * 4 * half + 255) / 256 * 256 : 0;
   if (dx || dw) {
     g.d = room;
@@ -417,14 +426,15 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
     typedef decltype(tile) T;
     parts = g.gm * T::WM;
     g.gn = (static_cast<int>(half) + T::kHeld - 1) / T::kHeld;  // the zeros up to d_half too
-    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn * g.split.count), dim3(T::kThreads), 0,
-                       rt->stream, g);
+    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn * g.split.count),
+                       dim3(T::kThreads), 0, rt->stream, g);
   });
   VK_TRY(vk::check_launch("gated_grad_kernel"));
   const char* d = static_cast<char*>(g.d);
   const auto pitch = static_cast<uint32_t>(4 * half);
   const int R = static_cast<int>(rows), values = static_cast<int>((in + 7) / 8 * 8);
-  const int D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden), both = static_cast<int>(2 * half);
+  const int D = static_cast<int>(in), H2 = static_cast<int>(2 * hidden);
+  const int both = static_cast<int>(2 * half);
   Product x{}, w{};
   if (dx) {
     x.a = Operand{d, R, pitch};
@@ -453,7 +463,8 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
   // (the first step's split sums are done with)
   const vkp::PlanTwo& two = plan.second;
   x.split = vkp::Split{two.splits[0], room + plan.work, rt->arrivals};
-  w.split = vkp::Split{two.splits[1], room + plan.work + plan.dx_sums, rt->arrivals + vkp::kMostTilesSplit};
+  w.split = vkp::Split{two.splits[1], room + plan.work + plan.dx_sums,
+                       rt->arrivals + vkp::kMostTilesSplit};
   // one launch, or dx in one of its own
   for (int part = two.together ? 1 : 0; part < 2; ++part) {
     vkp::with_tile<false>(two.tile[part], [&](auto tile) {
@@ -466,8 +477,8 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
       const int n_dx = part == 0 || two.together ? x.gm * x.gn * x.split.count : 0;
       const int n_dw = part == 0 ? 0 : w.gm * w.gn * w.split.count, biases = part == 0 ? 0 : n_bias;
       if (biases + n_dx + n_dw > 0)
-        hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(biases + n_dx + n_dw), dim3(T::kThreads), 0,
-                           rt->stream, x, w, sums, biases, n_dx);
+        hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(biases + n_dx + n_dw),
+                           dim3(T::kThreads), 0, rt->stream, x, w, sums, biases, n_dx);
     });
     VK_TRY(vk::check_launch("gradients_kernel"));
   }
@@ -475,10 +486,12 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
 }
 
 // ---------------------------------------------------------------- arguments
-int check16(const vk_runtime* rt, const vk_tensor* t, vk_dtype dtype, size_t len, const char* what) {
+int check16(const vk_runtime* rt, const vk_tensor* t, vk_dtype dtype, size_t len,
+            const char* what) {
   VK_REQUIRE(t && t->dtype == dtype && t->len == len,
              "gated: %s must hold %zu values of x's type (holds %zu)", what, len, t ? t->len : 0);
-  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0, "gated: %s must be 16-byte aligned", what);
+  VK_REQUIRE(reinterpret_cast<uintptr_t>(t->ptr) % 16 == 0, "gated: %s must be 16-byte aligned",
+             what);
   return vk::check_device(rt, t, what);
 }
 
@@ -489,20 +502,20 @@ int check_inputs(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const v
   VK_REQUIRE(in > 0 && hidden > 0, "gated: empty weights");
   VK_REQUIRE(act == VK_GATE_SILU || act == VK_GATE_GELU, "gated: unknown activation %d", act);
   // a tile addresses its rows of an operand by 31 bits
-  VK_UNSUPPORTED_IF(in > 0x100000 || hidden > 0x100000 || rows > 0x1000000, "gated: %zu x %zu -> %zu",
-                    rows, in, hidden);
-  VK_UNSUPPORTED_IF(2 * hidden * padded(in) * 2 > 0x7fffff00ULL, "gated: weights of %zu x %zu", 2 * hidden,
-                    in);
-  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((hidden + 31) / 32) > 0x7fffffULL, "gated: %zu x %zu outputs",
-                    rows, hidden);
+  VK_UNSUPPORTED_IF(in > 0x100000 || hidden > 0x100000 || rows > 0x1000000,
+                    "gated: %zu x %zu -> %zu", rows, in, hidden);
+  VK_UNSUPPORTED_IF(2 * hidden * padded(in) * 2 > 0x7fffff00ULL, "gated: weights of %zu x %zu",
+                    2 * hidden, in);
+  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((hidden + 31) / 32) > 0x7fffffULL,
+                    "gated: %zu x %zu outputs", rows, hidden);
   VK_TRY(check16(rt, x, x->dtype, rows * in, "x"));
   VK_TRY(check16(rt, w, x->dtype, 2 * hidden * in, "w"));
   if (bias) VK_TRY(check16(rt, bias, x->dtype, 2 * hidden, "bias"));
   return VK_OK;
 }
 
-Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
-                  size_t rows, size_t in, size_t hidden, int act) {
+Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
+                  const vk_tensor* bias, size_t rows, size_t in, size_t hidden, int act) {
   Args g{};
   const char* xp = static_cast<const char*>(x->ptr);
   const char* wp = static_cast<const char*>(w->ptr);
@@ -522,7 +535,8 @@ int align_operands(const vk_runtime* rt, Args& g, size_t in, char* room) {
   if (in % 8 == 0) return VK_OK;
   const size_t rows = g.a.rows, all = rows + g.b.rows, pieces = padded(in) / 8;
   VK_UNSUPPORTED_IF(all * pieces > 0x7fffffULL * 256, "gated: %zu rows of %zu", all, in);
-  hipLaunchKernelGGL(pad16_kernel, dim3((all * pieces + 255) / 256), dim3(256), 0, rt->stream, g.a.base,
+  hipLaunchKernelGGL(pad16_kernel, dim3((all * pieces + 255) / 256), dim3(256), 0, rt->stream,
+                     g.a.base,
                      g.b.base, rows, all, static_cast<int>(in), static_cast<int>(pieces), room);
   g.a.pitch = g.b.pitch = static_cast<uint32_t>(2 * padded(in));
   g.a.base = room;
@@ -535,11 +549,13 @@ int align_operands(const vk_runtime* rt, Args& g, size_t in, char* room) {
 extern "C" {
 
 int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const vk_tensor* bias,
-                     size_t rows, size_t in_features, size_t hidden, int activation, vk_tensor* out) {
+                     size_t rows, size_t in_features, size_t hidden, int activation,
+                     vk_tensor* out) {
   VK_TRY(vk::bind(rt));
   VK_TRY(check_inputs(rt, x, w, bias, rows, in_features, hidden, activation));
   VK_TRY(check16(rt, out, x->dtype, rows * hidden, "out"));
-  for (const vk_tensor* t : {x, w, bias}) VK_REQUIRE(!vk::overlap(out, t), "gated: out overlaps an input");
+  for (const vk_tensor* t : {x, w, bias})
+    VK_REQUIRE(!vk::overlap(out, t), "gated: out overlaps an input");
   if (rows == 0) return VK_OK;
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
   g.out = out->ptr;
@@ -570,7 +586,8 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
   for (int i = 0; i < 3; ++i) {
     for (const vk_tensor* t : {x, w, bias, grad})
       VK_REQUIRE(!vk::overlap(outs[i], t), "gated: a gradient overlaps an input");
-    for (int j = 0; j < i; ++j) VK_REQUIRE(!vk::overlap(outs[i], outs[j]), "gated: gradients overlap");
+    for (int j = 0; j < i; ++j)
+      VK_REQUIRE(!vk::overlap(outs[i], outs[j]), "gated: gradients overlap");
   }
   if (rows == 0) {  // sums of nothing
     if (dw) zero16(rt, dw->ptr, dw->len);

@@ -207,7 +207,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
   }
   const vkp::Place<T> place;
   vkp::i32x16 acc[T::MT][T::NT];
-  if (!vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place, stages_, acc))
+  if (!vkp::product_tile<kI8, T>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles, place,
+                                 stages_, acc))
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
@@ -228,7 +229,9 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
             const int j = jg + jj, c = T::b_row(wn, j) + 8 * q + 4 * (lane >> 5);
-            const auto at = [&](int p, int c_) { return *reinterpret_cast<const vkp::f32x4*>(&cols[p][c_]); };
+            const auto at = [&](int p, int c_) {
+              return *reinterpret_cast<const vkp::f32x4*>(&cols[p][c_]);
+            };
             const vkp::f32x4 s = at(0, c), b = at(1, c);
             vkp::f32x4 v;
 #pragma unroll
@@ -250,7 +253,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
             *C::at(chunk, lane, jj, q) = w;
           }
         vkd::wave_lds_fence();
-        C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg), g.N);
+        C::template store<END == kResidual>(chunk, lane, out, g.N, mb, g.M, n0 + T::b_row(wn, jg),
+                                            g.N);
         vkd::wave_lds_fence();
       }
     }
@@ -263,7 +267,8 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
 
 // What leaves after the waves' sums are joined: thread by thread.
 template <int END, typename V, int RT>
-__device__ __forceinline__ void few_finish(const Args& g, const char* smem, int n0, const float* scales) {
+__device__ __forceinline__ void few_finish(const Args& g, const char* smem, int n0,
+                                           const float* scales) {
   constexpr bool kPaired = END == kGated;
   for (int e = threadIdx.x; e < 256 * RT; e += vkp::kFewThreads) {
     const int m = e >> 4, n = n0 + (e & 15);
@@ -295,8 +300,8 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_few_kernel(Args g)
 }
 
 // Rows of at most kOwnBytes of codes in all: every workgroup quantises them for itself, in one
-// launch, while its weights are on their way.  Thread by thread eight values; sixteen lanes are of one
-// row, whose maximum meets in LDS.
+// launch, while its weights are on their way.  Thread by thread eight values; sixteen lanes are of
+// one row, whose maximum meets in LDS.
 template <typename XT>
 __device__ __forceinline__ void load8_of(const Args& g, int m, int at, float (&v)[8]) {
   load8(static_cast<const XT*>(g.x) + static_cast<size_t>(m) * g.K, at, g.K - at, v);
@@ -354,7 +359,8 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g
       },
       [&](int, int k) {
         vkp::i32x4 a = {0, 0, 0, 0};
-        if (c < g.M && k < g.k_bytes) a = *reinterpret_cast<const vkp::i32x4*>(codes + c * pitch + k);
+        if (c < g.M && k < g.k_bytes)
+          a = *reinterpret_cast<const vkp::i32x4*>(codes + c * pitch + k);
         return a;
       },
       [](int) { return vkp::i32x4{0, 0, 0, 0}; });
@@ -390,8 +396,8 @@ template <int END, typename V>
 int launch(vk_runtime* rt, Args& g, const vkp::Plan& p) {
   constexpr bool kPaired = END == kGated;
   if (g.x) {
-    hipLaunchKernelGGL((linear_i8_rows_kernel<END, V>), dim3((g.N + 15) / 16), dim3(vkp::kFewThreads), 0,
-                       rt->stream, g);
+    hipLaunchKernelGGL((linear_i8_rows_kernel<END, V>), dim3((g.N + 15) / 16),
+                       dim3(vkp::kFewThreads), 0, rt->stream, g);
     return vk::check_launch("linear_i8_rows_kernel");
   }
   if (p.few) {
@@ -409,8 +415,8 @@ int launch(vk_runtime* rt, Args& g, const vkp::Plan& p) {
     g.group = vkp::kGroupRows / T::TM;
     g.split.count = p.splits;
     g.split.arrivals = rt->arrivals;
-    hipLaunchKernelGGL((linear_i8_kernel<END, V, T>), dim3(g.gm * g.gn * p.splits), dim3(T::kThreads), 0,
-                       rt->stream, g);
+    hipLaunchKernelGGL((linear_i8_kernel<END, V, T>), dim3(g.gm * g.gn * p.splits),
+                       dim3(T::kThreads), 0, rt->stream, g);
   });
   return vk::check_launch("linear_i8_kernel");
 }
@@ -455,8 +461,8 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
   VK_REQUIRE(end != kResidual || out->dtype == VK_F32, "linear_i8: residual must be f32");
   VK_REQUIRE(!vk::overlap(x, out), "linear_i8: the output overlaps x");
   if (rows == 0) return VK_OK;
-  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((N + 31) / 32) > 0x7fffffULL, "linear_i8: %zu x %zu outputs",
-                    rows, N);
+  VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((N + 31) / 32) > 0x7fffffULL,
+                    "linear_i8: %zu x %zu outputs", rows, N);
 
   const int M = static_cast<int>(rows);
   const vkp::Plan p = vkp::plan(rt->cu_count, M, static_cast<long long>(lin->out_features),
@@ -468,7 +474,8 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
     g.x_type = x->dtype;
   } else {
     const size_t code_bytes = rows * lin->pitch, scale_bytes = (rows * 4 + 255) / 256 * 256;
-    const vkp::Shape shape{M, static_cast<long long>(lin->out_features), static_cast<long long>(lin->pitch)};
+    const vkp::Shape shape{M, static_cast<long long>(lin->out_features),
+                           static_cast<long long>(lin->pitch)};
     const size_t sums = p.few ? 0 : vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});
     VK_TRY(vk::ensure_work(rt, (code_bytes + scale_bytes + sums) / 4, "linear_i8"));
     char* codes = reinterpret_cast<char*>(rt->work);  // (code_bytes: a multiple of 128)
@@ -508,9 +515,10 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
 // ---------------------------------------------------------------- weights
 int check_prepare(size_t in, size_t out) {
   VK_REQUIRE(in > 0 && out > 0, "linear_i8: empty");
-  VK_UNSUPPORTED_IF(in > kMostK, "linear_i8: in_features=%zu (at most %zu: the int32 sum)", in, kMostK);
-  VK_UNSUPPORTED_IF(out > 0x7fffff00ULL / ((in + 127) / 128 * 128), "linear_i8: %zu x %zu weights", in,
-                    out);
+  VK_UNSUPPORTED_IF(in > kMostK, "linear_i8: in_features=%zu (at most %zu: the int32 sum)", in,
+                    kMostK);
+  VK_UNSUPPORTED_IF(out > 0x7fffff00ULL / ((in + 127) / 128 * 128), "linear_i8: %zu x %zu weights",
+                    in, out);
   return VK_OK;
 }
 
@@ -521,8 +529,8 @@ int upload(void** dev, const void* host, size_t bytes) {
 }
 
 // codes [out, pitch]
-int make(vk_runtime* rt, size_t in, size_t out, const std::vector<int8_t>& codes, const float* scale,
-         const float* bias, const float* ls, vk_linear_i8** res) {
+int make(vk_runtime* rt, size_t in, size_t out, const std::vector<int8_t>& codes,
+         const float* scale, const float* bias, const float* ls, vk_linear_i8** res) {
   auto* lin = new (std::nothrow) vk_linear_i8;
   if (!lin) return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
   lin->rt = rt;
@@ -584,7 +592,8 @@ int vk_linear_i8_prepare_f32(vk_runtime* rt, size_t in_features, size_t out_feat
   for (size_t i = 0; i < in_features; ++i)
     for (size_t o = 0; o < out_features; ++o)
       if (scale[o] > 0.0f)
-        w[o * pitch + i] = static_cast<int8_t>(std::nearbyint(weight_in_out[i * out_features + o] / scale[o]));
+        w[o * pitch + i] =
+            static_cast<int8_t>(std::nearbyint(weight_in_out[i * out_features + o] / scale[o]));
   return make(rt, in_features, out_features, w, scale.data(), bias, ls_gamma, out);
 } catch (const std::bad_alloc&) {
   return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");

@@ -71,9 +71,9 @@ struct Ops<kI8> {
 //   Rows (k contiguous): row r at base + r * pitch, k_bytes of k; what lies between k_bytes and
 //     the next multiple of 16 is zeros.
 //   Columns (16-bit types): k's values at base + k * pitch, `rows` of them, a multiple of
-//     8; `ks` of k.  With k_half > 0 (a multiple of 64) k comes in two halves: k < k_half is line k where
-//     that is below ks / 2, k >= k_half line ks / 2 + k - k_half where that is below ks; zeros
-//     otherwise.
+//     8; `ks` of k.  With k_half > 0 (a multiple of 64) k comes in two halves: k < k_half is line
+//     k where that is below ks / 2, k >= k_half line ks / 2 + k - k_half where that is below ks;
+//     zeros otherwise.
 struct Operand {
   const char* base;
   int rows;
@@ -91,21 +91,20 @@ constexpr uint32_t kMostBytes = 0x7ffffff0u;
 // the partners.
 // KG groups of waves share k out by stages and are added in their order at the end: for
 // grids of few tiles.
-template <int WM_, int WN_, int MT_, int NT_, bool PAIRED_, int S_, int R_, int KG_>
+template <int WM_, int WN_, int MT_, int NT_, bool PAIRED_, int R_, int KG_>
 struct Tile {
   static constexpr int WM = WM_, WN = WN_, MT = MT_, NT = NT_, KG = KG_;
-  static constexpr int S = S_, R = R_;  // bytes of k of a stage, stage buffers
+  static constexpr int R = R_;  // stage buffers
   static constexpr bool PAIRED = PAIRED_;
   static constexpr int kWaves = WM * WN;  // of a group
   static constexpr int kThreads = 64 * kWaves * KG;
   static constexpr int TM = 32 * WM * MT, TN = 32 * WN * NT;
   static constexpr int kHeld = PAIRED ? TN / 2 : TN;  // columns of the result
-  static constexpr int kRows = 1024 / S;  // rows of a wave's load
+  static constexpr int kRows = 1024 / kStage;  // rows of a wave's load
   static constexpr int kALoads = TM / kRows / kWaves, kBLoads = TN / kRows / kWaves;
-  static constexpr int kGroupBytes = (TM + TN) * S, kBytes = KG * kGroupBytes;
+  static constexpr int kGroupBytes = (TM + TN) * kStage, kBytes = KG * kGroupBytes;
   static_assert((KG - 1) * TM * TN * 4 <= kBytes, "a group's sums fit a stage buffer");
   static constexpr int kWavesASimd = MT * NT > 8 ? 1 : 2;  // by the registers of the sums
-  static_assert(S == 128 || S == 64, "a row's stage");
   static_assert(kALoads * kWaves * kRows == TM && kBLoads * kWaves * kRows == TN,
                 "loads divide evenly");
   static_assert(!PAIRED || NT % 2 == 0, "gates and partners");
@@ -124,14 +123,14 @@ struct Tile {
 template <bool PAIRED, typename F>
 void with_tile(TileSize size, F go) {
   if (size == kTile256) {
-    if constexpr (PAIRED) go(Tile<4, 2, 2, 4, true, 128, 2, 1>{});
-    else go(Tile<2, 4, 4, 2, false, 128, 2, 1>{});
+    if constexpr (PAIRED) go(Tile<4, 2, 2, 4, true, 2, 1>{});
+    else go(Tile<2, 4, 4, 2, false, 2, 1>{});
   } else if (size == kTile128) {
-    go(Tile<2, 2, 2, 2, PAIRED, 128, 2, 1>{});
+    go(Tile<2, 2, 2, 2, PAIRED, 2, 1>{});
   } else if (size == kTile64K) {
-    go(Tile<2, 1, 1, 2, PAIRED, 128, 4, 2>{});
+    go(Tile<2, 1, 1, 2, PAIRED, 4, 2>{});
   } else {
-    go(Tile<2, 1, 1, 2, PAIRED, 128, 2, 1>{});
+    go(Tile<2, 1, 1, 2, PAIRED, 2, 1>{});
   }
 }
 
@@ -162,8 +161,7 @@ __device__ __forceinline__ void tile_done() {
   __shared__ __align__(16) char s1_[T::kBytes];                          \
   __shared__ __align__(16) char s2_[T::R > 2 ? T::kBytes : 16];          \
   __shared__ __align__(16) char s3_[T::R > 3 ? T::kBytes : 16];          \
-  __shared__ __align__(16) char s4_[T::R > 4 ? T::kBytes : 16];          \
-  char* const stages_[5] = {s0_, s1_, s2_, s3_, s4_}
+  char* const stages_[4] = {s0_, s1_, s2_, s3_}
 
 // A buffer resource's parts.
 struct Source {
@@ -179,10 +177,10 @@ __device__ __forceinline__ Source rows_of(const Operand& o, int r0) {
 }
 
 // 16 bytes a lane from source + lane offset (zeros past its bytes) + k into LDS.  BY_HAND: the
-// instruction itself, which the compiler does not count: it would wait for every load under way before
-// a transposing read, whose buffer it does not see.  No register is written, and what has to be
-// waited for is waited for by stage_barrier and tile_done.  (The s_nop covers scalar operands that a
-// vector instruction may just have written.)
+// instruction itself, which the compiler does not count: it would wait for every load under way
+// before a transposing read, whose buffer it does not see.  No register is written, and what has to
+// be waited for is waited for by stage_barrier and tile_done.  (The s_nop covers scalar operands
+// that a vector instruction may just have written.)
 template <bool BY_HAND>
 __device__ __forceinline__ void load_lds(const Source& s, char* to, uint32_t lane_off, int k) {
   if constexpr (BY_HAND) {
@@ -191,8 +189,8 @@ __device__ __forceinline__ void load_lds(const Source& s, char* to, uint32_t lan
                      static_cast<int>(s.bytes), 0x00020000};
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds"
                  :
-                 : "s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(to)))), "v"(lane_off),
-                   "s"(r), "s"(k)
+                 : "s"(static_cast<uint32_t>(reinterpret_cast<uintptr_t>((lds_ptr)(to)))),
+                   "v"(lane_off), "s"(r), "s"(k)
                  : "memory", "m0");
   } else {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(vkd::buffer_rsrc(s.base, s.bytes), (lds_ptr)(to), 16,
@@ -219,7 +217,8 @@ __device__ __forceinline__ Source columns_of(const Operand& o, int st, int stop)
     }
   }
   const int lines = line < end && st < stop ? (end - line < 64 ? end - line : 64) : 0;
-  return Source{o.base + static_cast<size_t>(line) * o.pitch, static_cast<uint32_t>(lines) * o.pitch};
+  return Source{o.base + static_cast<size_t>(line) * o.pitch,
+                static_cast<uint32_t>(lines) * o.pitch};
 }
 
 // A lane's offsets in a stage's lines, of values c0 ...
@@ -232,7 +231,8 @@ __device__ __forceinline__ void columns_at(const Operand& o, int c0, int lane, i
     const int line = (wave + i * WAVES) * kLines + lane / kPieces;
     const int piece = (lane % kPieces) ^ column_turn<W>(line);
     const int c = c0 + piece * 8;
-    v[i] = c < o.rows ? static_cast<uint32_t>(line) * o.pitch + 2u * static_cast<uint32_t>(c) : kOutside;
+    const uint32_t at = static_cast<uint32_t>(line) * o.pitch + 2u * static_cast<uint32_t>(c);
+    v[i] = c < o.rows ? at : kOutside;
   }
 }
 
@@ -268,27 +268,28 @@ struct Place {
   }
 };
 
-// A launch may share a tile's k out over `count` workgroups: each leaves its sums in `partial`, and the
-// one that arrives last adds all of them, in their order whoever it is, and goes on.  For few tiles of
-// a long k.
+// A launch may share a tile's k out over `count` workgroups: each leaves its sums in `partial`, and
+// the one that arrives last adds all of them, in their order whoever it is, and goes on.  For few
+// tiles of a long k.
 struct Split {
   int count;
   char* partial;       // [count][tiles][a tile's sums]
   unsigned* arrivals;  // [tiles], zeros before and after a launch
 };
 
-// Leaves a wave's sums; whether its workgroup is its tile's last one, whose acc is then the sum of all
-// parts'.  Nobody waits for anybody.  The sums go past the L2 of the XCD, 8 bytes at a time, in both
-// directions (agent scope), so that they are where every XCD sees them once the wave's stores have
-// returned, and a fence, which would write back and drop the whole L2, is not needed: with fences a
-// launch of this kind took 44 us in place of 11.
+// Leaves a wave's sums; whether its workgroup is its tile's last one, whose acc is then the sum of
+// all parts'.  Nobody waits for anybody.  The sums go past the L2 of the XCD, 8 bytes at a time, in
+// both directions (agent scope), so that they are where every XCD sees them once the wave's stores
+// have returned, and a fence, which would write back and drop the whole L2, is not needed: with
+// fences a launch of this kind took 44 us in place of 11.
 template <Kind KIND, typename T>
 __device__ __forceinline__ bool last_of_split(const Split& split, int part, int tile, int tiles,
                                               const Place<T>& at,
                                               typename Ops<KIND>::Acc16 (&acc)[T::MT][T::NT]) {
   typedef decltype(typename Ops<KIND>::Acc4{}[0] + 0) S;
   typedef S S2 __attribute__((ext_vector_type(2)));
-  constexpr int kPairs = T::MT * T::NT * 8, kSums = T::kWaves * kPairs * 64;  // pairs of a lane, a tile
+  // pairs of a lane, a tile
+  constexpr int kPairs = T::MT * T::NT * 8, kSums = T::kWaves * kPairs * 64;
   __shared__ unsigned arrived;
   uint64_t* mine = reinterpret_cast<uint64_t*>(split.partial) + static_cast<size_t>(tile) * kSums +
                    at.wave * kPairs * 64 + at.lane;
@@ -303,7 +304,8 @@ __device__ __forceinline__ bool last_of_split(const Split& split, int part, int 
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's sums have arrived, then the count
   __syncthreads();
   if (threadIdx.x == 0)
-    arrived = __hip_atomic_fetch_add(&split.arrivals[tile], 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    arrived = __hip_atomic_fetch_add(&split.arrivals[tile], 1u, __ATOMIC_RELAXED,
+                                     __HIP_MEMORY_SCOPE_AGENT);
   __syncthreads();
   if (arrived + 1 != static_cast<unsigned>(split.count)) return false;
   if (threadIdx.x == 0)
@@ -338,28 +340,25 @@ __device__ __forceinline__ bool last_of_split(const Split& split, int part, int 
 }
 
 // acc[mt][nt] of this wave: the tile's rows from m0, columns from n0 (of the
-// hidden ones, where PAIRED), over all of k, where the wave is to go on with them: with KG > 1 those of
-// group 0, with a split those of the tile's last workgroup.  AC, BC: a, b as columns.
+// hidden ones, where PAIRED), over all of k, where the wave is to go on with them: with KG > 1
+// those of group 0, with a split those of the tile's last workgroup.  AC, BC: a, b as columns.
 template <Kind KIND, typename T, bool AC = false, bool BC = false>
 __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b, int k_bytes,
                                              int m0, int n0, const Split& split, int part, int tile,
                                              int tiles, const Place<T>& at,
-                                             char* const (&stages_)[5],
+                                             char* const (&stages_)[4],
                                              typename Ops<KIND>::Acc16 (&acc)[T::MT][T::NT]) {
-  constexpr int S = T::S, R = T::R, KG = T::KG, KS = S / 32;
+  constexpr int S = kStage, R = T::R, KG = T::KG, KS = S / 32;
   const int lane = at.lane, wave = at.wave, wm = at.wm, wn = at.wn;
   char* buf[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) buf[i] = stages_[i] + at.group * T::kGroupBytes;
 
-  // Loads of rows: 1 KiB an instruction, a lane 16 bytes.  With 128-byte rows bit 3 of a
-  // row is the lowest of the wave (rows from 8 (wave + i kWaves)).
+  // Loads of rows: 1 KiB an instruction, a lane 16 bytes.  Bit 3 of a row is the lowest of the
+  // wave (rows from 8 (wave + i kWaves)).
   static_assert(T::kWaves % 2 == 0, "the permutation of a lane's rows is one");
-  static_assert(S == 128 || !(AC || BC), "columns in stages of 64 k");
-  const int lr = S == 128 ? lane >> 3 : lane >> 2;
-  const uint32_t piece =
-      16u * static_cast<uint32_t>(S == 128 ? (lane & 7) ^ (4 * (wave & 1) + (lr >> 1))
-                                           : (lane & 3) ^ (lr >> 2));
+  const int lr = lane >> 3;
+  const uint32_t piece = 16u * static_cast<uint32_t>((lane & 7) ^ (4 * (wave & 1) + (lr >> 1)));
   uint32_t av[T::kALoads], bv[T::kBLoads];
   Source sa{}, sb{};
   if constexpr (!AC) sa = rows_of(a, m0);
@@ -418,7 +417,7 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
 
   // Fragment reads: step ks of a stage is pieces 2 ks + lane / 32.
   const int fr = lane & 31;
-  const int at0 = fr * S + (((lane >> 5) ^ (S == 128 ? (fr >> 1) & 7 : (fr >> 2) & 3)) << 4);
+  const int at0 = fr * S + (((lane >> 5) ^ ((fr >> 1) & 7)) << 4);
   const int a0 = at0 + wm * T::MT * 32 * S;
   i32x4 fa[2][T::MT], fb[2][T::NT];
   constexpr int kReads = T::MT + T::NT;
@@ -428,7 +427,8 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
       if constexpr (BC)
         fb[ks & 1][i] = read_columns<T::TN>(fb_at, lane, ks, T::b_row(wn, i));
       else
-        fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(fb_at + (at0 ^ (ks << 5)) + T::b_row(wn, i) * S);
+        fb[ks & 1][i] = *reinterpret_cast<const i32x4*>(fb_at + (at0 ^ (ks << 5)) +
+                                                        T::b_row(wn, i) * S);
     } else {
       const int r = i - T::NT;
       if constexpr (AC)
@@ -442,7 +442,8 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
   // load path holds the matrix pipe up.
   auto step = [&](auto reads, auto loads, int ks, const char* next, int nks, char* to, int t) {
     constexpr int kTiles = T::MT * T::NT;
-    constexpr int kReadsEach = (kReads + kTiles - 1) / kTiles, kLoadsEach = (kLoads + kTiles - 1) / kTiles;
+    constexpr int kReadsEach = (kReads + kTiles - 1) / kTiles;
+    constexpr int kLoadsEach = (kLoads + kTiles - 1) / kTiles;
 #pragma unroll
     for (int e = 0; e < kTiles; ++e) {
       const int i = e / T::NT, j = e % T::NT;
@@ -450,7 +451,8 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
       __builtin_amdgcn_sched_barrier(0);
       if constexpr (reads.value)
 #pragma unroll
-        for (int r = e * kReadsEach; r < (e + 1) * kReadsEach && r < kReads; ++r) read(next, nks, r);
+        for (int r = e * kReadsEach; r < (e + 1) * kReadsEach && r < kReads; ++r)
+          read(next, nks, r);
       if constexpr (loads.value)
 #pragma unroll
         for (int l = e * kLoadsEach; l < (e + 1) * kLoadsEach && l < kLoads; ++l) load(to, t, l);
@@ -494,7 +496,8 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
       const auto& v = acc[e / 4 / T::NT][e / 4 % T::NT];
       const int r = e % 4 * 4;
       if (at.group > 0)
-        sums[(at.group - 1) * T::kWaves * kWaveSums + e * 64] = Acc4{v[r], v[r + 1], v[r + 2], v[r + 3]};
+        sums[(at.group - 1) * T::kWaves * kWaveSums + e * 64] =
+            Acc4{v[r], v[r + 1], v[r + 2], v[r + 3]};
     }
     tile_done();
     if (at.group > 0) return false;
@@ -560,7 +563,8 @@ struct Chunk {
   static __device__ __forceinline__ void fill(char* c, int lane, const i32x4 (&v)[kFetch]) {
 #pragma unroll
     for (int p = 0; p < kFetch; ++p)
-      *reinterpret_cast<i32x4*>(c + slot(p * (64 / kPieces) + lane / kPieces, lane % kPieces)) = v[p];
+      *reinterpret_cast<i32x4*>(c + slot(p * (64 / kPieces) + lane / kPieces, lane % kPieces)) =
+          v[p];
   }
   // To rows m0 .. of `out` (pitch values a row), columns n0 .., of those below M and N.  ADD: added
   // to what is there (f32).
@@ -597,12 +601,13 @@ struct Chunk {
   }
 };
 
-// Sums over lanes 0 .. 31 and over lanes 32 .. 63 of N = 32 R values a lane: lane l is left with the
-// sums of values R (l % 32) .. + R.  A step adds half of the values of two lanes that
+// Sums over lanes 0 .. 31 and over lanes 32 .. 63 of N = 32 R values a lane: lane l is left with
+// the sums of values R (l % 32) .. + R.  A step adds half of the values of two lanes that
 // differ in one more bit (lanes l and l ^ 16, 15, 7, 3, 1), in a fixed order.
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
-  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf,
+                                                            0xf, true));
 }
 template <int N, int CTRL>
 __device__ __forceinline__ void halve(float* v, bool upper) {
@@ -665,8 +670,8 @@ __device__ __forceinline__ void gate_slope(float g, float* act, float* slope) {
   }
 }
 
-// f(std::integral_constant<int, ACT>) for the activation of a launch: one branch, so that the values of a
-// tile's end overlap one another's latencies.
+// f(std::integral_constant<int, ACT>) for the activation of a launch: one branch, so that the
+// values of a tile's end overlap one another's latencies.
 template <typename F>
 __device__ __forceinline__ void with_act(int act, F f) {
   if (act == VK_GATE_SILU)
@@ -704,8 +709,9 @@ struct FewSums {
   typename Ops<KIND>::Acc4 v[PAIRED ? 2 : 1][RT];
 };
 
-// The 16 bytes of a row from byte k, zeros where they are not all below `whole`, the row's whole pieces (one
-// at least).  The row may lie at any address.  No branch: a load in one would be waited for there.
+// The 16 bytes of a row from byte k, zeros where they are not all below `whole`, the row's whole
+// pieces (one at least).  The row may lie at any address.  No branch: a load in one would be waited
+// for there.
 __device__ __forceinline__ i32x4 row_piece(const char* row, int k, int whole) {
   i32x4 v;
   const bool in = k < whole;
@@ -752,7 +758,8 @@ __device__ __forceinline__ void few_join(const FewSums<KIND, RT, PAIRED>& s, cha
 #pragma unroll
   for (int p = 0; p < (PAIRED ? 2 : 1); ++p)
 #pragma unroll
-    for (int r = 0; r < RT; ++r) red[((wave * (PAIRED ? 2 : 1) + p) * RT + r) * 64 + lane] = s.v[p][r];
+    for (int r = 0; r < RT; ++r)
+      red[((wave * (PAIRED ? 2 : 1) + p) * RT + r) * 64 + lane] = s.v[p][r];
   __syncthreads();
 }
 
@@ -774,13 +781,13 @@ constexpr int few_bytes() {
   return kFewWaves * (PAIRED ? 2 : 1) * RT * 64 * 16;
 }
 
-// The product of the columns n0 .. with at most 16 RT rows: a_at(r, k) is the lane's 16 bytes from k
-// of row 16 r + lane % 16, zeros outside, a_rest(r) the values behind the whole pieces of a row of 16-bit
-// ones.  The first columns are on their way before `first()` runs, the next ones while a stage's
-// products do.
+// The product of the columns n0 .. with at most 16 RT rows: a_at(r, k) is the lane's 16 bytes from
+// k of row 16 r + lane % 16, zeros outside, a_rest(r) the values behind the whole pieces of a row
+// of 16-bit ones.  The first columns are on their way before `first()` runs, the next ones while a
+// stage's products do.
 template <Kind KIND, int RT, bool PAIRED, typename A, typename R, typename F>
-__device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n0, char* smem, F first,
-                                            A a_at, R a_rest) {
+__device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n0, char* smem,
+                                            F first, A a_at, R a_rest) {
   constexpr int U = 2, P = PAIRED ? 2 : 1;
   const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x >> 6));
   const int lane = threadIdx.x & 63, c = lane & 15, q = lane >> 4;
@@ -801,7 +808,8 @@ __device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n
 #pragma unroll
       for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) fa[u][r][h] = a_at(r, (t + u * kFewWaves) * kStage + q * 32 + h * 16);
+        for (int h = 0; h < 2; ++h)
+          fa[u][r][h] = a_at(r, (t + u * kFewWaves) * kStage + q * 32 + h * 16);
     if (t + U * kFewWaves < stages) fb.load(rows, q, t + U * kFewWaves, whole);
 #pragma unroll
     for (int u = 0; u < U; ++u)
@@ -830,7 +838,8 @@ __device__ __forceinline__ void few_product(const Operand& b, int k_bytes, int n
   few_join<KIND, RT, PAIRED>(s, smem, wave, lane);
 }
 
-// Rows 0 .. a.rows of a in memory (rows past the last one read the last one: their sums go nowhere).
+// Rows 0 .. a.rows of a in memory (rows past the last one read the last one: their sums go
+// nowhere).
 template <Kind KIND, int RT, bool PAIRED>
 __device__ __forceinline__ void few_product(const Operand& a, const Operand& b, int k_bytes, int n0,
                                             char* smem) {
@@ -842,7 +851,8 @@ __device__ __forceinline__ void few_product(const Operand& a, const Operand& b, 
     rows[r] = a.base + static_cast<size_t>(row < a.rows ? row : a.rows - 1) * a.pitch;
   }
   few_product<KIND, RT, PAIRED>(
-      b, k_bytes, n0, smem, [] {}, [&](int r, int k) { return row_piece(rows[r], k, k_bytes & ~15); },
+      b, k_bytes, n0, smem, [] {},
+      [&](int r, int k) { return row_piece(rows[r], k, k_bytes & ~15); },
       [&](int r) { return row_rest(rows[r], k_bytes); });
 }
 

@@ -47,8 +47,8 @@ inline long long split_bytes(TileSize tile, const Job& j) {
 }
 
 // Us of one workgroup where it has a CU to itself, and a CU's us a workgroup where it has many, as
-// measured on a card of 256 CUs (866 and 10,392 rows, 384 to 8192 wide): stages of 128 bytes, the two ends,
-// and the last one's reading of its tile's parts.
+// measured on a card of 256 CUs (866 and 10,392 rows, 384 to 8192 wide): stages of 128 bytes, the
+// two ends, and the last one's reading of its tile's parts.
 struct TileCost {
   double alone, many;
 };
@@ -126,8 +126,8 @@ inline Plan plan(int cus, long long m, long long n, long long k_bytes) {
   return plan(cus, Shape{m, n, k_bytes}, &us);
 }
 
-// Two products that do not wait for one another: in one launch of one tile, or each in its own, which
-// costs a launch more.
+// Two products that do not wait for one another: in one launch of one tile, or each in its own,
+// which costs a launch more.
 struct PlanTwo {
   bool together;
   TileSize tile[2];

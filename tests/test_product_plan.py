@@ -23,9 +23,10 @@ extern "C" int own(unsigned long long rows, unsigned long long bytes) {
   return own_rows(rows, bytes);
 }
 // few, tile, splits, tiles, bytes of sums
-extern "C" void one(int cus, long long m, long long n, long long k, long long* out) {
-  const Plan p = plan(cus, m, n, k);
-  const Job j{Shape{m, n, k}, p.splits};
+extern "C" void one(int cus, int paired, long long m, long long n, long long k, long long* out) {
+  const Shape s{m, n, k, paired != 0};
+  const Plan p = plan(cus, s);
+  const Job j{s, p.splits};
   out[0] = p.few; out[1] = p.tile; out[2] = p.splits; out[3] = tiles_of(p.tile, j.shape);
   out[4] = split_bytes(p.tile, j);
 }
@@ -40,8 +41,7 @@ extern "C" void two(int cus, const long long* a, const long long* b, long long* 
   }
 }
 """
-TILES = 4
-SIDE = (64, 64, 128, 256)
+SIDES = ((64, 64), (64, 64), (128, 128), (256, 192), (256, 256))
 
 
 @pytest.fixture(scope="module")
@@ -53,14 +53,14 @@ def lib():
         subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC",
                         "-I", plans._CSRC, src, "-o", out], check=True)
         lib = ctypes.CDLL(out)
-    lib.one.argtypes = [ctypes.c_int] + [ctypes.c_longlong] * 3 + [ctypes.c_void_p]
+    lib.one.argtypes = [ctypes.c_int] * 2 + [ctypes.c_longlong] * 3 + [ctypes.c_void_p]
     lib.own.argtypes = [ctypes.c_ulonglong] * 2
     return lib
 
 
-def one(lib, m, n, k, cus=256):
+def one(lib, m, n, k, cus=256, paired=False):
     out = (ctypes.c_longlong * 5)()
-    lib.one(cus, m, n, k, out)
+    lib.one(cus, paired, m, n, k, out)
     return tuple(out)
 
 
@@ -81,26 +81,28 @@ def sizes(n, seed):
     return [[int(2 ** rng.uniform(0, top)) for top in (15, 13, 14)] for _ in range(n)]
 
 
-def holds(tile, splits, tiles, sums, shape, cus):
+def holds(tile, splits, tiles, sums, shape, cus, paired=False):
     """What a launch relies on: counters for every tile that is shared out, parts of two stages
     at least, at most two workgroups a CU, and not for the largest tiles."""
-    assert 0 <= tile < TILES and splits >= 1
+    assert 0 <= tile < len(SIDES) and splits >= 1
     m, n, k = shape
-    assert tiles == -(-m // SIDE[tile]) * -(-n // SIDE[tile])
+    rows, cols = SIDES[tile][::-1] if paired else SIDES[tile]
+    assert tiles == -(-m // rows) * -(-n // cols)
     if splits == 1:
         assert sums == 0
         return
-    assert tile != 3 and tiles <= 1024 and tiles * splits <= 2 * cus
+    assert tile < 3 and tiles <= 1024 and tiles * splits <= 2 * cus
     assert 2 * splits <= -(-k // 128)
-    assert sums == tiles * splits * SIDE[tile] ** 2 * 4
+    assert sums == tiles * splits * rows * cols * 4
 
 
 @pytest.mark.parametrize("cus", [1, 64, 256, 304])
 def test_a_plan_stays_within_what_a_launch_holds(lib, cus):
     for m, k, n in sizes(4000, 3):
-        few, *p = one(lib, m, n, 2 * k, cus)
-        assert bool(few) == (m <= 32)
-        holds(*p, (m, n, 2 * k), cus)
+        for paired in (False, True):
+            few, *p = one(lib, m, n, 2 * k, cus, paired)
+            assert bool(few) == (m <= 32)
+            holds(*p, (m, n, 2 * k), cus, paired)
 
 
 @pytest.mark.parametrize("cus", [64, 256])
@@ -121,19 +123,20 @@ def test_a_product_that_is_not_asked_for(lib):
 
 def test_every_form_has_its_sizes(lib):
     """No tile, alone or shared out, that no size takes."""
+    for paired in (False, True):
+        whole, shared = set(), set()
+        for m, k, n in sizes(6000, 5):
+            few, tile, splits, *_ = one(lib, m, n, 2 * k, 256, paired)
+            if not few:
+                (whole if splits == 1 else shared).add(tile)
+        assert whole == set(range(5)) and shared >= {1, 2}, (paired, whole, shared)
     whole, shared, apart = set(), set(), 0
-    for m, k, n in sizes(6000, 5):
-        few, tile, splits, *_ = one(lib, m, n, 2 * k)
-        if not few:
-            (whole if splits == 1 else shared).add(tile)
-    assert whole == {0, 1, 2, 3} and shared >= {1, 2}, (whole, shared)
-    whole, shared = set(), set()
     for m, k, h in sizes(6000, 6):
         together, a, b = backward(lib, m, k, h)
         apart += not together
         for tile, splits, *_ in (a, b):
             (whole if splits == 1 else shared).add(tile)
-    assert whole == {0, 1, 2, 3} and shared >= {1, 2} and apart, (whole, shared, apart)
+    assert whole == set(range(5)) and shared >= {1, 2} and apart, (whole, shared, apart)
 
 
 def test_rows_that_each_workgroup_quantises(lib):

@@ -218,20 +218,11 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
                                             place, stages_, acc))
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
-  typedef vkp::Chunk<V, T::NT> C;
+  constexpr int J = T::NT % 2 ? 1 : 2;  // column tiles of 32 that leave together
+  typedef vkp::Chunk<V, J> C;
   char* chunk = stages_[0] + wave * C::kBytes;
 #pragma unroll
   for (int i = 0; i < T::MT; ++i) {
-#pragma unroll
-    for (int j = 0; j < T::NT; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        typename C::V4 w;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(acc[i][j][4 * q + e]);
-        *C::at(chunk, lane, j, q) = w;
-      }
-    vkd::wave_lds_fence();
     int mb = m0 + (wm * T::MT + i) * 32, end = g.M;
     if (g.m_half > 0) {  // 32 rows lie in one half: m_half is a multiple of 64
       end = g.M / 2;
@@ -240,9 +231,22 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
         end = g.M;
       }
     }
-    C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end,
-                             n0 + T::b_row(wn, 0), g.N);
-    vkd::wave_lds_fence();
+#pragma unroll
+    for (int jg = 0; jg < T::NT; jg += J) {
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          typename C::V4 w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(acc[i][jg + j][4 * q + e]);
+          *C::at(chunk, lane, j, q) = w;
+        }
+      vkd::wave_lds_fence();
+      C::template store<false>(chunk, lane, static_cast<V*>(g.out), g.N, mb, end,
+                               n0 + T::b_row(wn, jg), g.N);
+      vkd::wave_lds_fence();
+    }
   }
 }
 
@@ -353,7 +357,7 @@ void with_tile(vkp::TileSize size, Args& g, F go) {
   });
 }
 
-vkp::Shape forward_shape(const Args& g) { return vkp::Shape{g.M, 2LL * g.N, g.k_bytes}; }
+vkp::Shape forward_shape(const Args& g) { return vkp::Shape{g.M, 2LL * g.N, g.k_bytes, true}; }
 
 template <Kind KIND>
 int launch_forward(vk_runtime* rt, Args& g, const vkp::Plan& p) {
@@ -393,7 +397,7 @@ BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, 
   double us = 0;
   const size_t rows = g.M, half = padded(g.N);
   // the zeros up to d_half too
-  const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes};
+  const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes, true};
   p.first = vkp::plan(cus, step, &us);
   const auto D = static_cast<long long>(in);
   const vkp::Shape x{dx ? g.M : 0, D, static_cast<long long>(4 * half)};
@@ -560,7 +564,7 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, con
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
   g.out = out->ptr;
   const vkp::Shape shape = forward_shape(g);
-  const vkp::Plan p = vkp::plan(rt->cu_count, shape.m, shape.n, shape.k_bytes);
+  const vkp::Plan p = vkp::plan(rt->cu_count, shape);
   if (!p.few) {
     const size_t room = operands_room(rows, in_features, hidden);
     const size_t sums = vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});

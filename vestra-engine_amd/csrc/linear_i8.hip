@@ -212,7 +212,7 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void linear_i8_kernel(
     return;
   const int lane = place.lane, wave = place.wave, wm = place.wm, wn = place.wn;
   constexpr int kCols = T::PAIRED ? T::NT / 2 : T::NT;
-  constexpr int J = sizeof(V) == 4 ? 1 : (kCols < 2 ? kCols : 2);
+  constexpr int J = sizeof(V) == 4 || kCols % 2 ? 1 : 2;
   typedef vkp::Chunk<V, J> C;
   static_assert(T::kWaves * C::kBytes <= T::kBytes, "the chunks fit a stage buffer");
   char* chunk = stages_[0] + wave * C::kBytes;
@@ -465,8 +465,9 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
                     "linear_i8: %zu x %zu outputs", rows, N);
 
   const int M = static_cast<int>(rows);
-  const vkp::Plan p = vkp::plan(rt->cu_count, M, static_cast<long long>(lin->out_features),
-                                static_cast<long long>(lin->pitch));
+  const vkp::Shape shape{M, static_cast<long long>(lin->out_features),
+                         static_cast<long long>(lin->pitch), end == kGated};
+  const vkp::Plan p = vkp::plan(rt->cu_count, shape);
   Args g{};
   if (vkp::own_rows(rows, lin->pitch)) {
     g.x = x->ptr;
@@ -474,8 +475,6 @@ int run(vk_runtime* rt, const vk_linear_i8* lin, const vk_tensor* x, size_t rows
     g.x_type = x->dtype;
   } else {
     const size_t code_bytes = rows * lin->pitch, scale_bytes = (rows * 4 + 255) / 256 * 256;
-    const vkp::Shape shape{M, static_cast<long long>(lin->out_features),
-                           static_cast<long long>(lin->pitch)};
     const size_t sums = p.few ? 0 : vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});
     VK_TRY(vk::ensure_work(rt, (code_bytes + scale_bytes + sums) / 4, "linear_i8"));
     char* codes = reinterpret_cast<char*>(rt->work);  // (code_bytes: a multiple of 128)

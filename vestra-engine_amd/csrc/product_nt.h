@@ -122,7 +122,10 @@ struct Tile {
 // one line of 16-bit results.
 template <bool PAIRED, typename F>
 void with_tile(TileSize size, F go) {
-  if (size == kTile256) {
+  if (size == kTile192) {
+    if constexpr (PAIRED) go(Tile<2, 4, 3, 2, true, 2, 1>{});
+    else go(Tile<4, 2, 2, 3, false, 2, 1>{});
+  } else if (size == kTile256) {
     if constexpr (PAIRED) go(Tile<4, 2, 2, 4, true, 2, 1>{});
     else go(Tile<2, 4, 4, 2, false, 2, 1>{});
   } else if (size == kTile128) {
@@ -199,11 +202,12 @@ __device__ __forceinline__ void load_lds(const Source& s, char* to, uint32_t lan
 }
 
 // Columns: a stage is 64 lines of W values.  In LDS a line's 16-byte pieces are permuted by
-// piece ^ 4 (k % 4) (two 64-value lines to the 64 banks: by 4 (k / 2 % 2)): the 32 lanes of a
-// transposing read take 64 bytes each of four neighbouring lines, all banks once.
+// piece ^ 4 (k % 4) (where two lines differ by half of the 64 banks, of 64 and 192 values: by
+// 4 (k / 2 % 2)): the 32 lanes of a transposing read take 64 bytes each of four neighbouring lines,
+// all banks once.
 template <int W>
 __device__ __forceinline__ constexpr int column_turn(int k) {
-  return W == 64 ? ((k >> 1) & 1) * 4 : (k & 3) * 4;
+  return W % 128 ? ((k >> 1) & 1) * 4 : (k & 3) * 4;
 }
 
 // The lines of stage st, up to the last; none from stage `stop` on.
@@ -225,11 +229,11 @@ __device__ __forceinline__ Source columns_of(const Operand& o, int st, int stop)
 template <int W, int WAVES, int N>
 __device__ __forceinline__ void columns_at(const Operand& o, int c0, int lane, int wave,
                                            uint32_t (&v)[N]) {
-  constexpr int kPieces = W / 8, kLines = 64 / kPieces;  // of a line; lines a load
+  constexpr int kPieces = W / 8;  // of a line
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int line = (wave + i * WAVES) * kLines + lane / kPieces;
-    const int piece = (lane % kPieces) ^ column_turn<W>(line);
+    const int at_piece = (wave + i * WAVES) * 64 + lane, line = at_piece / kPieces;
+    const int piece = (at_piece % kPieces) ^ column_turn<W>(line);
     const int c = c0 + piece * 8;
     const uint32_t at = static_cast<uint32_t>(line) * o.pitch + 2u * static_cast<uint32_t>(c);
     v[i] = c < o.rows ? at : kOutside;
@@ -512,8 +516,8 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
       }
     }
   }
-  // (not for the largest tiles: 256 KiB of sums a workgroup cost more than they save)
-  if constexpr (T::TM < 256)
+  // (not for the largest tiles: 192 KiB of sums a workgroup and more cost more than they save)
+  if constexpr (T::TM < 192)
     if (split.count > 1) return last_of_split<KIND, T>(split, part, tile, tiles, at, acc);
   return true;
 }

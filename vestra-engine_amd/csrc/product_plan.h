@@ -16,20 +16,29 @@ inline bool own_rows(size_t rows, size_t bytes) {
   return rows <= kOwnRows && rows * bytes <= kOwnBytes;
 }
 
-// Tiles of 64 x 64 by one group of two waves or by four groups that share k, of 128 x 128 and
-// of 256 x 256.
-enum TileSize { kTile64 = 0, kTile64K = 1, kTile128 = 2, kTile256 = 3 };
+// Tiles of 64 x 64 by one group of two waves or by two groups that share k, of 128 x 128, of
+// 256 x 192 (gates and partners: 192 x 256) and of 256 x 256.
+enum TileSize { kTile64 = 0, kTile64K = 1, kTile128 = 2, kTile192 = 3, kTile256 = 4 };
+constexpr TileSize kTiles[] = {kTile64, kTile64K, kTile128, kTile192, kTile256};
 
-constexpr int kSide[] = {64, 64, 128, 256};
-
-inline long long tiles_of(int tile, long long m, long long n) {
-  return ((m + tile - 1) / tile) * ((n + tile - 1) / tile);
-}
-
-// A product's sizes; n: rows of b.
+// A product's sizes; n: rows of b, paired: gates and partners.
 struct Shape {
   long long m, n, k_bytes;
+  bool paired = false;
 };
+
+struct Sides {
+  int m, n;
+};
+constexpr Sides sides(TileSize tile, bool paired) {
+  switch (tile) {
+    case kTile64:
+    case kTile64K: return {64, 64};
+    case kTile128: return {128, 128};
+    case kTile192: return paired ? Sides{192, 256} : Sides{256, 192};
+    default: return {256, 256};
+  }
+}
 
 // A product as launched: `splits` workgroups share out a tile's k.
 struct Job {
@@ -38,49 +47,73 @@ struct Job {
 };
 
 inline long long tiles_of(TileSize tile, const Shape& p) {
-  return p.m > 0 ? tiles_of(kSide[tile], p.m, p.n) : 0;
+  const Sides s = sides(tile, p.paired);
+  return p.m > 0 ? ((p.m + s.m - 1) / s.m) * ((p.n + s.n - 1) / s.n) : 0;
 }
 
 // Bytes of a split tile's sums, of all workgroups.
 inline long long split_bytes(TileSize tile, const Job& j) {
-  return j.splits > 1 ? tiles_of(tile, j.shape) * j.splits * kSide[tile] * kSide[tile] * 4LL : 0;
+  const Sides s = sides(tile, j.shape.paired);
+  return j.splits > 1 ? tiles_of(tile, j.shape) * j.splits * s.m * s.n * 4LL : 0;
 }
 
-// Us of one workgroup where it has a CU to itself, and a CU's us a workgroup where it has many, as
-// measured on a card of 256 CUs (866 and 10,392 rows, 384 to 8192 wide): stages of 128 bytes, the
-// two ends, and the last one's reading of its tile's parts.
+// What a launch takes, in us, as measured on a card of 256 CUs (866 to 10,392 rows, 384 to 8192
+// wide).  A CU holds `held` workgroups of a tile, by their stage buffers; a stage of 128 bytes takes
+// `lone` where a CU has one (none but it, for the tiles that fill a CU: where the rest of the card
+// idles, whose power it then has) and `full` where all are there, in between in proportion.  To each
+// round of workgroups comes `between`, to the last one `end`.
 struct TileCost {
-  double alone, many;
+  int held;
+  double lone, full, between, end;
 };
-inline TileCost tile_cost(TileSize tile, const Job& j) {
-  const long long stages = (j.shape.k_bytes + 127) / 128;
-  const double s = static_cast<double>((stages + j.splits - 1) / j.splits);
-  const double join = j.splits > 1 ? 4 + j.splits * (kSide[tile] == 64 ? 0.4 : 1.3) : 0;
+constexpr TileCost tile_cost(TileSize tile) {
   switch (tile) {
-    case kTile64: return {0.47 * s + 3 + join, 0.2 * s + 0.7};
-    case kTile64K: return {0.23 * s + 3 + join, 0.25 * s + 3};
-    case kTile128: return {0.62 * s + 4 + join, 0.45 * s + 2};
-    default: return {1.1 * s + 6 + join, 1.3 * s + 5};
+    case kTile64: return {5, 0.47, 0.87, 3, 3};
+    case kTile64K: return {1, 0.23, 0.25, 3, 3};
+    case kTile128: return {2, 0.62, 0.9, 4, 4};
+    case kTile192: return {1, 0.85, 1.25, 4, 6};
+    default: return {1, 1.05, 1.5, 6, 6};
   }
 }
 
-// Us of up to two products in one launch of one tile.
+// The launch of up to two products.  Workgroups come in rounds of as many as the card holds; the
+// last round of two different products is half full, as it were.
 inline double launch_cost(int cus, TileSize tile, std::initializer_list<Job> jobs) {
-  double longest = 0, total = 0, end = 0, wgs = 0, sums = 0;
+  const TileCost c = tile_cost(tile);
+  const double room = static_cast<double>(cus) * c.held;
+  double wgs = 0, longest = 0, rounds = 0, sums = 0, join = 0;
+  int products = 0;
   for (const Job& j : jobs) {
-    if (j.shape.m <= 0) continue;
-    const double n = static_cast<double>(tiles_of(tile, j.shape) * j.splits);
-    const TileCost c = tile_cost(tile, j);
-    longest = c.alone > longest ? c.alone : longest;
-    end = c.many > end ? c.many : end;
-    total += n * c.many;
-    wgs += n;
-    sums += static_cast<double>(split_bytes(tile, j)) / 2e6;  // written and read
+    const long long n = tiles_of(tile, j.shape) * j.splits;
+    if (n == 0) continue;
+    ++products;
+    const long long stages = (j.shape.k_bytes + 127) / 128;
+    const auto s = static_cast<double>((stages + j.splits - 1) / j.splits);
+    wgs += static_cast<double>(n);
+    rounds += static_cast<double>(n) / room * (c.full * s + c.between);
+    longest = s > longest ? s : longest;
+    if (j.splits > 1) {  // the last one's reading of its tile's parts; they are written and read
+      const double parts = 4 + j.splits * (tile < kTile128 ? 0.4 : 1.3);
+      join = parts > join ? parts : join;
+      sums += static_cast<double>(split_bytes(tile, j)) / 2e6;
+    }
   }
-  const double share = wgs / cus;  // neighbours on a CU slow a tile down
-  const double crowded = longest * (share > 1 ? 1 + 0.15 * (share - 1) : 1);
-  const double busy = share > 1 ? total / cus + 0.5 * end : 0;
-  return (crowded > busy ? crowded : busy) + sums;
+  const auto last = [&](double n) {  // of n workgroups
+    const double u = n / cus, from = c.held > 1 ? 1 : 0;
+    const double x = u > from ? (u - from) / (c.held - from) : 0;
+    return (c.lone + (c.full - c.lone) * x) * longest + c.end;
+  };
+  double us = 0;
+  if (wgs <= room) {
+    us = last(wgs);
+  } else if (products == 1) {
+    const double whole = static_cast<double>(static_cast<long long>(wgs / room));
+    const double rest = wgs - whole * room;
+    us = whole * (c.full * longest + c.between) + (rest > 0 ? last(rest) : c.end - c.between);
+  } else {
+    us = rounds + 0.5 * last(room);
+  }
+  return us + join + sums;
 }
 
 constexpr int kMostTilesSplit = 1024;  // of a product, by its counters
@@ -88,7 +121,7 @@ constexpr int kMostTilesSplit = 1024;  // of a product, by its counters
 // How many workgroups a tile: no more than two to a CU.
 inline int splits_for(int cus, TileSize tile, const Shape& p) {
   const long long tiles = tiles_of(tile, p);
-  if (tile == kTile256 || tiles == 0 || tiles > kMostTilesSplit) return 1;
+  if (tile >= kTile192 || tiles == 0 || tiles > kMostTilesSplit) return 1;
   int best = 1;
   double least = launch_cost(cus, tile, {Job{p, 1}});
   for (int c : {2, 3, 4, 6, 8, 12, 16, 24, 32}) {
@@ -110,7 +143,7 @@ struct Plan {
 
 inline Plan plan(int cus, const Shape& p, double* us) {
   Plan best{p.m <= kFewRows, kTile64, 1};
-  for (TileSize t : {kTile64, kTile64K, kTile128, kTile256}) {
+  for (TileSize t : kTiles) {
     const int splits = splits_for(cus, t, p);
     const double c = launch_cost(cus, t, {Job{p, splits}});
     if (t != kTile64 && c >= *us) continue;
@@ -121,9 +154,9 @@ inline Plan plan(int cus, const Shape& p, double* us) {
   return best;
 }
 
-inline Plan plan(int cus, long long m, long long n, long long k_bytes) {
+inline Plan plan(int cus, const Shape& p) {
   double us = 0;
-  return plan(cus, Shape{m, n, k_bytes}, &us);
+  return plan(cus, p, &us);
 }
 
 // Two products that do not wait for one another: in one launch of one tile, or each in its own,
@@ -137,7 +170,7 @@ inline PlanTwo plan_two(int cus, const Shape& a, const Shape& b) {
   double one = 0, two = 0, least = 0;
   const Plan first = plan(cus, a, &one), second = plan(cus, b, &two);
   PlanTwo both{true, {kTile64, kTile64}, {1, 1}};
-  for (TileSize t : {kTile64, kTile64K, kTile128, kTile256}) {
+  for (TileSize t : kTiles) {
     const int sa = splits_for(cus, t, a), sb = splits_for(cus, t, b);
     const double us = launch_cost(cus, t, {Job{a, sa}, Job{b, sb}});
     if (t != kTile64 && us >= least) continue;

@@ -101,8 +101,15 @@ def test_a_plan_stays_within_what_a_launch_holds(lib, cus):
     for m, k, n in sizes(4000, 3):
         for paired in (False, True):
             few, *p = one(lib, m, n, 2 * k, cus, paired)
-            assert bool(few) == (m <= 32)
+            assert m <= 32 or not few
             holds(*p, (m, n, 2 * k), cus, paired)
+
+
+def test_few_rows_of_a_short_k_take_one_launch_of_their_own(lib):
+    for m in range(1, 40):
+        for k in (1, 8, 100, 128):
+            for paired in (False, True):
+                assert bool(one(lib, m, 1000, 2 * k, 256, paired)[0]) == (m <= 32)
 
 
 @pytest.mark.parametrize("cus", [64, 256])

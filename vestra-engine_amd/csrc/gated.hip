@@ -564,7 +564,8 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, con
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
   g.out = out->ptr;
   const vkp::Shape shape = forward_shape(g);
-  const vkp::Plan p = vkp::plan(rt->cu_count, shape);
+  // (rows that are no multiple of 16 bytes take a launch and its time to copy)
+  const vkp::Plan p = vkp::plan(rt->cu_count, shape, in_features % 8 == 0 ? 0 : 4);
   if (!p.few) {
     const size_t room = operands_room(rows, in_features, hidden);
     const size_t sums = vkp::split_bytes(p.tile, vkp::Job{shape, p.splits});

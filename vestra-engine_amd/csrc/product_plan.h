@@ -8,7 +8,7 @@
 namespace vkp {
 
 constexpr int kGroupRows = 1024;  // rows of a that an XCD walks the columns with
-constexpr int kFewRows = 32;      // most rows of the few-row kernels
+constexpr int kFewRows = 32;  // most rows of the few-row kernels
 // Rows of x that every workgroup of the 8-bit linear quantises for itself: a launch less, against
 // reading them that many times (from L2: 64 KiB of f32 at most).
 constexpr int kOwnRows = 16, kOwnBytes = 16384;
@@ -141,8 +141,21 @@ struct Plan {
   int splits;
 };
 
-inline Plan plan(int cus, const Shape& p, double* us) {
-  Plan best{p.m <= kFewRows, kTile64, 1};
+// The few-row kernels: a CU takes in 42 bytes of operands a ns, whoever shares them out, so that few
+// columns of a long k are better cut into tiles whose k many workgroups share (17 rows, 64 hidden
+// columns, bf16, us: k 1024 5.4 against 6.9, 2272 7.5 against 9.3, 4096 13.3 against 10.3, 8192 24.6
+// against 10.4; 4096 hidden columns: 5.4 against 7.1, 8.1 against 10.9, 15.1 against 16.1, 26
+// against 24.5).  `prepare`: what the tiles need before, in us.
+inline bool few_rows(int cus, const Shape& p, double tiles_us, double prepare) {
+  if (p.m > kFewRows) return false;
+  const double cols = p.paired ? 32 : 16, turns = static_cast<double>(p.n) / cols / cus;
+  const double us = 4 + (turns > 1 ? turns : 1) * 0.024 * (cols + static_cast<double>(p.m)) *
+                            static_cast<double>(p.k_bytes) / 1024;
+  return us <= 0.85 * (tiles_us > 4.5 ? tiles_us : 4.5) + 1.2 + prepare;
+}
+
+inline Plan plan(int cus, const Shape& p, double* us, double prepare = 0) {
+  Plan best{false, kTile64, 1};
   for (TileSize t : kTiles) {
     const int splits = splits_for(cus, t, p);
     const double c = launch_cost(cus, t, {Job{p, splits}});
@@ -151,12 +164,13 @@ inline Plan plan(int cus, const Shape& p, double* us) {
     best.tile = t;
     best.splits = splits;
   }
+  best.few = few_rows(cus, p, *us, prepare);
   return best;
 }
 
-inline Plan plan(int cus, const Shape& p) {
+inline Plan plan(int cus, const Shape& p, double prepare = 0) {
   double us = 0;
-  return plan(cus, p, &us);
+  return plan(cus, p, &us, prepare);
 }
 
 // Two products that do not wait for one another: in one launch of one tile, or each in its own,

@@ -250,26 +250,23 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
   }
 }
 
-// dbias: the tiles' sums of sixteen columns, eight runs of parts each in order, then the runs in
-// order.
+// dbias: the tiles' sums of COLS columns, eight runs of parts each in order, then the runs in order.
 struct BiasSums {
   const float* sums;  // [parts, cols]
   int parts, cols;
   void* out;
 };
 
-template <Kind KIND>
+template <Kind KIND, int COLS>
 __device__ __forceinline__ void bias_gradient(const BiasSums& g, int block, char* smem) {
-  float(*run)[16] = reinterpret_cast<float(*)[16]>(smem);
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = block * 16 + x;
-  if (y < 8) {
-    const int from = g.parts * y / 8, to = g.parts * (y + 1) / 8;
-    float s = 0.0f;
-    if (c < g.cols)
+  float(*run)[COLS] = reinterpret_cast<float(*)[COLS]>(smem);
+  const int x = threadIdx.x % COLS, y = threadIdx.x / COLS, c = block * COLS + x;
+  const int from = g.parts * y / 8, to = g.parts * (y + 1) / 8;
+  float part = 0.0f;
+  if (c < g.cols)
 #pragma unroll 8
-      for (int p = from; p < to; ++p) s += g.sums[static_cast<size_t>(p) * g.cols + c];
-    run[y][x] = s;
-  }
+    for (int p = from; p < to; ++p) part += g.sums[static_cast<size_t>(p) * g.cols + c];
+  run[y][x] = part;
   __syncthreads();
   if (y > 0 || c >= g.cols) return;
   float s = 0.0f;
@@ -279,19 +276,20 @@ __device__ __forceinline__ void bias_gradient(const BiasSums& g, int block, char
       static_cast<typename vkp::Value<KIND>::type>(s);
 }
 
-// Steps 2 to 4 in one launch: they need the same step before them, and few rows leave the card
-// half empty one after another.  Workgroups 0 .. n_bias are dbias, the next n_dx dx, the others dw.
+// Steps 2 to 4 in one launch, dx apart where that is cheaper: they need the same step before them,
+// and few rows leave the card half empty one after another.  The first n_dx workgroups are dx, the
+// next n_dw dw, the others dbias: short ones, for the CUs that the tiles leave.
 template <Kind KIND, typename T>
 __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gradients_kernel(
-    Product dx, Product dw, BiasSums bias, int n_bias, int n_dx) {
+    Product dx, Product dw, BiasSums bias, int n_dx, int n_dw) {
   VK_STAGES(T);
   const int wg = blockIdx.x;
-  if (wg < n_bias)
-    bias_gradient<KIND>(bias, wg, stages_[0]);
-  else if (wg < n_bias + n_dx)
-    product<KIND, T, false>(dx, wg - n_bias, stages_);
+  if (wg < n_dx)
+    product<KIND, T, false>(dx, wg, stages_);
+  else if (wg < n_dx + n_dw)
+    product<KIND, T, true>(dw, wg - n_dx, stages_);
   else
-    product<KIND, T, true>(dw, wg - n_bias - n_dx, stages_);
+    bias_gradient<KIND, T::kThreads / 8>(bias, wg - n_dx - n_dw, stages_[0]);
 }
 
 // Forward of at most 16 RT rows.
@@ -463,13 +461,12 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
     w.m_half = static_cast<int>(half);
   }
   BiasSums sums{g.sums, parts, H2, dbias ? dbias->ptr : nullptr};
-  const int n_bias = dbias ? (H2 + 15) / 16 : 0;
   // (the first step's split sums are done with)
   const vkp::PlanTwo& two = plan.second;
   x.split = vkp::Split{two.splits[0], room + plan.work, rt->arrivals};
   w.split = vkp::Split{two.splits[1], room + plan.work + plan.dx_sums,
                        rt->arrivals + vkp::kMostTilesSplit};
-  // one launch, or dx in one of its own
+  // one launch, or dx and dbias in one of their own
   for (int part = two.together ? 1 : 0; part < 2; ++part) {
     vkp::with_tile<false>(two.tile[part], [&](auto tile) {
       typedef decltype(tile) T;
@@ -479,10 +476,12 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
         p->group = vkp::kGroupRows / T::TM;
       }
       const int n_dx = part == 0 || two.together ? x.gm * x.gn * x.split.count : 0;
-      const int n_dw = part == 0 ? 0 : w.gm * w.gn * w.split.count, biases = part == 0 ? 0 : n_bias;
+      const int n_dw = part == 0 ? 0 : w.gm * w.gn * w.split.count;
+      constexpr int kCols = T::kThreads / 8;
+      const int biases = dbias && part == (two.together ? 1 : 0) ? (H2 + kCols - 1) / kCols : 0;
       if (biases + n_dx + n_dw > 0)
         hipLaunchKernelGGL((gradients_kernel<KIND, T>), dim3(biases + n_dx + n_dw),
-                           dim3(T::kThreads), 0, rt->stream, x, w, sums, biases, n_dx);
+                           dim3(T::kThreads), 0, rt->stream, x, w, sums, n_dx, n_dw);
     });
     VK_TRY(vk::check_launch("gradients_kernel"));
   }

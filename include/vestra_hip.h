@@ -655,7 +655,9 @@ int vk_linear_i8_prepare_f32(vk_runtime* rt, size_t in_features,
 int vk_linear_i8_destroy(vk_linear_i8* lin);
 size_t vk_linear_i8_input_features(const vk_linear_i8* lin);
 /* out [rows, out_features] = y [* gamma].  x and out are f32, f16 or bf16, each
- * of its own type; 16-bit results are rounded once.  out must not overlap x. */
+ * of its own type, and start on 16 bytes; 16-bit results are rounded once.  out
+ * must not overlap x.  Beyond 16 rows (or 16,384 codes) the codes of x go to the
+ * runtime's work buffer: run a call once before a capture. */
 int vk_linear_i8_run_into(vk_runtime* rt, const vk_linear_i8* lin,
                           const vk_tensor* x, size_t rows, vk_tensor* out);
 /* out = GELU(y), the erf of vk_gelu_f32_inplace.  No LayerScale. */
@@ -680,10 +682,13 @@ int vk_linear_i8_run_gated(vk_runtime* rt, const vk_linear_i8* lin,
 /* The gated feed-forward in 16 bits: g = x Wg^T + bg, u = x Wu^T + bu,
  * out = act(g) * u, in one kernel.  All tensors f16, or all bf16: x [rows,
  * in_features], w [2 hidden, in_features] (Wg's rows, then Wu's), bias
- * [2 hidden] or NULL, out [rows, hidden], overlapping no input.  Sums are f32,
- * out is rounded once.  in_features of a multiple of 8 are read where they lie;
- * any others are copied to the runtime's work buffer first (run such a call
- * once before a capture, which cannot grow it). */
+ * [2 hidden] or NULL, out [rows, hidden], overlapping no input; tensors start on
+ * 16 bytes.  Sums are f32, out is rounded once.  Beyond a few rows, in_features
+ * that are no multiple of 8 are copied to the runtime's work buffer first, and
+ * products of few outputs and a long sum leave partial sums there (run a call
+ * once before a capture, which cannot grow it).  The weights' rows, rounded up
+ * to 128 bytes, take less than 2 GiB; in_features and hidden at most 2^20, rows
+ * 2^24. */
 int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
                      const vk_tensor* bias, size_t rows, size_t in_features,
                      size_t hidden, int activation, vk_tensor* out);
@@ -997,7 +1002,8 @@ int vk_event_elapsed_ms(vk_event* start, vk_event* stop, float* ms);
  * while the stream captures: the runtime's work buffer (split-K partial sums
  * of linears over few rows, the key-split partials of attention over few
  * or unevenly spread query tiles, the row statistics of
- * vk_token_to_chw_f32) and its RoPE
+ * vk_token_to_chw_f32, codes, operands and partial sums of the feed-forward
+ * in fewer bits) and its RoPE
  * tables grow only outside capture, so a sequence is run once eagerly
  * before it is captured; a call that would grow them during capture fails
  * with an error and enqueues nothing.  Buffers they replace stay valid for

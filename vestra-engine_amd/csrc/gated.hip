@@ -250,7 +250,8 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
   }
 }
 
-// dbias: the tiles' sums of COLS columns, eight runs of parts each in order, then the runs in order.
+// dbias: the tiles' sums of COLS columns, eight runs of parts each in order, then the runs in
+// order.
 struct BiasSums {
   const float* sums;  // [parts, cols]
   int parts, cols;

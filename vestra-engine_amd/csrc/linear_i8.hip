@@ -121,7 +121,8 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
 
 // WPR waves a row (4 of them are a workgroup's, otherwise it has 4 rows).  NV steps of 8
 // values a lane stay in registers between the maximum and the codes; NV 0: any length, read
-// twice.
+// twice.  Bound by memory for many rows (10,392 x 1536 f32: 17.8 us, 4.5 TB/s of what is read and
+// written), by the chain row -> maximum -> codes for few.
 template <typename XT, int NV, int WPR>
 __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict__ x, int M, int K,
                                                             uint32_t pitch, char* codes,
@@ -368,27 +369,25 @@ __global__ __launch_bounds__(vkp::kFewThreads) void linear_i8_rows_kernel(Args g
 }
 
 // ---------------------------------------------------------------- launches
-// Four waves a row where a wave each would leave the card half empty.
+// Four waves a row of more than 1024 codes: shorter chains, and up to 8192 stay in registers (f32,
+// with a product of 64 columns behind it, us, one wave a row against four: 866 x 768 9.3 and 9.4,
+// 10,392 x 768 14.8 and 17.5; 866 x 1536 10.9 and 10.7, 10,392 x 1536 21.5 and 21.2; 866 x 4096
+// 15.0 and 14.5, 10,392 x 4096 44.0 and 42.1; 10,392 x 8192 146 and 102).
 template <typename XT>
 void quantise(const vk_runtime* rt, const XT* x, int M, int K, size_t pitch, char* codes,
               float* scales) {
-  const bool wide = pitch > 512 && M < 16 * (rt->cu_count > 0 ? rt->cu_count : 256);
+  const bool wide = pitch > 1024;
   const dim3 grid(wide ? M : (M + 3) / 4), block(256);
   const auto p = static_cast<uint32_t>(pitch);
-#define VK_LAUNCH(NV, WPR)                                                                          \
+#define VK_LAUNCH(NV, WPR)                                                                     \
   hipLaunchKernelGGL((quantise_rows_kernel<XT, NV, WPR>), grid, block, 0, rt->stream, x, M, K, \
                      p, codes, scales)
-  if (wide) {
-    if (pitch <= 2048) VK_LAUNCH(1, 4);
-    else if (pitch <= 4096) VK_LAUNCH(2, 4);
-    else VK_LAUNCH(0, 4);
-  } else {
-    if (pitch <= 512) VK_LAUNCH(1, 1);
-    else if (pitch <= 1024) VK_LAUNCH(2, 1);
-    else if (pitch <= 2048) VK_LAUNCH(4, 1);
-    else if (pitch <= 4096) VK_LAUNCH(8, 1);
-    else VK_LAUNCH(0, 1);
-  }
+  if (pitch <= 512) VK_LAUNCH(1, 1);
+  else if (pitch <= 1024) VK_LAUNCH(2, 1);
+  else if (pitch <= 2048) VK_LAUNCH(1, 4);
+  else if (pitch <= 4096) VK_LAUNCH(2, 4);
+  else if (pitch <= 8192) VK_LAUNCH(4, 4);
+  else VK_LAUNCH(0, 4);
 #undef VK_LAUNCH
 }
 

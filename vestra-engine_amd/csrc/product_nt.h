@@ -1,21 +1,31 @@
 // Products out[m, n] = sum_k a[m, k] b[n, k] on the gfx950 matrix cores: int8 with
 // int32 sums, f16 and bf16 with f32 sums.  An operand's rows are contiguous in k, or (16-bit
 // types) its columns are: then a stage lies in LDS as it lies in memory, and fragments are read
-// with the transposing LDS reads.
+// with the transposing LDS reads, so that a backward pass needs no transposed copies.
 //
 // All three types share one kernel, because they share one layout in bytes: an
 // operand of v_mfma_*_32x32x{32 int8, 16 f16/bf16} is 16 bytes a lane, lane l
 // holding k bytes 16 (l / 32) .. + 16 of row l % 32.  What a lane calls k only has
 // to agree between a and b.
 //
-// A workgroup owns a TM x TN tile and walks k in stages of 128 bytes a row:
-// both operands go from memory straight into LDS (16 bytes a lane, no
-// registers), two stage buffers, one barrier a stage -- a stage's loads run
-// while the stage before it is multiplied.  In LDS a row is 128 bytes, its
-// 16-byte pieces permuted by (piece ^ row / 2 % 8): a fragment read, whose lanes read the
-// same piece of 32 rows, then touches all 64 banks once with any 16 lanes that it takes
-// together (0-3, 12-15, 20-23 and 24-27 among them).  The permutation is applied to the
-// addresses that the loads read from.
+// A workgroup owns a TM x TN tile and walks k in stages of 128 bytes a row: both operands go from
+// memory straight into LDS (16 bytes a lane, no registers), two stage buffers (four where a tile is
+// alone on its CU and short of work), one barrier a stage.  Between two matrix instructions goes
+// one fragment read of the next step and one load of a later stage, so that neither LDS nor
+// the load path holds the matrix pipe up (10,392 x 1536 x 8192 in bf16: reads and loads in
+// bursts 237 us, one by one 204).  In LDS a row is 128 bytes, its 16-byte pieces permuted by
+// (piece ^ row / 2 % 8): a fragment read, whose lanes read the same piece of 32 rows, then
+// touches all 64 banks once with any 16 lanes that it takes together (0-3, 12-15, 20-23 and
+// 24-27 among them).  The permutation is applied to the addresses that the loads read from.
+//
+// What bounds it.  Large products: the stages' loads, which the L2s deliver at 10.5-11 TB/s (the
+// loads of the product above alone take 190 us, its matrix instructions alone some 150), and the
+// card's power (the same product of zeros: 154 us).  Bigger tiles load less but leave a larger
+// part of a last round of workgroups idle; product_plan.h weighs that.  It reaches 1,280 TFLOP/s
+// in bf16 and 1,770 TOP/s in int8 (with its gated end) where a library's plain product of the
+// same sizes reaches 1,415 and one of 8192^3 2,076.  Few tiles: the chain of stages, 0.23-0.47 us
+// each, which groups of waves share (Tile::KG) and, for a long k, workgroups (Split).  A few rows:
+// reading b (few_product).
 #pragma once
 
 #include <type_traits>
@@ -739,9 +749,9 @@ __device__ __forceinline__ i32x4 row_rest(const char* row, int k_bytes) {
 }
 
 // The stages of a workgroup's k from stage `first` on, around to it again: b's rows often lie a
-// power of two apart, where the same k of all of them is in one of the L2's channels, and workgroups
-// that all began at 0 would ask the same few of them together (8 rows, 8192 -> 4096 in bf16: 27 us
-// against 21; where the weights are in L2, no difference).
+// power of two apart, where the same k of all of them is in one of the L2's channels, and
+// workgroups that all began at 0 would ask the same few of them together (8 rows, 8192 -> 4096 in
+// bf16: 27 us against 21; where the weights are in L2, no difference).
 struct FewStages {
   int count, first, whole;  // whole: the bytes of k
   // First byte of the t-th one; past the last: none.

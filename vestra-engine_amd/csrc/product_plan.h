@@ -10,7 +10,8 @@ namespace vkp {
 constexpr int kGroupRows = 1024;  // rows of a that an XCD walks the columns with
 constexpr int kFewRows = 32;  // most rows of the few-row kernels
 // Rows of x that every workgroup of the 8-bit linear quantises for itself: a launch less, against
-// reading them that many times (from L2: 64 KiB of f32 at most).
+// reading them that many times (from L2: 64 KiB of f32 at most).  4 rows, 2272 -> 128: 6.2 us, 8
+// rows, which take two launches: 8.1; 16 rows, 1024 -> 128: 6.8, 17 rows: 8.0.
 constexpr int kOwnRows = 16, kOwnBytes = 16384;
 inline bool own_rows(size_t rows, size_t bytes) {
   return rows <= kOwnRows && rows * bytes <= kOwnBytes;
@@ -58,10 +59,10 @@ inline long long split_bytes(TileSize tile, const Job& j) {
 }
 
 // What a launch takes, in us, as measured on a card of 256 CUs (866 to 10,392 rows, 384 to 8192
-// wide).  A CU holds `held` workgroups of a tile, by their stage buffers; a stage of 128 bytes takes
-// `lone` where a CU has one (none but it, for the tiles that fill a CU: where the rest of the card
-// idles, whose power it then has) and `full` where all are there, in between in proportion.  To each
-// round of workgroups comes `between`, to the last one `end`.
+// wide).  A CU holds `held` workgroups of a tile, by their stage buffers; a stage of 128 bytes
+// takes `lone` where a CU has one (none but it, for the tiles that fill a CU: where the rest of the
+// card idles, whose power it then has) and `full` where all are there, in between in proportion. 
+// To each round of workgroups comes `between`, to the last one `end`.
 struct TileCost {
   int held;
   double lone, full, between, end;
@@ -141,11 +142,11 @@ struct Plan {
   int splits;
 };
 
-// The few-row kernels: a CU takes in 42 bytes of operands a ns, whoever shares them out, so that few
-// columns of a long k are better cut into tiles whose k many workgroups share (17 rows, 64 hidden
-// columns, bf16, us: k 1024 5.4 against 6.9, 2272 7.5 against 9.3, 4096 13.3 against 10.3, 8192 24.6
-// against 10.4; 4096 hidden columns: 5.4 against 7.1, 8.1 against 10.9, 15.1 against 16.1, 26
-// against 24.5).  `prepare`: what the tiles need before, in us.
+// The few-row kernels: a CU takes in 42 bytes of operands a ns, whoever shares them out, so that
+// few columns of a long k are better cut into tiles whose k many workgroups share (17 rows, 64
+// hidden columns, bf16, us: k 1024 5.4 against 6.9, 2272 7.5 against 9.3, 4096 13.3 against 10.3,
+// 8192 24.6 against 10.4; 4096 hidden columns: 5.4 against 7.1, 8.1 against 10.9, 15.1 against
+// 16.1, 26 against 24.5).  `prepare`: what the tiles need before, in us.
 inline bool few_rows(int cus, const Shape& p, double tiles_us, double prepare) {
   if (p.m > kFewRows) return false;
   const double cols = p.paired ? 32 : 16, turns = static_cast<double>(p.n) / cols / cus;

@@ -657,7 +657,7 @@ size_t vk_linear_i8_input_features(const vk_linear_i8* lin);
 /* out [rows, out_features] = y [* gamma].  x and out are f32, f16 or bf16, each
  * of its own type, and start on 16 bytes; 16-bit results are rounded once.  out
  * must not overlap x.  Beyond 16 rows (or 16,384 codes) the codes of x go to the
- * runtime's work buffer: run a call once before a capture. */
+ * runtime's work buffer: run a call once before a capture.  Less than 2^24 rows. */
 int vk_linear_i8_run_into(vk_runtime* rt, const vk_linear_i8* lin,
                           const vk_tensor* x, size_t rows, vk_tensor* out);
 /* out = GELU(y), the erf of vk_gelu_f32_inplace.  No LayerScale. */

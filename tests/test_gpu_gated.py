@@ -23,7 +23,8 @@ def up(rt, t, *arrays):
 
 SIZES = [(1, 64, 64), (1, 8, 1), (48, 2881, 173), (70, 4000, 64), (33, 2000, 7), (2, 136, 33),
          (5, 1024, 300), (16, 7, 40), (17, 513, 70), (32, 384, 96), (33, 100, 31),
-         (64, 64, 32), (70, 257, 65), (257, 384, 1023), (866, 768, 700), (1300, 96, 2050), (2100, 130, 1030)]
+         (64, 64, 32), (70, 257, 65), (17, 8192, 70), (20, 9001, 33),
+         (257, 384, 1023), (866, 768, 700), (1300, 96, 2050), (2100, 130, 1030)]
 
 
 @pytest.mark.parametrize("t", ["f16", "bf16"])

@@ -33,7 +33,7 @@ SIZES = [(1, 64, 64), (1, 1024, 4096), (2, 130, 33), (3, 5000, 40), (4, 4096, 20
          (5, 900, 70), (7, 1, 5), (16, 257, 96), (17, 512, 48),
          (31, 1031, 200), (32, 4096, 64), (33, 127, 65), (64, 128, 64), (65, 129, 127),
          (130, 768, 300), (257, 384, 257), (866, 768, 640), (1301, 770, 1999), (300, 5000, 96),
-         (40, 20000, 70), (129, 9000, 33),
+         (40, 20000, 70), (129, 9000, 33), (17, 9000, 50), (32, 20001, 130), (2, 20000, 96),
          (2600, 512, 2304)]
 
 
@@ -48,7 +48,8 @@ def test_sums_of_every_size(rt, rng, m, k, n):
     ff.assert_within(got, want, tol, (m, k, n))
 
 
-@pytest.mark.parametrize("m,k,n", [(1, 300, 70), (20, 256, 100), (200, 520, 130), (3000, 128, 2050)])
+@pytest.mark.parametrize("m,k,n", [(1, 300, 70), (20, 256, 100), (200, 520, 130),
+                                   (3000, 128, 2050)])
 @pytest.mark.parametrize("t,out", [("f32", "bf16"), ("f16", "f32"), ("bf16", "f16"), ("f16", "f16"),
                                    ("bf16", "bf16")])
 def test_types(rt, rng, m, k, n, t, out):
@@ -81,8 +82,8 @@ def test_epilogues(rt, rng, m, k, n):
 
 @pytest.mark.parametrize("act", [vh.VK_GATE_SILU, vh.VK_GATE_GELU])
 @pytest.mark.parametrize("m,k,h,out", [(1, 1536, 4096, "f32"), (1, 7, 1, "f32"),
-                                       (15, 130, 31, "bf16"), (32, 384, 96, "f16"), (33, 384, 33, "f32"),
-                                       (130, 257, 191, "f32"), (866, 256, 683, "bf16"),
+                                       (15, 130, 31, "bf16"), (32, 384, 96, "f16"),
+                                       (33, 384, 33, "f32"), (130, 257, 191, "f32"), (866, 256, 683, "bf16"),
                                        (2700, 200, 1365, "f32")])
 def test_gated(rt, rng, m, k, h, out, act):
     w, s = weights(rng, k, 2 * h)
@@ -230,6 +231,7 @@ def test_refusals(rt, rng):
 
     bad = vh.VK_ERR_INVALID
     refused(bad, lin.run_into, x, 3, y)
+    refused(vh.VK_ERR_UNSUPPORTED, lin.run_into, x, 1 << 24, y)
     refused(bad, lin.run_into, x, 2, rt.alloc_f32(2 * 32))
     refused(bad, lin.run_into, rt.alloc_u8(128), 2, y)
     refused(bad, lin.run_into, room.view(0, 128), 2, room.view(64, 66))

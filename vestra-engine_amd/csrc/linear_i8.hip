@@ -532,7 +532,7 @@ int upload(void** dev, const void* host, size_t bytes) {
 }
 
 // codes [out, pitch]
-int make(vk_runtime* rt, size_t in, size_t out, const std::vector<int8_t>& codes,
+int make(vk_runtime* rt, size_t in, size_t out, size_t pitch, const int8_t* codes,
          const float* scale, const float* bias, const float* ls, vk_linear_i8** res) {
   auto* lin = new (std::nothrow) vk_linear_i8;
   if (!lin) return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
@@ -540,8 +540,8 @@ int make(vk_runtime* rt, size_t in, size_t out, const std::vector<int8_t>& codes
   vk::retain(rt);
   lin->in_features = in;
   lin->out_features = out;
-  lin->pitch = codes.size() / out;
-  int s = upload(reinterpret_cast<void**>(&lin->codes), codes.data(), codes.size());
+  lin->pitch = pitch;
+  int s = upload(reinterpret_cast<void**>(&lin->codes), codes, out * pitch);
   if (s == VK_OK) s = upload(reinterpret_cast<void**>(&lin->scale), scale, out * 4);
   if (s == VK_OK && bias) s = upload(reinterpret_cast<void**>(&lin->bias), bias, out * 4);
   if (s == VK_OK && ls) s = upload(reinterpret_cast<void**>(&lin->ls_gamma), ls, out * 4);
@@ -564,10 +564,12 @@ int vk_linear_i8_prepare(vk_runtime* rt, size_t in_features, size_t out_features
   VK_REQUIRE(out && codes_out_in && scale, "null argument");
   VK_TRY(check_prepare(in_features, out_features));
   const size_t pitch = (in_features + 127) / 128 * 128;
+  if (pitch == in_features)
+    return make(rt, in_features, out_features, pitch, codes_out_in, scale, bias, ls_gamma, out);
   std::vector<int8_t> w(pitch * out_features, 0);
   for (size_t o = 0; o < out_features; ++o)
     std::memcpy(&w[o * pitch], codes_out_in + o * in_features, in_features);
-  return make(rt, in_features, out_features, w, scale, bias, ls_gamma, out);
+  return make(rt, in_features, out_features, pitch, w.data(), scale, bias, ls_gamma, out);
 } catch (const std::bad_alloc&) {
   return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
 }
@@ -597,7 +599,7 @@ int vk_linear_i8_prepare_f32(vk_runtime* rt, size_t in_features, size_t out_feat
       if (scale[o] > 0.0f)
         w[o * pitch + i] =
             static_cast<int8_t>(std::nearbyint(weight_in_out[i * out_features + o] / scale[o]));
-  return make(rt, in_features, out_features, w, scale.data(), bias, ls_gamma, out);
+  return make(rt, in_features, out_features, pitch, w.data(), scale.data(), bias, ls_gamma, out);
 } catch (const std::bad_alloc&) {
   return vk::set_error(VK_ERR_OOM, "linear_i8: out of host memory");
 }

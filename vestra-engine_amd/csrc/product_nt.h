@@ -657,16 +657,37 @@ __device__ __forceinline__ void tile_at(int tile, int gm, int gn, int group, int
 }
 
 // ---------------------------------------------------------------- activations
-// act(g): SiLU g / (1 + e^-g), GELU g Phi(g) by the GELU stream's erf (error below 1.5e-7: half
-// the instructions of erff, which a tile's end would wait for).  The exponential is v_exp_f32 of
-// g log2(e) and the quotient v_rcp_f32: some 2 ulp each, against results that are then
-// multiplied and, but for f32 outputs, rounded to 16 bits.
+// Phi(g), the normal distribution's integral, and e^(-g^2 / 2), which act' takes too.  From the
+// tail Phi(-a) = e^(-a^2 / 2) t P(t), t = 1 / (1 + 0.3055 a): P is of degree 7, fitted here to the
+// least relative error over a of 0 to 14.5 (1.4 u, u = 2^-24), so that gates far out keep their
+// value, where 1 + erf would cancel.  In f32 Phi(-a) is off by (19 + 1.3 a^2) u of itself (a^2 by the
+// exponent's own rounding), 1 - Phi(-a) by what that is of it; below 2^-126 (a > 12.9) it is 0.
+__device__ __forceinline__ float normal_below(float g, float* e) {
+  const float a = fabsf(g);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3055f, a, 1.0f));
+  float p = __builtin_fmaf(0.0366840921f, t, -0.152139843f);
+  p = __builtin_fmaf(p, t, 0.183085442f);
+  p = __builtin_fmaf(p, t, -0.0360131003f);
+  p = __builtin_fmaf(p, t, 0.120097294f);
+  p = __builtin_fmaf(p, t, 0.103812955f);
+  p = __builtin_fmaf(p, t, 0.122632049f);
+  p = __builtin_fmaf(p, t, 0.121841155f);
+  *e = __builtin_amdgcn_exp2f(a * a * -0.72134752f);
+  const float q = p * t * *e;
+  return g < 0.0f ? q : 1.0f - q;
+}
+
+// act(g): SiLU g / (1 + e^-g), GELU g Phi(g).  The exponential is v_exp_f32 of g log2(e) and
+// quotients v_rcp_f32, each 2 u off: some 20 instructions less than a correctly rounded
+// quotient and expf.  SiLU's exponent is rounded too, which takes it (8 + 2 |g|) u off where g is
+// below 0; below -87 it is 0 (e^-g above 2^126).
 template <int ACT>
 __device__ __forceinline__ float gate(float g) {
+  float e;
   if constexpr (ACT == VK_GATE_SILU)
     return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
   else
-    return vkd::gelu1<0>(g);
+    return g * normal_below(g, &e);
 }
 
 // act(g) and its derivative: SiLU's is s (1 + g (1 - s)), s = 1 / (1 + e^-g); GELU's
@@ -678,9 +699,10 @@ __device__ __forceinline__ void gate_slope(float g, float* act, float* slope) {
     *act = g * s;
     *slope = s * __builtin_fmaf(g, 1.0f - s, 1.0f);
   } else {
-    const float phi = 0.5f + 0.5f * vkd::erf_as7126(g * 0.70710678f);
+    float e;
+    const float phi = normal_below(g, &e);
     *act = g * phi;
-    *slope = __builtin_fmaf(g * 0.39894228f, __builtin_amdgcn_exp2f(g * g * -0.72134752f), phi);
+    *slope = __builtin_fmaf(g * 0.39894228f, e, phi);
   }
 }
 

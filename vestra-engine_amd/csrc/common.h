@@ -45,6 +45,7 @@ struct vk_runtime {
   size_t work_len = 0;
   // Counters of the workgroups that have left their part of a tile whose k is shared out over
   // several (product_nt.h): zeros between launches, since the last one to arrive clears its tile's.
+  // Null until ensure_work first allocates: creating a runtime allocates nothing.
   unsigned* arrivals = nullptr;
   // Replaced device buffers (work buffers, smaller RoPE tables): graphs
   // captured earlier may still name them, so they live until the runtime

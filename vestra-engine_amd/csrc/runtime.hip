@@ -163,6 +163,16 @@ int ensure_work(vk_runtime* rt, size_t floats, const char* who) {
   VK_REQUIRE(st == hipStreamCaptureStatusNone,
              "%s: the work buffer must grow to %zu floats before stream capture "
              "(run the sequence once eagerly first)", who, floats);
+  if (!rt->arrivals) {  // with the first buffer: who shares a tile's sums keeps them there
+    unsigned* a = nullptr;
+    VK_HIP(hipMalloc(reinterpret_cast<void**>(&a), kArrivals * sizeof(unsigned)));
+    const hipError_t e = hipMemsetAsync(a, 0, kArrivals * sizeof(unsigned), rt->stream);
+    if (e != hipSuccess) {
+      (void)hipFree(a);
+      return hip_fail(e, "hipMemsetAsync(arrival counters)");
+    }
+    rt->arrivals = a;
+  }
   size_t len = floats > 2 * rt->work_len ? floats : 2 * rt->work_len;
   if (len < (size_t{8} << 20)) len = size_t{8} << 20;
   float* p = nullptr;
@@ -354,15 +364,6 @@ int vk_runtime_create(int device, vk_runtime** out) {
   if (e != hipSuccess) {
     delete rt;
     return hip_fail(e, "hipStreamCreateWithFlags");
-  }
-  e = hipMalloc(reinterpret_cast<void**>(&rt->arrivals), kArrivals * sizeof(unsigned));
-  if (e == hipSuccess) e = hipMemsetAsync(rt->arrivals, 0, kArrivals * sizeof(unsigned), rt->stream);
-  if (e == hipSuccess) e = hipStreamSynchronize(rt->stream);
-  if (e != hipSuccess) {
-    if (rt->arrivals) (void)hipFree(rt->arrivals);
-    (void)hipStreamDestroy(rt->stream);
-    delete rt;
-    return hip_fail(e, "hipMalloc(arrival counters)");
   }
   *out = rt;
   return VK_OK;

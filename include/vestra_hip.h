@@ -670,7 +670,8 @@ int vk_linear_i8_run_residual(vk_runtime* rt, const vk_linear_i8* lin,
 
 /* The activation of a gated feed-forward, in f32 and right in relative terms on both sides:
  * SiLU off by (9 + 2 |g|) 2^-24 of itself (0 below g = -87), GELU by (20 + 1.3 g^2) 2^-24
- * (0 below g = -12.9).  vk_linear_i8_run_gelu has the GELU stream's erf, whose error is absolute. */
+ * (0 below g = -12.9).  vk_linear_i8_run_gelu has the GELU stream's erf, whose error is
+ * absolute. */
 #define VK_GATE_SILU 0 /* g / (1 + e^-g)                        */
 #define VK_GATE_GELU 1 /* 0.5 g (1 + erf(g / sqrt 2))           */
 /* The gated form: of the linear's out_features = 2 hidden columns the first
@@ -698,8 +699,10 @@ int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
  * hidden]; nothing is kept from the forward.  dx [rows, in_features], dw
  * [2 hidden, in_features], dbias [2 hidden] of x's type are overwritten; each may
  * be NULL (not computed), and overlaps no other tensor.  The gradients of g and u
- * are f32 up to one rounding to x's type, as operands of the products; dbias sums
- * them before that rounding.  The same call gives the same bits.  Intermediate
+ * are f32 up to one rounding to x's type, as operands of the products (in f16 times
+ * a power of two, where the largest of them is above 65,504 or below 2^-8: dx and dw
+ * do not hang on a loss's scale, a call takes longer there); dbias sums them before
+ * that rounding.  The same call gives the same bits.  Intermediate
  * values (2 rows x hidden and some) go to the runtime's work buffer: run it once
  * before a capture. */
 int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,

@@ -10,7 +10,9 @@
 // Backward, from x, w, b and the gradient dh, with nothing kept from the forward:
 //   1. g and u again, and in the same kernel dg = dh u act'(g), du = dh act(g), in
 //      f32 up to one rounding to x's type: the two products below take 16-bit
-//      operands.  Written as rows dg | du, with the f32 column sums of each tile;
+//      operands.  Written as rows dg | du, with the f32 column sums of each tile.  In f16, whose
+//      range is short, they are written times a power of two where their largest asks for
+//      it (Range);
 //   2. dx = [dg du] [Wg; Wu], w's lines being k;
 //   3. dw = [dg du]^T x, the lines of both being k;
 //   4. db: the tiles' column sums added in order;
@@ -24,6 +26,32 @@ using vkp::kBF16;
 using vkp::kF16;
 using vkp::Operand;
 
+// What f16 holds of dg and du.  Its numbers end at 65,504 and are whole multiples of 2^-24: a
+// loss's scale moves gradients past either end while dx and dw would be held.  So the first launch
+// of step 1 also finds the largest |dg|, |du| (a NaN aside): every workgroup leaves its tile's, the
+// last one to arrive takes the largest of all and with it the power of two that d is to be written
+// times. That is 1 from 2^-8 (below which values of a 64th of the largest would lose bits) to
+// 65,504, and for an infinity; otherwise a second launch writes d again, its largest in [2^14,
+// 2^15), and steps 2 and 3 take the power back in f32.  At a power of 1 the second launch ends at
+// once (10,392 x 1536 -> 2 x 4096: 4.5 us, and 270 where d is written again; a backward of 866 x
+// 768 -> 2 x 2048: 45 us, 58 written again, 41 with none of this).  bf16 has f32's range and none
+// of this.
+struct Range {
+  float* power;  // and 1 / power behind it; null: none of this
+  float* peaks;  // of each tile
+  unsigned* arrivals;  // 1 + kPeakGroups counters, a line each; zero before and after a launch
+  bool again;
+};
+// Tiles arrive by groups, and a group's last one for all of it: at one counter they would queue,
+// some 14 ns each (866 x 768 -> 2 x 2048, 896 tiles: 26.4 us against 19.3).
+constexpr int kPeakGroups = 32, kPeakLine = 16;
+__device__ __forceinline__ float power_for(float peak) {
+  const int e = static_cast<int>(__float_as_uint(peak) >> 23);
+  const bool held = peak == 0.0f || (peak >= 0x1p-8f && peak <= 65504.0f) || e == 255;
+  const int power = 268 - e < 240 ? 268 - e : 240;  // 2^14 over the peak's own power, biased
+  return held ? 1.0f : __uint_as_float(static_cast<uint32_t>(power) << 23);
+}
+
 struct Args {
   Operand a, b;
   int k_bytes;
@@ -33,6 +61,7 @@ struct Args {
   void* d;           // dg | du, rows of 2 d_half values, zeros from N to d_half of each half
   float* sums;       // [gm * WM, 2 N], or null
   int d_half;
+  Range range;       // of d in f16
   int M, N;
   int act;
   int gm, gn, group;
@@ -103,6 +132,47 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_kernel(Args
   });
 }
 
+// A workgroup's largest |dg|, |du|, from its waves'; behind the barrier wave 0 goes on alone, and
+// the last tile's takes the power.  Stores and loads of peaks go past the XCD's L2, as those of
+// shared sums do.
+template <typename T>
+__device__ __forceinline__ void leave_peak(const Range& range, int tile, int tiles, float peak,
+                                           const vkp::Place<T>& at, float* waves) {
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) peak = fmaxf(peak, __shfl_xor(peak, d, 64));
+  if (at.lane == 0) waves[at.wave] = peak;
+  __syncthreads();
+  if (at.wave > 0) return;
+#pragma unroll
+  for (int w = 0; w < T::kWaves; ++w) peak = fmaxf(peak, waves[w]);
+  int last = 0;
+  if (at.lane == 0) {
+    __hip_atomic_store(&range.peaks[tile], peak, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the peak is there, then the count
+    const auto arrive = [](unsigned* counter, int all) {
+      const unsigned n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED,
+                                                __HIP_MEMORY_SCOPE_AGENT);
+      if (n + 1 != static_cast<unsigned>(all)) return 0;
+      __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      return 1;
+    };
+    const int group = tile % kPeakGroups, groups = tiles < kPeakGroups ? tiles : kPeakGroups;
+    if (arrive(range.arrivals + (1 + group) * kPeakLine, (tiles - group - 1) / kPeakGroups + 1))
+      last = arrive(range.arrivals, groups);
+  }
+  if (__builtin_amdgcn_readfirstlane(last) == 0) return;
+  for (int t = at.lane; t < tiles; t += 64)
+    peak = fmaxf(peak, __hip_atomic_load(&range.peaks[t], __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT));
+#pragma unroll
+  for (int d = 32; d > 0; d >>= 1) peak = fmaxf(peak, __shfl_xor(peak, d, 64));
+  if (at.lane == 0) {
+    const float power = power_for(peak);
+    range.power[0] = power;
+    range.power[1] = 1.0f / power;
+  }
+}
+
 // Step 1 of the backward: the forward's products, then dg and du where h would be, through the same
 // LDS rows as e came in by.  10,392 x 1536 -> 2 x 4096 in bf16: 262-285 us, of which the 340 MB of
 // d are some 40 that no product covers.
@@ -111,6 +181,14 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
   typedef typename vkp::Value<KIND>::type V;
   VK_STAGES(T);
   __shared__ __align__(16) float bias[T::TN];
+  constexpr bool kRanged = KIND == kF16;
+  float power = 1.0f, peak = 0.0f;
+  if constexpr (kRanged) {
+    if (g.range.again) {
+      power = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(g.range.power[0])));
+      if (power == 1.0f) return;
+    }
+  }
   int mt, nt;
   const int tiles = g.gm * g.gn, tile = blockIdx.x % tiles, part = blockIdx.x / tiles;
   vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
@@ -164,8 +242,9 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
             const float fu = held ? h * a : 0.0f;
             v[j * 16 + 4 * q + e] = fg;
             v[kCols * 16 + j * 16 + 4 * q + e] = fu;
-            dg[e] = static_cast<V>(fg);
-            du[j][q][e] = static_cast<V>(fu);
+            if constexpr (kRanged) peak = fmaxf(fmaxf(peak, fabsf(fg)), fabsf(fu));
+            dg[e] = static_cast<V>(kRanged ? fg * power : fg);
+            du[j][q][e] = static_cast<V>(kRanged ? fu * power : fu);
           }
           *at = dg;
         }
@@ -197,6 +276,9 @@ __global__ __launch_bounds__(T::kThreads, T::kWavesASimd) void gated_grad_kernel
       if (n < g.N) g.sums[(static_cast<size_t>(mt * T::WM + wm) * 2 + part) * g.N + n] = sum[k];
     }
   }
+  if constexpr (kRanged)
+    if (g.range.power && !g.range.again)
+      leave_peak<T>(g.range, tile, tiles, peak, place, reinterpret_cast<float*>(stages_[1]));
 }
 
 // One of the products of steps 2 and 3: out[m, n] = sum_k a[m, k] b[n, k], rounded to the type; a
@@ -207,6 +289,7 @@ struct Product {
   Operand a, b;
   int k_bytes;
   void* out;
+  const float* back;  // what the sums are to be multiplied by, or null
   int M, N, m_half;
   int gm, gn, group;
   vkp::Split split;
@@ -220,6 +303,9 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
   vkp::tile_at(tile, g.gm, g.gn, g.group, &mt, &nt);
   const int m0 = mt * T::TM, n0 = nt * T::TN;
   const vkp::Place<T> place;
+  float back = 1.0f;
+  if constexpr (KIND == kF16)
+    back = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(*g.back)));
   vkp::f32x16 acc[T::MT][T::NT];
   if (!vkp::product_tile<KIND, T, AC, true>(g.a, g.b, g.k_bytes, m0, n0, g.split, part, tile, tiles,
                                             place, stages_, acc))
@@ -246,7 +332,10 @@ __device__ __forceinline__ void product(const Product& g, int wg, char* const (&
         for (int q = 0; q < 4; ++q) {
           typename C::V4 w;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) w[e] = static_cast<V>(acc[i][jg + j][4 * q + e]);
+          for (int e = 0; e < 4; ++e) {
+            const float v = acc[i][jg + j][4 * q + e];
+            w[e] = static_cast<V>(KIND == kF16 ? v * back : v);
+          }
           *C::at(chunk, lane, j, q) = w;
         }
       vkd::wave_lds_fence();
@@ -394,20 +483,28 @@ size_t operands_room(size_t rows, size_t in, size_t hidden) {
   return in % 8 == 0 ? 0 : (rows + 2 * hidden) * padded(in) * 2;
 }
 
-// What the backward's launches are and what they keep in the work buffer: d, the biases' sums, then
-// split tiles' sums, of the first step and after it of the products.
+// What the backward's launches are and what they keep in the work buffer: d, the biases' sums, d's
+// power and peaks (f16), then split tiles' sums, of the first step and after it of the products.
 struct BackwardPlan {
   vkp::Plan first;
   vkp::PlanTwo second;
-  size_t work, dx_sums, bytes;
+  bool ranged;
+  size_t range, work, dx_sums, bytes;
 };
-BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, bool dbias) {
+constexpr size_t kPowers = 64;  // bytes before the peaks
+static_assert(2 * vkp::kMostTilesSplit + (1 + kPeakGroups) * kPeakLine <= vk::kArrivals,
+              "counters of dx's and dw's shared tiles, then of the peaks");
+// Of the first step in f16: a larger tile's sums leave no registers for the power and the peak.
+constexpr vkp::TileSize kLargestRanged = vkp::kTile192;
+BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool f16, bool dx, bool dw,
+                           bool dbias) {
   BackwardPlan p{};
   double us = 0;
   const size_t rows = g.M, half = padded(g.N);
   // the zeros up to d_half too
   const vkp::Shape step{g.M, static_cast<long long>(2 * half), g.k_bytes, true};
-  p.first = vkp::plan(cus, step, &us);
+  p.ranged = f16 && (dx || dw);
+  p.first = vkp::plan(cus, step, &us, 0, f16 ? kLargestRanged : vkp::kTile256);
   const auto D = static_cast<long long>(in);
   const vkp::Shape x{dx ? g.M : 0, D, static_cast<long long>(4 * half)};
   const vkp::Shape w{dw ? static_cast<long long>(2 * half) : 0, D, 2LL * g.M};
@@ -416,6 +513,8 @@ BackwardPlan plan_backward(int cus, const Args& g, size_t in, bool dx, bool dw, 
   if (dx || dw) p.work += round(rows * 4 * half);
   // (a tile of 64 or 128 rows has two waves' sums, one of 256 four)
   if (dbias) p.work += round(((rows + 63) / 64 * 2 + 4) * 2 * g.N * 4);
+  p.range = p.work;
+  if (p.ranged) p.work += round(kPowers + vkp::tiles_of(p.first.tile, step) * 4);
   p.dx_sums = vkp::split_bytes(p.second.tile[0], vkp::Job{x, p.second.splits[0]});
   const size_t after =
       p.dx_sums + vkp::split_bytes(p.second.tile[1], vkp::Job{w, p.second.splits[1]});
@@ -433,14 +532,26 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
     g.d_half = static_cast<int>(half);
   }
   if (dbias) g.sums = reinterpret_cast<float*>(room + d_bytes);
+  const float* sums_of_tiles = g.sums;
+  if (plan.ranged)
+    g.range = Range{reinterpret_cast<float*>(room + plan.range),
+                    reinterpret_cast<float*>(room + plan.range + kPowers),
+                    rt->arrivals + 2 * vkp::kMostTilesSplit, false};
   g.split = vkp::Split{plan.first.splits, room + plan.work, rt->arrivals};
   int parts = 0;
   with_tile<true>(plan.first.tile, g, [&](auto tile) {
     typedef decltype(tile) T;
-    parts = g.gm * T::WM;
-    g.gn = (static_cast<int>(half) + T::kHeld - 1) / T::kHeld;  // the zeros up to d_half too
-    hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), dim3(g.gm * g.gn * g.split.count),
-                       dim3(T::kThreads), 0, rt->stream, g);
+    if constexpr (KIND != kF16 || !std::is_same_v<T, vkp::Tile<4, 2, 2, 4, true, 2, 1>>) {
+      parts = g.gm * T::WM;
+      g.gn = (static_cast<int>(half) + T::kHeld - 1) / T::kHeld;  // the zeros up to d_half too
+      const dim3 grid(g.gm * g.gn * g.split.count), block(T::kThreads);
+      hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), grid, block, 0, rt->stream, g);
+      if (plan.ranged) {  // d again, where another power holds it better; the biases' sums stand
+        g.range.again = true;
+        g.sums = nullptr;
+        hipLaunchKernelGGL((gated_grad_kernel<KIND, T>), grid, block, 0, rt->stream, g);
+      }
+    }
   });
   VK_TRY(vk::check_launch("gated_grad_kernel"));
   const char* d = static_cast<char*>(g.d);
@@ -457,6 +568,7 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
     x.b.k_half = static_cast<int>(half);
     x.k_bytes = 2 * both;
     x.out = dx->ptr;
+    if (plan.ranged) x.back = g.range.power + 1;
     x.M = R;
     x.N = D;
   }
@@ -467,11 +579,12 @@ int backward(vk_runtime* rt, Args& g, const BackwardPlan& plan, size_t rows, siz
     w.b.ks = R;
     w.k_bytes = 2 * R;
     w.out = dw->ptr;
+    if (plan.ranged) w.back = g.range.power + 1;
     w.M = H2;
     w.N = D;
     w.m_half = static_cast<int>(half);
   }
-  BiasSums sums{g.sums, parts, H2, dbias ? dbias->ptr : nullptr};
+  BiasSums sums{sums_of_tiles, parts, H2, dbias ? dbias->ptr : nullptr};
   // (the first step's split sums are done with)
   const vkp::PlanTwo& two = plan.second;
   x.split = vkp::Split{two.splits[0], room + plan.work, rt->arrivals};
@@ -611,7 +724,8 @@ int vk_gated_backward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, co
   }
   const size_t room = operands_room(rows, in_features, hidden);
   Args g = forward_args(rt, x, w, bias, rows, in_features, hidden, activation);
-  const BackwardPlan plan = plan_backward(rt->cu_count, g, in_features, dx, dw, dbias);
+  const BackwardPlan plan =
+      plan_backward(rt->cu_count, g, in_features, x->dtype == VK_F16, dx, dw, dbias);
   VK_TRY(vk::ensure_work(rt, (room + plan.bytes + 3) / 4, "gated_backward"));
   char* work = reinterpret_cast<char*>(rt->work);
   VK_TRY(align_operands(rt, g, in_features, work));

@@ -157,9 +157,12 @@ inline bool few_rows(int cus, const Shape& p, double tiles_us, double prepare) {
   return us <= 0.85 * (tiles_us > 4.5 ? tiles_us : 4.5) + 1.2 + prepare;
 }
 
-inline Plan plan(int cus, const Shape& p, double* us, double prepare = 0) {
+// `largest`: of the tiles to choose from.
+inline Plan plan(int cus, const Shape& p, double* us, double prepare = 0,
+                 TileSize largest = kTile256) {
   Plan best{false, kTile64, 1};
   for (TileSize t : kTiles) {
+    if (t > largest) break;
     const int splits = splits_for(cus, t, p);
     const double c = launch_cost(cus, t, {Job{p, splits}});
     if (t != kTile64 && c >= *us) continue;

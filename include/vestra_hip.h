@@ -656,8 +656,10 @@ int vk_linear_i8_destroy(vk_linear_i8* lin);
 size_t vk_linear_i8_input_features(const vk_linear_i8* lin);
 /* out [rows, out_features] = y [* gamma].  x and out are f32, f16 or bf16, each
  * of its own type, and start on 16 bytes; 16-bit results are rounded once.  out
- * must not overlap x.  Beyond 16 rows (or 16,384 codes) the codes of x go to the
- * runtime's work buffer: run a call once before a capture.  Less than 2^24 rows. */
+ * must not overlap x.  Beyond 16 rows, or 16,384 bytes of codes (each row takes
+ * in_features rounded up to 128), the codes of x go to the runtime's work buffer: run a
+ * call once before a capture.  Less than 2^24 rows, and rows / 64 times the columns of
+ * out / 32 (each rounded up) less than 2^23. */
 int vk_linear_i8_run_into(vk_runtime* rt, const vk_linear_i8* lin,
                           const vk_tensor* x, size_t rows, vk_tensor* out);
 /* out = GELU(y), the erf of vk_gelu_f32_inplace.  No LayerScale. */

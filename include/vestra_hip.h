@@ -693,7 +693,9 @@ int vk_linear_i8_run_gated(vk_runtime* rt, const vk_linear_i8* lin,
  * products of few outputs and a long sum leave partial sums there (run a call
  * once before a capture, which cannot grow it).  The weights' rows, rounded up
  * to 128 bytes, take less than 2 GiB; in_features and hidden at most 2^20, rows
- * 2^24. */
+ * 2^24, and rows / 64 times hidden / 32 (each rounded up) less than 2^23.  In_features
+ * that are no multiple of 8: x's and w's rows together, each rounded up to 128 bytes, take
+ * less than 32 GiB. */
 int vk_gated_forward(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
                      const vk_tensor* bias, size_t rows, size_t in_features,
                      size_t hidden, int activation, vk_tensor* out);

@@ -443,6 +443,7 @@ void zero16(const vk_runtime* rt, void* p, size_t n) {
 // ---------------------------------------------------------------- launches
 constexpr size_t kPitchValues = 64;  // rows of workspace start on 128-byte lines
 size_t padded(size_t n) { return (n + kPitchValues - 1) / kPitchValues * kPitchValues; }
+constexpr size_t kMostPieces = size_t{0x7fffff} * 256;  // of 16 bytes, that a launch copies
 
 template <bool PAIRED, typename F>
 void with_tile(vkp::TileSize size, Args& g, F go) {
@@ -635,6 +636,9 @@ int check_inputs(vk_runtime* rt, const vk_tensor* x, const vk_tensor* w, const v
                     2 * hidden, in);
   VK_UNSUPPORTED_IF(((rows + 63) / 64) * ((hidden + 31) / 32) > 0x7fffffULL,
                     "gated: %zu x %zu outputs", rows, hidden);
+  // the copies' launch (align_operands), a thread to 16 bytes
+  VK_UNSUPPORTED_IF(in % 8 != 0 && (rows + 2 * hidden) * (padded(in) / 8) > kMostPieces,
+                    "gated: %zu rows of %zu, no multiple of 8", rows + 2 * hidden, in);
   VK_TRY(check16(rt, x, x->dtype, rows * in, "x"));
   VK_TRY(check16(rt, w, x->dtype, 2 * hidden * in, "w"));
   if (bias) VK_TRY(check16(rt, bias, x->dtype, 2 * hidden, "bias"));
@@ -661,7 +665,6 @@ Args forward_args(const vk_runtime* rt, const vk_tensor* x, const vk_tensor* w,
 int align_operands(const vk_runtime* rt, Args& g, size_t in, char* room) {
   if (in % 8 == 0) return VK_OK;
   const size_t rows = g.a.rows, all = rows + g.b.rows, pieces = padded(in) / 8;
-  VK_UNSUPPORTED_IF(all * pieces > 0x7fffffULL * 256, "gated: %zu rows of %zu", all, in);
   hipLaunchKernelGGL(pad16_kernel, dim3((all * pieces + 255) / 256), dim3(256), 0, rt->stream,
                      g.a.base,
                      g.b.base, rows, all, static_cast<int>(in), static_cast<int>(pieces), room);

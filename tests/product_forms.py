@@ -82,14 +82,14 @@ def linear_i8(m, k, n, gated=False):
 FORWARD = [(1, 40, 71), (19, 39, 71), (1, 6760, 69), (36, 330, 71), (69, 300, 4149),
            (734, 8064, 333), (6591, 136, 292), (65, 3944, 4826), (645, 200, 5862), (9801, 250, 555)]
 BACKWARD = {
-    "bf16": [(78, 2696, 74), (74, 290, 5729), (76, 4200, 329), (70, 2283, 902), (1352, 1660, 78),
-             (76, 72, 1142), (2799, 104, 731), (3796, 1136, 70), (2196, 71, 70), (4122, 4779, 78),
-             (3349, 330, 1271), (962, 6072, 199), (91, 4290, 4358), (74, 5144, 4866),
-             (8482, 1368, 141), (658, 6056, 673), (973, 80, 5439)],
-    "f16": [(87, 2936, 72), (69, 285, 5416), (71, 5808, 260), (73, 2720, 727), (1291, 1902, 70),
-            (71, 96, 1052), (2896, 88, 728), (3423, 1192, 74), (70, 4174, 4237), (2199, 88, 69),
-            (3217, 352, 1247), (993, 6168, 200), (8755, 2064, 70), (69, 4107, 5175),
-            (3797, 4238, 109), (1033, 5472, 388)]}
+    "bf16": [(78, 2696, 74), (4113, 72, 70), (79, 3897, 329), (70, 3544, 842), (76, 72, 1142),
+             (2799, 104, 731), (4126, 4072, 69), (69, 1288, 3735), (4809, 1248, 76),
+             (3349, 330, 1271), (2772, 4776, 73), (135, 5888, 1401), (962, 6072, 199),
+             (1283, 5416, 370), (1108, 552, 6156), (4122, 5512, 69), (133, 2840, 5005)],
+    "f16": [(87, 2936, 72), (75, 3909, 328), (4117, 72, 71), (71, 96, 1052), (69, 3376, 1027),
+            (2615, 64, 879), (70, 4174, 4237), (1679, 3264, 77), (70, 1776, 3276),
+            (6885, 1160, 70), (3217, 352, 1247), (2737, 4992, 77), (993, 6168, 200),
+            (1033, 5472, 388), (140, 5821, 1309), (5291, 4483, 72), (82, 4456, 4838)]}
 LINEAR_I8 = [(1, 32, 70), (17, 300, 72), (3, 5864, 73), (34, 410, 69), (42, 4488, 72),
              (9808, 200, 69), (69, 16815, 4109), (8217, 264, 463), (67, 8036, 8268),
              (1560, 300, 5101), (2579, 390, 4481)]

@@ -10,9 +10,11 @@
 // Backward, from x, w, b and the gradient dh, with nothing kept from the forward:
 //   1. g and u again, and in the same kernel dg = dh u act'(g), du = dh act(g), in
 //      f32 up to one rounding to x's type: the two products below take 16-bit
-//      operands.  Written as rows dg | du, with the f32 column sums of each tile.  In f16, whose
-//      range is short, they are written times a power of two where their largest asks for
-//      it (Range);
+//      operands.  That rounding is as large as the result's own (10,392 x 1536 -> 2 x 4096 in
+//      bf16: off by 2.3e-3 of the norm with it, 1.7e-3 without); held as two 16-bit parts, the
+//      products below would have to be made twice, 430 us of 930.  Written as rows dg | du, with
+//      the f32 column sums of each tile.  In f16, whose range is short, they are written times a
+//      power of two where their largest asks for it (Range);
 //   2. dx = [dg du] [Wg; Wu], w's lines being k;
 //   3. dw = [dg du]^T x, the lines of both being k;
 //   4. db: the tiles' column sums added in order;
@@ -33,9 +35,9 @@ using vkp::Operand;
 // times. That is 1 from 2^-8 (below which values of a 64th of the largest would lose bits) to
 // 65,504, and for an infinity; otherwise a second launch writes d again, its largest in [2^14,
 // 2^15), and steps 2 and 3 take the power back in f32.  At a power of 1 the second launch ends at
-// once (10,392 x 1536 -> 2 x 4096: 4.5 us, and 270 where d is written again; a backward of 866 x
-// 768 -> 2 x 2048: 45 us, 58 written again, 41 with none of this).  bf16 has f32's range and none
-// of this.
+// once.  A backward of 257 x 384 -> 2 x 1023 takes 23.6 us (29 written again, 19.6 with none of
+// this), of 866 x 768 -> 2 x 2048 41.8 (52; 38.2), of 10,392 x 1536 -> 2 x 4096 715 (974; 690).
+// bf16 has f32's range and none of this.
 struct Range {
   float* power;  // and 1 / power behind it; null: none of this
   float* peaks;  // of each tile
@@ -43,7 +45,7 @@ struct Range {
   bool again;
 };
 // Tiles arrive by groups, and a group's last one for all of it: at one counter they would queue,
-// some 14 ns each (866 x 768 -> 2 x 2048, 896 tiles: 26.4 us against 19.3).
+// some 14 ns each (866 x 768 -> 2 x 2048 in 896 tiles of 64 x 64: 26.4 us against 19.3).
 constexpr int kPeakGroups = 32, kPeakLine = 16;
 __device__ __forceinline__ float power_for(float peak) {
   const int e = static_cast<int>(__float_as_uint(peak) >> 23);
@@ -85,7 +87,7 @@ __device__ __forceinline__ void load_bias(const Args& g, int n0, float* to) {
 
 // The forward's tiles.  A wave has gates and partners of the same columns in its sums, so nothing
 // but h leaves.  10,392 x 1536 -> 2 x 4096 in bf16: 235 us with SiLU (1.11 PFLOP/s; a library's
-// plain product of these sizes 278), 246 with GELU, whose erf no other work covers; 866 x 1024 -> 2
+// plain product of these sizes 278), 247 with GELU, whose Phi no other work covers; 866 x 1024 -> 2
 // x 2736 in f16 16.5, one round of tiles.  Bound by the products (product_nt.h) and the tiles'
 // ends.
 template <Kind KIND, typename T>

@@ -128,8 +128,9 @@ struct Tile {
   }
 };
 
-// The tile of a plan's size.  Gates and partners of the largest: a wave's 64 hidden columns are
-// one line of 16-bit results.
+// The tile of a plan's size.  16-bit results leave as whole lines where a wave has an even number
+// of 32-column tiles of them (gates and partners: of hidden columns, which only the largest tile
+// has), as halves of lines with the others.
 template <bool PAIRED, typename F>
 void with_tile(TileSize size, F go) {
   if (size == kTile192) {
@@ -533,9 +534,9 @@ __device__ __forceinline__ bool product_tile(const Operand& a, const Operand& b,
 }
 
 // A wave's sums lie with a row of a in each lane (lane % 32) and 16 columns in its registers:
-// register 4 q + e is column 8 q + 4 (lane / 32) + e of its 32.  Results leave through LDS, 32
-// rows at a time, so that a row's columns go to memory as whole lines: a Chunk is a wave's own
-// 32 rows of 32 J columns, in the stage buffers that the products are done with, its 16-byte
+// register 4 q + e is column 8 q + 4 (lane / 32) + e of its 32.  Results leave through LDS, 32 rows
+// at a time, so that a row's columns go to memory as lines or halves of them: a Chunk is a wave's
+// own 32 rows of 32 J columns, in the stage buffers that the products are done with, its 16-byte
 // pieces permuted as the stages' are.
 template <typename V, int J>
 struct Chunk {
@@ -660,8 +661,8 @@ __device__ __forceinline__ void tile_at(int tile, int gm, int gn, int group, int
 // Phi(g), the normal distribution's integral, and e^(-g^2 / 2), which act' takes too.  From the
 // tail Phi(-a) = e^(-a^2 / 2) t P(t), t = 1 / (1 + 0.3055 a): P is of degree 7, fitted here to the
 // least relative error over a of 0 to 14.5 (1.4 u, u = 2^-24), so that gates far out keep their
-// value, where 1 + erf would cancel.  In f32 Phi(-a) is off by (19 + 1.3 a^2) u of itself (a^2 by the
-// exponent's own rounding), 1 - Phi(-a) by what that is of it; below 2^-126 (a > 12.9) it is 0.
+// value, where 1 + erf would cancel.  In f32 Phi(-a) is off by (19 + 1.3 a^2) u of itself (a^2 by
+// the exponent's own rounding), 1 - Phi(-a) by what that is of it; below 2^-126 (a > 12.9) it is 0.
 __device__ __forceinline__ float normal_below(float g, float* e) {
   const float a = fabsf(g);
   const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3055f, a, 1.0f));

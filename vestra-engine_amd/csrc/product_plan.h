@@ -180,9 +180,9 @@ inline Plan plan(int cus, const Shape& p, double prepare = 0) {
 }
 
 // Two products that do not wait for one another: in one launch of one tile, or each in its own.
-// What the second launch costs is `kLaunch`, with the first one's end that covers nothing (110 sizes
-// of 34 to 9,735 rows, both ways timed: 6.3 us where both are one round of tiles; with 8 the choice
-// loses 0.5% against the better one on average, with 3 1.5%).
+// What the second launch costs is `kLaunch`, with the first one's end that covers nothing (110
+// sizes of 34 to 9,735 rows, both ways timed: 6.3 us where both are one round of tiles; with 8 the
+// choice loses 0.5% against the better one on average, with 3 1.5%).
 constexpr double kLaunch = 8;
 struct PlanTwo {
   bool together;

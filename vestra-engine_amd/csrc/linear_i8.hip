@@ -125,7 +125,7 @@ __device__ __forceinline__ uint32_t top_of(const float (&v)[8], uint32_t top) {
 
 // WPR waves a row (4 of them are a workgroup's, otherwise it has 4 rows).  NV steps of 8
 // values a lane stay in registers between the maximum and the codes; NV 0: any length, read
-// twice.  Bound by memory for many rows (10,392 x 1536 f32: 17.8 us, 4.5 TB/s of what is read and
+// twice.  Bound by memory for many rows (10,392 x 1536 f32: 16.6 us, 4.8 TB/s of what is read and
 // written), by the chain row -> maximum -> codes for few.
 template <typename XT, int NV, int WPR>
 __global__ __launch_bounds__(256) void quantise_rows_kernel(const XT* __restrict__ x, int M, int K,
